@@ -217,7 +217,7 @@ def prepare(case, seed):
         return s
     M, op = case["M"], case["op"]
     new = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="cuda")  # noqa: E731
-    lm = _lm()
+    lm = s["lm"] = _lm()
     if op == "norm":
         s["y"], s["rstd"] = new(M, case["N"], dtype=DTYPES[case["y"]]), new(M)
         s["total"] = torch.empty_like(s["x"]) if case["residual"] else None
@@ -246,7 +246,7 @@ def _lm():
 
 
 def _run_own(s):
-    lm, case = _lm(), s["case"]
+    lm, case = s["lm"], s["case"]
     op = case["op"]
     if op == "norm":
         lm.rms_norm_launch(s["x"], s["weight"], s["y"], residual=s.get("residual"), total=s["total"],
