@@ -1,0 +1,432 @@
+// Root-mean-square norm with the residual's addition, and its backward pass.
+//
+//   h = x + r;  rstd = (mean h^2 + eps)^(-1/2);  y = h rstd w
+//   8-bit y:    s = max |y| / Q (Q = 127 or 448),  q = y / s to nearest even
+//   backward:   t = dy w;  xh = h rstd;  dx = rstd (t - xh mean(t xh)) + dh;
+//               dw = sum over rows of dy xh
+//
+// Bound by memory: about one operation a byte. A row is read once and held in
+// registers between the sum and the output.
+#include "kernels.hpp"
+#include "lm_common.hpp"
+#include "lm_kernels.hpp"
+
+namespace edsl {
+namespace lm {
+namespace {
+
+// What y holds.
+enum : int { kOutSame = 0, kOutI8 = 1, kOutE4m3 = 2 };
+
+// (sum a, max b) over the TPR threads that share a row, in all of them. `lds`
+// holds two floats a wave; a barrier precedes its next use.
+template <int TPR>
+__device__ __forceinline__ void row_reduce(float& a, float& b, float* lds, bool want_b) {
+  a = wave_all<Sum>(a);
+  if (want_b) b = wave_all<MaxNan>(b);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) {
+      lds[2 * wave] = a;
+      lds[2 * wave + 1] = b;
+    }
+    __syncthreads();
+    a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) a += lds[2 * w];
+    if (want_b) {
+      b = lds[1];
+#pragma unroll
+      for (int w = 1; w < W; ++w) b = MaxNan::of(b, lds[2 * w + 1]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float weight_at(const void* w, bool f32, int64_t i) {
+  return f32 ? static_cast<const float*>(w)[i] : (float)static_cast<const T*>(w)[i];
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_weight(const void* w, bool f32, int64_t i0, int64_t n, float (&v)[VEC]) {
+  if (f32) {
+    const auto r = load_guarded<float, VEC>(static_cast<const float*>(w), i0, n);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = r.v[e];
+  } else {
+    const auto r = load_guarded<T, VEC>(static_cast<const T*>(w), i0, n);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (float)r.v[e];
+  }
+}
+
+template <typename T, int OUT, int VEC>
+__device__ __forceinline__ void store_y(void* y, int64_t row_at, int64_t i0, int64_t n, const float (&v)[VEC],
+                                        float inv) {
+  if constexpr (OUT == kOutSame) {
+    Packed<T, VEC> r;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = (T)v[e];
+    store_guarded<T, VEC>(static_cast<T*>(y) + row_at, i0, n, r);
+  } else {
+    Packed<uint8_t, VEC> r;
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      uint32_t code = 0;
+      if constexpr (OUT == kOutI8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float q = __builtin_amdgcn_fmed3f(rintf(v[e + j] * inv), -127.0f, 127.0f);
+          code |= ((uint32_t)(int)q & 0xffu) << (8 * j);
+        }
+      } else {
+        float q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f(v[e + j] * inv, -448.0f, 448.0f);
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+        code = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], c, true);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.v[e + j] = (uint8_t)(code >> (8 * j));
+    }
+    store_guarded<uint8_t, VEC>(static_cast<uint8_t*>(y) + row_at, i0, n, r);
+  }
+}
+
+// The scale of an 8-bit row whose largest |h w| is `amax`, and what y is multiplied by.
+template <int OUT>
+__device__ __forceinline__ void row_scale(float amax, float rstd, float& scale, float& inv) {
+  constexpr float kTop = OUT == kOutI8 ? 127.0f : 448.0f;
+  const float top = amax * rstd;
+  scale = top / kTop;
+  inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+}
+
+// TPR threads hold one row of up to TPR * NV vectors in registers; workgroups of
+// 256 threads (or TPR) take 256 / TPR rows.
+template <typename T, int OUT, int TPR, int NV>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_kernel(NormArgs a) {
+  constexpr int VEC = kVec<T>, BLOCK = TPR < 256 ? 256 : TPR, ROWS = BLOCK / TPR;
+  __shared__ float lds[2 * BLOCK / 64];
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if (row >= a.M) return;  // only where a row is one wave's, without barriers
+  const int t = threadIdx.x % TPR;
+  const bool wf32 = a.weight_type == kF32;
+  const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+  float h[NV][VEC], w[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const auto v = load_guarded<T, VEC>(x, ((int64_t)j * TPR + t) * VEC, a.N);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[j][e] = (float)v.v[e];
+  }
+  if (a.residual) {
+    const T* const r = static_cast<const T*>(a.residual) + row * a.ldr;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const auto v = load_guarded<T, VEC>(r, ((int64_t)j * TPR + t) * VEC, a.N);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[j][e] += (float)v.v[e];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) load_weight<T, VEC>(a.weight, wf32, ((int64_t)j * TPR + t) * VEC, a.N, w[j]);
+  float sum = 0.0f, amax = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      sum = fmaf(h[j][e], h[j][e], sum);
+      if constexpr (OUT != kOutSame) amax = MaxNan::of(amax, fabsf(h[j][e] * w[j][e]));
+    }
+  row_reduce<TPR>(sum, amax, lds, OUT != kOutSame);
+  const float rstd = 1.0f / sqrtf(sum / (float)a.N + a.eps);
+  float scale = 0.0f, inv = 1.0f;
+  if constexpr (OUT != kOutSame) {
+    row_scale<OUT>(amax, rstd, scale, inv);
+    if (t == 0) a.scales[row] = scale;
+  }
+  if (a.rstd && t == 0) a.rstd[row] = rstd;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int64_t i0 = ((int64_t)j * TPR + t) * VEC;
+    if (i0 >= a.N) break;
+    if (a.total) {
+      Packed<T, VEC> r;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r.v[e] = (T)h[j][e];
+      store_guarded<T, VEC>(static_cast<T*>(a.total) + row * a.ldt, i0, a.N, r);
+    }
+    float y[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] = h[j][e] * rstd * w[j][e];
+    store_y<T, OUT, VEC>(a.y, row * a.ldy, i0, a.N, y, inv);
+  }
+}
+
+// Rows of any length: one workgroup of 1024 threads reads the row twice, and
+// writes in the second pass only, so that the outputs may be the inputs.
+template <typename T, int OUT>
+__global__ void __launch_bounds__(1024) rms_norm_long_kernel(NormArgs a) {
+  constexpr int VEC = kVec<T>;
+  __shared__ float lds[32];
+  const int64_t row = blockIdx.x;
+  const bool wf32 = a.weight_type == kF32;
+  const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* const res = a.residual ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
+  float h[VEC], w[VEC], sum = 0.0f, amax = 0.0f;
+  const auto load = [&](int64_t i0) {
+    const auto v = load_guarded<T, VEC>(x, i0, a.N);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] = (float)v.v[e];
+    if (res) {
+      const auto r = load_guarded<T, VEC>(res, i0, a.N);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[e] += (float)r.v[e];
+    }
+    load_weight<T, VEC>(a.weight, wf32, i0, a.N, w);
+  };
+  for (int64_t i0 = (int64_t)threadIdx.x * VEC; i0 < a.N; i0 += 1024 * VEC) {
+    load(i0);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      sum = fmaf(h[e], h[e], sum);
+      if constexpr (OUT != kOutSame) amax = MaxNan::of(amax, fabsf(h[e] * w[e]));
+    }
+  }
+  row_reduce<1024>(sum, amax, lds, OUT != kOutSame);
+  const float rstd = 1.0f / sqrtf(sum / (float)a.N + a.eps);
+  float scale = 0.0f, inv = 1.0f;
+  if constexpr (OUT != kOutSame) {
+    row_scale<OUT>(amax, rstd, scale, inv);
+    if (threadIdx.x == 0) a.scales[row] = scale;
+  }
+  if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+  for (int64_t i0 = (int64_t)threadIdx.x * VEC; i0 < a.N; i0 += 1024 * VEC) {
+    load(i0);
+    if (a.total) {
+      Packed<T, VEC> r;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r.v[e] = (T)h[e];
+      store_guarded<T, VEC>(static_cast<T*>(a.total) + row * a.ldt, i0, a.N, r);
+    }
+    float y[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] = h[e] * rstd * w[e];
+    store_y<T, OUT, VEC>(a.y, row * a.ldy, i0, a.N, y, inv);
+  }
+}
+
+template <typename T, int OUT, int TPR, int NV>
+hipError_t launch_row(const NormArgs& a, hipStream_t stream) {
+  constexpr int BLOCK = TPR < 256 ? 256 : TPR, ROWS = BLOCK / TPR;
+  hipLaunchKernelGGL((rms_norm_kernel<T, OUT, TPR, NV>), dim3((unsigned)((a.M + ROWS - 1) / ROWS)), dim3(BLOCK), 0,
+                     stream, a);
+  return launched();
+}
+
+template <typename T, int OUT>
+hipError_t launch_norm(const NormArgs& a, hipStream_t stream, const char** plan) {
+  const int64_t vecs = (a.N + kVec<T> - 1) / kVec<T>;
+  if (vecs <= 64) return *plan = "row=64x1", launch_row<T, OUT, 64, 1>(a, stream);
+  if (vecs <= 256) return *plan = "row=256x1", launch_row<T, OUT, 256, 1>(a, stream);
+  if (vecs <= 512) return *plan = "row=256x2", launch_row<T, OUT, 256, 2>(a, stream);
+  if (vecs <= 1024) return *plan = "row=256x4", launch_row<T, OUT, 256, 4>(a, stream);
+  if (vecs <= 4096) return *plan = "row=1024x4", launch_row<T, OUT, 1024, 4>(a, stream);
+  *plan = "row=long";
+  hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), dim3((unsigned)a.M), dim3(1024), 0, stream, a);
+  return launched();
+}
+
+template <typename T>
+hipError_t launch_norm_out(const NormArgs& a, hipStream_t stream, const char** plan) {
+  if (a.y_type == kI8) return launch_norm<T, kOutI8>(a, stream, plan);
+  if (a.y_type == kE4m3) return launch_norm<T, kOutE4m3>(a, stream, plan);
+  return launch_norm<T, kOutSame>(a, stream, plan);
+}
+
+// ---------------------------------------------------------------- backward
+// A workgroup of TPR threads walks the rows group, group + groups, ...; a
+// thread keeps the same NV vectors of columns in each, its part of dweight in
+// registers.
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(TPR) rms_norm_backward_kernel(NormBackwardArgs a) {
+  constexpr int VEC = kVec<T>;
+  __shared__ float lds[2][2 * TPR / 64];
+  const int t = threadIdx.x;
+  const bool wf32 = a.weight_type == kF32;
+  float w[NV][VEC], dw[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    load_weight<T, VEC>(a.weight, wf32, ((int64_t)j * TPR + t) * VEC, a.N, w[j]);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[j][e] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.M; row += a.groups, turn ^= 1) {
+    const T* const pdy = static_cast<const T*>(a.dy) + row * a.lddy;
+    const T* const ph = static_cast<const T*>(a.h) + row * a.ldh;
+    Packed<T, VEC> dy[NV], h[NV], dh[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      dy[j] = load_guarded<T, VEC>(pdy, ((int64_t)j * TPR + t) * VEC, a.N);
+      h[j] = load_guarded<T, VEC>(ph, ((int64_t)j * TPR + t) * VEC, a.N);
+      if (a.dh)
+        dh[j] = load_guarded<T, VEC>(static_cast<const T*>(a.dh) + row * a.lddh, ((int64_t)j * TPR + t) * VEC, a.N);
+    }
+    const float rstd = a.rstd[row];
+    float dot = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float g = (float)dy[j].v[e], xh = (float)h[j].v[e] * rstd;
+        dot = fmaf(g * w[j][e], xh, dot);
+        dw[j][e] = fmaf(g, xh, dw[j][e]);
+      }
+    // Two buffers in turn: the barrier inside the next row's sum stands between
+    // the reads of one and its next writes.
+    row_reduce<TPR>(dot, none, lds[turn], false);
+    const float mean = dot / (float)a.N;
+    T* const pdx = static_cast<T*>(a.dx) + row * a.lddx;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t i0 = ((int64_t)j * TPR + t) * VEC;
+      if (i0 >= a.N) break;
+      Packed<T, VEC> r;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float xh = (float)h[j].v[e] * rstd;
+        float d = rstd * fmaf(-xh, mean, (float)dy[j].v[e] * w[j][e]);
+        if (a.dh) d += (float)dh[j].v[e];
+        r.v[e] = (T)d;
+      }
+      store_guarded<T, VEC>(pdx, i0, a.N, r);
+    }
+  }
+  if (!a.dweight) return;
+  float* const part = a.partials + (int64_t)blockIdx.x * a.N;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int64_t i0 = ((int64_t)j * TPR + t) * VEC;
+    if (i0 >= a.N) break;
+    Packed<float, VEC> r;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = dw[j][e];
+    store_guarded<float, VEC>(part, i0, a.N, r);
+  }
+}
+
+// Rows of any length, one workgroup a row at a time, each read twice; dweight is
+// added up in the workgroup's row of partials.
+template <typename T>
+__global__ void __launch_bounds__(1024) rms_norm_backward_long_kernel(NormBackwardArgs a) {
+  constexpr int VEC = kVec<T>;
+  __shared__ float lds[2][32];
+  const bool wf32 = a.weight_type == kF32;
+  float* const part = a.dweight ? a.partials + (int64_t)blockIdx.x * a.N : nullptr;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.M; row += a.groups, turn ^= 1) {
+    const T* const pdy = static_cast<const T*>(a.dy) + row * a.lddy;
+    const T* const ph = static_cast<const T*>(a.h) + row * a.ldh;
+    const float rstd = a.rstd[row];
+    float dot = 0.0f, none = 0.0f, w[VEC];
+    for (int64_t i0 = (int64_t)threadIdx.x * VEC; i0 < a.N; i0 += 1024 * VEC) {
+      const auto dy = load_guarded<T, VEC>(pdy, i0, a.N);
+      const auto h = load_guarded<T, VEC>(ph, i0, a.N);
+      load_weight<T, VEC>(a.weight, wf32, i0, a.N, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) dot = fmaf((float)dy.v[e] * w[e], (float)h.v[e] * rstd, dot);
+    }
+    row_reduce<1024>(dot, none, lds[turn], false);
+    const float mean = dot / (float)a.N;
+    for (int64_t i0 = (int64_t)threadIdx.x * VEC; i0 < a.N; i0 += 1024 * VEC) {
+      const auto dy = load_guarded<T, VEC>(pdy, i0, a.N);
+      const auto h = load_guarded<T, VEC>(ph, i0, a.N);
+      load_weight<T, VEC>(a.weight, wf32, i0, a.N, w);
+      Packed<T, VEC> dh, r;
+      if (a.dh) dh = load_guarded<T, VEC>(static_cast<const T*>(a.dh) + row * a.lddh, i0, a.N);
+      Packed<float, VEC> dw;
+      if (part && row != blockIdx.x) dw = load_guarded<float, VEC>(part, i0, a.N);
+      else
+        for (int e = 0; e < VEC; ++e) dw.v[e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float xh = (float)h.v[e] * rstd;
+        float d = rstd * fmaf(-xh, mean, (float)dy.v[e] * w[e]);
+        if (a.dh) d += (float)dh.v[e];
+        r.v[e] = (T)d;
+        dw.v[e] = fmaf((float)dy.v[e], xh, dw.v[e]);
+      }
+      store_guarded<T, VEC>(static_cast<T*>(a.dx) + row * a.lddx, i0, a.N, r);
+      if (part) store_guarded<float, VEC>(part, i0, a.N, dw);
+    }
+  }
+}
+
+// dweight[n] = the sum of the groups' partials, in their order: 64 columns a
+// workgroup, the groups in 16 interleaved parts, joined in order.
+__global__ void __launch_bounds__(1024) dweight_kernel(const float* partials, int groups, int64_t N, float* dweight) {
+  __shared__ float lds[16][64];
+  const int c = threadIdx.x % 64, part = threadIdx.x / 64;
+  const int64_t n = (int64_t)blockIdx.x * 64 + c;
+  float s = 0.0f;
+  if (n < N)
+    for (int g = part; g < groups; g += 16) s += partials[(int64_t)g * N + n];
+  lds[part][c] = s;
+  __syncthreads();
+  if (part == 0 && n < N) {
+#pragma unroll
+    for (int p = 1; p < 16; ++p) s += lds[p][c];
+    dweight[n] = s;
+  }
+}
+
+template <typename T>
+hipError_t launch_backward(const NormBackwardArgs& a, hipStream_t stream) {
+  const int64_t vecs = (a.N + kVec<T> - 1) / kVec<T>;
+  const dim3 grid((unsigned)a.groups);
+  if (a.M > 0) {
+    if (vecs <= 256)
+      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 256, 1>), grid, dim3(256), 0, stream, a);
+    else if (vecs <= 512)
+      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a);
+    else if (vecs <= 1024)
+      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 512, 2>), grid, dim3(512), 0, stream, a);
+    else if (vecs <= 2048)
+      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 1024, 2>), grid, dim3(1024), 0, stream, a);
+    else
+      hipLaunchKernelGGL((rms_norm_backward_long_kernel<T>), grid, dim3(1024), 0, stream, a);
+    if (const hipError_t e = launched(); e != hipSuccess) return e;
+  }
+  if (!a.dweight) return hipSuccess;
+  hipLaunchKernelGGL(dweight_kernel, dim3((unsigned)((a.N + 63) / 64)), dim3(1024), 0, stream, a.partials,
+                     a.M > 0 ? a.groups : 0, a.N, a.dweight);
+  return launched();
+}
+
+}  // namespace
+
+hipError_t launch_rms_norm(const NormArgs& a, int cus, hipStream_t stream, const char** plan) {
+  (void)cus;
+  if (a.type == kF32) return launch_norm_out<float>(a, stream, plan);
+  if (a.type == kBf16) return launch_norm_out<bf16>(a, stream, plan);
+  return launch_norm_out<f16>(a, stream, plan);
+}
+
+int rms_norm_backward_groups(int64_t M, int64_t N, int type, int cus) {
+  (void)N;
+  (void)type;
+  const int64_t most = 4 * (int64_t)cus;
+  return (int)(M < most ? (M > 0 ? M : 1) : most);
+}
+
+hipError_t launch_rms_norm_backward(const NormBackwardArgs& a, hipStream_t stream) {
+  if (a.type == kF32) return launch_backward<float>(a, stream);
+  if (a.type == kBf16) return launch_backward<bf16>(a, stream);
+  return launch_backward<f16>(a, stream);
+}
+
+}  // namespace lm
+}  // namespace edsl

@@ -83,6 +83,7 @@ struct DeviceState {
   DevBuf chain[2];  // intermediate activations of multi-layer programs (ping-pong)
   DevBuf gemv_partials{true};
   DevBuf i8_x{true}, i8_w{true}, i8_flags{true};
+  DevBuf lm_ws{true};  // partial results of the language-model operators (lm_runtime.cpp)
   // Ordering of the launches that use the library scratch above (split-K
   // partials, packed int8 operands and flag) across streams.
   hipStream_t ws_stream = nullptr;  // stream of the last such launch
@@ -916,6 +917,20 @@ void dense_f32_launch(const float* X, int64_t ldx, const float* W, int64_t ldw, 
   DenseLaunch L{EDSL_DTYPE_F32, epilogue, alpha, X, ldx, W, ldw, bias, Y, ldy, M, N, K};
   L.plan_bias = plan_bias;
   launch_dense(ds, L, static_cast<hipStream_t>(stream), fixed);
+}
+
+void device_launch(size_t bytes, void* stream, const std::function<void(char*, int)>& enqueue) {
+  std::lock_guard<std::mutex> lock(g_mu);
+  DeviceState& ds = device_state(nullptr);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (bytes == 0) {
+    enqueue(nullptr, ds.cus);
+    return;
+  }
+  char* const ws = static_cast<char*>(ds.lm_ws.ensure(bytes));
+  scratch_begin(ds, s);
+  enqueue(ws, ds.cus);
+  scratch_end(ds, s);
 }
 
 }  // namespace rt

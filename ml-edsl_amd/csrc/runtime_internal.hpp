@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <exception>
+#include <functional>
 #include <memory>
 #include <string>
 
@@ -124,6 +125,15 @@ struct FixedScratch {
   char* base;    // device address, 256-byte aligned
   size_t bytes;  // capacity; a plan that needs more is rejected (kErrLimit)
 };
+
+// Runs enqueue(workspace, number of CUs) for a device launch of `bytes` of
+// library workspace (none: null) on the current device, under the launch lock;
+// the workspace is ordered between the launches of several streams as the
+// split-K partials are (runtime.cpp), and kept once grown. Throws Failure.
+void device_launch(size_t bytes, void* stream, const std::function<void(char*, int)>& enqueue);
+
+// The description that edsl_hip_last_plan() gives of the calling thread's call.
+void set_plan(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 
 // Body of edsl_hip_dense_f32_launch (argument checks, plan, launch); with
 // `fixed` non-null every scratch buffer comes from it. `plan_bias`, when not

@@ -37,6 +37,11 @@ MEMREF_ENTRY_POINTS = {
     "edsl_hip_matmul_if_relu_f32": MEMREF2 * 3,
 }
 
+LM_ENTRY_POINTS = ("edsl_hip_rms_norm_launch", "edsl_hip_rms_norm_backward_launch",
+                   "edsl_hip_token_logprobs_launch", "edsl_hip_token_logprobs_backward_launch")
+LM_F32, LM_BF16, LM_F16, LM_I8, LM_E4M3 = range(5)  # EDSL_LM_* element types
+LM_MAX_TOP = 32  # EDSL_LM_MAX_TOP
+
 
 class NativeLibraryError(ImportError):
     pass
@@ -86,6 +91,18 @@ def _declare(L: ctypes.CDLL) -> None:
     L.edsl_hip_f32_config_count.restype = c_int
     L.edsl_hip_f32_config_name.argtypes = [c_int, ctypes.c_char_p, ctypes.c_size_t]
     L.edsl_hip_f32_config_name.restype = c_int
+
+    # include/edsl_hip_lm.h
+    L.edsl_hip_rms_norm_launch.argtypes = [vp, i64, vp, i64, vp, c_int, vp, i64, vp, i64, c_int, vp, vp, i64, i64,
+                                           c_int, c_float, vp]
+    L.edsl_hip_rms_norm_backward_launch.argtypes = [vp, i64, vp, i64, vp, c_int, vp, vp, i64, vp, i64, vp, i64, i64,
+                                                    c_int, vp]
+    L.edsl_hip_token_logprobs_launch.argtypes = [vp, i64, c_int, vp, c_int, vp, vp, vp, vp, vp, c_int, i64, i64,
+                                                 c_float, vp]
+    L.edsl_hip_token_logprobs_backward_launch.argtypes = [vp, i64, c_int, vp, c_int, vp, vp, vp, vp, vp, i64, i64,
+                                                          i64, c_float, vp]
+    for name in LM_ENTRY_POINTS:
+        getattr(L, name).restype = c_int
 
 
 def _share_torch_hip_runtime() -> None:
