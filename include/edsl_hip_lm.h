@@ -83,6 +83,31 @@ int edsl_hip_token_logprobs_backward_launch(const void *logits, int64_t ldl, int
                                             const float *dentropy, void *dlogits, int64_t lddl, int64_t M, int64_t V,
                                             float scale, void *stream);
 
+/* The dense layer on 4-bit weights with a scale and, optionally, a zero point
+ * for each column and group of `group` successive k (32, 64 or a multiple of
+ * 128; the last group may be shorter):
+ *   W[k][n] = scales[k / group][n] * (q[k][n] - zeros[k / group][n]),
+ * q and zeros integers 0 .. 15 (the low four bits of their bytes), zeros 8 where
+ * there are none. edsl_hip_q4_pack_launch lays the weights out once, in
+ * edsl_hip_q4_packed_bytes bytes (-1: arguments that it does not take, with the
+ * message in edsl_hip_last_error) at a 256-byte aligned address; scales are F32,
+ * BF16 or F16 and kept as they are. */
+int64_t edsl_hip_q4_packed_bytes(int64_t K, int64_t N, int group, int scale_type, int has_zeros);
+int edsl_hip_q4_pack_launch(const uint8_t *q, int64_t ldq, const void *scales, int64_t lds, int scale_type,
+                            const uint8_t *zeros, int64_t ldz, int64_t K, int64_t N, int group, void *packed,
+                            size_t packed_bytes, void *stream);
+
+/* Y[M,N] = epilogue(x_scales[m] * X[M,K] @ W (+ bias)), EDSL_EPI_* epilogues of
+ * include/edsl_hip_device.h. X is F32, BF16, F16, I8 or E4M3, x_scales[M] (f32)
+ * optional; Y is F32, BF16 or F16, bias[N] of any of these; K, N, group,
+ * scale_type and has_zeros as packed. Products are exact and sums 32-bit: no
+ * weight or activation is rounded, f32 ones included. Sums are taken in a fixed
+ * order. A row of X that holds an infinity or NaN gives NaN in all of Y's row. */
+int edsl_hip_q4_dense_launch(const void *X, int64_t ldx, int x_type, const float *x_scales, const void *packed,
+                             const void *bias, int bias_type, void *Y, int64_t ldy, int y_type, int64_t M, int64_t N,
+                             int64_t K, int group, int scale_type, int has_zeros, int epilogue, float alpha,
+                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif

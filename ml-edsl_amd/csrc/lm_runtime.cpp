@@ -2,11 +2,13 @@
 // split of the work over the chip, and the launches.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/edsl_hip_lm.h"
 #include "dev_buf.hpp"
 #include "lm_kernels.hpp"
+#include "q4.hpp"
 #include "runtime_internal.hpp"
 
 namespace edsl {
@@ -134,6 +136,128 @@ void token_logprobs_backward(lm::LogprobsBackwardArgs a, void* stream) {
   });
 }
 
+// ------------------------------------------------------------ 4-bit layer
+lm::Q4Layout q4_checked_layout(int64_t K, int64_t N, int group, int scale_type, bool zeros) {
+  check_sizes(K, N, "K", "N");
+  check_float_type(scale_type, "scales");
+  if (group != 32 && group != 64 && (group <= 0 || group % 128 != 0))
+    fail(kErrArgument, "group=%d is not 32, 64 or a multiple of 128", group);
+  return lm::q4_layout(K, N, group, scale_type, zeros);
+}
+
+void check_packed(const void* p, const char* name) {
+  if (!p) fail(kErrArgument, "%s is null", name);
+  if (reinterpret_cast<uintptr_t>(p) % 256 != 0) fail(kErrArgument, "%s is not 256-byte aligned", name);
+}
+
+void q4_pack(lm::Q4PackArgs a, size_t bytes, void* stream) {
+  a.layout = q4_checked_layout(a.K, a.N, a.group, a.scale_type, a.zeros != nullptr);
+  if (bytes < (size_t)a.layout.bytes)
+    fail(kErrArgument, "packed: %zu bytes, %lld are needed", bytes, (long long)a.layout.bytes);
+  if (a.layout.bytes == 0) return set_plan("empty");
+  const int64_t groups = (a.K + a.group - 1) / a.group;
+  check_mat(a.q, a.ldq, a.K, a.N, "q");
+  check_mat(a.scales, a.lds, groups, a.N, "scales");
+  if (a.zeros) check_mat(a.zeros, a.ldz, groups, a.N, "zeros");
+  check_packed(a.packed, "packed");
+  check_grid(a.layout.tiles_n, a.layout.blocks);
+  device_launch(0, stream, [&](char*, int) {
+    check_hip(lm::launch_q4_pack(a, as_stream(stream)), "q4_pack launch");
+    set_plan("q4_pack group=%d", a.group);
+  });
+}
+
+size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// Up to 16 rows: column tiles of a workgroup, and how many workgroups split K,
+// so that there is one for each CU.
+void q4_small_plan(const lm::Q4Args& a, int cus, int* nt, int* ksplit) {
+  const int64_t tiles = (a.N + 15) / 16;
+  *nt = tiles >= 4 * (int64_t)cus ? 4 : tiles >= 2 * (int64_t)cus ? 2 : 1;
+  const int64_t wgs = (tiles + *nt - 1) / *nt;
+  const int64_t most = std::max(1, a.blocks / 8);
+  *ksplit = (int)std::clamp<int64_t>(cus / wgs, 1, std::min<int64_t>(most, 16));
+}
+
+int q4_tile_plan(const lm::Q4Args& a, int cus, int* ksplit) {
+  const int64_t tiles = (a.N + 15) / 16;
+  const auto count = [&](int bm) { return (a.M + bm - 1) / bm * ((tiles + 7) / 8); };
+  const int config = a.M <= 32                                              ? lm::kQ4Tile32x128
+                     : a.M <= 64 || a.x_type == lm::kF32 || count(128) < cus ? lm::kQ4Tile64x128
+                                                                             : lm::kQ4Tile128x128;
+  const int64_t wgs = count(config == lm::kQ4Tile32x128 ? 32 : config == lm::kQ4Tile64x128 ? 64 : 128);
+  check_grid(wgs, 16);
+  *ksplit = (int)std::clamp<int64_t>(cus / wgs, 1, std::clamp(a.blocks / 4, 1, 16));
+  return config;
+}
+
+void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, bool zeros, void* stream) {
+  check_sizes(M, K, "M", "K");
+  const lm::Q4Layout l = q4_checked_layout(K, N, group, a.scale_type, zeros);
+  if (a.x_type < lm::kF32 || a.x_type > lm::kE4m3) fail(kErrDtype, "X: unknown type %d", a.x_type);
+  check_float_type(a.y_type, "Y");
+  if (a.epi < 0 || a.epi > 7) fail(kErrArgument, "bad epilogue code %d", a.epi);
+  if (M == 0 || N == 0) return set_plan("empty");
+  if (a.epi & 1) {
+    if (!a.bias) fail(kErrArgument, "epilogue adds a bias but bias is null");
+    check_float_type(a.bias_type, "bias");
+  } else {
+    a.bias = nullptr;
+  }
+  check_mat(a.x, a.ldx, M, K, "X");
+  check_mat(a.y, a.ldy, M, N, "Y");
+  if (K > 0) check_packed(a.w, "packed");
+  a.M = (int)M, a.N = (int)N, a.K = (int)K;
+  a.scales_at = l.scales_at, a.zeros_at = l.zeros_at;
+  a.blocks = (int)l.blocks, a.scale_blocks = (int)l.scale_blocks, a.blocks_per_scale = l.blocks_per_scale;
+  int cus = 0;
+  device_launch(0, stream, [&](char*, int n) { cus = n; });
+  const hipStream_t s = as_stream(stream);
+  if (M <= 16) {
+    int nt;
+    q4_small_plan(a, cus, &nt, &a.ksplit);
+    const size_t bytes = a.ksplit > 1 ? (size_t)a.ksplit * a.M * a.N * sizeof(float) : 0;
+    device_launch(bytes, stream, [&](char* ws, int) {
+      a.partials = reinterpret_cast<float*>(ws);
+      hipError_t (*const launch)(const lm::Q4Args&, int, int, bool, hipStream_t) =
+          a.x_type == lm::kF32    ? lm::launch_q4_small<lm::kF32>
+          : a.x_type == lm::kBf16 ? lm::launch_q4_small<lm::kBf16>
+          : a.x_type == lm::kF16  ? lm::launch_q4_small<lm::kF16>
+          : a.x_type == lm::kI8   ? lm::launch_q4_small<lm::kI8>
+                                  : lm::launch_q4_small<lm::kE4m3>;
+      check_hip(launch(a, nt, l.spb, zeros, s), "q4_small launch");
+      if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
+      set_plan("q4_small %s cols=%d ksplit=%d%s", type_name(a.x_type), 16 * nt, a.ksplit, a.ksplit > 1 ? " +join" : "");
+    });
+    return;
+  }
+  const int config = q4_tile_plan(a, cus, &a.ksplit);
+  lm::Q4PrepArgs p{};
+  p.x = a.x, p.ldx = a.ldx, p.M = a.M, p.K = a.K, p.blocks = a.blocks, p.spb = l.spb, p.x_type = a.x_type;
+  p.factor = zeros ? -1.0f : -8.0f;
+  p.xs_ld = (M + 127) / 128 * 128;
+  // x itself where the tiles can read it: 16 bits, whole blocks, 16-byte aligned rows.
+  const bool copy = !((a.x_type == lm::kBf16 || a.x_type == lm::kF16) && K % 128 == 0 && a.ldx % 8 == 0 &&
+                      reinterpret_cast<uintptr_t>(a.x) % 16 == 0);
+  p.ldp = l.blocks * 128, p.plane = M * p.ldp;
+  const size_t sums = aligned((size_t)l.blocks * l.spb * p.xs_ld * sizeof(float));
+  const size_t planes = copy ? aligned((size_t)(a.x_type == lm::kF32 ? 3 : 1) * p.plane * 2) : 0;
+  const size_t parts = a.ksplit > 1 ? (size_t)a.ksplit * M * N * sizeof(float) : 0;
+  device_launch(sums + planes + parts, stream, [&](char* ws, int) {
+    p.xs = reinterpret_cast<float*>(ws);
+    p.xp = copy ? ws + sums : nullptr;
+    a.xs = p.xs, a.xs_ld = p.xs_ld;
+    a.xp = copy ? p.xp : a.x, a.ldp = copy ? p.ldp : a.ldx, a.plane = p.plane;
+    a.partials = reinterpret_cast<float*>(ws + sums + planes);
+    if (a.blocks > 0) check_hip(lm::launch_q4_prep(p, s), "q4_prep launch");
+    check_hip(lm::launch_q4_tile(a, config, l.spb, zeros, s), "q4_tile launch");
+    if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
+    static const char* const names[] = {"32x128", "64x128", "128x128"};
+    set_plan("q4_prep%s+q4_tile %s tile=%s ksplit=%d%s", copy ? "_copy" : "", type_name(a.x_type), names[config],
+             a.ksplit, a.ksplit > 1 ? " +join" : "");
+  });
+}
+
 }  // namespace
 }  // namespace rt
 }  // namespace edsl
@@ -187,6 +311,36 @@ int edsl_hip_token_logprobs_backward_launch(const void* logits, int64_t ldl, int
     a.dx = dlogits, a.ldx = ldl, a.lddx = lddl, a.M = M, a.V = V, a.scale = scale, a.type = type;
     a.ids64 = ids64 != 0;
     rt::token_logprobs_backward(a, stream);
+  });
+}
+
+int64_t edsl_hip_q4_packed_bytes(int64_t K, int64_t N, int group, int scale_type, int has_zeros) {
+  int64_t bytes = -1;
+  rt::guarded([&] { bytes = rt::q4_checked_layout(K, N, group, scale_type, has_zeros != 0).bytes; });
+  return bytes;
+}
+
+int edsl_hip_q4_pack_launch(const uint8_t* q, int64_t ldq, const void* scales, int64_t lds, int scale_type,
+                            const uint8_t* zeros, int64_t ldz, int64_t K, int64_t N, int group, void* packed,
+                            size_t packed_bytes, void* stream) {
+  return rt::guarded([&] {
+    lm::Q4PackArgs a{};
+    a.q = q, a.scales = scales, a.zeros = zeros, a.packed = static_cast<char*>(packed);
+    a.ldq = ldq, a.lds = lds, a.ldz = ldz, a.K = K, a.N = N, a.group = group, a.scale_type = scale_type;
+    rt::q4_pack(a, packed_bytes, stream);
+  });
+}
+
+int edsl_hip_q4_dense_launch(const void* X, int64_t ldx, int x_type, const float* x_scales, const void* packed,
+                             const void* bias, int bias_type, void* Y, int64_t ldy, int y_type, int64_t M, int64_t N,
+                             int64_t K, int group, int scale_type, int has_zeros, int epilogue, float alpha,
+                             void* stream) {
+  return rt::guarded([&] {
+    lm::Q4Args a{};
+    a.x = X, a.x_scales = x_scales, a.w = static_cast<const char*>(packed), a.bias = bias, a.y = Y;
+    a.ldx = ldx, a.ldy = ldy, a.x_type = x_type, a.scale_type = scale_type, a.y_type = y_type;
+    a.bias_type = bias_type, a.epi = epilogue, a.alpha = alpha;
+    rt::q4_dense(a, M, N, K, group, has_zeros != 0, stream);
   });
 }
 

@@ -10,6 +10,8 @@ and what the library refuses raises ``RuntimeError``.
 
 * ``rms_norm_launch``, ``rms_norm_backward_launch``: the root-mean-square norm
   with the residual's addition, its output in the input's type or in 8 bits.
+* ``q4_pack``, ``q4_dense_launch``: the dense layer on 4-bit weights with group
+  scales, and ``q4_quantize`` to make them.
 * ``token_logprobs_launch``, ``token_logprobs_backward_launch``: log
   probabilities of given tokens, log-sum-exp, entropy, top alternatives.
 """
@@ -130,6 +132,95 @@ def rms_norm_backward_launch(dY, H, weight, rstd, dX, dweight=None, dh=None, str
             rstd.data_ptr(), _ptr(dh), _ld(dh), dX.data_ptr(), dX.stride(0), _ptr(dweight), M, N, _types[dY.dtype],
             _stream(stream)):
         _native.raise_on_error("rms_norm_backward_launch")
+
+
+class Q4Weight:
+    """4-bit weights of a [K, N] layer as ``q4_pack`` laid them out."""
+
+    __slots__ = ("packed", "K", "N", "group_size", "scale_type", "has_zeros")
+
+    def __init__(self, packed, K, N, group_size, scale_type, has_zeros):
+        self.packed, self.K, self.N = packed, K, N
+        self.group_size, self.scale_type, self.has_zeros = group_size, scale_type, has_zeros
+
+    def __repr__(self):
+        return (f"Q4Weight({self.K}x{self.N}, group_size={self.group_size}, "
+                f"{'zeros, ' if self.has_zeros else ''}{self.packed.numel()} bytes on {self.packed.device})")
+
+
+def q4_quantize(W, group_size: int = 128, symmetric: bool = False):
+    """4-bit integers, scales and zero points (None when symmetric) of a float
+    matrix [K, N], each group's extremes at the ends of its range: what
+    ``q4_pack`` takes. Torch arithmetic, for the time a model is loaded."""
+    torch = _torch()
+    if W.dim() != 2 or not W.is_floating_point():
+        raise ValueError(f"W must be a 2-D float matrix, got {tuple(W.shape)} {W.dtype}")
+    K, N = W.shape
+    G = -(-K // group_size)
+    w = torch.nn.functional.pad(W.float(), (0, 0, 0, G * group_size - K)).view(G, group_size, N)
+    if symmetric:
+        scales, zeros, z = w.abs().amax(1) / 7, None, 8.0
+    else:
+        low, high = w.amin(1).clamp(max=0), w.amax(1).clamp(min=0)
+        scales = (high - low) / 15
+        z = torch.where(scales > 0, -low / scales, 0.0).round()
+        zeros, z = z.to(torch.uint8), z[:, None]
+    q = torch.where(scales[:, None] > 0, w / scales[:, None], 0.0).round() + z
+    return q.clamp(0, 15).to(torch.uint8).view(G * group_size, N)[:K].contiguous(), scales, zeros
+
+
+def q4_pack(Q, scales, zeros=None, group_size: int = 128) -> Q4Weight:
+    """Lays 4-bit weights out for ``q4_dense_launch``, once:
+    ``W[k, n] = scales[k // group_size, n] * (Q[k, n] - zeros[k // group_size, n])``.
+
+    Q [K, N] uint8 of 0 .. 15; scales [G, N] f32, bf16 or f16 with G = K /
+    group_size rounded up; zeros [G, N] uint8 of 0 .. 15, 8 where left out.
+    group_size is 32, 64 or a multiple of 128. Enqueued on the current stream."""
+    torch = _torch()
+    K, N = _matrix(Q, "Q", (torch.uint8,))
+    scale_type = _types.get(scales.dtype, -1) if scales.dtype in _floats(torch) else -1
+    bytes_ = _native.lib().edsl_hip_q4_packed_bytes(K, N, group_size, max(scale_type, 0), zeros is not None)
+    if bytes_ < 0:
+        _native.raise_on_error("q4_pack")
+    G = -(-K // group_size)
+    _operand(scales, "scales", (G, N), _floats(torch), Q)
+    if zeros is not None:
+        _operand(zeros, "zeros", (G, N), (torch.uint8,), Q)
+    packed = torch.empty(bytes_, dtype=torch.uint8, device=Q.device)
+    if _native.lib().edsl_hip_q4_pack_launch(
+            Q.data_ptr(), Q.stride(0), scales.data_ptr(), scales.stride(0), scale_type, _ptr(zeros), _ld(zeros), K, N,
+            group_size, packed.data_ptr(), bytes_, _stream(None)):
+        _native.raise_on_error("q4_pack")
+    return Q4Weight(packed, K, N, group_size, scale_type, zeros is not None)
+
+
+def q4_dense_launch(X, W: Q4Weight, b, Y, epilogue: int = _native.EPI_NONE, alpha: float = 0.0, x_scales=None,
+                    stream=None) -> None:
+    """``Y = epilogue(x_scales[:, None] * X @ W (+ b))``, with the epilogues of
+    ``device.dense_launch``.
+
+    X is [M, K] in f32, bf16, f16, int8 or float8_e4m3fn, x_scales [M] f32
+    (the 8-bit norm's, say), W from ``q4_pack``, Y [M, N] and b [N] in f32, bf16
+    or f16. Nothing is rounded before the 32-bit sums. A row of X with an
+    infinity or NaN gives a row of NaN."""
+    torch = _torch()
+    if not isinstance(W, Q4Weight):
+        raise TypeError("W is not a Q4Weight")
+    M, K = _matrix(X, "X", tuple(_types))
+    if K != W.K:
+        raise ValueError(f"shape mismatch: X{tuple(X.shape)} W{(W.K, W.N)}")
+    if W.packed.device != X.device:
+        raise ValueError(f"W is on {W.packed.device}, not on {X.device}")
+    _operand(Y, "Y", (M, W.N), _floats(torch), X)
+    if b is not None:
+        _list(b, "b", (W.N,), _floats(torch), X)
+    if x_scales is not None:
+        _list(x_scales, "x_scales", (M,), (torch.float32,), X)
+    if _native.lib().edsl_hip_q4_dense_launch(
+            X.data_ptr(), X.stride(0), _types[X.dtype], _ptr(x_scales), W.packed.data_ptr(), _ptr(b),
+            _types[b.dtype] if b is not None else 0, Y.data_ptr(), Y.stride(0), _types[Y.dtype], M, W.N, K,
+            W.group_size, W.scale_type, W.has_zeros, epilogue, alpha, _stream(stream)):
+        _native.raise_on_error("q4_dense_launch")
 
 
 def _tokens(torch, tokens, logits):
