@@ -88,7 +88,7 @@ int edsl_hip_token_logprobs_backward_launch(const void *logits, int64_t ldl, int
  * 128; the last group may be shorter):
  *   W[k][n] = scales[k / group][n] * (q[k][n] - zeros[k / group][n]),
  * q and zeros integers 0 .. 15 (the low four bits of their bytes), zeros 8 where
- * there are none. edsl_hip_q4_pack_launch lays the weights out once, in
+ * there are none. K <= 2^23. edsl_hip_q4_pack_launch lays the weights out once, in
  * edsl_hip_q4_packed_bytes bytes (-1: arguments that it does not take, with the
  * message in edsl_hip_last_error) at a 256-byte aligned address; scales are F32,
  * BF16 or F16 and kept as they are. */

@@ -16,6 +16,7 @@ namespace rt {
 namespace {
 
 constexpr int64_t kMostDim = int64_t(1) << 30;
+constexpr int64_t kMostDepth = int64_t(1) << 23;  // of a 4-bit layer: 128 rows of x within 32-bit offsets
 constexpr int64_t kMostVocabulary = int64_t(1) << 21;
 
 void check_sizes(int64_t rows, int64_t cols, const char* rn, const char* cn) {
@@ -139,6 +140,7 @@ void token_logprobs_backward(lm::LogprobsBackwardArgs a, void* stream) {
 // ------------------------------------------------------------ 4-bit layer
 lm::Q4Layout q4_checked_layout(int64_t K, int64_t N, int group, int scale_type, bool zeros) {
   check_sizes(K, N, "K", "N");
+  if (K > kMostDepth) fail(kErrLimit, "K=%lld beyond 2^23", (long long)K);
   check_float_type(scale_type, "scales");
   if (group != 32 && group != 64 && (group <= 0 || group % 128 != 0))
     fail(kErrArgument, "group=%d is not 32, 64 or a multiple of 128", group);
@@ -208,7 +210,7 @@ void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, bool zer
   check_mat(a.y, a.ldy, M, N, "Y");
   if (K > 0) check_packed(a.w, "packed");
   a.M = (int)M, a.N = (int)N, a.K = (int)K;
-  a.scales_at = l.scales_at, a.zeros_at = l.zeros_at;
+  a.scales_at = l.scales_at, a.zeros_at = l.zeros_at, a.scale_bytes = l.scale_bytes;
   a.blocks = (int)l.blocks, a.scale_blocks = (int)l.scale_blocks, a.blocks_per_scale = l.blocks_per_scale;
   int cus = 0;
   device_launch(0, stream, [&](char*, int n) { cus = n; });
@@ -234,11 +236,11 @@ void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, bool zer
   const int config = q4_tile_plan(a, cus, &a.ksplit);
   lm::Q4PrepArgs p{};
   p.x = a.x, p.ldx = a.ldx, p.M = a.M, p.K = a.K, p.blocks = a.blocks, p.spb = l.spb, p.x_type = a.x_type;
-  p.factor = zeros ? -1.0f : -8.0f;
+  p.factor = zeros ? -1.0f : -8.0f - lm::q4_offset(a.x_type);
   p.xs_ld = (M + 127) / 128 * 128;
   // x itself where the tiles can read it: 16 bits, whole blocks, 16-byte aligned rows.
   const bool copy = !((a.x_type == lm::kBf16 || a.x_type == lm::kF16) && K % 128 == 0 && a.ldx % 8 == 0 &&
-                      reinterpret_cast<uintptr_t>(a.x) % 16 == 0);
+                      reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx <= kMostDepth);
   p.ldp = l.blocks * 128, p.plane = M * p.ldp;
   const size_t sums = aligned((size_t)l.blocks * l.spb * p.xs_ld * sizeof(float));
   const size_t planes = copy ? aligned((size_t)(a.x_type == lm::kF32 ? 3 : 1) * p.plane * 2) : 0;

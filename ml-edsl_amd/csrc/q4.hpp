@@ -4,7 +4,7 @@
 //   y = epi(xs[m] * sum_k x[m][k] s[g][n] (q[k][n] - z[g][n]) + b[n]),  g = k / group
 //
 // Products are exact: q in 0..15 and the integers of an 8-bit x are exact in
-// bf16 (q in f16 too), bf16 and f16 x are what the matrix cores take, and an
+// bf16 and f16, bf16 and f16 x are what the matrix cores take, and an
 // f32 x is the exact sum of three bf16 terms. Sums are 32-bit. Inside a group
 //   sum x (q - z) = sum x q - z sum x,
 // with the second term the starting value of the accumulator, so that a weight
@@ -26,9 +26,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Packed weights: blocks of 16 columns x 128 k, [N/16][K/128] rounded up, 1024
 // bytes each: lane l of a wave has 16 bytes, column l % 16, and word s of them
-// holds k = 32 s + 8 (l / 16) + j, j = 0..3 in the low and j = 4..7 in the high
-// nibbles of its bytes. That is the operand of the 16x16x32 matrix instruction,
-// lane for lane, four in a row: a wave's load is one 1024-byte line of memory.
+// holds k = 32 s + 8 (l / 16) + j, even j in nibble j / 2 of its lower half, odd
+// ones in the upper half's. That is the operand of the 16x16x32 matrix
+// instruction, lane for lane, four in a row: a wave's load is one 1024-byte run.
 // Behind them the scales [N/16][SB][16][spb] and zero points likewise in bytes:
 // spb = 128 / group scales of a column in a block and SB = K/128 where the group
 // is less than 128, else spb = 1 and SB = K/group. All padding is zero.
@@ -52,6 +52,7 @@ inline Q4Layout q4_layout(int64_t K, int64_t N, int group, int scale_type, bool 
   l.scales_at = l.tiles_n * l.blocks * 1024;
   l.zeros_at = l.scales_at + (scales * l.scale_bytes + 255) / 256 * 256;
   l.bytes = l.zeros_at + (zeros ? (scales + 255) / 256 * 256 : 0);
+  if (l.bytes > 0) l.bytes += 256;  // what a 32-bit load of the last scale reads past it
   return l;
 }
 
@@ -66,13 +67,14 @@ struct Q4Args {
   int M, N, K;
   int blocks, scale_blocks, blocks_per_scale;
   int ksplit;  // workgroups that split K
+  int scale_bytes;
   int x_type, scale_type, y_type, bias_type, epi;
   float alpha;
   // Tiles of many rows: x prepared (q4_prep_kernel), or x itself where its rows
   // are whole 16-byte aligned blocks.
   const void* xp;       // [planes][M][ldp]
   int64_t ldp, plane;   // elements
-  const float* xs;      // [blocks * spb][xs_ld]: minus (8 times, without zero points) the sums of x in each group
+  const float* xs;      // [blocks * spb][xs_ld]: minus the sums of x in each group, times offset + 8 without zero points
   int64_t xs_ld;
 };
 
@@ -84,17 +86,8 @@ struct Q4Elem<false> {
   static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  // Eight weights of a word. As an 8-bit float of 4 exponent bits the byte n in
-  // 0..15 is n / 512 (0..7 subnormal), so that the conversion with a factor of
-  // 512 gives n: 7 instructions for 8 weights, no table.
-  static __device__ __forceinline__ V weights(uint32_t w) {
-    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false);
-    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false);
-    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
-    return V{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-  }
+  static constexpr int kShift = 3;            // of a weight in the mantissa of 16 .. 31
+  static constexpr uint32_t kBase = 0x41804180u;  // 16, twice
 };
 template <>
 struct Q4Elem<true> {
@@ -102,22 +95,51 @@ struct Q4Elem<true> {
   static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ V weights(uint32_t w) {
-    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false);
-    const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
-    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false);
-    const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
-    return V{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-  }
+  static constexpr int kShift = 6;
+  static constexpr uint32_t kBase = 0x4c004c00u;
 };
 
-// Scale i of an array of this type, as f32.
-__device__ __forceinline__ float q4_scale(const char* p, int type, int64_t i) {
-  if (type == kF32) return reinterpret_cast<const float*>(p)[i];
-  const uint32_t h = reinterpret_cast<const uint16_t*>(p)[i];
-  if (type == kBf16) return __builtin_bit_cast(float, h << 16);
-  return (float)__builtin_bit_cast(f16, (uint16_t)h);
+// Eight weights of a word, in the order of k, as kQ4Offset + q: in the mantissa
+// of 16 .. 31 an integer 0 .. 15 is its own bits, so two weights cost one shift
+// and one and-or, and the 16 goes with the zero point. The sums then hold
+// 16 sum x more than they need, which costs up to two of their bits.
+constexpr float kQ4Offset = 16.0f;
+template <bool F16>
+__device__ __forceinline__ typename Q4Elem<F16>::V q4_weights(uint32_t w) {
+  using E = Q4Elem<F16>;
+  constexpr uint32_t mask = (15u << E::kShift) * 0x10001u;
+  u32x4 r;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int s = 4 * p - E::kShift;
+    r[p] = ((s >= 0 ? w >> s : w << -s) & mask) | E::kBase;
+  }
+  return __builtin_bit_cast(typename E::V, r);
+}
+// For f32 x, as q itself: as an 8-bit float of 4 exponent bits the byte n in
+// 0 .. 15 is n / 512 (0 .. 7 subnormal), so the conversion with a factor of 512
+// gives n. They come in the order k = 0 4 1 5 2 6 3 7, in which x is split too.
+__device__ __forceinline__ bf16x8 q4_weights_f32(uint32_t w) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// What a weight is held above q for x of this type.
+constexpr float q4_offset(int x_type) { return x_type == kF32 ? 0.0f : kQ4Offset; }
+
+// Scale i of an array, as it lies in memory: 32 bits from its address on (the
+// packed weights' end leaves room). Read one way for all types and decoded where
+// it is used, so that no load waits at a branch.
+__device__ __forceinline__ uint32_t q4_scale_bits(const char* p, int bytes, int64_t i) {
+  return load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(p + i * bytes)).v[0] |
+         (uint32_t)load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(p + i * bytes)).v[1] << 16;
+}
+__device__ __forceinline__ float q4_scale(uint32_t bits, int type) {
+  const float half = (float)__builtin_bit_cast(f16, (uint16_t)bits);
+  return type == kF32 ? __builtin_bit_cast(float, bits) : type == kBf16 ? __builtin_bit_cast(float, bits << 16) : half;
 }
 
 // Three bf16 terms whose sum is v, to the last bit of it while they are normal:
@@ -135,24 +157,66 @@ __device__ __forceinline__ Split3 split3(float v) {
   return r;
 }
 
+// Eight elements of an f32 x as operands of three products, in the order of
+// q4_weights_f32.
+__device__ __forceinline__ void split3_operands(const float (&v)[8], u32x4 (&p)[3]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const Split3 a = split3(v[j]), b = split3(v[j + 4]);
+    p[0][j] = (a.hi >> 16) | b.hi;
+    p[1][j] = (a.mid >> 16) | b.mid;
+    p[2][j] = (a.lo >> 16) | b.lo;
+  }
+}
+
 __device__ __forceinline__ float q4_load_as_float(const void* p, int type, int64_t i) {
   if (type == kF32) return static_cast<const float*>(p)[i];
   if (type == kBf16) return (float)static_cast<const bf16*>(p)[i];
   return (float)static_cast<const f16*>(p)[i];
 }
 
-// y[m][n] from the sum over k.
-__device__ __forceinline__ void q4_store(const Q4Args& a, int m, int n, float v) {
-  if (a.x_scales) v *= a.x_scales[m];
-  const float b = a.bias ? q4_load_as_float(a.bias, a.bias_type, n) : 0.0f;
-  v = epilogue_rt(v, b, a.alpha, a.epi);
-  const int64_t at = (int64_t)m * a.ldy + n;
-  if (a.y_type == kF32)
-    static_cast<float*>(a.y)[at] = v;
-  else if (a.y_type == kBf16)
-    static_cast<bf16*>(a.y)[at] = (bf16)v;
-  else
-    static_cast<f16*>(a.y)[at] = (f16)v;
+// Writes C outputs of a lane, y[m[i]][n[i]], from their sums over k; `in`: those
+// that exist. The branches are taken once for all of them.
+template <int C>
+__device__ __forceinline__ void q4_store(const Q4Args& a, const int (&m)[C], const int (&n)[C], const bool (&in)[C],
+                                         float (&v)[C]) {
+  if (a.x_scales)
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (in[i]) v[i] *= a.x_scales[m[i]];
+  if (a.bias)
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (in[i]) v[i] = __fadd_rn(v[i], q4_load_as_float(a.bias, a.bias_type, n[i]));
+  switch (epi_act(a.epi)) {
+    case ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = apply_epilogue_f32<epi_code(false, ACT_RELU)>(v[i], 0.0f, 0.0f);
+      break;
+    case ACT_LEAKY:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = apply_epilogue_f32<epi_code(false, ACT_LEAKY)>(v[i], 0.0f, a.alpha);
+      break;
+    case ACT_IF_RELU:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = apply_epilogue_f32<epi_code(false, ACT_IF_RELU)>(v[i], 0.0f, 0.0f);
+      break;
+    default:
+      break;
+  }
+  if (a.y_type == kF32) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (in[i]) static_cast<float*>(a.y)[(int64_t)m[i] * a.ldy + n[i]] = v[i];
+  } else if (a.y_type == kBf16) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (in[i]) static_cast<bf16*>(a.y)[(int64_t)m[i] * a.ldy + n[i]] = (bf16)v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (in[i]) static_cast<f16*>(a.y)[(int64_t)m[i] * a.ldy + n[i]] = (f16)v[i];
+  }
 }
 
 // q4_small.hpp, one source file for each type of x.
@@ -167,7 +231,7 @@ struct Q4PrepArgs {
   float* xs;
   int64_t ldx, ldp, plane, xs_ld;
   int M, K, blocks, spb, x_type;
-  float factor;  // of the sums: -1, or -8 without zero points
+  float factor;  // of the sums
 };
 hipError_t launch_q4_prep(const Q4PrepArgs& a, hipStream_t stream);
 hipError_t launch_q4_join(const Q4Args& a, hipStream_t stream);

@@ -45,13 +45,7 @@ struct SmallX<kF32> {
   static constexpr int kPlanes = 3;
   static __device__ __forceinline__ void operands(const Packed<T, 8>& r, bf16x8 (&o)[3]) {
     u32x4 p[3];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const Split3 a = split3(r.v[2 * j]), b = split3(r.v[2 * j + 1]);
-      p[0][j] = (a.hi >> 16) | b.hi;
-      p[1][j] = (a.mid >> 16) | b.mid;
-      p[2][j] = (a.lo >> 16) | b.lo;
-    }
+    split3_operands(r.v, p);
 #pragma unroll
     for (int i = 0; i < 3; ++i) o[i] = __builtin_bit_cast(bf16x8, p[i]);
   }
@@ -89,7 +83,7 @@ template <int XT, int NT, int SPB, bool ZEROS>
 struct SmallBlock {
   Packed<typename SmallX<XT>::T, 8> x[4];
   u32x4 w[NT];
-  float scale[NT][SPB], zero[ZEROS ? NT : 1][SPB];
+  uint32_t scale[NT][SPB], zero[ZEROS ? NT : 1][SPB];  // as read
 };
 
 template <int XT, int NT, int SPB, bool ZEROS>
@@ -105,20 +99,21 @@ __device__ __forceinline__ void small_load(const Q4Args& a, const typename Small
     const int64_t at = (((tile + t) * a.scale_blocks + sb) * 16 + lane % 16) * SPB;
 #pragma unroll
     for (int g = 0; g < SPB; ++g) {
-      r.scale[t][g] = q4_scale(a.w + a.scales_at, a.scale_type, at + g);
-      if constexpr (ZEROS) r.zero[t][g] = (float)reinterpret_cast<const uint8_t*>(a.w + a.zeros_at)[at + g];
+      r.scale[t][g] = q4_scale_bits(a.w + a.scales_at, a.scale_bytes, at + g);
+      if constexpr (ZEROS) r.zero[t][g] = reinterpret_cast<const uint8_t*>(a.w + a.zeros_at)[at + g];
     }
   }
 }
 
 template <int XT, int NT, int SPB, bool ZEROS>
-__device__ __forceinline__ void small_block(const SmallBlock<XT, NT, SPB, ZEROS>& r, f32x4 (&sum)[NT]) {
+__device__ __forceinline__ void small_block(const Q4Args& a, const SmallBlock<XT, NT, SPB, ZEROS>& r,
+                                            f32x4 (&sum)[NT]) {
   using X = SmallX<XT>;
   using V = typename X::E::V;
   constexpr int STEPS = 4 / SPB;
   V minus;  // the constant operand of the sums of x
 #pragma unroll
-  for (int j = 0; j < 8; ++j) minus[j] = ZEROS ? -1.0f : -8.0f;
+  for (int j = 0; j < 8; ++j) minus[j] = ZEROS ? -1.0f : -8.0f - q4_offset(XT);
 #pragma unroll
   for (int g = 0; g < SPB; ++g) {
     V o[STEPS][X::kPlanes];
@@ -132,17 +127,24 @@ __device__ __forceinline__ void small_block(const SmallBlock<XT, NT, SPB, ZEROS>
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       f32x4 acc = xs;
-      if constexpr (ZEROS)
+      if constexpr (ZEROS) {
+        const float zero = q4_offset(XT) + (float)r.zero[t][g];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= r.zero[t][g];
+        for (int i = 0; i < 4; ++i) acc[i] *= zero;
+      }
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        const V w = X::E::weights(r.w[t][g * STEPS + s]);
+        V w;
+        if constexpr (XT == kF32)
+          w = q4_weights_f32(r.w[t][g * STEPS + s]);
+        else
+          w = q4_weights<XT == kF16>(r.w[t][g * STEPS + s]);
 #pragma unroll
         for (int p = X::kPlanes - 1; p >= 0; --p) acc = X::E::mfma(o[s][p], w, acc);
       }
+      const float scale = q4_scale(r.scale[t][g], a.scale_type);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[t][i] = fmaf(acc[i], r.scale[t][g], sum[t][i]);
+      for (int i = 0; i < 4; ++i) sum[t][i] = fmaf(acc[i], scale, sum[t][i]);
     }
   }
 }
@@ -151,7 +153,7 @@ template <int XT, int NT, int SPB, bool ZEROS>
 __global__ void __launch_bounds__(64 * kSmallWaves) q4_small_kernel(Q4Args a) {
   using T = typename SmallX<XT>::T;
   __shared__ float part[kSmallWaves][16][16 * NT];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int64_t tiles = (a.N + 15) / 16;
   const int64_t first = (int64_t)(blockIdx.x / a.ksplit) * NT;
   const int slice = blockIdx.x % a.ksplit;
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(64 * kSmallWaves) q4_small_kernel(Q4Args a) {
   while (b < b1) {
     const int after = b + kSmallWaves;
     if (after < b1) small_load<XT, NT, SPB, ZEROS>(a, x, tile, after, lane, next);
-    small_block<XT, NT, SPB, ZEROS>(now, sum);
+    small_block<XT, NT, SPB, ZEROS>(a, now, sum);
     now = next;
     b = after;
   }
@@ -189,10 +191,12 @@ __global__ void __launch_bounds__(64 * kSmallWaves) q4_small_kernel(Q4Args a) {
     float v = 0.0f;
 #pragma unroll
     for (int w = 0; w < kSmallWaves; ++w) v += part[w][m][c];
-    if (a.ksplit > 1)
+    if (a.ksplit > 1) {
       a.partials[((int64_t)slice * a.M + m) * a.N + n] = v;
-    else
-      q4_store(a, m, (int)n, v);
+    } else {
+      float out[1] = {v};
+      q4_store<1>(a, {m}, {(int)n}, {true}, out);
+    }
   }
 }
 

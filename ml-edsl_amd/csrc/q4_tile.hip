@@ -1,9 +1,9 @@
 // The 4-bit layer on more than 16 rows: tiles on the matrix cores.
 //
 // A workgroup of 4 waves takes 16 MT WM rows x 16 NT WN columns. A wave loads and
-// unpacks the weights of its own columns in registers; x goes through LDS, one
-// block of 128 k ahead, in operand order with 16-byte chunks exchanged by row so
-// that reads hit all banks. Each group's accumulators start at the prepared
+// unpacks the weights of its own columns in registers, a block of 128 k ahead; x
+// and its groups' sums go from memory straight to LDS, a stage ahead, with 16-byte
+// chunks exchanged by row so that reads hit all banks. Each group's accumulators start at the prepared
 // -zero * sum x and are scaled into the 32-bit totals at its end.
 #include "q4.hpp"
 
@@ -11,15 +11,27 @@ namespace edsl {
 namespace lm {
 namespace {
 
+// 16 bytes a lane from memory to LDS, at `to` + 16 lane (`to` the wave's own).
+__device__ __forceinline__ void to_lds(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
+                                   (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
+}
+
+// Waits for the wave's loads, those to LDS among them (vmcnt 0).
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 template <bool F16, int PLANES, int MT, int NT, int WM, int WN, int SPB, bool ZEROS>
-__global__ void __launch_bounds__(256) q4_tile_kernel(Q4Args a) {
+__global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   using E = Q4Elem<F16>;
   using V = typename E::V;
   constexpr int BM = 16 * MT * WM, STEPS = 4 / SPB;
   static_assert(WM * WN == 4, "four waves");
-  constexpr int CHUNKS = PLANES * BM * 16 / 256;  // 16-byte chunks of a block of x, a thread's
-  __shared__ u32x4 lds[2][PLANES * BM * 16];
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  // A stage of x in LDS: SS steps of 32 k, CPR 16-byte chunks a row.
+  constexpr int SS = PLANES == 3 ? 2 : 4, CPR = 4 * SS, STAGES = 4 / SS;
+  constexpr int CHUNKS = PLANES * BM * CPR / 256;  // a thread's
+  __shared__ u32x4 lds[2][PLANES * BM * CPR];
+  __shared__ f32x4 sums[2][SPB * BM / 4];  // a block's sums of x
+  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int wm = wave % WM, wn = wave / WM;
   const int64_t tiles = (a.N + 15) / 16;
   const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (int)((tiles + NT * WN - 1) / (NT * WN));
@@ -30,118 +42,145 @@ __global__ void __launch_bounds__(256) q4_tile_kernel(Q4Args a) {
   const int m0 = tm * BM;
   const int b0 = (int)((int64_t)a.blocks * slice / a.ksplit), b1 = (int)((int64_t)a.blocks * (slice + 1) / a.ksplit);
 
-  // Chunk i of a block: row i / 16 of the planes, its k chunk (i % 16) ^ (row % 16).
-  const char* src[CHUNKS];
+  // Row r's chunk c lies at c ^ swizzle(r): 16 rows' reads of one chunk meet all banks.
+  const auto swizzle = [](int r) { return CPR == 16 ? r % 16 : (r / 2) % 8; };
+  // Addresses are a uniform base and 32 bits a lane, so that they stay out of the
+  // vector registers (the runtime bounds K for it); rows past M repeat the last.
+  static_assert(BM * CPR % 256 == 0, "a chunk is of one plane");
+  uint32_t src[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const int i = c * 256 + tid, r = i / 16, plane = r / BM, row = m0 + r % BM;
-    const int64_t at = plane * a.plane + (int64_t)(row < a.M ? row : a.M - 1) * a.ldp + 8 * ((i % 16) ^ (r % 16));
-    src[c] = static_cast<const char*>(a.xp) + 2 * at;
+    const int i = c * 256 + tid, r = i / CPR, row = m0 + r % BM;
+    src[c] = (uint32_t)(((int64_t)(row < a.M ? row : a.M - 1) - m0) * a.ldp + 8 * ((i % CPR) ^ swizzle(r))) * 2u;
   }
-  u32x4 xr[CHUNKS];
-  const auto load_x = [&](int b) {
+  const char* const xp = static_cast<const char*>(a.xp) + 2 * m0 * a.ldp;
+  const auto load_x = [&](int stage, int buf) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) xr[c] = *reinterpret_cast<const u32x4*>(src[c] + (int64_t)b * 256);
+    for (int c = 0; c < CHUNKS; ++c)
+      to_lds(xp + 2 * (c * 256 / (BM * CPR)) * a.plane + (int64_t)stage * (16 * CPR) + src[c],
+             &lds[buf][c * 256 + wave * 64]);
   };
-  const auto store_x = [&](int buf) {
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) lds[buf][c * 256 + tid] = xr[c];
+  const auto load_sums = [&](int b) {
+    // 16-byte pieces of SPB runs of BM sums.
+    if (tid < SPB * BM / 4)
+      to_lds(a.xs + ((int64_t)b * SPB + tid / (BM / 4)) * a.xs_ld + m0 + 4 * (tid % (BM / 4)),
+             &sums[b & 1][wave * 64]);
   };
-  u32x4 w[2][NT];
-  const auto load_w = [&](int b, u32x4 (&r)[NT]) {
+  struct Weights {
+    u32x4 w[NT];
+    uint32_t scale[NT][SPB], zero[ZEROS ? NT : 1][SPB];  // as read
+  };
+  const auto load_w = [&](int b, Weights& r) {
+    const int sb = b / a.blocks_per_scale;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int64_t tile = first + t < tiles ? first + t : tiles - 1;
-      r[t] = *reinterpret_cast<const u32x4*>(a.w + (tile * a.blocks + b) * 1024 + 16 * lane);
+      r.w[t] = *reinterpret_cast<const u32x4*>(a.w + (tile * a.blocks + b) * 1024 + 16 * lane);
+      const int64_t at = ((tile * a.scale_blocks + sb) * 16 + lane % 16) * SPB;
+#pragma unroll
+      for (int g = 0; g < SPB; ++g) {
+        r.scale[t][g] = q4_scale_bits(a.w + a.scales_at, a.scale_bytes, at + g);
+        if constexpr (ZEROS) r.zero[t][g] = reinterpret_cast<const uint8_t*>(a.w + a.zeros_at)[at + g];
+      }
     }
   };
-  f32x4 sum[MT][NT];
+  f32x4 sum[MT][NT], acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int t = 0; t < NT; ++t) sum[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
+  Weights now, next;
   if (b0 < b1) {
-    load_x(b0);
-    load_w(b0, w[0]);
-    store_x(0);
+    load_x(b0 * STAGES, 0);
+    load_sums(b0);
+    load_w(b0, now);
   }
   for (int b = b0; b < b1; ++b) {
-    const int buf = (b - b0) & 1;
-    __syncthreads();
-    const bool more = b + 1 < b1;
-    if (more) {
-      load_x(b + 1);
-      load_w(b + 1, w[1]);
-    }
-    const int sb = b / a.blocks_per_scale;
 #pragma unroll
-    for (int g = 0; g < SPB; ++g) {
-      float scale[NT], zero[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int64_t tile = first + t < tiles ? first + t : tiles - 1;
-        const int64_t at = ((tile * a.scale_blocks + sb) * 16 + lane % 16) * SPB + g;
-        scale[t] = q4_scale(a.w + a.scales_at, a.scale_type, at);
-        if constexpr (ZEROS) zero[t] = (float)reinterpret_cast<const uint8_t*>(a.w + a.zeros_at)[at];
+    for (int stage = 0; stage < STAGES; ++stage) {
+      const int buf = STAGES == 2 ? stage : (b - b0) & 1;
+      wait_loads();
+      __syncthreads();
+      const bool last = stage == STAGES - 1;
+      if (!last || b + 1 < b1) load_x(b * STAGES + stage + 1, buf ^ 1);
+      if (stage == 0 && b + 1 < b1) {
+        load_sums(b + 1);
+        load_w(b + 1, next);
       }
-      f32x4 acc[MT][NT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int m = m0 + 16 * (wm * MT + i) + 4 * (lane / 16);
-        const f32x4 xs = *reinterpret_cast<const f32x4*>(a.xs + ((int64_t)b * SPB + g) * a.xs_ld + m);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          acc[i][t] = xs;
+      for (int s = 0; s < SS; ++s) {
+        const int step = stage * SS + s, g = step / STEPS;
+        if (step % STEPS == 0) {
+          float zero[NT];
           if constexpr (ZEROS)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][t][e] *= zero[t];
-        }
-      }
+            for (int t = 0; t < NT; ++t) zero[t] = (PLANES == 3 ? 0.0f : kQ4Offset) + (float)now.zero[t][g];
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int step = g * STEPS + s;
+          for (int i = 0; i < MT; ++i) {
+            const f32x4 xs = sums[b & 1][g * (BM / 4) + 4 * (wm * MT + i) + lane / 16];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              acc[i][t] = xs;
+              if constexpr (ZEROS)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][t][e] *= zero[t];
+            }
+          }
+        }
         V q[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) q[t] = E::weights(w[0][t][step]);
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (PLANES == 3)
+            q[t] = q4_weights_f32(now.w[t][step]);
+          else
+            q[t] = q4_weights<F16>(now.w[t][step]);
+        }
 #pragma unroll
         for (int p = PLANES - 1; p >= 0; --p)
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             const int r = p * BM + 16 * (wm * MT + i) + lane % 16;
-            const V x = __builtin_bit_cast(V, lds[buf][r * 16 + ((4 * step + lane / 16) ^ (r % 16))]);
+            const V x = __builtin_bit_cast(V, lds[buf][r * CPR + ((4 * s + lane / 16) ^ swizzle(r))]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[i][t] = E::mfma(x, q[t], acc[i][t]);
           }
+        if (step % STEPS == STEPS - 1) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float scale = q4_scale(now.scale[t][g], a.scale_type);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[i][t][e] = fmaf(acc[i][t][e], scale, sum[i][t][e]);
+          }
+        }
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[i][t][e] = fmaf(acc[i][t][e], scale[t], sum[i][t][e]);
     }
-    if (more) {
-      store_x(buf ^ 1);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) w[0][t] = w[1][t];
-    }
+    now = next;
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = 16 * (first + t) + lane % 16;
-    if (n >= a.N) continue;
+  for (int i = 0; i < MT; ++i) {
+    int m[4 * NT], n[4 * NT];
+    bool in[4 * NT];
+    float v[4 * NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int m = m0 + 16 * (wm * MT + i) + 4 * (lane / 16) + e;
-        if (m >= a.M) continue;
-        if (a.ksplit > 1)
-          a.partials[((int64_t)slice * a.M + m) * a.N + n] = sum[i][t][e];
-        else
-          q4_store(a, m, (int)n, sum[i][t][e]);
+        const int j = 4 * t + e;
+        m[j] = m0 + 16 * (wm * MT + i) + 4 * (lane / 16) + e;
+        n[j] = (int)(16 * (first + t)) + lane % 16;
+        in[j] = m[j] < a.M && n[j] < a.N;
+        v[j] = sum[i][t][e];
       }
+    if (a.ksplit > 1) {
+#pragma unroll
+      for (int j = 0; j < 4 * NT; ++j)
+        if (in[j]) a.partials[((int64_t)slice * a.M + m[j]) * a.N + n[j]] = v[j];
+    } else {
+      q4_store<4 * NT>(a, m, n, in, v);
+    }
   }
 }
 
@@ -215,16 +254,14 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(Q4PrepArgs a) {
       for (int j = 0; j < 8; ++j) v[j] = (float)r.v[j];
     }
     if (a.xp) {
-      if constexpr (XT != kF16) {
+      if constexpr (XT == kF32) {
+        split3_operands(v, out);
+      } else if constexpr (XT != kF16) {
+        // Exact in bf16: its upper half.
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Split3 p = split3(v[2 * j]), q = split3(v[2 * j + 1]);
-          out[0][j] = (p.hi >> 16) | q.hi;
-          if constexpr (XT == kF32) {
-            out[1][j] = (p.mid >> 16) | q.mid;
-            out[2][j] = (p.lo >> 16) | q.lo;
-          }
-        }
+        for (int j = 0; j < 4; ++j)
+          out[0][j] = (__builtin_bit_cast(uint32_t, v[2 * j]) >> 16) |
+                      (__builtin_bit_cast(uint32_t, v[2 * j + 1]) & 0xffff0000u);
       }
 #pragma unroll
       for (int p = 0; p < (XT == kF32 ? 3 : 1); ++p)
@@ -245,7 +282,8 @@ __global__ void __launch_bounds__(256) q4_join_kernel(Q4Args a) {
   if (i >= all) return;
   float v = 0.0f;
   for (int s = 0; s < a.ksplit; ++s) v += a.partials[s * all + i];
-  q4_store(a, (int)(i / a.N), (int)(i % a.N), v);
+  float out[1] = {v};
+  q4_store<1>(a, {(int)(i / a.N)}, {(int)(i % a.N)}, {true}, out);
 }
 
 // ------------------------------------------------------------------ packing
@@ -259,7 +297,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(Q4PackArgs a) {
   if (n < a.N)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (k0 + j < a.K) w |= (uint32_t)(a.q[(k0 + j) * a.ldq + n] & 15) << (j < 4 ? 8 * j : 8 * (j - 4) + 4);
+      if (k0 + j < a.K) w |= (uint32_t)(a.q[(k0 + j) * a.ldq + n] & 15) << (4 * (j / 2) + 16 * (j % 2));
   reinterpret_cast<uint32_t*>(a.packed + (tile * a.layout.blocks + block) * 1024)[4 * lane + step] = w;
   // Its scales and zero points, by the first block of each group.
   const int spb = a.layout.spb, bps = a.layout.blocks_per_scale;
