@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/edsl_hip_device.h"
+#include "torch_lm.hpp"
 
 namespace {
 
@@ -97,9 +98,16 @@ PyObject* dense_launch(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+#define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
+
 PyMethodDef methods[] = {
     {"dense_launch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense_launch)), METH_FASTCALL,
      "dense_launch(X, W, b, Y, epilogue, alpha, stream, current) -> status, or None when the arguments are not taken"},
+    {"rms_norm", FAST(edsl_torch_rms_norm), "rms_norm_launch of lm.py"},
+    {"rms_norm_backward", FAST(edsl_torch_rms_norm_backward), "rms_norm_backward_launch of lm.py"},
+    {"q4_dense", FAST(edsl_torch_q4_dense), "q4_dense_launch of lm.py"},
+    {"token_logprobs", FAST(edsl_torch_token_logprobs), "token_logprobs_launch of lm.py"},
+    {"token_logprobs_backward", FAST(edsl_torch_token_logprobs_backward), "token_logprobs_backward_launch of lm.py"},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -98,7 +98,7 @@ def build_torch_launch_module() -> str:
     return _link_module("_torch_launch", [
         cxx, "-O2", "-std=c++17", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         f'-DEDSL_TORCH_BUILD_ID="{torch_build_id(torch)}"', *[f"-isystem{p}" for p in include_paths()],
-        os.path.join(CSRC, "torch_launch.cpp"), f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10"])
+        os.path.join(CSRC, "torch_launch.cpp"), os.path.join(CSRC, "lm_torch.cpp"), f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10"])
 
 
 def build_optional_torch_launch_module() -> list[str]:

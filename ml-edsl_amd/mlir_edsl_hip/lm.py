@@ -20,16 +20,29 @@ from __future__ import annotations
 from . import _native, device
 
 _types = None  # torch dtype -> EDSL_LM_* code
+_native_module = None  # the checks below and the calls, natively (csrc/lm_torch.cpp), where device.py may use it
 
 
 def _torch():
     """torch; the first call also maps the library and the stream accessor (device.py)."""
-    global _types
+    global _types, _native_module
     torch = device._torch if device._torch is not None else device._torch_module()
     if _types is None:
         _types = {torch.float32: _native.LM_F32, torch.bfloat16: _native.LM_BF16, torch.float16: _native.LM_F16,
                   torch.int8: _native.LM_I8, torch.float8_e4m3fn: _native.LM_E4M3}
+        if device._native_launch is not None:
+            from . import _torch_launch as _native_module
     return torch
+
+
+def _done(rc, what) -> bool:
+    """Whether a native call was taken; its error is raised. None: the Python
+    path runs, and names what is wrong with the arguments."""
+    if rc == 0:
+        return True
+    if rc is not None:
+        _native.raise_on_error(what)
+    return rc is not None
 
 
 def _stream(stream):
@@ -89,6 +102,10 @@ def rms_norm_launch(X, weight, Y, residual=None, total=None, scales=None, rstd=N
     is that of h in 32 bits. total may be X or residual, and Y any of the three
     in their type."""
     torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.rms_norm(X, weight, Y, residual, total, scales, rstd, eps, stream, device._raw_stream),
+            "rms_norm_launch"):
+        return
     shape = _matrix(X, "X", _floats(torch))
     eight = (torch.int8, torch.float8_e4m3fn)
     _list(weight, "weight", shape[1:], (X.dtype, torch.float32), X)
@@ -117,6 +134,10 @@ def rms_norm_backward_launch(dY, H, weight, rstd, dX, dweight=None, dh=None, str
     f32 the weight's, summed over the rows in a fixed order. dX may be dY, H or
     dh."""
     torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.rms_norm_backward(dY, H, weight, rstd, dX, dweight, dh, stream, device._raw_stream),
+            "rms_norm_backward_launch"):
+        return
     shape = _matrix(dY, "dY", _floats(torch))
     _operand(H, "H", shape, (dY.dtype,), dY)
     _list(weight, "weight", shape[1:], (dY.dtype, torch.float32), dY)
@@ -206,6 +227,10 @@ def q4_dense_launch(X, W: Q4Weight, b, Y, epilogue: int = _native.EPI_NONE, alph
     torch = _torch()
     if not isinstance(W, Q4Weight):
         raise TypeError("W is not a Q4Weight")
+    if _native_module is not None and _done(
+            _native_module.q4_dense(X, W.packed, W.K, W.N, W.group_size, W.scale_type, W.has_zeros, b, Y, epilogue,
+                                    alpha, x_scales, stream, device._raw_stream), "q4_dense_launch"):
+        return
     M, K = _matrix(X, "X", tuple(_types))
     if K != W.K:
         raise ValueError(f"shape mismatch: X{tuple(X.shape)} W{(W.K, W.N)}")
@@ -241,6 +266,10 @@ def token_logprobs_launch(logits, tokens=None, logprobs=None, lse=None, entropy=
     probabilities are -inf and the entropy 0. A row with a NaN or +inf gives
     NaN and ids -1."""
     torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.token_logprobs(logits, tokens, logprobs, lse, entropy, top_logprobs, top_ids, scale, stream,
+                                          device._raw_stream), "token_logprobs_launch"):
+        return
     M, V = _matrix(logits, "logits", _floats(torch))
     ids64 = _tokens(torch, tokens, logits) if tokens is not None else True
     for t, name in ((logprobs, "logprobs"), (lse, "lse"), (entropy, "entropy")):
@@ -273,6 +302,10 @@ def token_logprobs_backward_launch(logits, tokens, lse, dlogits, dlogprobs=None,
     forward pass's. A padding token's dlogprobs counts as 0, and so does
     everything in a row of -inf alone. dlogits may be logits."""
     torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.token_logprobs_backward(logits, tokens, lse, dlogits, dlogprobs, entropy, dentropy, scale,
+                                                   stream, device._raw_stream), "token_logprobs_backward_launch"):
+        return
     M, V = _matrix(logits, "logits", _floats(torch))
     ids64 = _tokens(torch, tokens, logits) if tokens is not None else True
     _list(lse, "lse", (M,), (torch.float32,), logits)
