@@ -171,20 +171,31 @@ void q4_pack(lm::Q4PackArgs a, size_t bytes, void* stream) {
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Up to 16 rows: column tiles of a workgroup, and how many workgroups split K,
-// so that there is one for each CU.
+// Up to 32 rows: column tiles of a workgroup, one where that is one workgroup a
+// CU at most (1 x 4096 x 4096 in 5.0 us against 7.6 on half the CUs), else two (1 x
+// 8192 x 8192 in 9.0 against 9.6); and how many workgroups split K, whose sums
+// take a second kernel: up to four where CUs would be idle, from K = 16384 on (1
+// x 16384 x 1024 in 8.1 us against 9.7 unsplit; 1 x 8192 x 1024 in 6.4 unsplit
+// against 7.2).
 void q4_small_plan(const lm::Q4Args& a, int cus, int* nt, int* ksplit) {
   const int64_t tiles = (a.N + 15) / 16;
-  *nt = tiles >= 4 * (int64_t)cus ? 4 : tiles >= 2 * (int64_t)cus ? 2 : 1;
+  *nt = tiles > cus ? 2 : 1;
   const int64_t wgs = (tiles + *nt - 1) / *nt;
-  const int64_t most = std::max(1, a.blocks / 8);
-  *ksplit = (int)std::clamp<int64_t>(cus / wgs, 1, std::min<int64_t>(most, 16));
+  *ksplit = a.blocks >= 128 ? (int)std::clamp<int64_t>(cus / wgs, 1, 4) : 1;
+}
+
+// Whether the small kernel takes the layer: up to 16 rows, and up to 32 of a
+// layer that is not wide (17 x 8192 x 8192 in 12.6 us against 23.6 on tiles, 17 x
+// 4096 x 50256 in 44 against 34) nor f32, whose operands do not fit.
+bool q4_small_takes(const lm::Q4Args& a, int cus) {
+  if (a.M <= 16) return true;
+  return a.M <= 32 && a.x_type != lm::kF32 && (a.N + 15) / 16 <= 4 * (int64_t)cus;
 }
 
 int q4_tile_plan(const lm::Q4Args& a, int cus, int* ksplit) {
   const int64_t tiles = (a.N + 15) / 16;
   const auto count = [&](int bm) { return (a.M + bm - 1) / bm * ((tiles + 7) / 8); };
-  const int config = a.M <= 32                                              ? lm::kQ4Tile32x128
+  const int config = a.M <= 32 ? lm::kQ4Tile32x128
                      : a.M <= 64 || a.x_type == lm::kF32 || count(128) < cus ? lm::kQ4Tile64x128
                                                                              : lm::kQ4Tile128x128;
   const int64_t wgs = count(config == lm::kQ4Tile32x128 ? 32 : config == lm::kQ4Tile64x128 ? 64 : 128);
@@ -193,9 +204,16 @@ int q4_tile_plan(const lm::Q4Args& a, int cus, int* ksplit) {
   return config;
 }
 
-void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, bool zeros, void* stream) {
+// Even slices of K, none of them empty.
+void q4_slices(lm::Q4Args& a) {
+  a.slice_blocks = (a.blocks + a.ksplit - 1) / a.ksplit;
+  if (a.slice_blocks > 0) a.ksplit = (a.blocks + a.slice_blocks - 1) / a.slice_blocks;
+}
+
+void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, int scale_type, bool zeros, void* stream) {
   check_sizes(M, K, "M", "K");
-  const lm::Q4Layout l = q4_checked_layout(K, N, group, a.scale_type, zeros);
+  const lm::Q4Layout l = q4_checked_layout(K, N, group, scale_type, zeros);
+  a.scale_mask = lm::q4_scale_mask(scale_type);
   if (a.x_type < lm::kF32 || a.x_type > lm::kE4m3) fail(kErrDtype, "X: unknown type %d", a.x_type);
   check_float_type(a.y_type, "Y");
   if (a.epi < 0 || a.epi > 7) fail(kErrArgument, "bad epilogue code %d", a.epi);
@@ -211,46 +229,52 @@ void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, bool zer
   if (K > 0) check_packed(a.w, "packed");
   a.M = (int)M, a.N = (int)N, a.K = (int)K;
   a.scales_at = l.scales_at, a.zeros_at = l.zeros_at, a.scale_bytes = l.scale_bytes;
-  a.blocks = (int)l.blocks, a.scale_blocks = (int)l.scale_blocks, a.blocks_per_scale = l.blocks_per_scale;
+  a.zero_step = zeros ? 1 : 0;
+  a.blocks = (int)l.blocks, a.scale_blocks = (int)l.scale_blocks;
+  const uint64_t per = l.blocks_per_scale;
+  a.scale_magic = per > 1 ? (uint32_t)((0x100000000ull + per - 1) / per) : 0;
   int cus = 0;
   device_launch(0, stream, [&](char*, int n) { cus = n; });
   const hipStream_t s = as_stream(stream);
-  if (M <= 16) {
+  lm::Q4PrepArgs p{};
+  p.x = a.x, p.ldx = a.ldx, p.M = a.M, p.K = a.K, p.blocks = a.blocks, p.spb = l.spb, p.x_type = a.x_type;
+  p.ldp = l.blocks * 128, p.plane = M * p.ldp;
+  const size_t planes = aligned((size_t)(a.x_type == lm::kF32 ? 3 : 1) * p.plane * 2);
+  if (q4_small_takes(a, cus)) {
     int nt;
     q4_small_plan(a, cus, &nt, &a.ksplit);
+    q4_slices(a);
     const size_t bytes = a.ksplit > 1 ? (size_t)a.ksplit * a.M * a.N * sizeof(float) : 0;
     device_launch(bytes, stream, [&](char* ws, int) {
       a.partials = reinterpret_cast<float*>(ws);
-      hipError_t (*const launch)(const lm::Q4Args&, int, int, bool, hipStream_t) =
+      hipError_t (*const launch)(const lm::Q4Args&, int, int, hipStream_t) =
           a.x_type == lm::kF32    ? lm::launch_q4_small<lm::kF32>
           : a.x_type == lm::kBf16 ? lm::launch_q4_small<lm::kBf16>
           : a.x_type == lm::kF16  ? lm::launch_q4_small<lm::kF16>
           : a.x_type == lm::kI8   ? lm::launch_q4_small<lm::kI8>
                                   : lm::launch_q4_small<lm::kE4m3>;
-      check_hip(launch(a, nt, l.spb, zeros, s), "q4_small launch");
+      check_hip(launch(a, nt, l.spb, s), "q4_small launch");
       if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
       set_plan("q4_small %s cols=%d ksplit=%d%s", type_name(a.x_type), 16 * nt, a.ksplit, a.ksplit > 1 ? " +join" : "");
     });
     return;
   }
   const int config = q4_tile_plan(a, cus, &a.ksplit);
-  lm::Q4PrepArgs p{};
-  p.x = a.x, p.ldx = a.ldx, p.M = a.M, p.K = a.K, p.blocks = a.blocks, p.spb = l.spb, p.x_type = a.x_type;
+  q4_slices(a);
   p.factor = zeros ? -1.0f : -8.0f - lm::q4_offset(a.x_type);
   p.xs_ld = (M + 127) / 128 * 128;
   // x itself where the tiles can read it: 16 bits, whole blocks, 16-byte aligned rows.
   const bool copy = !((a.x_type == lm::kBf16 || a.x_type == lm::kF16) && K % 128 == 0 && a.ldx % 8 == 0 &&
                       reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx <= kMostDepth);
-  p.ldp = l.blocks * 128, p.plane = M * p.ldp;
   const size_t sums = aligned((size_t)l.blocks * l.spb * p.xs_ld * sizeof(float));
-  const size_t planes = copy ? aligned((size_t)(a.x_type == lm::kF32 ? 3 : 1) * p.plane * 2) : 0;
+  const size_t copied = copy ? planes : 0;
   const size_t parts = a.ksplit > 1 ? (size_t)a.ksplit * M * N * sizeof(float) : 0;
-  device_launch(sums + planes + parts, stream, [&](char* ws, int) {
+  device_launch(sums + copied + parts, stream, [&](char* ws, int) {
     p.xs = reinterpret_cast<float*>(ws);
     p.xp = copy ? ws + sums : nullptr;
     a.xs = p.xs, a.xs_ld = p.xs_ld;
     a.xp = copy ? p.xp : a.x, a.ldp = copy ? p.ldp : a.ldx, a.plane = p.plane;
-    a.partials = reinterpret_cast<float*>(ws + sums + planes);
+    a.partials = reinterpret_cast<float*>(ws + sums + copied);
     if (a.blocks > 0) check_hip(lm::launch_q4_prep(p, s), "q4_prep launch");
     check_hip(lm::launch_q4_tile(a, config, l.spb, zeros, s), "q4_tile launch");
     if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
@@ -340,9 +364,9 @@ int edsl_hip_q4_dense_launch(const void* X, int64_t ldx, int x_type, const float
   return rt::guarded([&] {
     lm::Q4Args a{};
     a.x = X, a.x_scales = x_scales, a.w = static_cast<const char*>(packed), a.bias = bias, a.y = Y;
-    a.ldx = ldx, a.ldy = ldy, a.x_type = x_type, a.scale_type = scale_type, a.y_type = y_type;
+    a.ldx = ldx, a.ldy = ldy, a.x_type = x_type, a.y_type = y_type;
     a.bias_type = bias_type, a.epi = epilogue, a.alpha = alpha;
-    rt::q4_dense(a, M, N, K, group, has_zeros != 0, stream);
+    rt::q4_dense(a, M, N, K, group, scale_type, has_zeros != 0, stream);
   });
 }
 

@@ -29,7 +29,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // holds k = 32 s + 8 (l / 16) + j, even j in nibble j / 2 of its lower half, odd
 // ones in the upper half's. That is the operand of the 16x16x32 matrix
 // instruction, lane for lane, four in a row: a wave's load is one 1024-byte run.
-// Behind them the scales [N/16][SB][16][spb] and zero points likewise in bytes:
+// Behind them the scales [N/16][SB][16][spb] and the zero points in bytes likewise:
 // spb = 128 / group scales of a column in a block and SB = K/128 where the group
 // is less than 128, else spb = 1 and SB = K/group. All padding is zero.
 struct Q4Layout {
@@ -51,9 +51,19 @@ inline Q4Layout q4_layout(int64_t K, int64_t N, int group, int scale_type, bool 
   const int64_t scales = l.tiles_n * l.scale_blocks * 16 * l.spb;
   l.scales_at = l.tiles_n * l.blocks * 1024;
   l.zeros_at = l.scales_at + (scales * l.scale_bytes + 255) / 256 * 256;
+  // At the end room for what a 32-bit load of the last scale reads past it, and,
+  // without zero points, an 8 that stands for all of them.
   l.bytes = l.zeros_at + (zeros ? (scales + 255) / 256 * 256 : 0);
-  if (l.bytes > 0) l.bytes += 256;  // what a 32-bit load of the last scale reads past it
+  if (l.bytes > 0) l.bytes += 256;
   return l;
+}
+
+// Which reading of a scale's bits is kept (q4_scale).
+struct Q4ScaleMask {
+  uint32_t f32, bf16, f16;
+};
+inline Q4ScaleMask q4_scale_mask(int type) {
+  return {type == kF32 ? ~0u : 0u, type == kBf16 ? ~0u : 0u, type == kF16 ? ~0u : 0u};
 }
 
 struct Q4Args {
@@ -65,18 +75,26 @@ struct Q4Args {
   float* partials;  // [ksplit][M][N] sums where ksplit > 1
   int64_t ldx, ldy, scales_at, zeros_at;
   int M, N, K;
-  int blocks, scale_blocks, blocks_per_scale;
+  int blocks, scale_blocks;
+  uint32_t scale_magic;  // block / blocks_per_scale = block * magic >> 32, blocks up to 2^16
   int ksplit;  // workgroups that split K
+  int slice_blocks;  // blocks of a slice of K (the last may have fewer)
   int scale_bytes;
-  int x_type, scale_type, y_type, bias_type, epi;
+  int64_t zero_step;  // of a group's zero point: 1, or 0 where all are the one at zeros_at
+  int x_type, y_type, bias_type, epi;
+  Q4ScaleMask scale_mask;
   float alpha;
   // Tiles of many rows: x prepared (q4_prep_kernel), or x itself where its rows
-  // are whole 16-byte aligned blocks.
+  // are whole 16-byte aligned blocks of 16 bits.
   const void* xp;       // [planes][M][ldp]
   int64_t ldp, plane;   // elements
   const float* xs;      // [blocks * spb][xs_ld]: minus the sums of x in each group, times offset + 8 without zero points
   int64_t xs_ld;
 };
+
+__device__ __forceinline__ int q4_scale_block(const Q4Args& a, int block) {
+  return a.scale_magic ? (int)__umulhi((uint32_t)block, a.scale_magic) : block;
+}
 
 template <bool F16>
 struct Q4Elem;
@@ -107,12 +125,15 @@ constexpr float kQ4Offset = 16.0f;
 template <bool F16>
 __device__ __forceinline__ typename Q4Elem<F16>::V q4_weights(uint32_t w) {
   using E = Q4Elem<F16>;
-  constexpr uint32_t mask = (15u << E::kShift) * 0x10001u;
+  // One of the two constants in a vector register: an instruction takes one scalar.
+  const uint32_t mask = (15u << E::kShift) * 0x10001u;
+  uint32_t base = E::kBase;
+  asm("" : "+v"(base));
   u32x4 r;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int s = 4 * p - E::kShift;
-    r[p] = ((s >= 0 ? w >> s : w << -s) & mask) | E::kBase;
+    r[p] = ((s >= 0 ? w >> s : w << -s) & mask) | base;
   }
   return __builtin_bit_cast(typename E::V, r);
 }
@@ -137,9 +158,10 @@ __device__ __forceinline__ uint32_t q4_scale_bits(const char* p, int bytes, int6
   return load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(p + i * bytes)).v[0] |
          (uint32_t)load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(p + i * bytes)).v[1] << 16;
 }
-__device__ __forceinline__ float q4_scale(uint32_t bits, int type) {
-  const float half = (float)__builtin_bit_cast(f16, (uint16_t)bits);
-  return type == kF32 ? __builtin_bit_cast(float, bits) : type == kBf16 ? __builtin_bit_cast(float, bits << 16) : half;
+// All three readings, one kept: a branch would wait for the load.
+__device__ __forceinline__ float q4_scale(uint32_t bits, const Q4ScaleMask& k) {
+  const uint32_t half = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(f16, (uint16_t)bits));
+  return __builtin_bit_cast(float, (bits & k.f32) | ((bits << 16) & k.bf16) | (half & k.f16));
 }
 
 // Three bf16 terms whose sum is v, to the last bit of it while they are normal:
@@ -221,14 +243,14 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, const int (&m)[C], con
 
 // q4_small.hpp, one source file for each type of x.
 template <int XT>
-hipError_t launch_q4_small(const Q4Args& a, int nt, int spb, bool zeros, hipStream_t stream);
+hipError_t launch_q4_small(const Q4Args& a, int nt, int spb, hipStream_t stream);
 // q4_tile.hip; f32 has the first two only.
 enum : int { kQ4Tile32x128 = 0, kQ4Tile64x128 = 1, kQ4Tile128x128 = 2 };
 hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, bool zeros, hipStream_t stream);
 struct Q4PrepArgs {
   const void* x;
-  void* xp;  // or nullptr: sums only
-  float* xs;
+  void* xp;   // or nullptr: sums only
+  float* xs;  // or nullptr: a copy only
   int64_t ldx, ldp, plane, xs_ld;
   int M, K, blocks, spb, x_type;
   float factor;  // of the sums

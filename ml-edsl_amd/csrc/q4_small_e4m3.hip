@@ -1,8 +1,8 @@
-// The 4-bit layer on up to 16 rows (q4_small.hpp), x in e4m3.
+// The 4-bit layer on up to 32 rows (q4_small.hpp), x in e4m3.
 #include "q4_small.hpp"
 
 namespace edsl {
 namespace lm {
-template hipError_t launch_q4_small<kE4m3>(const Q4Args& a, int nt, int spb, bool zeros, hipStream_t stream);
+template hipError_t launch_q4_small<kE4m3>(const Q4Args& a, int nt, int spb, hipStream_t stream);
 }  // namespace lm
 }  // namespace edsl

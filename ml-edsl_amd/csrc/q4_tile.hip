@@ -11,10 +11,17 @@ namespace edsl {
 namespace lm {
 namespace {
 
-// 16 bytes a lane from memory to LDS, at `to` + 16 lane (`to` the wave's own).
-__device__ __forceinline__ void to_lds(const void* from, void* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
-                                   (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
+// 16 bytes a lane from memory, `base` (uniform) + `offset`, to LDS, `to` (the
+// wave's own) + 16 lane. As the instruction itself: for its intrinsic the
+// compiler lets every later read of LDS wait for it, whichever buffer it reads,
+// which left nothing on the way while a stage was multiplied. It has no result
+// register; wait_loads() is what waits for it. (m0 holds nothing between uses.)
+__device__ __forceinline__ void to_lds(const void* base, uint32_t offset, void* to) {
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)at)), "v"(offset), "s"(base)
+               : "memory");
 }
 
 // Waits for the wave's loads, those to LDS among them (vmcnt 0).
@@ -40,7 +47,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   tile_coords(blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
   const int64_t first = ((int64_t)tn * WN + wn) * NT;
   const int m0 = tm * BM;
-  const int b0 = (int)((int64_t)a.blocks * slice / a.ksplit), b1 = (int)((int64_t)a.blocks * (slice + 1) / a.ksplit);
+  const int b0 = slice * a.slice_blocks, b1 = min(a.blocks, b0 + a.slice_blocks);
 
   // Row r's chunk c lies at c ^ swizzle(r): 16 rows' reads of one chunk meet all banks.
   const auto swizzle = [](int r) { return CPR == 16 ? r % 16 : (r / 2) % 8; };
@@ -54,24 +61,24 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
     src[c] = (uint32_t)(((int64_t)(row < a.M ? row : a.M - 1) - m0) * a.ldp + 8 * ((i % CPR) ^ swizzle(r))) * 2u;
   }
   const char* const xp = static_cast<const char*>(a.xp) + 2 * m0 * a.ldp;
-  const auto load_x = [&](int stage, int buf) {
+  const auto load_x = [&](int stage, u32x4* to) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
-      to_lds(xp + 2 * (c * 256 / (BM * CPR)) * a.plane + (int64_t)stage * (16 * CPR) + src[c],
-             &lds[buf][c * 256 + wave * 64]);
+      to_lds(xp + 2 * (c * 256 / (BM * CPR)) * a.plane + (int64_t)stage * (16 * CPR), src[c],
+             to + c * 256 + wave * 64);
   };
-  const auto load_sums = [&](int b) {
+  const auto load_sums = [&](int b, f32x4* to) {
     // 16-byte pieces of SPB runs of BM sums.
     if (tid < SPB * BM / 4)
-      to_lds(a.xs + ((int64_t)b * SPB + tid / (BM / 4)) * a.xs_ld + m0 + 4 * (tid % (BM / 4)),
-             &sums[b & 1][wave * 64]);
+      to_lds(a.xs + (int64_t)b * SPB * a.xs_ld + m0,
+             4u * (uint32_t)(tid / (BM / 4) * a.xs_ld + 4 * (tid % (BM / 4))), to + wave * 64);
   };
   struct Weights {
     u32x4 w[NT];
     uint32_t scale[NT][SPB], zero[ZEROS ? NT : 1][SPB];  // as read
   };
   const auto load_w = [&](int b, Weights& r) {
-    const int sb = b / a.blocks_per_scale;
+    const int sb = q4_scale_block(a, b);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int64_t tile = first + t < tiles ? first + t : tiles - 1;
@@ -91,71 +98,77 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
     for (int t = 0; t < NT; ++t) sum[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   Weights now, next;
+  // One stage: starts the next one's loads, and multiplies this one.
+  const auto turn = [&](int b, int stage, const u32x4* x_now, u32x4* x_next, const f32x4* sums_now,
+                        f32x4* sums_next) {
+    wait_loads();
+    __syncthreads();
+    if (stage < STAGES - 1 || b + 1 < b1) load_x(b * STAGES + stage + 1, x_next);
+    if (stage == 0 && b + 1 < b1) {
+      load_sums(b + 1, sums_next);
+      load_w(b + 1, next);
+    }
+#pragma unroll
+    for (int s = 0; s < SS; ++s) {
+      const int step = stage * SS + s, g = step / STEPS;
+      if (step % STEPS == 0) {
+        float zero[NT];
+        if constexpr (ZEROS)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) zero[t] = (PLANES == 3 ? 0.0f : kQ4Offset) + (float)now.zero[t][g];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const f32x4 xs = sums_now[g * (BM / 4) + 4 * (wm * MT + i) + lane / 16];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            acc[i][t] = xs;
+            if constexpr (ZEROS)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][t][e] *= zero[t];
+          }
+        }
+      }
+      V q[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (PLANES == 3)
+          q[t] = q4_weights_f32(now.w[t][step]);
+        else
+          q[t] = q4_weights<F16>(now.w[t][step]);
+      }
+#pragma unroll
+      for (int p = PLANES - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int r = p * BM + 16 * (wm * MT + i) + lane % 16;
+          const V x = __builtin_bit_cast(V, x_now[r * CPR + ((4 * s + lane / 16) ^ swizzle(r))]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[i][t] = E::mfma(x, q[t], acc[i][t]);
+        }
+      if (step % STEPS == STEPS - 1) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float scale = q4_scale(now.scale[t][g], a.scale_mask);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[i][t][e] = fmaf(acc[i][t][e], scale, sum[i][t][e]);
+        }
+      }
+    }
+  };
   if (b0 < b1) {
-    load_x(b0 * STAGES, 0);
-    load_sums(b0);
+    load_x(b0 * STAGES, lds[0]);
+    load_sums(b0, sums[0]);
     load_w(b0, now);
   }
   for (int b = b0; b < b1; ++b) {
-#pragma unroll
-    for (int stage = 0; stage < STAGES; ++stage) {
-      const int buf = STAGES == 2 ? stage : (b - b0) & 1;
-      wait_loads();
-      __syncthreads();
-      const bool last = stage == STAGES - 1;
-      if (!last || b + 1 < b1) load_x(b * STAGES + stage + 1, buf ^ 1);
-      if (stage == 0 && b + 1 < b1) {
-        load_sums(b + 1);
-        load_w(b + 1, next);
-      }
-#pragma unroll
-      for (int s = 0; s < SS; ++s) {
-        const int step = stage * SS + s, g = step / STEPS;
-        if (step % STEPS == 0) {
-          float zero[NT];
-          if constexpr (ZEROS)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) zero[t] = (PLANES == 3 ? 0.0f : kQ4Offset) + (float)now.zero[t][g];
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const f32x4 xs = sums[b & 1][g * (BM / 4) + 4 * (wm * MT + i) + lane / 16];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              acc[i][t] = xs;
-              if constexpr (ZEROS)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][t][e] *= zero[t];
-            }
-          }
-        }
-        V q[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if constexpr (PLANES == 3)
-            q[t] = q4_weights_f32(now.w[t][step]);
-          else
-            q[t] = q4_weights<F16>(now.w[t][step]);
-        }
-#pragma unroll
-        for (int p = PLANES - 1; p >= 0; --p)
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const int r = p * BM + 16 * (wm * MT + i) + lane % 16;
-            const V x = __builtin_bit_cast(V, lds[buf][r * CPR + ((4 * s + lane / 16) ^ swizzle(r))]);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[i][t] = E::mfma(x, q[t], acc[i][t]);
-          }
-        if (step % STEPS == STEPS - 1) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const float scale = q4_scale(now.scale[t][g], a.scale_type);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sum[i][t][e] = fmaf(acc[i][t][e], scale, sum[i][t][e]);
-          }
-        }
-      }
+    const int odd = (b - b0) & 1;
+    if constexpr (STAGES == 1) {
+      turn(b, 0, lds[odd], lds[odd ^ 1], sums[odd], sums[odd ^ 1]);
+    } else {
+      turn(b, 0, lds[0], lds[1], sums[odd], sums[odd ^ 1]);
+      turn(b, 1, lds[1], lds[0], sums[odd], sums[odd ^ 1]);
     }
     now = next;
   }
@@ -272,7 +285,7 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(Q4PrepArgs a) {
     s += dpp<0x4E>(s);
     if (lanes > 4) s += dpp<0x141>(s);
     if (lanes > 8) s += dpp<0x140>(s);
-    if (lane % lanes == 0) a.xs[(int64_t)(k0 / (8 * lanes)) * a.xs_ld + row] = a.factor * s;
+    if (a.xs && lane % lanes == 0) a.xs[(int64_t)(k0 / (8 * lanes)) * a.xs_ld + row] = a.factor * s;
   }
 }
 
@@ -301,6 +314,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(Q4PackArgs a) {
   reinterpret_cast<uint32_t*>(a.packed + (tile * a.layout.blocks + block) * 1024)[4 * lane + step] = w;
   // Its scales and zero points, by the first block of each group.
   const int spb = a.layout.spb, bps = a.layout.blocks_per_scale;
+  if (!a.zeros && blockIdx.x == 0 && threadIdx.x < 16) a.packed[a.layout.zeros_at + threadIdx.x] = 8;
   if (block % bps != 0 || threadIdx.x >= 16 * spb) return;
   const int c = threadIdx.x / spb, g = threadIdx.x % spb;
   const int64_t col = 16 * tile + c, sb = block / bps, group = sb * spb + g, groups = (a.K + a.group - 1) / a.group;
