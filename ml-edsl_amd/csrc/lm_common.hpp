@@ -65,8 +65,10 @@ struct MaxNan {
   static __device__ __forceinline__ float of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 };
 
-// The combination over a wave's 64 lanes, in every lane: lanes 1 and 2 apart,
-// mirrored in 8 and in 16 by DPP, then 16 and 32 apart.
+// The combination over a wave's 64 lanes: lanes 1 and 2 apart, mirrored in 8 and
+// in 16 by DPP, then 16 and 32 apart. Every lane has the first one's, bit for
+// bit: its own may differ where the compiler fuses the caller's product into its
+// side of the first sum.
 template <typename Op>
 __device__ __forceinline__ float wave_all(float v) {
   v = Op::of(v, dpp<0xB1>(v));
@@ -75,7 +77,7 @@ __device__ __forceinline__ float wave_all(float v) {
   v = Op::of(v, dpp<0x140>(v));
   v = Op::of(v, __shfl_xor(v, 16));
   v = Op::of(v, __shfl_xor(v, 32));
-  return v;
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 
 // hipSuccess or the first error of a launch.

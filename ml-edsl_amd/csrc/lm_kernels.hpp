@@ -60,6 +60,7 @@ struct LogprobsArgs {
   float scale;
   int k;       // 0: no alternatives
   int chunks;  // parts of a row, one workgroup each
+  bool many;   // more rows than CUs
   int type;
   bool ids64;
 };

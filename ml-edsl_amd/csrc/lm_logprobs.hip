@@ -26,10 +26,13 @@ namespace edsl {
 namespace lm {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
-constexpr int kList = 512;   // candidates of one workgroup
-constexpr int kMaxChunks = 64;  // parts of a row: one lane each in the join
+constexpr int kVectors = 256;  // vectors that hold candidates, of one workgroup
+constexpr int kList = 512;     // its candidates
+constexpr int kMaxChunks = 64; // parts of a row: one lane each in the join
 constexpr int kNoIndex = 0x7fffffff;
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -79,35 +82,60 @@ __device__ __forceinline__ void put_id(void* ids, bool ids64, int64_t i, int v) 
     static_cast<int32_t*>(ids)[i] = v;
 }
 
-// The results of a row, by one thread, from its whole sums.
+// The given token's logit, read early by the thread that writes the results.
+struct Given {
+  bool in;  // inside the vocabulary
+  float x;
+};
 template <typename T>
-__device__ __forceinline__ void finish_row(const LogprobsArgs& a, int64_t row, Part p, bool none, float log_s) {
-  if (a.lse) a.lse[row] = none ? neg_inf() : fmaf(kLn2, log_s, a.scale * p.m);
-  if (a.entropy) a.entropy[row] = none ? 0.0f : kLn2 * (log_s - p.t / p.s);
+__device__ __forceinline__ Given read_given(const LogprobsArgs& a, int64_t row) {
+  Given g{false, 0.0f};
   if (a.logprobs) {
     const int64_t id = id_at(a.tokens, a.ids64, row);
-    float lp = 0.0f;
-    if (id >= 0 && id < a.V) {
-      const float x = (float)static_cast<const T*>(a.x)[row * a.ldx + id];
-      lp = none ? neg_inf() : fmaf(-kLn2, log_s, (x - p.m) * a.scale);
-    }
-    a.logprobs[row] = lp;
+    g.in = id >= 0 && id < a.V;
+    if (g.in) g.x = (float)static_cast<const T*>(a.x)[row * a.ldx + id];
   }
+  return g;
 }
 
-// One part's place in the workspace: Part, then k (value, index) pairs.
-__device__ __forceinline__ char* part_at(char* base, int64_t row, int chunk, int chunks, int k) {
-  return base + (row * chunks + chunk) * (int64_t)(16 + 8 * k);
+// The results of a row, by one thread, from its whole sums.
+__device__ __forceinline__ void finish_row(const LogprobsArgs& a, int64_t row, Given g, Part p, bool none, float log_s) {
+  if (a.lse) a.lse[row] = none ? neg_inf() : fmaf(kLn2, log_s, a.scale * p.m);
+  if (a.entropy) a.entropy[row] = none ? 0.0f : kLn2 * (log_s - p.t / p.s);
+  if (a.logprobs) a.logprobs[row] = !g.in ? 0.0f : none ? neg_inf() : fmaf(-kLn2, log_s, (g.x - p.m) * a.scale);
+}
+
+// The workspace: the parts of all rows, then k (value, index) pairs of each.
+struct Pair {
+  float v;
+  int i;
+};
+__device__ __forceinline__ Part* parts_of(const LogprobsArgs& a, int64_t row) {
+  return reinterpret_cast<Part*>(a.partials) + row * a.chunks;
+}
+__device__ __forceinline__ Pair* pairs_of(const LogprobsArgs& a, int64_t row) {
+  return reinterpret_cast<Pair*>(a.partials + (a.M * a.chunks * (int64_t)sizeof(Part) + 15) / 16 * 16) +
+         row * a.chunks * a.k;
+}
+
+// An alternative of a row, to its results.
+__device__ __forceinline__ void put_top(const LogprobsArgs& a, int64_t row, int r, float value, int index, Part p,
+                                        bool bad, bool none, float log_s) {
+  a.top[row * a.k + r] = bad ? __builtin_nanf("") : none ? neg_inf() : fmaf(-kLn2, log_s, (value - p.m) * a.scale);
+  put_id(a.top_ids, a.ids64, row * a.k + r, bad ? -1 : index);
 }
 
 template <typename T, int THREADS, int NV, bool TOP>
-__global__ void __launch_bounds__(THREADS) logprobs_kernel(LogprobsArgs a, int64_t part_len) {
+__global__ void __launch_bounds__(THREADS, NV <= 8 ? 8 : 4) logprobs_kernel(LogprobsArgs a, int64_t part_len) {
   constexpr int VEC = kVec<T>, WAVES = THREADS / 64;
+  using Vals = Packed<T, VEC>;
   __shared__ float maxima[TOP ? WAVES : 1][64];
   __shared__ Part parts[WAVES];
   __shared__ float list_v[TOP ? kList : 1];
   __shared__ int list_i[TOP ? kList : 1];
-  __shared__ int count;
+  __shared__ u32x4 vector_v[TOP ? kVectors : 1];
+  __shared__ int vector_i[TOP ? kVectors : 1];
+  __shared__ int vectors, count;
   __shared__ float best_v[WAVES];
   __shared__ int best_i[WAVES];
   const int64_t row = (int64_t)blockIdx.x / a.chunks;
@@ -117,30 +145,63 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(LogprobsArgs a, int64
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx + first;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const float c = a.scale * kLog2e;
-  if (tid == 0) count = 0;
+  Given given{};
+  if (tid == 0) {
+    vectors = count = 0;
+    if (a.chunks == 1) given = read_given<T>(a, row);
+  }
 
-  Packed<T, VEC> v[NV];
+  // The part stays in registers in its own type: 16-byte vectors, whole ones
+  // without a check, -inf past the end.
+  u32x4 v[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) v[j] = load_guarded<T, VEC>(x, (j * THREADS + tid) * VEC, n, (T)neg_inf());
+  for (int j = 0; j < NV; ++j) {
+    const int at = (j * THREADS + tid) * VEC;
+    if ((j + 1) * THREADS * VEC <= n)
+      v[j] = __builtin_bit_cast(u32x4, load_packed<T, VEC>(x + at));
+    else
+      v[j] = __builtin_bit_cast(u32x4, load_guarded<T, VEC>(x, at, n, (T)neg_inf()));
+  }
   float top = neg_inf();
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    const auto r = __builtin_bit_cast(Vals, v[j]);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) top = fmaxf(top, (float)v[j].v[e]);
+    for (int e = 0; e < VEC; ++e) top = fmaxf(top, (float)r.v[e]);
+    // Else the compiler keeps all elements in 32 bits, twice the registers.
+    asm("" : "+v"(v[j]));
+  }
   if constexpr (TOP) maxima[wave][lane] = top;
   const bool any = top > neg_inf();
   Part p{any ? top : 0.0f, 0.0f, 0.0f};
+  const auto add_up = [&](auto u_of) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (j * THREADS * VEC >= n) break;
+    for (int j = 0; j < NV; ++j) {
+      if (j * THREADS * VEC >= n) break;
+      const auto r = __builtin_bit_cast(Vals, v[j]);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float u = ((float)v[j].v[e] - p.m) * c;
-      const float w = __builtin_amdgcn_exp2f(u);
-      p.s += w;
-      p.t = fmaf(w, fmaxf(u, -200.0f), p.t);  // 0 for -inf: e is 0 there
+      for (int e = 0; e < VEC; ++e) {
+        const float u = u_of((float)r.v[e]);
+        const float w = __builtin_amdgcn_exp2f(u);
+        p.s += w;
+        p.t = fmaf(w, fmaxf(u, -200.0f), p.t);  // 0 for -inf: w is 0 there
+      }
     }
+  };
+  // One fma an element, where m c is far from overflow.
+  const float mc = p.m * c;
+  if (__all(fabsf(mc) < 1e37f)) {
+    add_up([&](float x) { return fmaf(x, c, -mc); });
+    // What was subtracted is m c rounded: back to m itself.
+    const float d = fmaf(p.m, c, -mc), f = __builtin_amdgcn_exp2f(-d);
+    p.t = (p.t - d * p.s) * f;
+    p.s *= f;
+  } else {
+    add_up([&](float x) { return (x - p.m) * c; });
   }
+  if constexpr (TOP)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) asm("" : "+v"(v[j]));
   p = wave_join(p, any, c);
   if (lane == 0) parts[wave] = p;
   __syncthreads();
@@ -151,52 +212,70 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(LogprobsArgs a, int64
   const bool none = !bad && all.s == 0.0f;
   const float log_s = log2f(all.s);
 
-  char* const out = a.chunks > 1 ? part_at(a.partials, row, chunk, a.chunks, a.k) : nullptr;
+  const bool whole = a.chunks == 1;
   if (tid == 0) {
-    if (out)
-      *reinterpret_cast<Part*>(out) = all;
+    if (whole)
+      finish_row(a, row, given, all, none, log_s);
     else
-      finish_row<T>(a, row, all, none, log_s);
+      parts_of(a, row)[chunk] = all;
   }
   if constexpr (TOP) {
     const int k = a.k;
     // The r-th alternative: to the row's results, or to the join.
     const auto put = [&](int r, float value, int index) {
-      if (out) {
-        float* const q = reinterpret_cast<float*>(out + 16) + 2 * r;
-        q[0] = value;
-        reinterpret_cast<int*>(q)[1] = index == kNoIndex ? index : (int)first + index;
-      } else {
-        a.top[row * k + r] = none ? neg_inf() : fmaf(-kLn2, log_s, (value - all.m) * a.scale);
-        put_id(a.top_ids, a.ids64, row * k + r, index);
-      }
+      if (whole)
+        put_top(a, row, r, value, index, all, bad, none, log_s);
+      else
+        pairs_of(a, row)[chunk * k + r] = {value, index == kNoIndex ? index : (int)first + index};
     };
     if (bad) {
-      if (tid < k) put(tid, __builtin_nanf(""), out ? kNoIndex : -1);
+      if (tid < k) put(tid, neg_inf(), kNoIndex);
       return;
     }
-    float classes = maxima[0][lane];
+    // By the first wave: the others leave the CU to its other workgroups.
+    if (wave == 0) {
+      float classes = maxima[0][lane];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) classes = fmaxf(classes, maxima[w][lane]);
-    const float least = kth_of_lanes(classes, k);
-    if (any && top >= least) {
+      for (int w = 1; w < WAVES; ++w) classes = fmaxf(classes, maxima[w][lane]);
+      const float t = kth_of_lanes(classes, k);
+      if (lane == 0) best_v[0] = t;
+    }
+    __syncthreads();
+    const float least = best_v[0];
+    // Vectors with an element that reaches it, then those elements.
+    if (__any(any && top >= least)) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        if (j * THREADS * VEC >= n) break;
+        const auto r = __builtin_bit_cast(Vals, v[j]);
+        float most = neg_inf();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float value = (float)v[j].v[e];
-          if (value >= least && value > neg_inf()) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kList) {
-              list_v[at] = value;
-              list_i[at] = (j * THREADS + tid) * VEC + e;
-            }
+        for (int e = 0; e < VEC; ++e) most = fmaxf(most, (float)r.v[e]);
+        if (most >= least && most > neg_inf()) {
+          const int at = atomicAdd(&vectors, 1);
+          if (at < kVectors) {
+            vector_v[at] = v[j];
+            vector_i[at] = (j * THREADS + tid) * VEC;
           }
         }
+        asm("" : "+v"(v[j]));
+      }
+    }
+    __syncthreads();
+    const int held = vectors;
+    for (int i = tid; i < (held < kVectors ? held : kVectors) * VEC; i += THREADS) {
+      const float value = (float)reinterpret_cast<const T*>(vector_v)[i];
+      if (value >= least && value > neg_inf()) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kList) {
+          list_v[at] = value;
+          list_i[at] = vector_i[i / VEC] + i % VEC;
+        }
+      }
     }
     __syncthreads();
     const int found = count;
-    if (found <= kList) {
+    if (held <= kVectors && found <= kList) {
       for (int i = tid; i < found; i += THREADS) {
         const float value = list_v[i];
         const int index = list_i[i];
@@ -216,23 +295,25 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(LogprobsArgs a, int64
       }
       return;
     }
-    // One alternative after the other: the best that follows the last one.
+    // One alternative after the other: the best that follows the last one. From
+    // memory again, which leaves the registers to the other workgroups' rows.
+    // (best_v is free: its readers are past a barrier.)
     float last_v = __builtin_inff();
     int last_i = -1;
     for (int r = 0; r < k; ++r) {
       float bv = neg_inf();
       int bi = kNoIndex;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int at = tid * VEC; at < n; at += THREADS * VEC) {
+        const auto vals = load_guarded<T, VEC>(x, at, n, (T)neg_inf());
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float value = (float)v[j].v[e];
-          const int index = (j * THREADS + tid) * VEC + e;
-          if (index < n && better(last_v, last_i, value, index) && better(value, index, bv, bi)) {
+          const float value = (float)vals.v[e];
+          if (at + e < n && better(last_v, last_i, value, at + e) && better(value, at + e, bv, bi)) {
             bv = value;
-            bi = index;
+            bi = at + e;
           }
         }
+      }
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) {
         const float ov = __shfl_xor(bv, d);
@@ -262,33 +343,63 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(LogprobsArgs a, int64
   }
 }
 
-// Joins the parts of a row, one a lane. Each part's alternatives are in order: the
-// row's are taken from the heads of the lists.
+// Joins the parts of a row, one a lane, in one wave; its alternatives come from
+// the parts' by the same way as theirs from the logits.
 template <typename T>
 __global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsArgs a) {
-  __shared__ float heads_v[kMaxChunks * kMaxTop];
-  __shared__ int heads_i[kMaxChunks * kMaxTop];
+  constexpr int kFew = 128;
+  __shared__ Pair pairs[kMaxChunks * kMaxTop];
+  __shared__ Pair list[kFew];
+  __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x, k = a.k;
-  const char* const mine = part_at(a.partials, row, lane < a.chunks ? lane : 0, a.chunks, k);
-  Part p = lane < a.chunks ? *reinterpret_cast<const Part*>(mine) : Part{0.0f, 0.0f, 0.0f};
-  if (lane < a.chunks)
-    for (int r = 0; r < k; ++r) {
-      heads_v[lane * kMaxTop + r] = reinterpret_cast<const float*>(mine + 16)[2 * r];
-      heads_i[lane * kMaxTop + r] = reinterpret_cast<const int*>(mine + 16)[2 * r + 1];
-    }
+  const int lane = threadIdx.x, k = a.k, n = a.chunks * k;
+  const Given given = read_given<T>(a, row);
+  Part p = lane < a.chunks ? parts_of(a, row)[lane] : Part{0.0f, 0.0f, 0.0f};
+  const Pair* const from = pairs_of(a, row);
+  float top = neg_inf();
+#pragma unroll 4
+  for (int i = lane; i < n; i += 64) {
+    const Pair q = from[i];
+    pairs[i] = q;
+    top = fmaxf(top, q.v);
+  }
+  if (lane == 0) count = 0;
   const float c = a.scale * kLog2e;
   p = wave_join(p, p.s > 0.0f || p.s != p.s, c);
   const bool bad = p.s != p.s, none = !bad && p.s == 0.0f;
   const float log_s = log2f(p.s);
-  if (lane == 0) finish_row<T>(a, row, p, none, log_s);
-  int at = 0;  // a lane reads its own entries only
+  if (lane == 0) finish_row(a, row, given, p, none, log_s);
+  if (k == 0) return;
+  if (bad) {
+    if (lane < k) put_top(a, row, lane, 0.0f, 0, p, bad, none, log_s);
+    return;
+  }
+  const float least = kth_of_lanes(top, k);
+  __syncthreads();
+  for (int i = lane; i < n; i += 64)
+    if (pairs[i].v >= least && pairs[i].i != kNoIndex) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kFew) list[at] = pairs[i];
+    }
+  __syncthreads();
+  const int found = count;
+  if (found <= kFew && found >= k) {
+    for (int i = lane; i < found; i += 64) {
+      const Pair q = list[i];
+      int rank = 0;
+      for (int j = 0; j < found; ++j) rank += better(list[j].v, list[j].i, q.v, q.i);
+      if (rank < k) put_top(a, row, rank, q.v, q.i, p, bad, none, log_s);
+    }
+    return;
+  }
+  // Many equal ones: each part's are in order, so the row's are taken from the
+  // heads of the parts' lists.
+  int at = 0;
   for (int r = 0; r < k; ++r) {
-    const bool has = lane < a.chunks && at < k && !bad;
-    const float v = has ? heads_v[lane * kMaxTop + at] : neg_inf();
-    const int i = has ? heads_i[lane * kMaxTop + at] : kNoIndex;
-    float bv = v;
-    int bi = i;
+    const bool has = lane < a.chunks && at < k;
+    const Pair q = has ? pairs[lane * k + at] : Pair{neg_inf(), kNoIndex};
+    float bv = q.v;
+    int bi = q.i;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const float ov = __shfl_xor(bv, d);
@@ -298,11 +409,8 @@ __global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsArgs a) {
         bi = oi;
       }
     }
-    if (has && i == bi && i != kNoIndex) ++at;
-    if (lane == 0) {
-      a.top[row * k + r] = bad ? __builtin_nanf("") : none ? neg_inf() : fmaf(-kLn2, log_s, (bv - p.m) * a.scale);
-      put_id(a.top_ids, a.ids64, row * k + r, bad ? -1 : bi);
-    }
+    if (has && q.i == bi && q.i != kNoIndex) ++at;
+    if (lane == 0) put_top(a, row, r, bv, bi, p, bad, none, log_s);
   }
 }
 
@@ -328,16 +436,20 @@ hipError_t launch_logprobs(const LogprobsArgs& a, hipStream_t stream) {
   hipError_t e;
   if (vecs <= 256)
     e = launch_parts<T, 256, 1>(a, len, stream);
-  else if (vecs <= 512)
+  else if (a.many && vecs <= 512)
     e = launch_parts<T, 256, 2>(a, len, stream);
-  else if (vecs <= 1024)
+  else if (a.many && vecs <= 1024)
     e = launch_parts<T, 256, 4>(a, len, stream);
+  else if (vecs <= 1024)
+    e = launch_parts<T, 1024, 1>(a, len, stream);
   else if (vecs <= 2048)
     e = launch_parts<T, 1024, 2>(a, len, stream);
   else if (vecs <= 4096)
     e = launch_parts<T, 1024, 4>(a, len, stream);
-  else
+  else if (vecs <= 8192)
     e = launch_parts<T, 1024, 8>(a, len, stream);
+  else
+    e = launch_parts<T, 1024, 16>(a, len, stream);
   if (e != hipSuccess || a.chunks == 1) return e;
   hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)a.M), dim3(64), 0, stream, a);
   return launched();
@@ -402,23 +514,20 @@ hipError_t launch_backward(const LogprobsBackwardArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// One workgroup a row where there are rows enough for the chip or the row is
-// short; else as many parts as there are CUs for, of 2048 elements at least.
+// As few parts of a row as fit a workgroup's registers: with one there is no join
+// (1 x 50256 in 8.3 us, in 24 parts 10.4; 65 x 32001 in 9.7, in 3 parts 16.5).
+// Twice the registers where there is no second row for the CU.
 int logprobs_chunks(int64_t M, int64_t V, int type, int cus) {
-  const int64_t most = 1024 * 8 * (16 / type_bytes(type));  // what a workgroup holds
-  const int64_t least = (V + most - 1) / most;
-  int64_t want = M > 0 ? cus / M : 1;
-  if (want > V / 2048) want = V / 2048;
-  if (want > kMaxChunks) want = kMaxChunks;
-  if (want < least) want = least;
   const int vec = 16 / type_bytes(type);
+  const int64_t most = 1024 * (M <= cus ? 16 : 8) * vec;
+  const int64_t want = (V + most - 1) / most;
   // Rounding the length up to vectors may leave the last parts empty: fewer, then.
   const int64_t len = part_length(V, (int)want, vec);
   return (int)((V + len - 1) / len);
 }
 
 size_t logprobs_partial_bytes(int64_t M, int chunks, int k) {
-  return chunks > 1 ? (size_t)M * chunks * (16 + 8 * (size_t)k) : 0;
+  return chunks > 1 ? ((size_t)M * chunks * sizeof(Part) + 15) / 16 * 16 + (size_t)M * chunks * k * sizeof(Pair) : 0;
 }
 
 hipError_t launch_token_logprobs(const LogprobsArgs& a, hipStream_t stream) {

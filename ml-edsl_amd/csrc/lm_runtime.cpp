@@ -114,6 +114,7 @@ void token_logprobs(lm::LogprobsArgs a, void* stream) {
   int cus = 0;
   device_launch(0, stream, [&](char*, int n) { cus = n; });
   a.chunks = lm::logprobs_chunks(a.M, a.V, a.type, cus);
+  a.many = a.M > cus;
   check_grid(a.M, a.chunks);
   device_launch(lm::logprobs_partial_bytes(a.M, a.chunks, a.k), stream, [&](char* ws, int) {
     a.partials = ws;

@@ -67,14 +67,15 @@ def check(x, tokens, k=0, scale=1.0):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("M,V,k", [(1, 1, 1), (3, 2, 2), (2, 31, 31), (5, 64, 32), (4, 100, 3), (7, 1000, 5),
                                    (2, 2049, 8), (1, 8191, 32), (3, 16385, 4), (300, 2500, 2), (1, 50256, 8),
-                                   (270, 50257, 5), (2, 131072, 20), (260, 70001, 32)])
+                                   (270, 50257, 5), (2, 131072, 20), (260, 70001, 32),
+                                   (3, 200003, 32), (300, 66000, 5)])
 def test_sizes(M, V, k, dtype):
     x, tokens = make(M, V, dtype, V % 5, V)
     check(x, tokens, k, 1.25)
 
 
 def test_one_launch_or_parts():
-    x, tokens = make(1, 50256, F32)
+    x, tokens = make(1, 131073, BF16)
     call(x, tokens, 4)
     assert "+join" in last_plan()
     x, tokens = make(512, 4096, BF16)
