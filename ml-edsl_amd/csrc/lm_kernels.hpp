@@ -39,7 +39,7 @@ struct NormBackwardArgs {
   float* dweight;   // or nullptr
   float* partials;  // [groups][N], where dweight is wanted
   int64_t lddy, ldh, lddh, lddx, M, N;
-  int groups;  // workgroups, each with the rows group, group + groups, ...
+  int groups;  // workgroups, each with a row of partials
   int type, weight_type;
 };
 int rms_norm_backward_groups(int64_t M, int64_t N, int type, int cus);

@@ -458,45 +458,66 @@ hipError_t launch_logprobs(const LogprobsArgs& a, hipStream_t stream) {
 // ---------------------------------------------------------------- backward
 // p_j = exp(d_j), d_j = scale x_j - lse (one rounding, exact where p is near 1);
 // dx_j = scale (dlp ([j == token] - p_j) - dent p_j (d_j + entropy)).
+// The bracket is one fma of d and g + dent entropy. The token's own element is
+// put right by the thread that has it.
 constexpr int kBackThreads = 256, kBackVecs = 4;
 
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(LogprobsBackwardArgs a, int chunks) {
   constexpr int VEC = kVec<T>;
+  using Vals = Packed<T, VEC>;
   const int64_t row = (int64_t)blockIdx.x / chunks;
-  const int64_t first = ((int64_t)blockIdx.x - row * chunks) * (kBackThreads * kBackVecs * VEC);
-  const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
-  T* const dx = static_cast<T*>(a.dx) + row * a.lddx;
+  const int first = (int)((int64_t)blockIdx.x - row * chunks) * (kBackThreads * kBackVecs * VEC);
+  const int n = (int)a.V - first;
+  const T* const x = static_cast<const T*>(a.x) + row * a.ldx + first;
+  T* const dx = static_cast<T*>(a.dx) + row * a.lddx + first;
+  Vals v[kBackVecs];
+  const bool full = n >= kBackThreads * kBackVecs * VEC;
+  if (full) {
+#pragma unroll
+    for (int j = 0; j < kBackVecs; ++j) v[j] = load_packed<T, VEC>(x + (j * kBackThreads + threadIdx.x) * VEC);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kBackVecs; ++j)
+      v[j] = load_guarded<T, VEC>(x, (j * kBackThreads + threadIdx.x) * VEC, n, (T)neg_inf());
+  }
   const float lse = a.lse[row];
-  const bool none = lse == neg_inf();
-  int64_t id = -1;
+  int id = -1;  // the token's place here
   float g = 0.0f;
   if (a.dlogprobs) {
-    id = id_at(a.tokens, a.ids64, row);
-    if (id >= 0 && id < a.V) g = a.scale * a.dlogprobs[row];
-    else id = -1;
+    const int64_t t = id_at(a.tokens, a.ids64, row);
+    if (t >= 0 && t < a.V) {
+      g = a.scale * a.dlogprobs[row];
+      id = (int)t - first;
+    }
   }
-  const float h = ENT ? a.entropy[row] : 0.0f, gh = ENT ? a.scale * a.dentropy[row] : 0.0f;
-  Packed<T, VEC> v[kBackVecs];
-#pragma unroll
-  for (int j = 0; j < kBackVecs; ++j)
-    v[j] = load_guarded<T, VEC>(x, first + (j * kBackThreads + threadIdx.x) * VEC, a.V, (T)neg_inf());
+  float gh = ENT ? a.scale * a.dentropy[row] : 0.0f;
+  float base = ENT ? fmaf(gh, a.entropy[row], g) : g;
+  const bool none = lse == neg_inf();
+  if (none) g = gh = base = 0.0f;
+  const float offset = none ? 0.0f : lse;  // p is 0 there: every logit is -inf, or its gradient counts as 0
 #pragma unroll
   for (int j = 0; j < kBackVecs; ++j) {
-    const int64_t i0 = first + (j * kBackThreads + threadIdx.x) * VEC;
-    if (i0 >= a.V) break;
-    Packed<T, VEC> r;
+    const int i0 = (j * kBackThreads + threadIdx.x) * VEC;
+    Vals r;
+    float out[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float d = fmaf((float)v[j].v[e], a.scale, -lse);
-      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
-      float q = g;
-      if constexpr (ENT) q = fmaf(gh, fmaxf(d, -200.0f) + h, g);  // p is 0 below
-      float out = -p * q;
-      if (i0 + e == id) out += g;
-      r.v[e] = (T)(none ? 0.0f : out);
+      const float d = fmaf((float)v[j].v[e], a.scale, -offset);
+      const float p = none ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
+      float q = base;
+      if constexpr (ENT) q = fmaf(gh, fmaxf(d, -200.0f), base);  // p is 0 below
+      out[e] = -p * q;
     }
-    store_guarded<T, VEC>(dx, i0, a.V, r);
+    if ((unsigned)(id - i0) < (unsigned)VEC)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out[e] += i0 + e == id ? g : 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = (T)out[e];
+    if (full)
+      *reinterpret_cast<Vals*>(dx + i0) = r;
+    else if (i0 < n)
+      store_guarded<T, VEC>(dx, i0, n, r);
   }
 }
 

@@ -7,6 +7,8 @@
 //
 // Bound by memory: about one operation a byte. A row is read once and held in
 // registers between the sum and the output.
+#include <type_traits>
+
 #include "kernels.hpp"
 #include "lm_common.hpp"
 #include "lm_kernels.hpp"
@@ -14,6 +16,8 @@
 namespace edsl {
 namespace lm {
 namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // What y holds.
 enum : int { kOutSame = 0, kOutI8 = 1, kOutE4m3 = 2 };
@@ -103,6 +107,43 @@ __device__ __forceinline__ void row_scale(float amax, float rstd, float& scale, 
   inv = scale > 0.0f ? 1.0f / scale : 0.0f;
 }
 
+// A thread's vectors of a row: no check where the threads' vectors are the row,
+// one a vector where it is whole vectors (then no load waits for another), one an
+// element else.
+template <typename T, int TPR, int NV>
+__device__ __forceinline__ void load_row(const T* row, int t, int64_t n, Packed<T, kVec<T>> (&v)[NV]) {
+  constexpr int VEC = kVec<T>;
+  if (n == (int64_t)TPR * NV * VEC) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = load_packed<T, VEC>(row + (j * TPR + t) * VEC);
+  } else if (n % VEC == 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      v[j] = Packed<T, VEC>{};
+      if ((j * TPR + t) * VEC < n) v[j] = load_packed<T, VEC>(row + (j * TPR + t) * VEC);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = load_guarded<T, VEC>(row, (j * TPR + t) * VEC, n);
+  }
+}
+
+template <typename T, int TPR, int NV>
+__device__ __forceinline__ void load_weights(const void* w, bool f32, int t, int64_t n, float (&v)[NV][kVec<T>]) {
+  constexpr int VEC = kVec<T>;
+  if (f32 && sizeof(T) != 4) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) load_weight<T, VEC>(w, true, (j * TPR + t) * VEC, n, v[j]);
+    return;
+  }
+  Packed<T, VEC> p[NV];
+  load_row<T, TPR, NV>(static_cast<const T*>(w), t, n, p);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[j][e] = (float)p[j].v[e];
+}
+
 // TPR threads hold one row of up to TPR * NV vectors in registers; workgroups of
 // 256 threads (or TPR) take 256 / TPR rows.
 template <typename T, int OUT, int TPR, int NV>
@@ -115,23 +156,19 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_kernel(NormArg
   const bool wf32 = a.weight_type == kF32;
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
   float h[NV][VEC], w[NV][VEC];
+  Packed<T, VEC> px[NV], pr[NV];
+  load_row<T, TPR, NV>(x, t, a.N, px);
+  if (a.residual) load_row<T, TPR, NV>(static_cast<const T*>(a.residual) + row * a.ldr, t, a.N, pr);
+  load_weights<T, TPR, NV>(a.weight, wf32, t, a.N, w);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const auto v = load_guarded<T, VEC>(x, ((int64_t)j * TPR + t) * VEC, a.N);
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) h[j][e] = (float)v.v[e];
-  }
-  if (a.residual) {
-    const T* const r = static_cast<const T*>(a.residual) + row * a.ldr;
+    for (int e = 0; e < VEC; ++e) h[j][e] = (float)px[j].v[e];
+  if (a.residual)
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const auto v = load_guarded<T, VEC>(r, ((int64_t)j * TPR + t) * VEC, a.N);
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) h[j][e] += (float)v.v[e];
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < NV; ++j) load_weight<T, VEC>(a.weight, wf32, ((int64_t)j * TPR + t) * VEC, a.N, w[j]);
+      for (int e = 0; e < VEC; ++e) h[j][e] += (float)pr[j].v[e];
   float sum = 0.0f, amax = 0.0f;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -247,65 +284,120 @@ hipError_t launch_norm_out(const NormArgs& a, hipStream_t stream, const char** p
 }
 
 // ---------------------------------------------------------------- backward
-// A workgroup of TPR threads walks the rows group, group + groups, ...; a
-// thread keeps the same NV vectors of columns in each, its part of dweight in
-// registers.
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR) rms_norm_backward_kernel(NormBackwardArgs a) {
-  constexpr int VEC = kVec<T>;
-  __shared__ float lds[2][2 * TPR / 64];
-  const int t = threadIdx.x;
-  const bool wf32 = a.weight_type == kF32;
-  float w[NV][VEC], dw[NV][VEC];
+// The backward pass. A workgroup of 1024 threads is 1024 / TPR teams with a row
+// each; a thread keeps the same NV vectors of columns in every row, its part of
+// dweight in registers, and the teams join theirs through LDS at the end, so that
+// there is one row of partials a CU. Where the registers hold it, the next row is
+// on its way while one is summed. WF32: the weight is f32 and x is not.
+template <typename T, int TPR, int NV, bool WF32>
+__global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackwardArgs a) {
+  constexpr int VEC = kVec<T>, TEAMS = 1024 / TPR, WAVES = TPR / 64;
+  constexpr bool AHEAD = NV * VEC <= 8;  // registers for the next row
+  using Vals = Packed<T, VEC>;
+  using W = std::conditional_t<WF32, float, T>;
+  __shared__ float lds[2][16];
+  __shared__ float joined[TEAMS > 1 ? TPR * NV * VEC : 1];
+  const int team = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  Packed<W, VEC> w[NV];
+  if constexpr (WF32) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    load_weight<T, VEC>(a.weight, wf32, ((int64_t)j * TPR + t) * VEC, a.N, w[j]);
+    for (int j = 0; j < NV; ++j)
+      w[j] = load_guarded<W, VEC>(static_cast<const W*>(a.weight), (j * TPR + t) * VEC, a.N);
+  } else {
+    load_row<T, TPR, NV>(static_cast<const T*>(a.weight), t, a.N, w);
+  }
+  float dw[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[j][e] = 0.0f;
-  }
-  int turn = 0;
-  for (int64_t row = blockIdx.x; row < a.M; row += a.groups, turn ^= 1) {
-    const T* const pdy = static_cast<const T*>(a.dy) + row * a.lddy;
-    const T* const ph = static_cast<const T*>(a.h) + row * a.ldh;
-    Packed<T, VEC> dy[NV], h[NV], dh[NV];
+  struct Row {
+    Vals dy[NV], h[NV], dh[NV];
+    float rstd;
+  };
+  // Rows stay packed: opened for the sum and again for the gradient, they take
+  // half of the registers.
+  const auto keep_packed = [](Vals (&v)[NV]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      dy[j] = load_guarded<T, VEC>(pdy, ((int64_t)j * TPR + t) * VEC, a.N);
-      h[j] = load_guarded<T, VEC>(ph, ((int64_t)j * TPR + t) * VEC, a.N);
-      if (a.dh)
-        dh[j] = load_guarded<T, VEC>(static_cast<const T*>(a.dh) + row * a.lddh, ((int64_t)j * TPR + t) * VEC, a.N);
+      u32x4 raw = __builtin_bit_cast(u32x4, v[j]);
+      asm("" : "+v"(raw));
+      v[j] = __builtin_bit_cast(Vals, raw);
     }
-    const float rstd = a.rstd[row];
-    float dot = 0.0f, none = 0.0f;
+  };
+  const auto load = [&](int64_t row, Row& r) {
+    if (row >= a.M) row = a.M - 1;  // not used: the last turn of a team without a row
+    load_row<T, TPR, NV>(static_cast<const T*>(a.dy) + row * a.lddy, t, a.N, r.dy);
+    load_row<T, TPR, NV>(static_cast<const T*>(a.h) + row * a.ldh, t, a.N, r.h);
+    if (a.dh) load_row<T, TPR, NV>(static_cast<const T*>(a.dh) + row * a.lddh, t, a.N, r.dh);
+    r.rstd = a.rstd[row];
+  };
+  const int64_t step = (int64_t)a.groups * TEAMS;
+  int64_t first = (int64_t)blockIdx.x * TEAMS;  // the first team's row; every team turns as often
+  Row now, next;
+  if (AHEAD && first < a.M) load(first + team, now);
+  for (int turn = 0; first < a.M; first += step, turn ^= 1) {
+    const int64_t row = first + team;
+    if (!AHEAD)
+      load(row, now);
+    else if (first + step < a.M)
+      load(row + step, next);
+    const float rstd = now.rstd;
+    const bool in = row < a.M;
+    float dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float g = (float)dy[j].v[e], xh = (float)h[j].v[e] * rstd;
-        dot = fmaf(g * w[j][e], xh, dot);
+        const float g = in ? (float)now.dy[j].v[e] : 0.0f, xh = in ? (float)now.h[j].v[e] * rstd : 0.0f;
+        dot = fmaf(g * (float)w[j].v[e], xh, dot);
         dw[j][e] = fmaf(g, xh, dw[j][e]);
       }
-    // Two buffers in turn: the barrier inside the next row's sum stands between
-    // the reads of one and its next writes.
-    row_reduce<TPR>(dot, none, lds[turn], false);
+    keep_packed(now.dy);
+    keep_packed(now.h);
+    // Two buffers in turn: the barrier of the next row stands between the reads
+    // of one and its next writes.
+    dot = wave_all<Sum>(dot);
+    if constexpr (WAVES > 1) {
+      if (t % 64 == 0) lds[turn][threadIdx.x / 64] = dot;
+      __syncthreads();
+      dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) dot += lds[turn][team * WAVES + i];
+    }
     const float mean = dot / (float)a.N;
     T* const pdx = static_cast<T*>(a.dx) + row * a.lddx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t i0 = ((int64_t)j * TPR + t) * VEC;
-      if (i0 >= a.N) break;
-      Packed<T, VEC> r;
+      if (!in || i0 >= a.N) break;
+      Vals r;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float xh = (float)h[j].v[e] * rstd;
-        float d = rstd * fmaf(-xh, mean, (float)dy[j].v[e] * w[j][e]);
-        if (a.dh) d += (float)dh[j].v[e];
+        const float xh = (float)now.h[j].v[e] * rstd;
+        float d = rstd * fmaf(-xh, mean, (float)now.dy[j].v[e] * (float)w[j].v[e]);
+        if (a.dh) d += (float)now.dh[j].v[e];
         r.v[e] = (T)d;
       }
       store_guarded<T, VEC>(pdx, i0, a.N, r);
     }
+    if (AHEAD) now = next;
   }
   if (!a.dweight) return;
+  if constexpr (TEAMS > 1) {
+    for (int i = 0; i < TEAMS; ++i) {
+      if (team == i)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            float& s = joined[(j * TPR + t) * VEC + e];
+            s = i == 0 ? dw[j][e] : s + dw[j][e];
+          }
+      __syncthreads();
+    }
+  }
+  if (team != 0) return;
   float* const part = a.partials + (int64_t)blockIdx.x * a.N;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -313,7 +405,7 @@ __global__ void __launch_bounds__(TPR) rms_norm_backward_kernel(NormBackwardArgs
     if (i0 >= a.N) break;
     Packed<float, VEC> r;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) r.v[e] = dw[j][e];
+    for (int e = 0; e < VEC; ++e) r.v[e] = TEAMS > 1 ? joined[i0 + e] : dw[j][e];
     store_guarded<float, VEC>(part, i0, a.N, r);
   }
 }
@@ -348,8 +440,10 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_long_kernel(NormBackwa
       Packed<T, VEC> dh, r;
       if (a.dh) dh = load_guarded<T, VEC>(static_cast<const T*>(a.dh) + row * a.lddh, i0, a.N);
       Packed<float, VEC> dw;
-      if (part && row != blockIdx.x) dw = load_guarded<float, VEC>(part, i0, a.N);
+      if (part && row != blockIdx.x)
+        dw = load_guarded<float, VEC>(part, i0, a.N);
       else
+#pragma unroll
         for (int e = 0; e < VEC; ++e) dw.v[e] = 0.0f;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -365,43 +459,73 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_long_kernel(NormBackwa
   }
 }
 
-// dweight[n] = the sum of the groups' partials, in their order: 64 columns a
-// workgroup, the groups in 16 interleaved parts, joined in order.
+// dweight[n] = the sum of the groups' partials, in a fixed order: 16 columns a
+// workgroup, so that there is one for most CUs, the groups in 64 interleaved
+// parts that are then joined in order.
 __global__ void __launch_bounds__(1024) dweight_kernel(const float* partials, int groups, int64_t N, float* dweight) {
-  __shared__ float lds[16][64];
-  const int c = threadIdx.x % 64, part = threadIdx.x / 64;
-  const int64_t n = (int64_t)blockIdx.x * 64 + c;
+  __shared__ float lds[64][17];
+  const int c = threadIdx.x % 16, part = threadIdx.x / 16;
+  const int64_t n = (int64_t)blockIdx.x * 16 + c;
   float s = 0.0f;
   if (n < N)
-    for (int g = part; g < groups; g += 16) s += partials[(int64_t)g * N + n];
+#pragma unroll 4
+    for (int g = part; g < groups; g += 64) s += partials[(int64_t)g * N + n];
   lds[part][c] = s;
   __syncthreads();
-  if (part == 0 && n < N) {
+  if (threadIdx.x < 256) {  // sixteen threads a column
+    const int col = threadIdx.x / 16, first = threadIdx.x % 16 * 4;
+    float v = 0.0f;
 #pragma unroll
-    for (int p = 1; p < 16; ++p) s += lds[p][c];
-    dweight[n] = s;
+    for (int p = 0; p < 4; ++p) v += lds[first + p][col];
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    const int64_t at = (int64_t)blockIdx.x * 16 + col;
+    if (first == 0 && at < N) dweight[at] = v;
   }
+}
+
+// Threads of a row, 0 for rows of any length: a vector each, two of f32 (4096 x
+// 4096 f32 in 52 us, with one in 59).
+int backward_threads(int64_t N, int type) {
+  int64_t vecs = (N * type_bytes(type) + 15) / 16;
+  if (vecs > 2048) return 0;
+  if (type == kF32) vecs = (vecs + 1) / 2;
+  return vecs <= 64 ? 64 : vecs <= 128 ? 128 : vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
+}
+
+template <typename T, int TPR, int NV>
+void launch_backward_rows(const NormBackwardArgs& a, hipStream_t stream) {
+  if (sizeof(T) != 4 && a.weight_type == kF32)
+    hipLaunchKernelGGL((rms_norm_backward_kernel<T, TPR, NV, sizeof(T) != 4>), dim3(a.groups), dim3(1024), 0, stream, a);
+  else
+    hipLaunchKernelGGL((rms_norm_backward_kernel<T, TPR, NV, false>), dim3(a.groups), dim3(1024), 0, stream, a);
 }
 
 template <typename T>
 hipError_t launch_backward(const NormBackwardArgs& a, hipStream_t stream) {
+  constexpr int NV = sizeof(T) == 4 ? 2 : 1;
   const int64_t vecs = (a.N + kVec<T> - 1) / kVec<T>;
-  const dim3 grid((unsigned)a.groups);
   if (a.M > 0) {
-    if (vecs <= 256)
-      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 256, 1>), grid, dim3(256), 0, stream, a);
-    else if (vecs <= 512)
-      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a);
-    else if (vecs <= 1024)
-      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 512, 2>), grid, dim3(512), 0, stream, a);
-    else if (vecs <= 2048)
-      hipLaunchKernelGGL((rms_norm_backward_kernel<T, 1024, 2>), grid, dim3(1024), 0, stream, a);
-    else
-      hipLaunchKernelGGL((rms_norm_backward_long_kernel<T>), grid, dim3(1024), 0, stream, a);
+    switch (backward_threads(a.N, a.type)) {
+      case 64: launch_backward_rows<T, 64, NV>(a, stream); break;
+      case 128: launch_backward_rows<T, 128, NV>(a, stream); break;
+      case 256: launch_backward_rows<T, 256, NV>(a, stream); break;
+      case 512: launch_backward_rows<T, 512, NV>(a, stream); break;
+      case 1024:
+        if (vecs <= 1024 * NV)
+          launch_backward_rows<T, 1024, NV>(a, stream);
+        else
+          launch_backward_rows<T, 1024, 2>(a, stream);
+        break;
+      default:
+        hipLaunchKernelGGL((rms_norm_backward_long_kernel<T>), dim3(a.groups), dim3(1024), 0, stream, a);
+    }
     if (const hipError_t e = launched(); e != hipSuccess) return e;
   }
   if (!a.dweight) return hipSuccess;
-  hipLaunchKernelGGL(dweight_kernel, dim3((unsigned)((a.N + 63) / 64)), dim3(1024), 0, stream, a.partials,
+  hipLaunchKernelGGL(dweight_kernel, dim3((unsigned)((a.N + 15) / 16)), dim3(1024), 0, stream, a.partials,
                      a.M > 0 ? a.groups : 0, a.N, a.dweight);
   return launched();
 }
@@ -416,10 +540,10 @@ hipError_t launch_rms_norm(const NormArgs& a, int cus, hipStream_t stream, const
 }
 
 int rms_norm_backward_groups(int64_t M, int64_t N, int type, int cus) {
-  (void)N;
-  (void)type;
-  const int64_t most = 4 * (int64_t)cus;
-  return (int)(M < most ? (M > 0 ? M : 1) : most);
+  const int tpr = backward_threads(N, type);
+  const int64_t teams = tpr > 0 ? 1024 / tpr : 1;
+  const int64_t wgs = (M + teams - 1) / teams;
+  return (int)(wgs < 1 ? 1 : wgs < cus ? wgs : cus);
 }
 
 hipError_t launch_rms_norm_backward(const NormBackwardArgs& a, hipStream_t stream) {

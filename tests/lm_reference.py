@@ -37,31 +37,30 @@ def token_logprobs(logits, tokens, k=0, scale=1.0):
     """logprobs, lse, entropy, top values, top ids: by the rules of
     include/edsl_hip_lm.h for masked rows, padding and rows without probabilities."""
     scale = as_f32(scale)
-    l = scale * d(logits)
+    x = d(logits)
+    l = scale * x
     M, V = l.shape
-    lse, entropy, lp = torch.empty(M, dtype=torch.float64), torch.empty(M, dtype=torch.float64), torch.zeros(M, dtype=torch.float64)
-    top, ids = torch.empty(M, k, dtype=torch.float64), torch.empty(M, k, dtype=torch.int64)
-    for r in range(M):
-        row = l[r]
-        bad = bool(torch.isnan(row).any() or (row == math.inf).any())
-        none = not bad and bool((row == -math.inf).all())
-        if bad:
-            lse[r] = entropy[r] = math.nan
-            logp = torch.full_like(row, math.nan)
-        elif none:
-            lse[r], entropy[r] = -math.inf, 0.0
-            logp = row
-        else:
-            lse[r] = torch.logsumexp(row, 0)
-            logp = torch.log_softmax(row, 0)
-            p = logp.exp()
-            entropy[r] = -(p[p > 0] * logp[p > 0]).sum()
-        if tokens is not None and 0 <= int(tokens[r]) < V:
-            lp[r] = logp[int(tokens[r])]
-        if k:
-            order = torch.sort(d(logits)[r], descending=True, stable=True).indices[:k]
-            ids[r] = -1 if bad else order
-            top[r] = math.nan if bad else logp[order]
+    bad = torch.isnan(l).any(1) | (l == math.inf).any(1)
+    none = ~bad & (l == -math.inf).all(1)
+    logp = torch.log_softmax(torch.where((bad | none)[:, None], 0.0, l), 1)
+    lse = torch.logsumexp(torch.where(bad[:, None], 0.0, l), 1)
+    entropy = -torch.where(logp > -math.inf, logp.exp() * logp, 0.0).sum(1)
+    logp[none], lse[none], entropy[none] = -math.inf, -math.inf, 0.0
+    logp[bad], lse[bad], entropy[bad] = math.nan, math.nan, math.nan
+    lp = torch.zeros(M, dtype=torch.float64)
+    if tokens is not None:
+        tokens = tokens.cpu().long()
+        given = (tokens >= 0) & (tokens < V)
+        lp = torch.where(given, logp[torch.arange(M), torch.where(given, tokens, 0)], 0.0)
+    # Falling, equal ones by their index: a stable sort of no more than the values that can matter.
+    ids = torch.empty(M, k, dtype=torch.int64)
+    if k:
+        least = torch.where(bad[:, None], 0.0, x).topk(k, 1).values[:, -1:]
+        for r in range(M):
+            some = (x[r] >= least[r]).nonzero()[:, 0] if not bad[r] else torch.arange(k)
+            ids[r] = some[torch.sort(x[r, some], descending=True, stable=True).indices[:k]]
+    top = logp.gather(1, ids) if k else torch.empty(M, 0, dtype=torch.float64)
+    ids[bad] = -1
     return lp, lse, entropy, top, ids
 
 
