@@ -193,15 +193,23 @@ bool q4_small_takes(const lm::Q4Args& a, int cus) {
   return a.M <= 32 && a.x_type != lm::kF32 && (a.N + 15) / 16 <= 4 * (int64_t)cus;
 }
 
+// Tiles: 64 rows (32 for up to 32) until tiles of 128 rows are two a CU (1024 x
+// 4096 x 4096 bf16 in 49 us on the former, 56 on the latter); K split towards two
+// workgroups a CU (33 x 8192 x 8192 in 60, 42, 28, 27 us on 1, 2, 4, 8 slices), and
+// by two where there is one but K is long (256 x 8192 x 8192 in 58 against 63, 512
+// x 4096 x 4096 in 38 against 35).
 int q4_tile_plan(const lm::Q4Args& a, int cus, int* ksplit) {
   const int64_t tiles = (a.N + 15) / 16;
   const auto count = [&](int bm) { return (a.M + bm - 1) / bm * ((tiles + 7) / 8); };
-  const int config = a.M <= 32 ? lm::kQ4Tile32x128
-                     : a.M <= 64 || a.x_type == lm::kF32 || count(128) < cus ? lm::kQ4Tile64x128
+  const int config = a.M <= 32                                              ? lm::kQ4Tile32x128
+                     : a.x_type == lm::kF32 || count(128) < 2 * (int64_t)cus ? lm::kQ4Tile64x128
                                                                              : lm::kQ4Tile128x128;
   const int64_t wgs = count(config == lm::kQ4Tile32x128 ? 32 : config == lm::kQ4Tile64x128 ? 64 : 128);
   check_grid(wgs, 16);
-  *ksplit = (int)std::clamp<int64_t>(cus / wgs, 1, std::clamp(a.blocks / 4, 1, 16));
+  if (wgs >= cus)
+    *ksplit = wgs < 2 * (int64_t)cus && a.blocks >= 64 ? 2 * cus / wgs : 1;
+  else
+    *ksplit = (int)std::clamp<int64_t>(2 * cus / wgs, 1, std::clamp(a.blocks / 4, 1, 16));
   return config;
 }
 

@@ -225,7 +225,7 @@ hipError_t launch_tile_config(const Q4Args& a, int config, int spb, bool zeros, 
 }
 
 // ------------------------------------------------------------------- x
-// A wave takes a row of x, 8 elements a lane: converts them where a copy is
+// A wave takes 512 k of a row of x, 8 elements a lane: converts them where a copy is
 // wanted (bf16 terms of f32, bf16 of 8 bits; zeros past K) and adds up each
 // group's.
 template <int XT>
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(Q4PrepArgs a) {
   const int row = blockIdx.x * 4 + threadIdx.x / 64;
   if (row >= a.M) return;
   const int lanes = 16 / a.spb;  // of a group
-  for (int k0 = 8 * lane; k0 < 128 * a.blocks; k0 += 512) {
+  if (const int k0 = 512 * blockIdx.y + 8 * lane; k0 < 128 * a.blocks) {
     float v[8];
     u32x4 out[3];
     if constexpr (XT == kE4m3) {
@@ -300,23 +300,43 @@ __global__ void __launch_bounds__(256) q4_join_kernel(Q4Args a) {
 }
 
 // ------------------------------------------------------------------ packing
-// A workgroup of 256 threads packs a block of 16 columns x 128 k, a word each.
+// A workgroup of 256 threads packs a block of 128 k of four tiles: reads rows of 64
+// columns, 4 bytes a thread, into LDS, and each wave puts its tile's words together.
 __global__ void __launch_bounds__(256) q4_pack_kernel(Q4PackArgs a) {
-  const int64_t tile = blockIdx.x / a.layout.blocks, block = blockIdx.x % a.layout.blocks;
-  // Threads of a wave take 16 columns by 4 runs of 8 k of one step.
-  const int lane = threadIdx.x % 64, step = threadIdx.x / 64;
-  const int64_t n = 16 * tile + lane % 16, k0 = 128 * block + 32 * step + 8 * (lane / 16);
-  uint32_t w = 0;
-  if (n < a.N)
+  constexpr int PITCH = 68;  // bytes of a row in LDS
+  __shared__ uint8_t q[128 * PITCH];
+  const int64_t first = 4 * (blockIdx.x / a.layout.blocks), block = blockIdx.x % a.layout.blocks;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  {
+    const int c = threadIdx.x % 16 * 4;
+    const int64_t n = 16 * first + c;
+#pragma unroll 8
+    for (int r = threadIdx.x / 16; r < 128; r += 16) {
+      const int64_t k = 128 * block + r;
+      Packed<uint8_t, 4> v{};
+      if (k < a.K && n < a.N) v = load_guarded<uint8_t, 4>(a.q + k * a.ldq, n, a.N);
+      *reinterpret_cast<uint32_t*>(&q[r * PITCH + c]) = __builtin_bit_cast(uint32_t, v);
+    }
+  }
+  __syncthreads();
+  const int64_t tile = first + wave;
+  if (tile >= a.layout.tiles_n) return;
+  u32x4 words;
+#pragma unroll
+  for (int step = 0; step < 4; ++step) {
+    uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (k0 + j < a.K) w |= (uint32_t)(a.q[(k0 + j) * a.ldq + n] & 15) << (4 * (j / 2) + 16 * (j % 2));
-  reinterpret_cast<uint32_t*>(a.packed + (tile * a.layout.blocks + block) * 1024)[4 * lane + step] = w;
+      w |= (uint32_t)(q[(32 * step + 8 * (lane / 16) + j) * PITCH + 16 * wave + lane % 16] & 15)
+           << (4 * (j / 2) + 16 * (j % 2));
+    words[step] = w;
+  }
+  reinterpret_cast<u32x4*>(a.packed + (tile * a.layout.blocks + block) * 1024)[lane] = words;
   // Its scales and zero points, by the first block of each group.
   const int spb = a.layout.spb, bps = a.layout.blocks_per_scale;
   if (!a.zeros && blockIdx.x == 0 && threadIdx.x < 16) a.packed[a.layout.zeros_at + threadIdx.x] = 8;
-  if (block % bps != 0 || threadIdx.x >= 16 * spb) return;
-  const int c = threadIdx.x / spb, g = threadIdx.x % spb;
+  if (block % bps != 0 || lane >= 16 * spb) return;
+  const int c = lane / spb, g = lane % spb;
   const int64_t col = 16 * tile + c, sb = block / bps, group = sb * spb + g, groups = (a.K + a.group - 1) / a.group;
   const bool in = col < a.N && group < groups;
   const int64_t at = ((tile * a.layout.scale_blocks + sb) * 16 + c) * spb + g;
@@ -339,7 +359,7 @@ hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, bool zeros, hipS
 }
 
 hipError_t launch_q4_prep(const Q4PrepArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.M + 3) / 4)), block(256);
+  const dim3 grid((unsigned)((a.M + 3) / 4), (unsigned)((a.blocks + 3) / 4)), block(256);
   switch (a.x_type) {
     case kF32: hipLaunchKernelGGL((q4_prep_kernel<kF32>), grid, block, 0, stream, a); break;
     case kBf16: hipLaunchKernelGGL((q4_prep_kernel<kBf16>), grid, block, 0, stream, a); break;
@@ -358,7 +378,8 @@ hipError_t launch_q4_join(const Q4Args& a, hipStream_t stream) {
 
 hipError_t launch_q4_pack(const Q4PackArgs& a, hipStream_t stream) {
   if (a.layout.blocks == 0 || a.layout.tiles_n == 0) return hipSuccess;
-  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)(a.layout.tiles_n * a.layout.blocks)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)((a.layout.tiles_n + 3) / 4 * a.layout.blocks)), dim3(256), 0,
+                     stream, a);
   return launched();
 }
 
