@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   static_assert(WM * WN == 4, "four waves");
   // A stage of x in LDS: SS steps of 32 k, CPR 16-byte chunks a row.
   constexpr int SS = PLANES == 3 ? 2 : 4, CPR = 4 * SS, STAGES = 4 / SS;
-  constexpr int CHUNKS = PLANES * BM * CPR / 256;  // a thread's
-  __shared__ u32x4 lds[2][PLANES * BM * CPR];
+  constexpr int ALL = PLANES * BM * CPR, CHUNKS = (ALL + 255) / 256;  // a thread's
+  __shared__ u32x4 lds[2][ALL];
   __shared__ f32x4 sums[2][SPB * BM / 4];  // a block's sums of x
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int wm = wave % WM, wn = wave / WM;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   const auto swizzle = [](int r) { return CPR == 16 ? r % 16 : (r / 2) % 8; };
   // Addresses are a uniform base and 32 bits a lane, so that they stay out of the
   // vector registers (the runtime bounds K for it); rows past M repeat the last.
-  static_assert(BM * CPR % 256 == 0, "a chunk is of one plane");
+  static_assert(BM * CPR % 64 == 0, "a wave's chunk is of one plane");
   uint32_t src[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
@@ -63,9 +63,13 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   const char* const xp = static_cast<const char*>(a.xp) + 2 * m0 * a.ldp;
   const auto load_x = [&](int stage, u32x4* to) {
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-      to_lds(xp + 2 * (c * 256 / (BM * CPR)) * a.plane + (int64_t)stage * (16 * CPR), src[c],
-             to + c * 256 + wave * 64);
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int i = c * 256 + wave * 64;
+      if (ALL % 256 == 0 || i < ALL)
+        to_lds(xp + 2 * (BM * CPR % 256 == 0 ? c * 256 / (BM * CPR) : i / (BM * CPR)) * a.plane +
+                   (int64_t)stage * (16 * CPR),
+               src[c], to + i);
+    }
   };
   const auto load_sums = [&](int b, f32x4* to) {
     // 16-byte pieces of SPB runs of BM sums.
@@ -220,8 +224,10 @@ template <bool F16, int PLANES>
 hipError_t launch_tile_config(const Q4Args& a, int config, int spb, bool zeros, hipStream_t stream) {
   if (config == kQ4Tile32x128) return launch_tile_spb<F16, PLANES, 2, 2, 1, 4>(a, spb, zeros, stream);
   if (config == kQ4Tile64x128) return launch_tile_spb<F16, PLANES, 4, 2, 1, 4>(a, spb, zeros, stream);
-  if constexpr (PLANES == 1) return launch_tile_spb<F16, 1, 4, 4, 2, 2>(a, spb, zeros, stream);
-  return hipErrorInvalidValue;
+  if constexpr (PLANES == 3)
+    return launch_tile_spb<F16, 3, 3, 2, 1, 4>(a, spb, zeros, stream);
+  else
+    return launch_tile_spb<F16, 1, 4, 4, 2, 2>(a, spb, zeros, stream);
 }
 
 // ------------------------------------------------------------------- x
