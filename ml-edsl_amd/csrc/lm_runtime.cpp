@@ -193,21 +193,17 @@ bool q4_small_takes(const lm::Q4Args& a, int cus) {
   return a.M <= 32 && a.x_type != lm::kF32 && (a.N + 15) / 16 <= 4 * (int64_t)cus;
 }
 
-// Tiles: 64 rows (32 for up to 32) until tiles of 128 rows are two a CU (1024 x
-// 4096 x 4096 bf16 in 49 us on the former, 56 on the latter), of f32 of 48 where
-// that is fewer rows in all; K split towards two
-// workgroups a CU (33 x 8192 x 8192 in 60, 42, 28, 27 us on 1, 2, 4, 8 slices), and
-// by two where there is one but K is long (256 x 8192 x 8192 in 58 against 63, 512
-// x 4096 x 4096 in 38 against 35).
+// Tiles: 64 rows, 32 for up to 32, of f32 48 where that is fewer rows in all (48 x
+// 4096 x 50256 in 66 us against 79); K split towards two workgroups a CU (33 x 8192
+// x 8192 in 60, 42, 28, 27 us on 1, 2, 4, 8 slices), and by two where there is one
+// but K is long (256 x 8192 x 8192 in 58 against 63, 512 x 4096 x 4096 in 38
+// against 35).
 int q4_tile_plan(const lm::Q4Args& a, int cus, int* ksplit) {
-  const int64_t tiles = (a.N + 15) / 16;
-  const auto count = [&](int bm) { return (a.M + bm - 1) / bm * ((tiles + 7) / 8); };
-  static const int rows[] = {32, 64, 48, 128};
-  const bool f32 = a.x_type == lm::kF32;
+  static const int rows[] = {32, 64, 48};
   int config = a.M <= 32 ? lm::kQ4Tile32x128 : lm::kQ4Tile64x128;
-  if (a.M > 32 && f32 && (a.M + 47) / 48 * 48 < (a.M + 63) / 64 * 64) config = lm::kQ4Tile48x128;
-  if (!f32 && count(128) >= 2 * (int64_t)cus) config = lm::kQ4Tile128x128;
-  const int64_t wgs = count(rows[config]);
+  if (a.M > 32 && a.x_type == lm::kF32 && ((int64_t)a.M + 47) / 48 * 48 < ((int64_t)a.M + 63) / 64 * 64)
+    config = lm::kQ4Tile48x128;
+  const int64_t wgs = ((int64_t)a.M + rows[config] - 1) / rows[config] * (((int64_t)a.N + 127) / 128);
   check_grid(wgs, 16);
   if (wgs >= cus)
     *ksplit = wgs < 2 * (int64_t)cus && a.blocks >= 64 ? 2 * cus / wgs : 1;
@@ -290,7 +286,7 @@ void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, int scal
     if (a.blocks > 0) check_hip(lm::launch_q4_prep(p, s), "q4_prep launch");
     check_hip(lm::launch_q4_tile(a, config, l.spb, zeros, s), "q4_tile launch");
     if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
-    static const char* const names[] = {"32x128", "64x128", "48x128", "128x128"};
+    static const char* const names[] = {"32x128", "64x128", "48x128"};
     set_plan("q4_prep%s+q4_tile %s tile=%s ksplit=%d%s", copy ? "_copy" : "", type_name(a.x_type), names[config],
              a.ksplit, a.ksplit > 1 ? " +join" : "");
   });

@@ -151,12 +151,13 @@ __device__ __forceinline__ bf16x8 q4_weights_f32(uint32_t w) {
 // What a weight is held above q for x of this type.
 constexpr float q4_offset(int x_type) { return x_type == kF32 ? 0.0f : kQ4Offset; }
 
-// Scale i of an array, as it lies in memory: 32 bits from its address on (the
-// packed weights' end leaves room). Read one way for all types and decoded where
-// it is used, so that no load waits at a branch.
-__device__ __forceinline__ uint32_t q4_scale_bits(const char* p, int bytes, int64_t i) {
-  return load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(p + i * bytes)).v[0] |
-         (uint32_t)load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(p + i * bytes)).v[1] << 16;
+// A scale as it lies in memory: 32 bits from its address on (the packed weights'
+// end leaves room). Read one way for all types and decoded where it is used, so
+// that no load waits at a branch. `row`: uniform, of a tile's column 0 and first
+// group; the lane's part of the address is 32 bits.
+__device__ __forceinline__ uint32_t q4_scale_bits(const char* row, uint32_t offset) {
+  const auto v = load_packed<uint16_t, 2>(reinterpret_cast<const uint16_t*>(row + offset));
+  return v.v[0] | (uint32_t)v.v[1] << 16;
 }
 // All three readings, one kept: a branch would wait for the load.
 __device__ __forceinline__ float q4_scale(uint32_t bits, const Q4ScaleMask& k) {
@@ -244,8 +245,8 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, const int (&m)[C], con
 // q4_small.hpp, one source file for each type of x.
 template <int XT>
 hipError_t launch_q4_small(const Q4Args& a, int nt, int spb, hipStream_t stream);
-// q4_tile.hip; the third is of f32, the fourth of the others.
-enum : int { kQ4Tile32x128 = 0, kQ4Tile64x128 = 1, kQ4Tile48x128 = 2, kQ4Tile128x128 = 3 };
+// q4_tile.hip; the third is of f32 only.
+enum : int { kQ4Tile32x128 = 0, kQ4Tile64x128 = 1, kQ4Tile48x128 = 2 };
 hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, bool zeros, hipStream_t stream);
 struct Q4PrepArgs {
   const void* x;

@@ -76,11 +76,14 @@ __device__ __forceinline__ void small_load(const Q4Args& a, const SmallRows<XT, 
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     r.w[t] = __builtin_bit_cast(u32x4, raw_buffer_load_i32x4(rsrc[t], 1024 * block + 16 * lane, 0, 0));
-    const int64_t at = ((int64_t)((tile + t) * (int64_t)a.scale_blocks + sb) * 16 + lane % 16) * SPB;
+    // Uniform bases, 32 bits a lane.
+    const int64_t at = ((tile + t) * (int64_t)a.scale_blocks + sb) * (16 * SPB);
+    const char* const scales = a.w + a.scales_at + at * a.scale_bytes;
+    const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(a.w + a.zeros_at) + at * a.zero_step;
 #pragma unroll
     for (int g = 0; g < SPB; ++g) {
-      r.scale[t][g] = q4_scale_bits(a.w + a.scales_at, a.scale_bytes, at + g);
-      r.zero[t][g] = reinterpret_cast<const uint8_t*>(a.w + a.zeros_at)[(at + g) * a.zero_step];
+      r.scale[t][g] = q4_scale_bits(scales + g * a.scale_bytes, (uint32_t)(lane % 16 * SPB * a.scale_bytes));
+      r.zero[t][g] = zeros[(uint32_t)((lane % 16 * SPB + g) * (int)a.zero_step)];
     }
   }
 }

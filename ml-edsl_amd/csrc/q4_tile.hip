@@ -1,10 +1,18 @@
 // The 4-bit layer on more than 16 rows: tiles on the matrix cores.
 //
-// A workgroup of 4 waves takes 16 MT WM rows x 16 NT WN columns. A wave loads and
+// A workgroup of 4 waves takes 16 MT rows x 64 NT columns. A wave loads and
 // unpacks the weights of its own columns in registers, a block of 128 k ahead; x
 // and its groups' sums go from memory straight to LDS, a stage ahead, with 16-byte
 // chunks exchanged by row so that reads hit all banks. Each group's accumulators start at the prepared
 // -zero * sum x and are scaled into the 32-bit totals at its end.
+//
+// Bound by power and by the matrix cores and vector ALUs together where M is
+// large: 4096^3 in 153 us without zero points and 163 with them, the preparation of
+// x included (898 and 843 TFLOP/s, 80 and 75 % of what the vendor's bf16 product
+// reaches there), 8192^3 with them in 1098 us (1.0 PFLOP/s, 80 %). Tiles of 128x128
+// and 128x256 (half and a third of the traffic) are no faster, 164 to 172 us, nor
+// are fragments read ahead or a forced order of products and unpacking. With few
+// rows the loads' latency bounds it.
 #include "q4.hpp"
 
 namespace edsl {
@@ -27,25 +35,23 @@ __device__ __forceinline__ void to_lds(const void* base, uint32_t offset, void* 
 // Waits for the wave's loads, those to LDS among them (vmcnt 0).
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
-template <bool F16, int PLANES, int MT, int NT, int WM, int WN, int SPB, bool ZEROS>
+template <bool F16, int PLANES, int MT, int NT, int SPB, bool ZEROS>
 __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   using E = Q4Elem<F16>;
   using V = typename E::V;
-  constexpr int BM = 16 * MT * WM, STEPS = 4 / SPB;
-  static_assert(WM * WN == 4, "four waves");
+  constexpr int BM = 16 * MT, STEPS = 4 / SPB;
   // A stage of x in LDS: SS steps of 32 k, CPR 16-byte chunks a row.
   constexpr int SS = PLANES == 3 ? 2 : 4, CPR = 4 * SS, STAGES = 4 / SS;
   constexpr int ALL = PLANES * BM * CPR, CHUNKS = (ALL + 255) / 256;  // a thread's
   __shared__ u32x4 lds[2][ALL];
   __shared__ f32x4 sums[2][SPB * BM / 4];  // a block's sums of x
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  const int wm = wave % WM, wn = wave / WM;
   const int64_t tiles = (a.N + 15) / 16;
-  const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (int)((tiles + NT * WN - 1) / (NT * WN));
+  const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (int)((tiles + 4 * NT - 1) / (4 * NT));
   const int slice = blockIdx.x / (tiles_m * tiles_n);
   int tm, tn;
   tile_coords(blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
-  const int64_t first = ((int64_t)tn * WN + wn) * NT;
+  const int64_t first = ((int64_t)tn * 4 + wave) * NT;
   const int m0 = tm * BM;
   const int b0 = slice * a.slice_blocks, b1 = min(a.blocks, b0 + a.slice_blocks);
 
@@ -77,6 +83,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
       to_lds(a.xs + (int64_t)b * SPB * a.xs_ld + m0,
              4u * (uint32_t)(tid / (BM / 4) * a.xs_ld + 4 * (tid % (BM / 4))), to + wave * 64);
   };
+  const uint32_t scale_offset = lane % 16 * SPB * a.scale_bytes;
   struct Weights {
     u32x4 w[NT];
     uint32_t scale[NT][SPB], zero[ZEROS ? NT : 1][SPB];  // as read
@@ -85,13 +92,16 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
     const int sb = q4_scale_block(a, b);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      // Uniform bases, 32 bits a lane: no vector instruction goes into addresses.
       const int64_t tile = first + t < tiles ? first + t : tiles - 1;
-      r.w[t] = *reinterpret_cast<const u32x4*>(a.w + (tile * a.blocks + b) * 1024 + 16 * lane);
-      const int64_t at = ((tile * a.scale_blocks + sb) * 16 + lane % 16) * SPB;
+      r.w[t] = *reinterpret_cast<const u32x4*>(a.w + (tile * a.blocks + b) * 1024 + (uint32_t)(16 * lane));
+      const int64_t at = (tile * a.scale_blocks + sb) * (16 * SPB);
+      const char* const scales = a.w + a.scales_at + at * a.scale_bytes;
+      const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(a.w + a.zeros_at) + at;
 #pragma unroll
       for (int g = 0; g < SPB; ++g) {
-        r.scale[t][g] = q4_scale_bits(a.w + a.scales_at, a.scale_bytes, at + g);
-        if constexpr (ZEROS) r.zero[t][g] = reinterpret_cast<const uint8_t*>(a.w + a.zeros_at)[at + g];
+        r.scale[t][g] = q4_scale_bits(scales + g * a.scale_bytes, scale_offset);
+        if constexpr (ZEROS) r.zero[t][g] = zeros[(uint32_t)(lane % 16 * SPB + g)];
       }
     }
   };
@@ -122,7 +132,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
           for (int t = 0; t < NT; ++t) zero[t] = (PLANES == 3 ? 0.0f : kQ4Offset) + (float)now.zero[t][g];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const f32x4 xs = sums_now[g * (BM / 4) + 4 * (wm * MT + i) + lane / 16];
+          const f32x4 xs = sums_now[g * (BM / 4) + 4 * i + lane / 16];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             acc[i][t] = xs;
@@ -144,7 +154,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
       for (int p = PLANES - 1; p >= 0; --p)
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const int r = p * BM + 16 * (wm * MT + i) + lane % 16;
+          const int r = p * BM + 16 * i + lane % 16;
           const V x = __builtin_bit_cast(V, x_now[r * CPR + ((4 * s + lane / 16) ^ swizzle(r))]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) acc[i][t] = E::mfma(x, q[t], acc[i][t]);
@@ -186,7 +196,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = 4 * t + e;
-        m[j] = m0 + 16 * (wm * MT + i) + 4 * (lane / 16) + e;
+        m[j] = m0 + 16 * i + 4 * (lane / 16) + e;
         n[j] = (int)(16 * (first + t)) + lane % 16;
         in[j] = m[j] < a.M && n[j] < a.N;
         v[j] = sum[i][t][e];
@@ -201,33 +211,31 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   }
 }
 
-template <bool F16, int PLANES, int MT, int NT, int WM, int WN, int SPB>
+template <bool F16, int PLANES, int MT, int NT, int SPB>
 hipError_t launch_tile_zeros(const Q4Args& a, bool zeros, hipStream_t stream) {
   const int64_t tiles = (a.N + 15) / 16;
-  const int64_t tm = (a.M + 16 * MT * WM - 1) / (16 * MT * WM), tn = (tiles + NT * WN - 1) / (NT * WN);
+  const int64_t tm = (a.M + 16 * MT - 1) / (16 * MT), tn = (tiles + 4 * NT - 1) / (4 * NT);
   const dim3 grid((unsigned)(tm * tn * a.ksplit)), block(256);
   if (zeros)
-    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, WM, WN, SPB, true>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, SPB, true>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, WM, WN, SPB, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, SPB, false>), grid, block, 0, stream, a);
   return launched();
 }
 
-template <bool F16, int PLANES, int MT, int NT, int WM, int WN>
+template <bool F16, int PLANES, int MT, int NT>
 hipError_t launch_tile_spb(const Q4Args& a, int spb, bool zeros, hipStream_t stream) {
-  if (spb == 4) return launch_tile_zeros<F16, PLANES, MT, NT, WM, WN, 4>(a, zeros, stream);
-  if (spb == 2) return launch_tile_zeros<F16, PLANES, MT, NT, WM, WN, 2>(a, zeros, stream);
-  return launch_tile_zeros<F16, PLANES, MT, NT, WM, WN, 1>(a, zeros, stream);
+  if (spb == 4) return launch_tile_zeros<F16, PLANES, MT, NT, 4>(a, zeros, stream);
+  if (spb == 2) return launch_tile_zeros<F16, PLANES, MT, NT, 2>(a, zeros, stream);
+  return launch_tile_zeros<F16, PLANES, MT, NT, 1>(a, zeros, stream);
 }
 
 template <bool F16, int PLANES>
 hipError_t launch_tile_config(const Q4Args& a, int config, int spb, bool zeros, hipStream_t stream) {
-  if (config == kQ4Tile32x128) return launch_tile_spb<F16, PLANES, 2, 2, 1, 4>(a, spb, zeros, stream);
-  if (config == kQ4Tile64x128) return launch_tile_spb<F16, PLANES, 4, 2, 1, 4>(a, spb, zeros, stream);
-  if constexpr (PLANES == 3)
-    return launch_tile_spb<F16, 3, 3, 2, 1, 4>(a, spb, zeros, stream);
-  else
-    return launch_tile_spb<F16, 1, 4, 4, 2, 2>(a, spb, zeros, stream);
+  if (config == kQ4Tile32x128) return launch_tile_spb<F16, PLANES, 2, 2>(a, spb, zeros, stream);
+  if (config == kQ4Tile64x128) return launch_tile_spb<F16, PLANES, 4, 2>(a, spb, zeros, stream);
+  if constexpr (PLANES == 3) return launch_tile_spb<F16, 3, 3, 2>(a, spb, zeros, stream);
+  return hipErrorInvalidValue;
 }
 
 // ------------------------------------------------------------------- x

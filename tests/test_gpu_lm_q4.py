@@ -119,7 +119,7 @@ def test_epilogues(epi, y_dtype, M):
 def test_plans():
     for M, K, N, what in [(1, 16384, 64, "q4_small bf16 cols=16 ksplit=4 +join"), (16, 512, 8192, "cols=32 ksplit=1"),
                           (20, 512, 512, "q4_small bf16 cols=16 ksplit=1"), (20, 128, 20000, "tile=32x128"), (64, 4096, 8192, "tile=64x128 ksplit=8"),
-                          (2048, 128, 4096, "q4_prep+q4_tile bf16 tile=128x128 ksplit=1"),
+                          (2048, 128, 4096, "q4_prep+q4_tile bf16 tile=64x128 ksplit=1"),
                           (2048, 130, 4096, "q4_prep_copy+q4_tile")]:
         layer(M, K, N, 128, BF16)
         assert what in last_plan(), last_plan()
