@@ -80,6 +80,14 @@ __device__ __forceinline__ float wave_all(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 
+// A grid of n workgroups along x and y: a launch takes less than 2^32 threads along
+// each. block_of() numbers them; the last ones may be past n, which is less than 2^31.
+inline dim3 grid_of(int64_t n) {
+  constexpr int64_t kRow = int64_t(1) << 20;
+  return n <= kRow ? dim3((unsigned)n) : dim3((unsigned)kRow, (unsigned)((n + kRow - 1) / kRow));
+}
+__device__ __forceinline__ uint32_t block_of() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // hipSuccess or the first error of a launch.
 inline hipError_t launched() { return hipGetLastError(); }
 

@@ -138,8 +138,9 @@ __global__ void __launch_bounds__(THREADS, NV <= 8 ? 8 : 4) logprobs_kernel(Logp
   __shared__ int vectors, count;
   __shared__ float best_v[WAVES];
   __shared__ int best_i[WAVES];
-  const int64_t row = (int64_t)blockIdx.x / a.chunks;
-  const int chunk = (int)((int64_t)blockIdx.x - row * a.chunks);
+  const int64_t row = block_of() / (uint32_t)a.chunks;
+  if (row >= a.M) return;
+  const int chunk = (int)(block_of() - row * a.chunks);
   const int64_t first = chunk * part_len;
   const int n = (int)(first + part_len < a.V ? part_len : a.V - first);  // > 0
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx + first;
@@ -351,7 +352,8 @@ __global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsArgs a) {
   __shared__ Pair pairs[kMaxChunks * kMaxTop];
   __shared__ Pair list[kFew];
   __shared__ int count;
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_of();
+  if (row >= a.M) return;
   const int lane = threadIdx.x, k = a.k, n = a.chunks * k;
   const Given given = read_given<T>(a, row);
   Part p = lane < a.chunks ? parts_of(a, row)[lane] : Part{0.0f, 0.0f, 0.0f};
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsArgs a) {
 
 template <typename T, int THREADS, int NV>
 hipError_t launch_parts(const LogprobsArgs& a, int64_t part_len, hipStream_t stream) {
-  const dim3 grid((unsigned)(a.M * a.chunks));
+  const dim3 grid = grid_of(a.M * a.chunks);
   if (a.k > 0)
     hipLaunchKernelGGL((logprobs_kernel<T, THREADS, NV, true>), grid, dim3(THREADS), 0, stream, a, part_len);
   else
@@ -451,7 +453,7 @@ hipError_t launch_logprobs(const LogprobsArgs& a, hipStream_t stream) {
   else
     e = launch_parts<T, 1024, 16>(a, len, stream);
   if (e != hipSuccess || a.chunks == 1) return e;
-  hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)a.M), dim3(64), 0, stream, a);
+  hipLaunchKernelGGL((logprobs_join_kernel<T>), grid_of(a.M), dim3(64), 0, stream, a);
   return launched();
 }
 
@@ -466,8 +468,9 @@ template <typename T, bool ENT>
 __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(LogprobsBackwardArgs a, int chunks) {
   constexpr int VEC = kVec<T>;
   using Vals = Packed<T, VEC>;
-  const int64_t row = (int64_t)blockIdx.x / chunks;
-  const int first = (int)((int64_t)blockIdx.x - row * chunks) * (kBackThreads * kBackVecs * VEC);
+  const int64_t row = block_of() / (uint32_t)chunks;
+  if (row >= a.M) return;
+  const int first = (int)(block_of() - row * chunks) * (kBackThreads * kBackVecs * VEC);
   const int n = (int)a.V - first;
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx + first;
   T* const dx = static_cast<T*>(a.dx) + row * a.lddx + first;
@@ -525,7 +528,7 @@ template <typename T>
 hipError_t launch_backward(const LogprobsBackwardArgs& a, hipStream_t stream) {
   const int64_t per = kBackThreads * kBackVecs * kVec<T>;
   const int chunks = (int)((a.V + per - 1) / per);
-  const dim3 grid((unsigned)(a.M * chunks)), block(kBackThreads);
+  const dim3 grid = grid_of(a.M * chunks), block(kBackThreads);
   if (a.dentropy)
     hipLaunchKernelGGL((logprobs_backward_kernel<T, true>), grid, block, 0, stream, a, chunks);
   else

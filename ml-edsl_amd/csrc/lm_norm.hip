@@ -104,7 +104,7 @@ __device__ __forceinline__ void row_scale(float amax, float rstd, float& scale, 
   constexpr float kTop = OUT == kOutI8 ? 127.0f : 448.0f;
   const float top = amax * rstd;
   scale = top / kTop;
-  inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+  inv = scale >= 0x1p-126f ? 1.0f / scale : 0.0f;  // below, the reciprocal may be infinite
 }
 
 // A thread's vectors of a row: no check where the threads' vectors are the row,
@@ -150,8 +150,8 @@ template <typename T, int OUT, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_kernel(NormArgs a) {
   constexpr int VEC = kVec<T>, BLOCK = TPR < 256 ? 256 : TPR, ROWS = BLOCK / TPR;
   __shared__ float lds[2 * BLOCK / 64];
-  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-  if (row >= a.M) return;  // only where a row is one wave's, without barriers
+  const int64_t row = (int64_t)block_of() * ROWS + threadIdx.x / TPR;
+  if (row >= a.M) return;  // by waves where a row is one wave's, without barriers, else by workgroups
   const int t = threadIdx.x % TPR;
   const bool wf32 = a.weight_type == kF32;
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -208,7 +208,8 @@ template <typename T, int OUT>
 __global__ void __launch_bounds__(1024) rms_norm_long_kernel(NormArgs a) {
   constexpr int VEC = kVec<T>;
   __shared__ float lds[32];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_of();
+  if (row >= a.M) return;
   const bool wf32 = a.weight_type == kF32;
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* const res = a.residual ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
@@ -258,8 +259,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(NormArgs a) {
 template <typename T, int OUT, int TPR, int NV>
 hipError_t launch_row(const NormArgs& a, hipStream_t stream) {
   constexpr int BLOCK = TPR < 256 ? 256 : TPR, ROWS = BLOCK / TPR;
-  hipLaunchKernelGGL((rms_norm_kernel<T, OUT, TPR, NV>), dim3((unsigned)((a.M + ROWS - 1) / ROWS)), dim3(BLOCK), 0,
-                     stream, a);
+  hipLaunchKernelGGL((rms_norm_kernel<T, OUT, TPR, NV>), grid_of((a.M + ROWS - 1) / ROWS), dim3(BLOCK), 0, stream, a);
   return launched();
 }
 
@@ -272,7 +272,7 @@ hipError_t launch_norm(const NormArgs& a, hipStream_t stream, const char** plan)
   if (vecs <= 1024) return *plan = "row=256x4", launch_row<T, OUT, 256, 4>(a, stream);
   if (vecs <= 4096) return *plan = "row=1024x4", launch_row<T, OUT, 1024, 4>(a, stream);
   *plan = "row=long";
-  hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), dim3((unsigned)a.M), dim3(1024), 0, stream, a);
+  hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), grid_of(a.M), dim3(1024), 0, stream, a);
   return launched();
 }
 
@@ -532,8 +532,7 @@ hipError_t launch_backward(const NormBackwardArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_rms_norm(const NormArgs& a, int cus, hipStream_t stream, const char** plan) {
-  (void)cus;
+hipError_t launch_rms_norm(const NormArgs& a, hipStream_t stream, const char** plan) {
   if (a.type == kF32) return launch_norm_out<float>(a, stream, plan);
   if (a.type == kBf16) return launch_norm_out<bf16>(a, stream, plan);
   return launch_norm_out<f16>(a, stream, plan);

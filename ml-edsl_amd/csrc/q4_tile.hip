@@ -245,7 +245,8 @@ hipError_t launch_tile_config(const Q4Args& a, int config, int spb, bool zeros, 
 template <int XT>
 __global__ void __launch_bounds__(256) q4_prep_kernel(Q4PrepArgs a) {
   const int lane = threadIdx.x % 64;
-  const int row = blockIdx.x * 4 + threadIdx.x / 64;
+  // Rows along x and z (a launch takes less than 2^32 threads along each).
+  const int64_t row = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 4 + threadIdx.x / 64;
   if (row >= a.M) return;
   const int lanes = 16 / a.spb;  // of a group
   if (const int k0 = 512 * blockIdx.y + 8 * lane; k0 < 128 * a.blocks) {
@@ -373,7 +374,7 @@ hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, bool zeros, hipS
 }
 
 hipError_t launch_q4_prep(const Q4PrepArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.M + 3) / 4), (unsigned)((a.blocks + 3) / 4)), block(256);
+  const dim3 rows = grid_of(((int64_t)a.M + 3) / 4), grid(rows.x, (unsigned)((a.blocks + 3) / 4), rows.y), block(256);
   switch (a.x_type) {
     case kF32: hipLaunchKernelGGL((q4_prep_kernel<kF32>), grid, block, 0, stream, a); break;
     case kBf16: hipLaunchKernelGGL((q4_prep_kernel<kBf16>), grid, block, 0, stream, a); break;
