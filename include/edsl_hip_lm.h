@@ -10,7 +10,10 @@
  * the message in edsl_hip_last_error(). Rows of any length, stride (at least
  * the row) and alignment to their element are taken; a pointer of an optional
  * operand may be null. Sizes go up to 2^30 in each dimension, offsets are 64
- * bits. An output may not overlap an input except where stated.
+ * bits; work beyond one launch (2^31 workgroups) is refused. Sums, maxima and
+ * norms are 32-bit floats: rows whose squares, or products with weights, leave
+ * their range have results of 0, infinities or NaN. An output may not overlap an input except where
+ * stated.
  */
 #ifndef EDSL_HIP_LM_H
 #define EDSL_HIP_LM_H
@@ -36,7 +39,8 @@ extern "C" {
  * F16), weight that type or F32. The norm is that of h in 32 bits, not of the
  * rounded total. y has type `type`, or an 8-bit type with scales[M], one a row:
  * y = q * scales with scales = max_n |y| / 127 (I8) or / 448 (E4M3), q rounded
- * to nearest even; a row of zeros has scale 0. A row whose norm is not finite
+ * to nearest even; a row of zeros has scale 0, and
+ * one whose scale is under 2^-126 codes of 0. A row whose norm is not finite
  * or whose values are NaN has a NaN scale and unspecified codes. rstd[M] is
  * optional, for the backward pass. total may be x or residual, and y may be
  * x, residual or total's memory in the same type and stride. */
