@@ -27,7 +27,7 @@ struct NormArgs {
   float eps;
   int type, weight_type, y_type;
 };
-hipError_t launch_rms_norm(const NormArgs& a, hipStream_t stream, const char** plan);
+hipError_t launch_rms_norm(const NormArgs& a, int cus, hipStream_t stream, const char** plan);
 
 struct NormBackwardArgs {
   const void* dy;

@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kBackThreads) logprobs_backward_kernel(Logprob
 #pragma unroll
     for (int e = 0; e < VEC; ++e) r.v[e] = (T)out[e];
     if (full)
-      *reinterpret_cast<Vals*>(dx + i0) = r;
+      store_streamed<T, VEC>(dx + i0, r);
     else if (i0 < n)
       store_guarded<T, VEC>(dx, i0, n, r);
   }

@@ -59,9 +59,9 @@ void rms_norm(lm::NormArgs a, void* stream) {
   check_mat(a.y, a.ldy, a.M, a.N, "y");
   if (a.residual) check_mat(a.residual, a.ldr, a.M, a.N, "residual");
   if (a.total) check_mat(a.total, a.ldt, a.M, a.N, "total");
-  device_launch(0, stream, [&](char*, int) {
+  device_launch(0, stream, [&](char*, int cus) {
     const char* plan = "";
-    check_hip(lm::launch_rms_norm(a, as_stream(stream), &plan), "rms_norm launch");
+    check_hip(lm::launch_rms_norm(a, cus, as_stream(stream), &plan), "rms_norm launch");
     set_plan("rms_norm %s->%s %s", type_name(a.type), type_name(a.y_type), plan);
   });
 }
