@@ -194,22 +194,28 @@ bool q4_small_takes(const lm::Q4Args& a, int cus) {
 }
 
 // Tiles: 64 rows, 32 for up to 32, of f32 48 where that is fewer rows in all (48 x
-// 4096 x 50256 in 66 us against 79); K split towards two workgroups a CU (33 x 8192
-// x 8192 in 60, 42, 28, 27 us on 1, 2, 4, 8 slices), and by two where there is one
-// but K is long (256 x 8192 x 8192 in 58 against 63, 512 x 4096 x 4096 in 38
-// against 35).
-int q4_tile_plan(const lm::Q4Args& a, int cus, int* ksplit) {
+// 4096 x 50256 in 66 us against 79). Under two tiles a CU, two teams in a workgroup
+// take K's blocks in turn (512 x 4096 x 4096 in 29 us against 33; 48 x 4096 x 50256
+// f32 in 65 against 66.5), not from there on (2048 x 4096 x 4096 in 88 against 85;
+// 1024 x 4096 x 4096 f32 in 106 against 99). Under one a CU (`few`), workgroups split
+// K too (33 x 8192 x 8192 bf16 in 49, 29, 20, 22 us on 1, 2, 4, 8 slices), and sum
+// their x themselves where they read it in place: the prepared sums' launch costs
+// more (128 x 4096 x 4096 in 16.8 us against 18.8; 1024 rows in 54 against 47).
+struct Q4TilePlan {
+  int config, teams, ksplit;
+  bool few;  // fewer tiles than CUs
+};
+Q4TilePlan q4_tile_plan(const lm::Q4Args& a, int cus) {
   static const int rows[] = {32, 64, 48};
-  int config = a.M <= 32 ? lm::kQ4Tile32x128 : lm::kQ4Tile64x128;
+  Q4TilePlan p{a.M <= 32 ? lm::kQ4Tile32x128 : lm::kQ4Tile64x128, 1, 1, false};
   if (a.M > 32 && a.x_type == lm::kF32 && ((int64_t)a.M + 47) / 48 * 48 < ((int64_t)a.M + 63) / 64 * 64)
-    config = lm::kQ4Tile48x128;
-  const int64_t wgs = ((int64_t)a.M + rows[config] - 1) / rows[config] * (((int64_t)a.N + 127) / 128);
-  check_grid(wgs, 16);
-  if (wgs >= cus)
-    *ksplit = wgs < 2 * (int64_t)cus && a.blocks >= 64 ? 2 * cus / wgs : 1;
-  else
-    *ksplit = (int)std::clamp<int64_t>(2 * cus / wgs, 1, std::clamp(a.blocks / 4, 1, 16));
-  return config;
+    p.config = lm::kQ4Tile48x128;
+  const int64_t wgs = ((int64_t)a.M + rows[p.config] - 1) / rows[p.config] * (((int64_t)a.N + 127) / 128);
+  check_grid(wgs, 8);
+  p.few = wgs < cus;
+  p.teams = wgs < 2 * (int64_t)cus ? 2 : 1;
+  if (p.few) p.ksplit = (int)std::clamp<int64_t>(cus / wgs, 1, std::clamp(a.blocks / 4, 1, 8));
+  return p;
 }
 
 // Even slices of K, none of them empty.
@@ -267,28 +273,30 @@ void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, int scal
     });
     return;
   }
-  const int config = q4_tile_plan(a, cus, &a.ksplit);
+  const Q4TilePlan plan = q4_tile_plan(a, cus);
+  a.ksplit = plan.ksplit;
   q4_slices(a);
   p.factor = zeros ? -1.0f : -8.0f - lm::q4_offset(a.x_type);
   p.xs_ld = (M + 127) / 128 * 128;
   // x itself where the tiles can read it: 16 bits, whole blocks, 16-byte aligned rows.
   const bool copy = !((a.x_type == lm::kBf16 || a.x_type == lm::kF16) && K % 128 == 0 && a.ldx % 8 == 0 &&
                       reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx <= kMostDepth);
-  const size_t sums = aligned((size_t)l.blocks * l.spb * p.xs_ld * sizeof(float));
+  const bool own_sums = !copy && plan.few;
+  const size_t sums = own_sums ? 0 : aligned((size_t)l.blocks * l.spb * p.xs_ld * sizeof(float));
   const size_t copied = copy ? planes : 0;
   const size_t parts = a.ksplit > 1 ? (size_t)a.ksplit * M * N * sizeof(float) : 0;
   device_launch(sums + copied + parts, stream, [&](char* ws, int) {
-    p.xs = reinterpret_cast<float*>(ws);
+    p.xs = own_sums ? nullptr : reinterpret_cast<float*>(ws);
     p.xp = copy ? ws + sums : nullptr;
     a.xs = p.xs, a.xs_ld = p.xs_ld;
     a.xp = copy ? p.xp : a.x, a.ldp = copy ? p.ldp : a.ldx, a.plane = p.plane;
     a.partials = reinterpret_cast<float*>(ws + sums + copied);
-    if (a.blocks > 0) check_hip(lm::launch_q4_prep(p, s), "q4_prep launch");
-    check_hip(lm::launch_q4_tile(a, config, l.spb, zeros, s), "q4_tile launch");
+    if (a.blocks > 0 && !own_sums) check_hip(lm::launch_q4_prep(p, s), "q4_prep launch");
+    check_hip(lm::launch_q4_tile(a, plan.config, l.spb, plan.teams, zeros, s), "q4_tile launch");
     if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
     static const char* const names[] = {"32x128", "64x128", "48x128"};
-    set_plan("q4_prep%s+q4_tile %s tile=%s ksplit=%d%s", copy ? "_copy" : "", type_name(a.x_type), names[config],
-             a.ksplit, a.ksplit > 1 ? " +join" : "");
+    set_plan("%sq4_tile %s tile=%s teams=%d ksplit=%d%s", own_sums ? "" : copy ? "q4_prep_copy+" : "q4_prep+", type_name(a.x_type), names[plan.config],
+             plan.teams, a.ksplit, a.ksplit > 1 ? " +join" : "");
   });
 }
 

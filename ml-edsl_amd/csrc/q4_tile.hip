@@ -1,18 +1,21 @@
 // The 4-bit layer on more than 16 rows: tiles on the matrix cores.
 //
-// A workgroup of 4 waves takes 16 MT rows x 64 NT columns. A wave loads and
-// unpacks the weights of its own columns in registers, a block of 128 k ahead; x
-// and its groups' sums go from memory straight to LDS, a stage ahead, with 16-byte
-// chunks exchanged by row so that reads hit all banks. Each group's accumulators start at the prepared
-// -zero * sum x and are scaled into the 32-bit totals at its end.
+// A workgroup takes 16 MT rows x 64 NT columns by teams of 4 waves; the blocks of 128
+// k go to the teams in turn, whose sums meet in LDS at the end. A wave loads and
+// unpacks the weights of its own columns in registers, a block ahead; x and its
+// groups' sums go from memory straight to LDS, a stage ahead, with 16-byte chunks
+// exchanged by row so that reads hit all banks. Each group's accumulators start at
+// the prepared -zero * sum x and are scaled into the 32-bit totals at its end; with
+// OWN_SUMS a matrix instruction with a constant operand sums x instead.
 //
 // Bound by power and by the matrix cores and vector ALUs together where M is
-// large: 4096^3 in 153 us without zero points and 163 with them, the preparation of
+// large: 4096^3 in 153 us without zero points and 163 with them, the sums of
 // x included (898 and 843 TFLOP/s, 80 and 75 % of what the vendor's bf16 product
 // reaches there), 8192^3 with them in 1098 us (1.0 PFLOP/s, 80 %). Tiles of 128x128
 // and 128x256 (half and a third of the traffic) are no faster, 164 to 172 us, nor
 // are fragments read ahead or a forced order of products and unpacking. With few
-// rows the loads' latency bounds it.
+// rows a block's loads and the launches bound it: 33 x 8192 x 8192 in 20 us, 7 of
+// them the weights' bytes, 5 the join's launch.
 #include "q4.hpp"
 
 namespace edsl {
@@ -35,17 +38,20 @@ __device__ __forceinline__ void to_lds(const void* base, uint32_t offset, void* 
 // Waits for the wave's loads, those to LDS among them (vmcnt 0).
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
-template <bool F16, int PLANES, int MT, int NT, int SPB, bool ZEROS>
-__global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
+template <bool F16, int PLANES, int MT, int NT, int SPB, bool ZEROS, int TEAMS, bool OWN_SUMS>
+__global__ void __launch_bounds__(256 * TEAMS, 2) q4_tile_kernel(Q4Args a) {
   using E = Q4Elem<F16>;
   using V = typename E::V;
   constexpr int BM = 16 * MT, STEPS = 4 / SPB;
   // A stage of x in LDS: SS steps of 32 k, CPR 16-byte chunks a row.
   constexpr int SS = PLANES == 3 ? 2 : 4, CPR = 4 * SS, STAGES = 4 / SS;
   constexpr int ALL = PLANES * BM * CPR, CHUNKS = (ALL + 255) / 256;  // a thread's
-  __shared__ u32x4 lds[2][ALL];
-  __shared__ f32x4 sums[2][SPB * BM / 4];  // a block's sums of x
-  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  __shared__ u32x4 lds_all[TEAMS][2][ALL];
+  __shared__ f32x4 sums_all[TEAMS][2][SPB * BM / 4];  // a block's sums of x
+  const int tid = threadIdx.x % 256, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 256) : 0;
+  auto& lds = lds_all[team];
+  auto& sums = sums_all[team];
   const int64_t tiles = (a.N + 15) / 16;
   const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (int)((tiles + 4 * NT - 1) / (4 * NT));
   const int slice = blockIdx.x / (tiles_m * tiles_n);
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   };
   const auto load_sums = [&](int b, f32x4* to) {
     // 16-byte pieces of SPB runs of BM sums.
-    if (tid < SPB * BM / 4)
+    if (!OWN_SUMS && tid < SPB * BM / 4)
       to_lds(a.xs + (int64_t)b * SPB * a.xs_ld + m0,
              4u * (uint32_t)(tid / (BM / 4) * a.xs_ld + 4 * (tid % (BM / 4))), to + wave * 64);
   };
@@ -105,7 +111,10 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
       }
     }
   };
-  f32x4 sum[MT][NT], acc[MT][NT];
+  f32x4 sum[MT][NT], acc[MT][NT], own[OWN_SUMS ? MT : 1];
+  V minus;  // the constant operand of the sums of x
+#pragma unroll
+  for (int j = 0; j < 8; ++j) minus[j] = -1.0f;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -117,10 +126,14 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
                         f32x4* sums_next) {
     wait_loads();
     __syncthreads();
-    if (stage < STAGES - 1 || b + 1 < b1) load_x(b * STAGES + stage + 1, x_next);
-    if (stage == 0 && b + 1 < b1) {
-      load_sums(b + 1, sums_next);
-      load_w(b + 1, next);
+    if (TEAMS > 1 && b >= b1) return;  // the last turn of a team without a block
+    if (stage < STAGES - 1)
+      load_x(b * STAGES + stage + 1, x_next);
+    else if (b + TEAMS < b1)
+      load_x((b + TEAMS) * STAGES, x_next);
+    if (stage == 0 && b + TEAMS < b1) {
+      load_sums(b + TEAMS, sums_next);
+      load_w(b + TEAMS, next);
     }
 #pragma unroll
     for (int s = 0; s < SS; ++s) {
@@ -132,6 +145,12 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
           for (int t = 0; t < NT; ++t) zero[t] = (PLANES == 3 ? 0.0f : kQ4Offset) + (float)now.zero[t][g];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
+          if constexpr (OWN_SUMS) {
+            own[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[i][t] = own[i];
+            continue;
+          }
           const f32x4 xs = sums_now[g * (BM / 4) + 4 * i + lane / 16];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -156,6 +175,7 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
         for (int i = 0; i < MT; ++i) {
           const int r = p * BM + 16 * i + lane % 16;
           const V x = __builtin_bit_cast(V, x_now[r * CPR + ((4 * s + lane / 16) ^ swizzle(r))]);
+          if constexpr (OWN_SUMS) own[i] = E::mfma(x, minus, own[i]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) acc[i][t] = E::mfma(x, q[t], acc[i][t]);
         }
@@ -163,21 +183,26 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const float scale = q4_scale(now.scale[t][g], a.scale_mask);
+          const float zero = kQ4Offset + (ZEROS ? (float)now.zero[ZEROS ? t : 0][g] : 8.0f);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[i][t][e] = fmaf(acc[i][t][e], scale, sum[i][t][e]);
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (OWN_SUMS) acc[i][t][e] = fmaf(own[i][e], zero, acc[i][t][e]);
+              sum[i][t][e] = fmaf(acc[i][t][e], scale, sum[i][t][e]);
+            }
         }
       }
     }
   };
-  if (b0 < b1) {
-    load_x(b0 * STAGES, lds[0]);
-    load_sums(b0, sums[0]);
-    load_w(b0, now);
+  if (b0 + team < b1) {
+    load_x((b0 + team) * STAGES, lds[0]);
+    load_sums(b0 + team, sums[0]);
+    load_w(b0 + team, now);
   }
-  for (int b = b0; b < b1; ++b) {
-    const int odd = (b - b0) & 1;
+  int odd = 0;
+  for (int first_b = b0; first_b < b1; first_b += TEAMS, odd ^= 1) {
+    const int b = first_b + team;
     if constexpr (STAGES == 1) {
       turn(b, 0, lds[odd], lds[odd ^ 1], sums[odd], sums[odd ^ 1]);
     } else {
@@ -185,6 +210,25 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
       turn(b, 1, lds[1], lds[0], sums[odd], sums[odd ^ 1]);
     }
     now = next;
+  }
+  if constexpr (TEAMS > 1) {
+    // The first team adds the others' sums to its own, in their order.
+    static_assert(MT * NT * 256 <= 2 * ALL, "a team's sums fit its stages of x");
+    __syncthreads();
+    if (team > 0)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) lds[0][(i * NT + t) * 256 + tid] = __builtin_bit_cast(u32x4, sum[i][t]);
+    __syncthreads();
+    if (team > 0) return;
+#pragma unroll
+    for (int other = 1; other < TEAMS; ++other)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          sum[i][t] += __builtin_bit_cast(f32x4, lds_all[other][0][(i * NT + t) * 256 + tid]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -211,30 +255,42 @@ __global__ void __launch_bounds__(256, 2) q4_tile_kernel(Q4Args a) {
   }
 }
 
-template <bool F16, int PLANES, int MT, int NT, int SPB>
-hipError_t launch_tile_zeros(const Q4Args& a, bool zeros, hipStream_t stream) {
+template <bool F16, int PLANES, int MT, int NT, int SPB, bool ZEROS>
+hipError_t launch_tile_teams(const Q4Args& a, int teams, hipStream_t stream) {
   const int64_t tiles = (a.N + 15) / 16;
   const int64_t tm = (a.M + 16 * MT - 1) / (16 * MT), tn = (tiles + 4 * NT - 1) / (4 * NT);
-  const dim3 grid((unsigned)(tm * tn * a.ksplit)), block(256);
-  if (zeros)
-    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, SPB, true>), grid, block, 0, stream, a);
+  const dim3 grid((unsigned)(tm * tn * a.ksplit));
+  if constexpr (PLANES == 1) {
+    if (teams == 2 && !a.xs) {
+      hipLaunchKernelGGL((q4_tile_kernel<F16, 1, MT, NT, SPB, ZEROS, 2, true>), grid, dim3(512), 0, stream, a);
+      return launched();
+    }
+  }
+  if (teams == 2)
+    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, SPB, ZEROS, 2, false>), grid, dim3(512), 0, stream, a);
   else
-    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, SPB, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((q4_tile_kernel<F16, PLANES, MT, NT, SPB, ZEROS, 1, false>), grid, dim3(256), 0, stream, a);
   return launched();
 }
 
+template <bool F16, int PLANES, int MT, int NT, int SPB>
+hipError_t launch_tile_zeros(const Q4Args& a, int teams, bool zeros, hipStream_t stream) {
+  return zeros ? launch_tile_teams<F16, PLANES, MT, NT, SPB, true>(a, teams, stream)
+               : launch_tile_teams<F16, PLANES, MT, NT, SPB, false>(a, teams, stream);
+}
+
 template <bool F16, int PLANES, int MT, int NT>
-hipError_t launch_tile_spb(const Q4Args& a, int spb, bool zeros, hipStream_t stream) {
-  if (spb == 4) return launch_tile_zeros<F16, PLANES, MT, NT, 4>(a, zeros, stream);
-  if (spb == 2) return launch_tile_zeros<F16, PLANES, MT, NT, 2>(a, zeros, stream);
-  return launch_tile_zeros<F16, PLANES, MT, NT, 1>(a, zeros, stream);
+hipError_t launch_tile_spb(const Q4Args& a, int spb, int teams, bool zeros, hipStream_t stream) {
+  if (spb == 4) return launch_tile_zeros<F16, PLANES, MT, NT, 4>(a, teams, zeros, stream);
+  if (spb == 2) return launch_tile_zeros<F16, PLANES, MT, NT, 2>(a, teams, zeros, stream);
+  return launch_tile_zeros<F16, PLANES, MT, NT, 1>(a, teams, zeros, stream);
 }
 
 template <bool F16, int PLANES>
-hipError_t launch_tile_config(const Q4Args& a, int config, int spb, bool zeros, hipStream_t stream) {
-  if (config == kQ4Tile32x128) return launch_tile_spb<F16, PLANES, 2, 2>(a, spb, zeros, stream);
-  if (config == kQ4Tile64x128) return launch_tile_spb<F16, PLANES, 4, 2>(a, spb, zeros, stream);
-  if constexpr (PLANES == 3) return launch_tile_spb<F16, 3, 3, 2>(a, spb, zeros, stream);
+hipError_t launch_tile_config(const Q4Args& a, int config, int spb, int teams, bool zeros, hipStream_t stream) {
+  if (config == kQ4Tile32x128) return launch_tile_spb<F16, PLANES, 2, 2>(a, spb, teams, zeros, stream);
+  if (config == kQ4Tile64x128) return launch_tile_spb<F16, PLANES, 4, 2>(a, spb, teams, zeros, stream);
+  if constexpr (PLANES == 3) return launch_tile_spb<F16, 3, 3, 2>(a, spb, teams, zeros, stream);
   return hipErrorInvalidValue;
 }
 
@@ -367,10 +423,10 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(Q4PackArgs a) {
 
 }  // namespace
 
-hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, bool zeros, hipStream_t stream) {
-  if (a.x_type == kF16) return launch_tile_config<true, 1>(a, config, spb, zeros, stream);
-  if (a.x_type == kF32) return launch_tile_config<false, 3>(a, config, spb, zeros, stream);
-  return launch_tile_config<false, 1>(a, config, spb, zeros, stream);
+hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, int teams, bool zeros, hipStream_t stream) {
+  if (a.x_type == kF16) return launch_tile_config<true, 1>(a, config, spb, teams, zeros, stream);
+  if (a.x_type == kF32) return launch_tile_config<false, 3>(a, config, spb, teams, zeros, stream);
+  return launch_tile_config<false, 1>(a, config, spb, teams, zeros, stream);
 }
 
 hipError_t launch_q4_prep(const Q4PrepArgs& a, hipStream_t stream) {

@@ -95,7 +95,7 @@ def layer(M, K, N, group, x_dtype, y_dtype=None, scales=F32, zeros=True, epi="no
     (1, 1, 1, 32), (1, 128, 16, 128), (2, 31, 17, 32), (1, 1000, 100, 64), (16, 257, 33, 128), (5, 4096, 130, 128),
     (3, 2050, 520, 256), (16, 640, 4200, 64), (1, 384, 20000, 32), (17, 100, 20, 32), (31, 300, 129, 64),
     (33, 1024, 300, 128), (64, 129, 70, 32), (65, 512, 1000, 256), (130, 1000, 257, 64), (300, 384, 2100, 128),
-    (513, 256, 4100, 32)])
+    (513, 256, 4100, 32), (1100, 300, 4100, 64), (1060, 384, 4097, 32), (2000, 512, 2200, 128)])
 def test_sizes(M, K, N, group, x_dtype):
     layer(M, K, N, group, x_dtype, zeros=(M + N) % 2 == 0, pad=N % 3, seed=M + K)
 
@@ -118,8 +118,10 @@ def test_epilogues(epi, y_dtype, M):
 
 def test_plans():
     for M, K, N, what in [(1, 16384, 64, "q4_small bf16 cols=16 ksplit=4 +join"), (16, 512, 8192, "cols=32 ksplit=1"),
-                          (20, 512, 512, "q4_small bf16 cols=16 ksplit=1"), (20, 128, 20000, "tile=32x128"), (64, 4096, 8192, "tile=64x128 ksplit=8"),
-                          (2048, 128, 4096, "q4_prep+q4_tile bf16 tile=64x128 ksplit=1"),
+                          (20, 512, 512, "q4_small bf16 cols=16 ksplit=1"), (20, 128, 20000, "q4_tile bf16 tile=32x128 teams=2 ksplit=1"),
+                          (64, 4096, 8192, "q4_tile bf16 tile=64x128 teams=2 ksplit=4 +join"),
+                          (512, 128, 4096, "q4_prep+q4_tile bf16 tile=64x128 teams=2 ksplit=1"),
+                          (2048, 128, 4096, "q4_prep+q4_tile bf16 tile=64x128 teams=1 ksplit=1"),
                           (2048, 130, 4096, "q4_prep_copy+q4_tile")]:
         layer(M, K, N, 128, BF16)
         assert what in last_plan(), last_plan()
