@@ -497,10 +497,11 @@ __global__ void __launch_bounds__(1024) dweight_kernel(const float* partials, in
 }
 
 // Threads of a row, 0 for rows of any length: a vector each, two of f32 (4096 x
-// 4096 f32 in 52 us, with one in 59).
+// 4096 f32 in 52 us, with one in 59); twice that of the longest rows, though four of f32 spill (2048 x
+// 16384 in 135 us, read twice in 173).
 int backward_threads(int64_t N, int type) {
   int64_t vecs = (N * type_bytes(type) + 15) / 16;
-  if (vecs > 2048) return 0;
+  if (vecs > (type == kF32 ? 4096 : 2048)) return 0;
   if (type == kF32) vecs = (vecs + 1) / 2;
   return vecs <= 64 ? 64 : vecs <= 128 ? 128 : vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
 }
@@ -527,7 +528,7 @@ hipError_t launch_backward(const NormBackwardArgs& a, hipStream_t stream) {
         if (vecs <= 1024 * NV)
           launch_backward_rows<T, 1024, NV>(a, stream);
         else
-          launch_backward_rows<T, 1024, 2>(a, stream);
+          launch_backward_rows<T, 1024, 2 * NV>(a, stream);
         break;
       default:
         hipLaunchKernelGGL((rms_norm_backward_long_kernel<T>), dim3(a.groups), dim3(1024), 0, stream, a);

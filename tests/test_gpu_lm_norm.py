@@ -109,7 +109,7 @@ def test_outputs_in_the_inputs_memory(N):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("M,N", SIZES + [(1500, 130), (3000, 9)])
+@pytest.mark.parametrize("M,N", SIZES + [(1500, 130), (3000, 9), (300, 16384), (3, 12001)])
 def test_backward(M, N, dtype):
     x, dy, dh = rows(M, N, dtype, 1, 10), rows(M, N, dtype, 0, 11), rows(M, N, dtype, 2, 12)
     w = (1 + 0.2 * torch.randn(N, generator=torch.Generator().manual_seed(13))).to(dtype).cuda()
