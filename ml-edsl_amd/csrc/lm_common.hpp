@@ -75,19 +75,25 @@ struct MaxNan {
   static __device__ __forceinline__ float of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 };
 
-// The combination over a wave's 64 lanes: lanes 1 and 2 apart, mirrored in 8 and
-// in 16 by DPP, then 16 and 32 apart. Every lane has the first one's, bit for
-// bit: its own may differ where the compiler fuses the caller's product into its
-// side of the first sum.
-template <typename Op>
-__device__ __forceinline__ float wave_all(float v) {
+// The combination over runs of LANES lanes (16, 32, 64): lanes 1 and 2 apart,
+// mirrored in 8 and in 16 by DPP, then 16 and 32 apart. Every lane of a run has the
+// same bits: both sides of each step add the same two values, which holds as long
+// as the compiler does not fuse the caller's product into its side of the first.
+template <typename Op, int LANES>
+__device__ __forceinline__ float lanes_all(float v) {
+  asm("" : "+v"(v));
   v = Op::of(v, dpp<0xB1>(v));
   v = Op::of(v, dpp<0x4E>(v));
   v = Op::of(v, dpp<0x141>(v));
   v = Op::of(v, dpp<0x140>(v));
-  v = Op::of(v, __shfl_xor(v, 16));
-  v = Op::of(v, __shfl_xor(v, 32));
-  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  if constexpr (LANES > 16) v = Op::of(v, __shfl_xor(v, 16));
+  if constexpr (LANES > 32) v = Op::of(v, __shfl_xor(v, 32));
+  return v;
+}
+// Over the wave, in a scalar register.
+template <typename Op>
+__device__ __forceinline__ float wave_all(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, lanes_all<Op, 64>(v))));
 }
 
 // A grid of n workgroups along x and y: a launch takes less than 2^32 threads along

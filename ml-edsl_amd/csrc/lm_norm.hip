@@ -29,8 +29,13 @@ enum : int { kOutSame = 0, kOutI8 = 1, kOutE4m3 = 2 };
 // holds two floats a wave; a barrier precedes its next use.
 template <int TPR>
 __device__ __forceinline__ void row_reduce(float& a, float& b, float* lds, bool want_b) {
-  a = wave_all<Sum>(a);
-  if (want_b) b = wave_all<MaxNan>(b);
+  if constexpr (TPR < 64) {
+    a = lanes_all<Sum, TPR>(a);
+    if (want_b) b = lanes_all<MaxNan, TPR>(b);
+  } else {
+    a = wave_all<Sum>(a);
+    if (want_b) b = wave_all<MaxNan>(b);
+  }
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     const int wave = threadIdx.x / 64;
@@ -154,7 +159,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_kernel(NormArg
   constexpr int VEC = kVec<T>, BLOCK = TPR < 256 ? 256 : TPR, ROWS = BLOCK / TPR;
   __shared__ float lds[2 * BLOCK / 64];
   const int64_t row = (int64_t)block_of() * ROWS + threadIdx.x / TPR;
-  if (row >= a.M) return;  // by waves where a row is one wave's, without barriers, else by workgroups
+  if (row >= a.M) return;  // by lanes or waves where they hold a row, without barriers, else by workgroups
   const int t = threadIdx.x % TPR;
   const bool wf32 = a.weight_type == kF32;
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -266,7 +271,9 @@ hipError_t launch_row(const NormArgs& a, hipStream_t stream) {
   return launched();
 }
 
-// Threads of a row x vectors of a thread. More threads rather than vectors from 513
+// Threads of a row x vectors of a thread. Short rows share a wave (262144 x 128 bf16
+// in 22 us on 16 threads each against 57 on 64) or take one without a barrier (65536
+// x 1024 in 38 on 64x2 against 57 on 256x1). More threads rather than vectors from 513
 // vectors on (4096 x 8192 bf16 to 8 bits 51 us on 512x2 against 56 on 256x4; 2048 x
 // 16384 49 on 1024x2 against 55 on 1024x4), and below where a CU has one row at most
 // (`few`; 256 x 4096 bf16 3.7 against 4.1), but not for many (2001 x 2001 f32 7.6 on
@@ -274,7 +281,10 @@ hipError_t launch_row(const NormArgs& a, hipStream_t stream) {
 template <typename T, int OUT>
 hipError_t launch_norm(const NormArgs& a, bool few, hipStream_t stream, const char** plan) {
   const int64_t vecs = (a.N + kVec<T> - 1) / kVec<T>;
+  if (vecs <= 16) return *plan = "row=16x1", launch_row<T, OUT, 16, 1>(a, stream);
+  if (vecs <= 32) return *plan = "row=32x1", launch_row<T, OUT, 32, 1>(a, stream);
   if (vecs <= 64) return *plan = "row=64x1", launch_row<T, OUT, 64, 1>(a, stream);
+  if (vecs <= 128) return *plan = "row=64x2", launch_row<T, OUT, 64, 2>(a, stream);
   if (vecs <= 256) return *plan = "row=256x1", launch_row<T, OUT, 256, 1>(a, stream);
   if (vecs <= 512 && few) return *plan = "row=512x1", launch_row<T, OUT, 512, 1>(a, stream);
   if (vecs <= 512) return *plan = "row=256x2", launch_row<T, OUT, 256, 2>(a, stream);
@@ -367,7 +377,10 @@ __global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackward
     keep_packed(now.h);
     // Two buffers in turn: the barrier of the next row stands between the reads
     // of one and its next writes.
-    dot = wave_all<Sum>(dot);
+    if constexpr (TPR < 64)
+      dot = lanes_all<Sum, TPR>(dot);
+    else
+      dot = wave_all<Sum>(dot);
     if constexpr (WAVES > 1) {
       if (t % 64 == 0) lds[turn][threadIdx.x / 64] = dot;
       __syncthreads();
@@ -498,12 +511,12 @@ __global__ void __launch_bounds__(1024) dweight_kernel(const float* partials, in
 
 // Threads of a row, 0 for rows of any length: a vector each, two of f32 (4096 x
 // 4096 f32 in 52 us, with one in 59); twice that of the longest rows, though four of f32 spill (2048 x
-// 16384 in 135 us, read twice in 173).
+// 16384 in 135 us, read twice in 173). 65536 x 128 bf16 in 23.5 us, 42 on 64 threads.
 int backward_threads(int64_t N, int type) {
   int64_t vecs = (N * type_bytes(type) + 15) / 16;
   if (vecs > (type == kF32 ? 4096 : 2048)) return 0;
   if (type == kF32) vecs = (vecs + 1) / 2;
-  return vecs <= 64 ? 64 : vecs <= 128 ? 128 : vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
+  return vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 ? 64 : vecs <= 128 ? 128 : vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
 }
 
 template <typename T, int TPR, int NV>
@@ -520,6 +533,8 @@ hipError_t launch_backward(const NormBackwardArgs& a, hipStream_t stream) {
   const int64_t vecs = (a.N + kVec<T> - 1) / kVec<T>;
   if (a.M > 0) {
     switch (backward_threads(a.N, a.type)) {
+      case 16: launch_backward_rows<T, 16, NV>(a, stream); break;
+      case 32: launch_backward_rows<T, 32, NV>(a, stream); break;
       case 64: launch_backward_rows<T, 64, NV>(a, stream); break;
       case 128: launch_backward_rows<T, 128, NV>(a, stream); break;
       case 256: launch_backward_rows<T, 256, NV>(a, stream); break;

@@ -38,7 +38,7 @@ def rows(M, N, dtype, pad=0, seed=0, scale=1.0):
     return t
 
 
-SIZES = [(1, 1), (3, 7), (5, 64), (2, 257), (7, 512), (4, 1000), (3, 2001), (2, 4096), (3, 8200), (2, 16384),
+SIZES = [(1, 1), (3, 7), (5, 64), (37, 128), (41, 250), (2, 257), (7, 512), (4, 1000), (3, 2001), (2, 4096), (3, 8200), (2, 16384),
          (2, 32771), (1, 70001)]
 
 
