@@ -8,8 +8,8 @@
 // Bound by memory: about one operation a byte. A row is read once and held in
 // registers between the sum and the output. 4096 x 8192 bf16 with a residual to 8
 // bits: 44 us, 5.3 TB/s; a copy of 1 GiB reaches 5.0. The backward pass reads dy, h
-// and dh once and leaves one row of partials a CU: 4096 x 4096 bf16 in 33 us, 4.1
-// TB/s, the join of the partials (3 us) included. One row takes 4 us, a launch's time.
+// and dh once and leaves one row of partials a CU: 4096 x 4096 bf16 in 30 us, 4.5
+// TB/s, the join of the partials (4 us) included. One row takes 4 us, a launch's time.
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -307,18 +307,22 @@ hipError_t launch_norm_out(const NormArgs& a, bool few, hipStream_t stream, cons
 // The backward pass. A workgroup of 1024 threads is 1024 / TPR teams with a row
 // each; a thread keeps the same NV vectors of columns in every row, its part of
 // dweight in registers, and the teams join theirs through LDS at the end, so that
-// there is one row of partials a CU. Where the registers hold it, the next row is
-// on its way while one is summed. WF32: the weight is f32 and x is not.
-template <typename T, int TPR, int NV, bool WF32>
+// there is one row of partials a CU. Where the registers hold it, the next row is on
+// its way while one is summed, in registers of its own and by the same loads every
+// turn, whatever the row: a load under a branch, or a copied register, would wait
+// for all of them (4096 x 4096 bf16 30 us against 33, 4096 x 8192 53 against 59).
+// WF32: the weight is f32 and x is not. DH: dh is there. WHOLE: rows are whole
+// vectors.
+template <typename T, int TPR, int NV, bool WF32, bool DH, bool WHOLE>
 __global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackwardArgs a) {
   constexpr int VEC = kVec<T>, TEAMS = 1024 / TPR, WAVES = TPR / 64;
-  constexpr bool AHEAD = NV * VEC <= 8;  // registers for the next row
+  constexpr int DEPTH = NV * VEC > 8 ? 1 : 2;  // rows in registers; three were no faster
   using Vals = Packed<T, VEC>;
   using W = std::conditional_t<WF32, float, T>;
   __shared__ float lds[2][16];
   __shared__ float joined[TEAMS > 1 ? TPR * NV * VEC : 1];
   const int team = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  Packed<W, VEC> w[NV];
+  Packed<W, VEC> w[NV];  // zeros past the row's end
   if constexpr (WF32) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackward
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[j][e] = 0.0f;
   struct Row {
-    Vals dy[NV], h[NV], dh[NV];
+    Vals dy[NV], h[NV], dh[DH ? NV : 1];
     float rstd;
   };
   // Rows stay packed: opened for the sum and again for the gradient, they take
@@ -345,23 +349,30 @@ __global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackward
       v[j] = __builtin_bit_cast(Vals, raw);
     }
   };
+  // Vectors past a whole row's end repeat its last one: their weights are zero.
+  const auto load_vectors = [&](const void* p, int64_t at, auto& v) {
+    const T* const row = static_cast<const T*>(p) + at;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i0 = (j * TPR + t) * VEC;
+      if constexpr (WHOLE)
+        v[j] = load_packed<T, VEC>(row + (i0 < (int)a.N ? i0 : (int)a.N - VEC));
+      else
+        v[j] = load_guarded<T, VEC>(row, i0, a.N);
+    }
+  };
   const auto load = [&](int64_t row, Row& r) {
-    if (row >= a.M) row = a.M - 1;  // not used: the last turn of a team without a row
-    load_row<T, TPR, NV>(static_cast<const T*>(a.dy) + row * a.lddy, t, a.N, r.dy);
-    load_row<T, TPR, NV>(static_cast<const T*>(a.h) + row * a.ldh, t, a.N, r.h);
-    if (a.dh) load_row<T, TPR, NV>(static_cast<const T*>(a.dh) + row * a.lddh, t, a.N, r.dh);
+    if (row >= a.M) row = a.M - 1;  // not used
+    load_vectors(a.dy, row * a.lddy, r.dy);
+    load_vectors(a.h, row * a.ldh, r.h);
+    if constexpr (DH) load_vectors(a.dh, row * a.lddh, r.dh);
     r.rstd = a.rstd[row];
   };
   const int64_t step = (int64_t)a.groups * TEAMS;
   int64_t first = (int64_t)blockIdx.x * TEAMS;  // the first team's row; every team turns as often
-  Row now, next;
-  if (AHEAD && first < a.M) load(first + team, now);
-  for (int turn = 0; first < a.M; first += step, turn ^= 1) {
+  int turn = 0;
+  const auto one = [&](Row& now) {
     const int64_t row = first + team;
-    if (!AHEAD)
-      load(row, now);
-    else if (first + step < a.M)
-      load(row + step, next);
     const float rstd = now.rstd;
     const bool in = row < a.M;
     float dot = 0.0f;
@@ -387,6 +398,7 @@ __global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackward
       dot = 0.0f;
 #pragma unroll
       for (int i = 0; i < WAVES; ++i) dot += lds[turn][team * WAVES + i];
+      turn ^= 1;
     }
     const float mean = dot / (float)a.N;
     T* const pdx = static_cast<T*>(a.dx) + row * a.lddx;
@@ -399,12 +411,29 @@ __global__ void __launch_bounds__(1024, 4) rms_norm_backward_kernel(NormBackward
       for (int e = 0; e < VEC; ++e) {
         const float xh = (float)now.h[j].v[e] * rstd;
         float d = rstd * fmaf(-xh, mean, (float)now.dy[j].v[e] * (float)w[j].v[e]);
-        if (a.dh) d += (float)now.dh[j].v[e];
+        if constexpr (DH) d += (float)now.dh[j].v[e];
         r.v[e] = (T)d;
       }
       store_guarded<T, VEC>(pdx, i0, a.N, r);
     }
-    if (AHEAD) now = next;
+  };
+  Row rows[DEPTH];
+  if (first < a.M) {
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) load(first + d * step + team, rows[d]);
+    bool more = true;
+    while (more) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        if (more) {
+          load(first + (DEPTH - 1) * step + team, rows[(d + DEPTH - 1) % DEPTH]);
+          __builtin_amdgcn_sched_barrier(0);
+          one(rows[d]);
+          first += step;
+          more = first < a.M;
+        }
+      }
+    }
   }
   if (!a.dweight) return;
   if constexpr (TEAMS > 1) {
@@ -511,7 +540,7 @@ __global__ void __launch_bounds__(1024) dweight_kernel(const float* partials, in
 
 // Threads of a row, 0 for rows of any length: a vector each, two of f32 (4096 x
 // 4096 f32 in 52 us, with one in 59); twice that of the longest rows, though four of f32 spill (2048 x
-// 16384 in 135 us, read twice in 173). 65536 x 128 bf16 in 23.5 us, 42 on 64 threads.
+// 16384 in 142 us, read twice in 173). 65536 x 128 bf16 in 22 us, 42 on 64 threads.
 int backward_threads(int64_t N, int type) {
   int64_t vecs = (N * type_bytes(type) + 15) / 16;
   if (vecs > (type == kF32 ? 4096 : 2048)) return 0;
@@ -519,12 +548,22 @@ int backward_threads(int64_t N, int type) {
   return vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 64 ? 64 : vecs <= 128 ? 128 : vecs <= 256 ? 256 : vecs <= 512 ? 512 : 1024;
 }
 
+template <typename T, int TPR, int NV, bool WF32, bool DH>
+void launch_backward_whole(const NormBackwardArgs& a, hipStream_t stream) {
+  if (a.N % kVec<T> == 0)
+    hipLaunchKernelGGL((rms_norm_backward_kernel<T, TPR, NV, WF32, DH, true>), dim3(a.groups), dim3(1024), 0, stream, a);
+  else
+    hipLaunchKernelGGL((rms_norm_backward_kernel<T, TPR, NV, WF32, DH, false>), dim3(a.groups), dim3(1024), 0, stream, a);
+}
+
 template <typename T, int TPR, int NV>
 void launch_backward_rows(const NormBackwardArgs& a, hipStream_t stream) {
   if (sizeof(T) != 4 && a.weight_type == kF32)
-    hipLaunchKernelGGL((rms_norm_backward_kernel<T, TPR, NV, sizeof(T) != 4>), dim3(a.groups), dim3(1024), 0, stream, a);
+    a.dh ? launch_backward_whole<T, TPR, NV, sizeof(T) != 4, true>(a, stream)
+         : launch_backward_whole<T, TPR, NV, sizeof(T) != 4, false>(a, stream);
   else
-    hipLaunchKernelGGL((rms_norm_backward_kernel<T, TPR, NV, false>), dim3(a.groups), dim3(1024), 0, stream, a);
+    a.dh ? launch_backward_whole<T, TPR, NV, false, true>(a, stream)
+         : launch_backward_whole<T, TPR, NV, false, false>(a, stream);
 }
 
 template <typename T>
