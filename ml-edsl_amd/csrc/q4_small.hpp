@@ -217,7 +217,8 @@ __global__ void __launch_bounds__(64 * kSmallWaves, (kSmallOccupancy<XT, NT, MT,
   __shared__ u32x4 lds[BYTES / 16];  // the waves' pieces, then their sums
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int tiles = (a.N + 15) / 16;
-  const int first = blockIdx.x * NT, slice = blockIdx.y;
+  const int first = (int)(blockIdx.z * gridDim.x + blockIdx.x) * NT, slice = blockIdx.y;
+  if (first >= tiles) return;  // whole workgroups
   // The last workgroup's tiles may reach past the end: it repeats the last ones
   // and stores each column once.
   const int tile = first + NT <= tiles ? first : tiles - NT;
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(64 * kSmallWaves, (kSmallOccupancy<XT, NT, MT,
 template <int XT, int NT, int MT>
 hipError_t launch_small_spb(const Q4Args& a, int spb, hipStream_t stream) {
   const int tiles = (a.N + 15) / 16;
-  const dim3 grid((unsigned)((tiles + NT - 1) / NT), (unsigned)a.ksplit), block(64 * kSmallWaves);
+  const dim3 columns = grid_of((tiles + NT - 1) / NT), block(64 * kSmallWaves);
+  const dim3 grid(columns.x, (unsigned)a.ksplit, columns.y);
   if (spb == 4)
     hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 4>), grid, block, 0, stream, a);
   else if (spb == 2)

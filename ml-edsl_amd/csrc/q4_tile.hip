@@ -54,9 +54,11 @@ __global__ void __launch_bounds__(256 * TEAMS, 2) q4_tile_kernel(Q4Args a) {
   auto& sums = sums_all[team];
   const int64_t tiles = (a.N + 15) / 16;
   const int tiles_m = (a.M + BM - 1) / BM, tiles_n = (int)((tiles + 4 * NT - 1) / (4 * NT));
-  const int slice = blockIdx.x / (tiles_m * tiles_n);
+  const int block = (int)block_of();
+  const int slice = block / (tiles_m * tiles_n);
+  if (slice >= a.ksplit) return;  // whole workgroups
   int tm, tn;
-  tile_coords(blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
+  tile_coords(block % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
   const int64_t first = ((int64_t)tn * 4 + wave) * NT;
   const int m0 = tm * BM;
   const int b0 = slice * a.slice_blocks, b1 = min(a.blocks, b0 + a.slice_blocks);
@@ -259,7 +261,7 @@ template <bool F16, int PLANES, int MT, int NT, int SPB, bool ZEROS>
 hipError_t launch_tile_teams(const Q4Args& a, int teams, hipStream_t stream) {
   const int64_t tiles = (a.N + 15) / 16;
   const int64_t tm = (a.M + 16 * MT - 1) / (16 * MT), tn = (tiles + 4 * NT - 1) / (4 * NT);
-  const dim3 grid((unsigned)(tm * tn * a.ksplit));
+  const dim3 grid = grid_of(tm * tn * a.ksplit);
   if constexpr (PLANES == 1) {
     if (teams == 2 && !a.xs) {
       hipLaunchKernelGGL((q4_tile_kernel<F16, 1, MT, NT, SPB, ZEROS, 2, true>), grid, dim3(512), 0, stream, a);
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(256) q4_join_kernel(Q4Args a) {
 __global__ void __launch_bounds__(256) q4_pack_kernel(Q4PackArgs a) {
   constexpr int PITCH = 68;  // bytes of a row in LDS
   __shared__ uint8_t q[128 * PITCH];
-  const int64_t first = 4 * (blockIdx.x / a.layout.blocks), block = blockIdx.x % a.layout.blocks;
+  const int64_t first = 4 * (block_of() / a.layout.blocks), block = block_of() % a.layout.blocks;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   {
     const int c = threadIdx.x % 16 * 4;
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(Q4PackArgs a) {
   reinterpret_cast<u32x4*>(a.packed + (tile * a.layout.blocks + block) * 1024)[lane] = words;
   // Its scales and zero points, by the first block of each group.
   const int spb = a.layout.spb, bps = a.layout.blocks_per_scale;
-  if (!a.zeros && blockIdx.x == 0 && threadIdx.x < 16) a.packed[a.layout.zeros_at + threadIdx.x] = 8;
+  if (!a.zeros && block_of() == 0 && threadIdx.x < 16) a.packed[a.layout.zeros_at + threadIdx.x] = 8;
   if (block % bps != 0 || lane >= 16 * spb) return;
   const int c = lane / spb, g = lane % spb;
   const int64_t col = 16 * tile + c, sb = block / bps, group = sb * spb + g, groups = (a.K + a.group - 1) / a.group;
@@ -449,8 +451,7 @@ hipError_t launch_q4_join(const Q4Args& a, hipStream_t stream) {
 
 hipError_t launch_q4_pack(const Q4PackArgs& a, hipStream_t stream) {
   if (a.layout.blocks == 0 || a.layout.tiles_n == 0) return hipSuccess;
-  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)((a.layout.tiles_n + 3) / 4 * a.layout.blocks)), dim3(256), 0,
-                     stream, a);
+  hipLaunchKernelGGL(q4_pack_kernel, grid_of((a.layout.tiles_n + 3) / 4 * a.layout.blocks), dim3(256), 0, stream, a);
   return launched();
 }
 

@@ -149,3 +149,33 @@ def test_q4_of_large_weights(M):
     lm.q4_dense_launch(X, W, None, Y)
     cols = torch.tensor([0, 1, N // 2, 2 ** 20 - 1, 2 ** 20, N - 17, N - 1], device="cuda")
     q4_check(Y[:, cols], X, q[:, cols], s[:, cols], group)
+
+
+# More threads than a launch takes along one axis (2^32).
+def test_norm_backward_of_a_row_of_many_columns():
+    N = 2 ** 26 + 21
+    g = torch.Generator("cuda").manual_seed(3)
+    dy, h = (torch.empty(1, N, device="cuda").normal_(generator=g) for _ in range(2))
+    w, rstd = torch.ones(N, device="cuda"), torch.ones(1, device="cuda")
+    dX, dw = torch.empty_like(dy), torch.full((N,), float("nan"), device="cuda")
+    lm.rms_norm_backward_launch(dy, h, w, rstd, dX, dw)
+    assert torch.equal(dw, (dy * h)[0])  # one row, rstd 1: the rounded product
+
+
+def test_q4_of_many_columns():
+    K, N, group = 1, 2 ** 30, 128  # 2^26 tiles of columns, 6.9e10 bytes of packed weights
+    q, s = q4_weights(K, N, group)
+    W = lm.q4_pack(q, s, group_size=group)
+    X, Y = normal(1, K, dtype=BF16).cuda(), torch.full((1, N), float("nan"), dtype=BF16, device="cuda")
+    lm.q4_dense_launch(X, W, None, Y)
+    cols = torch.tensor([0, 1, N // 2 - 1, N // 2, 2 ** 29 + 2 ** 24, N - 17, N - 1], device="cuda")
+    q4_check(Y[:, cols], X, q[:, cols], s[:, cols], group)
+    assert not bool(Y.isnan().any())
+
+
+def test_q4_without_depth_of_many_rows():
+    M, N = 2 ** 30, 1  # 2^24 tiles of rows; no element of X is there: Y is the bias
+    W = lm.q4_pack(torch.empty(0, N, dtype=torch.uint8, device="cuda"), torch.empty(0, N, device="cuda"))
+    Y = torch.full((M, N), float("nan"), dtype=BF16, device="cuda")
+    lm.q4_dense_launch(torch.empty(M, 0, dtype=BF16, device="cuda"), W, torch.full((N,), 1.5, device="cuda"), Y, 1)
+    assert bool((Y == 1.5).all())
