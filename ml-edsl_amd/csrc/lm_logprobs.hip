@@ -12,7 +12,7 @@
 // Bound by memory: a logit is read once, into registers, where its workgroup
 // finds the maximum, the sums and the alternatives. Second come the vector ALUs,
 // some seven operations and an exponential an element: 2048 x 50256 in bf16 46 us
-// (4.4 TB/s), with five alternatives 48, in f32 70 (5.9 TB/s). The gradient of 2048
+// (4.5 TB/s), with five alternatives 47, in f32 70 (5.9 TB/s). The gradient of 2048
 // x 50256 bf16 logits takes 71 us (5.8 TB/s). One row of 50256 takes 6.1 us, with
 // eight alternatives 8.2: one workgroup's latency.
 //
