@@ -177,11 +177,23 @@ size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // 8192 x 8192 in 9.0 against 9.6); and how many workgroups split K, whose sums
 // take a second kernel: up to four where CUs would be idle, from K = 16384 on (1
 // x 16384 x 1024 in 8.1 us against 9.7 unsplit; 1 x 8192 x 1024 in 6.4 unsplit
-// against 7.2).
-void q4_small_plan(const lm::Q4Args& a, int cus, int* nt, int* ksplit) {
+// against 7.2). Eight waves of a workgroup split K's blocks, but four where there
+// are no two for each (1 x 1024 x 32064 bf16 in 6.4 us, on eight 9.7), in very wide
+// layers (1 x 4096 x 50176 in 26.5, on eight 28.3; but 16 x 8192 x 20000 in 22.9 and
+// 22.6), and for f32, where a CU holds one workgroup of eight (1 x 4096 x 50176 in
+// 45, on eight 58); and two for up to four blocks of a very wide layer (1 x 448 x
+// 50176 in 7.6, on four 9.4, on eight 13.3; but 16 x 448 x 32064 in 6.9 and 6.5).
+void q4_small_plan(const lm::Q4Args& a, int cus, int* nt, int* waves, int* ksplit) {
   const int64_t tiles = (a.N + 15) / 16;
   *nt = tiles > cus ? 2 : 1;
   const int64_t wgs = (tiles + *nt - 1) / *nt;
+  *waves = 8;
+  if (*nt == 2) {
+    if (a.blocks <= 4 && wgs > 4 * (int64_t)cus)
+      *waves = 2;
+    else if (a.blocks <= 8 || (a.x_type == lm::kF32 && wgs > cus) || wgs > 3 * (int64_t)cus)
+      *waves = 4;
+  }
   *ksplit = a.blocks >= 128 ? (int)std::clamp<int64_t>(cus / wgs, 1, 4) : 1;
 }
 
@@ -255,21 +267,23 @@ void q4_dense(lm::Q4Args a, int64_t M, int64_t N, int64_t K, int group, int scal
   p.ldp = l.blocks * 128, p.plane = M * p.ldp;
   const size_t planes = aligned((size_t)(a.x_type == lm::kF32 ? 3 : 1) * p.plane * 2);
   if (q4_small_takes(a, cus)) {
-    int nt;
-    q4_small_plan(a, cus, &nt, &a.ksplit);
+    int nt, waves;
+    q4_small_plan(a, cus, &nt, &waves, &a.ksplit);
     q4_slices(a);
     const size_t bytes = a.ksplit > 1 ? (size_t)a.ksplit * a.M * a.N * sizeof(float) : 0;
     device_launch(bytes, stream, [&](char* ws, int) {
       a.partials = reinterpret_cast<float*>(ws);
-      hipError_t (*const launch)(const lm::Q4Args&, int, int, hipStream_t) =
+      hipError_t (*const launch)(const lm::Q4Args&, int, int, int, hipStream_t) =
           a.x_type == lm::kF32    ? lm::launch_q4_small<lm::kF32>
           : a.x_type == lm::kBf16 ? lm::launch_q4_small<lm::kBf16>
           : a.x_type == lm::kF16  ? lm::launch_q4_small<lm::kF16>
           : a.x_type == lm::kI8   ? lm::launch_q4_small<lm::kI8>
                                   : lm::launch_q4_small<lm::kE4m3>;
-      check_hip(launch(a, nt, l.spb, s), "q4_small launch");
+      check_hip(launch(a, nt, waves, l.spb, s), "q4_small launch");
       if (a.ksplit > 1) check_hip(lm::launch_q4_join(a, s), "q4_join launch");
-      set_plan("q4_small %s cols=%d ksplit=%d%s", type_name(a.x_type), 16 * nt, a.ksplit, a.ksplit > 1 ? " +join" : "");
+      static const char* const fewer[] = {"", "", " waves=2", "", " waves=4"};
+      set_plan("q4_small %s cols=%d ksplit=%d%s%s", type_name(a.x_type), 16 * nt, a.ksplit,
+               a.ksplit > 1 ? " +join" : "", waves < 8 ? fewer[waves] : "");
     });
     return;
   }

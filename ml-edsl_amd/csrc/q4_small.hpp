@@ -1,8 +1,8 @@
 // The 4-bit layer on up to 32 rows: the weights' bytes are the time.
 //
-// A workgroup of 8 waves takes NT tiles of 16 columns; its waves split K by
-// blocks of 128 in turn, so that together they read 8 KB runs of a tile, and
-// their sums meet in LDS. A wave's 16-byte load of a lane is its operand for four
+// A workgroup of 8 waves (4 or 2 of wide layers) takes NT tiles of 16 columns; its
+// waves split K by blocks of 128 in turn, so that together they read 8 KB runs of a
+// tile, and their sums meet in LDS. A wave's 16-byte load of a lane is its operand for four
 // matrix instructions. x comes from the caches in whole lines, 16 bytes of a row
 // to a lane, and takes operand order through a few KB of LDS that are the wave's
 // own (no barrier): loaded in operand order, where neighbouring lanes are rows,
@@ -22,8 +22,6 @@
 
 namespace edsl {
 namespace lm {
-
-constexpr int kSmallWaves = 8;
 
 // How x of a type is read: bytes of an element, operands that it makes.
 template <int XT>
@@ -208,12 +206,12 @@ constexpr int kSmallOccupancy = 2 * (4 * MT * SmallX<XT>::kLoads + 4 * NT + 2 * 
                                     ? 4
                                     : 2;
 
-template <int XT, int NT, int MT, int SPB>
-__global__ void __launch_bounds__(64 * kSmallWaves, (kSmallOccupancy<XT, NT, MT, SPB>)) q4_small_kernel(Q4Args a) {
+template <int XT, int NT, int MT, int SPB, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, (kSmallOccupancy<XT, NT, MT, SPB>)) q4_small_kernel(Q4Args a) {
   using X = SmallX<XT>;
   constexpr int PIECE = 16 * MT * X::kChunks;  // of a wave, in chunks
   constexpr int ROWS = 16 * MT, COLS = 16 * NT;
-  constexpr int BYTES = kSmallWaves * (PIECE * 16 > ROWS * COLS * 4 ? PIECE * 16 : ROWS * COLS * 4);
+  constexpr int BYTES = WAVES * (PIECE * 16 > ROWS * COLS * 4 ? PIECE * 16 : ROWS * COLS * 4);
   __shared__ u32x4 lds[BYTES / 16];  // the waves' pieces, then their sums
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int tiles = (a.N + 15) / 16;
@@ -253,16 +251,16 @@ __global__ void __launch_bounds__(64 * kSmallWaves, (kSmallOccupancy<XT, NT, MT,
     do {
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
-        small_load<false>(a, rows, tile, b + kSmallWaves, full - 1, lane, rsrc, buf[d ^ 1]);
+        small_load<false>(a, rows, tile, b + WAVES, full - 1, lane, rsrc, buf[d ^ 1]);
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t on = b < full ? ~0u : 0u;
         small_block({a.scale_mask.f32 & on, a.scale_mask.bf16 & on, a.scale_mask.f16 & on}, buf[d], piece, lane, sum);
-        b += kSmallWaves;
+        b += WAVES;
         __builtin_amdgcn_sched_barrier(0);
       }
     } while (b < full);
   }
-  if (full < b1 && wave == (full - b0) % kSmallWaves) {
+  if (full < b1 && wave == (full - b0) % WAVES) {
     small_load<true>(a, rows, tile, full, full, lane, rsrc, buf[0]);
     small_block(a.scale_mask, buf[0], piece, lane, sum);
   }
@@ -276,13 +274,13 @@ __global__ void __launch_bounds__(64 * kSmallWaves, (kSmallOccupancy<XT, NT, MT,
       for (int e = 0; e < 4; ++e)
         part[(wave * ROWS + 16 * i + 4 * (lane / 16) + e) * COLS + 16 * t + lane % 16] = sum[i][t][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < a.M * COLS; i += 64 * kSmallWaves) {
+  for (int i = threadIdx.x; i < a.M * COLS; i += 64 * WAVES) {
     const int m = i / COLS, c = i % COLS;
     const int n = 16 * tile + c;
     if (n >= a.N || n < 16 * first) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kSmallWaves; ++w) v += part[(w * ROWS + m) * COLS + c];
+    for (int w = 0; w < WAVES; ++w) v += part[(w * ROWS + m) * COLS + c];
     if (a.ksplit > 1) {
       a.partials[((int64_t)slice * a.M + m) * a.N + n] = v;
     } else {
@@ -292,27 +290,30 @@ __global__ void __launch_bounds__(64 * kSmallWaves, (kSmallOccupancy<XT, NT, MT,
   }
 }
 
-template <int XT, int NT, int MT>
+template <int XT, int NT, int MT, int WAVES>
 hipError_t launch_small_spb(const Q4Args& a, int spb, hipStream_t stream) {
   const int tiles = (a.N + 15) / 16;
-  const dim3 columns = grid_of((tiles + NT - 1) / NT), block(64 * kSmallWaves);
+  const dim3 columns = grid_of((tiles + NT - 1) / NT), block(64 * WAVES);
   const dim3 grid(columns.x, (unsigned)a.ksplit, columns.y);
   if (spb == 4)
-    hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 4>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 4, WAVES>), grid, block, 0, stream, a);
   else if (spb == 2)
-    hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 2>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 2, WAVES>), grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((q4_small_kernel<XT, NT, MT, 1, WAVES>), grid, block, 0, stream, a);
   return launched();
 }
 
 template <int XT>
-hipError_t launch_q4_small(const Q4Args& a, int nt, int spb, hipStream_t stream) {
+hipError_t launch_q4_small(const Q4Args& a, int nt, int waves, int spb, hipStream_t stream) {
   if constexpr (XT != kF32) {  // three operands of 32 rows do not fit the registers
     if (a.M > 16)
-      return nt == 2 ? launch_small_spb<XT, 2, 2>(a, spb, stream) : launch_small_spb<XT, 1, 2>(a, spb, stream);
+      return nt == 2 ? launch_small_spb<XT, 2, 2, 8>(a, spb, stream) : launch_small_spb<XT, 1, 2, 8>(a, spb, stream);
   }
-  return nt == 2 ? launch_small_spb<XT, 2, 1>(a, spb, stream) : launch_small_spb<XT, 1, 1>(a, spb, stream);
+  if (nt == 1) return launch_small_spb<XT, 1, 1, 8>(a, spb, stream);
+  if (waves == 2) return launch_small_spb<XT, 2, 1, 2>(a, spb, stream);
+  if (waves == 4) return launch_small_spb<XT, 2, 1, 4>(a, spb, stream);
+  return launch_small_spb<XT, 2, 1, 8>(a, spb, stream);
 }
 
 }  // namespace lm

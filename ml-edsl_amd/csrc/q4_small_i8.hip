@@ -3,6 +3,6 @@
 
 namespace edsl {
 namespace lm {
-template hipError_t launch_q4_small<kI8>(const Q4Args& a, int nt, int spb, hipStream_t stream);
+template hipError_t launch_q4_small<kI8>(const Q4Args& a, int nt, int waves, int spb, hipStream_t stream);
 }  // namespace lm
 }  // namespace edsl

@@ -176,6 +176,17 @@ def test_what_lies_around_x_is_not_read_into_it():
             check(y, want, size, 233)
 
 
+# Wide layers on four and two waves of a workgroup: blocks of K that the waves do
+# not share evenly, odd widths, whole and broken last blocks.
+@pytest.mark.parametrize("x_dtype", [F32, BF16, F16, I8, E4M3])
+@pytest.mark.parametrize("M,K,N,group,waves", [
+    (1, 130, 8161, 64, 4), (7, 1024, 8200, 128, 4), (16, 897, 4129, 32, 4), (3, 1200, 25000, 128, 4),
+    (1, 1, 33001, 32, 2), (16, 448, 33000, 256, 2), (5, 512, 32801, 64, 2)])
+def test_fewer_waves(M, K, N, group, waves, x_dtype):
+    layer(M, K, N, group, x_dtype, zeros=(M + N) % 2 == 0, epi="bias", pad=N % 3, seed=M + K)
+    assert f"cols=32 ksplit=1 waves={waves}" in last_plan(), last_plan()
+
+
 def test_no_rows_no_columns_no_depth():
     q, s, z = make_weights(64, 40, 64)
     W = lm.q4_pack(q, s, z, group_size=64)
