@@ -205,9 +205,12 @@ bool q4_small_takes(const lm::Q4Args& a, int cus) {
   return a.M <= 32 && a.x_type != lm::kF32 && (a.N + 15) / 16 <= 4 * (int64_t)cus;
 }
 
-// Tiles: 64 rows, 32 for up to 32, of f32 48 where that is fewer rows in all (48 x
-// 4096 x 50256 in 66 us against 79). Under two tiles a CU, two teams in a workgroup
-// take K's blocks in turn (512 x 4096 x 4096 in 29 us against 33; 48 x 4096 x 50256
+// Tiles: 64 rows, 32 for up to 32, and 48 where that is fewer rows in all: of f32
+// always (48 x 4096 x 50256 in 66 us against 79), of the others under three tiles a
+// CU (270 x 4096 x 4096 bf16 in 23.2 against 27.6, 1100 rows in 56 against 61) and
+// where it is a fifth fewer (144 x 3968 x 42834 in 78 against 86; but 330 rows of
+// that layer in 168 against 163, 2000 x 4096 x 4096 in 98 against 85). Under two
+// tiles a CU, two teams in a workgroup take K's blocks in turn (512 x 4096 x 4096 in 29 us against 33; 48 x 4096 x 50256
 // f32 in 65 against 66.5), not from there on (2048 x 4096 x 4096 in 88 against 85;
 // 1024 x 4096 x 4096 f32 in 106 against 99). Under one a CU (`few`), workgroups split
 // K too (33 x 8192 x 8192 bf16 in 49, 29, 20, 22 us on 1, 2, 4, 8 slices), and sum
@@ -220,9 +223,12 @@ struct Q4TilePlan {
 Q4TilePlan q4_tile_plan(const lm::Q4Args& a, int cus) {
   static const int rows[] = {32, 64, 48};
   Q4TilePlan p{a.M <= 32 ? lm::kQ4Tile32x128 : lm::kQ4Tile64x128, 1, 1, false};
-  if (a.M > 32 && a.x_type == lm::kF32 && ((int64_t)a.M + 47) / 48 * 48 < ((int64_t)a.M + 63) / 64 * 64)
+  const int64_t rows48 = ((int64_t)a.M + 47) / 48 * 48, rows64 = ((int64_t)a.M + 63) / 64 * 64;
+  const int64_t tiles_n = ((int64_t)a.N + 127) / 128;
+  if (a.M > 32 && rows48 < rows64 &&
+      (a.x_type == lm::kF32 || rows64 / 64 * tiles_n < 3 * (int64_t)cus || 5 * rows48 <= 4 * rows64))
     p.config = lm::kQ4Tile48x128;
-  const int64_t wgs = ((int64_t)a.M + rows[p.config] - 1) / rows[p.config] * (((int64_t)a.N + 127) / 128);
+  const int64_t wgs = ((int64_t)a.M + rows[p.config] - 1) / rows[p.config] * tiles_n;
   check_grid(wgs, 8);
   p.few = wgs < cus;
   p.teams = wgs < 2 * (int64_t)cus ? 2 : 1;

@@ -245,7 +245,7 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, const int (&m)[C], con
 // q4_small.hpp, one source file for each type of x.
 template <int XT>
 hipError_t launch_q4_small(const Q4Args& a, int nt, int waves, int spb, hipStream_t stream);
-// q4_tile.hip; the third is of f32 only.
+// q4_tile.hip.
 enum : int { kQ4Tile32x128 = 0, kQ4Tile64x128 = 1, kQ4Tile48x128 = 2 };
 hipError_t launch_q4_tile(const Q4Args& a, int config, int spb, int teams, bool zeros, hipStream_t stream);
 struct Q4PrepArgs {

@@ -292,8 +292,7 @@ template <bool F16, int PLANES>
 hipError_t launch_tile_config(const Q4Args& a, int config, int spb, int teams, bool zeros, hipStream_t stream) {
   if (config == kQ4Tile32x128) return launch_tile_spb<F16, PLANES, 2, 2>(a, spb, teams, zeros, stream);
   if (config == kQ4Tile64x128) return launch_tile_spb<F16, PLANES, 4, 2>(a, spb, teams, zeros, stream);
-  if constexpr (PLANES == 3) return launch_tile_spb<F16, 3, 3, 2>(a, spb, teams, zeros, stream);
-  return hipErrorInvalidValue;
+  return launch_tile_spb<F16, PLANES, 3, 2>(a, spb, teams, zeros, stream);
 }
 
 // ------------------------------------------------------------------- x
