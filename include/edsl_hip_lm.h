@@ -38,9 +38,10 @@ extern "C" {
  * x, residual (optional) and total (optional) have type `type` (F32, BF16,
  * F16), weight that type or F32. The norm is that of h in 32 bits, not of the
  * rounded total. y has type `type`, or an 8-bit type with scales[M], one a row:
- * y = q * scales with scales = max_n |y| / 127 (I8) or / 448 (E4M3), q rounded
- * to nearest even; a row of zeros has scale 0, and
- * one whose scale is under 2^-126 codes of 0. A row whose norm is not finite
+ * y = q * scales with scales = max_n |y| / Q, Q = 127 (I8) or 448 (E4M3), and
+ * q = h * weight * Q / max_n |h * weight| rounded to nearest even (from 32-bit
+ * products and a 32-bit quotient); a row of zeros has scale 0, and one whose
+ * scale is under 2^-126 codes of 0. A row whose norm is not finite
  * or whose values are NaN has a NaN scale and unspecified codes. rstd[M] is
  * optional, for the backward pass. total may be x or residual, and y may be
  * x, residual or total's memory in the same type and stride. */
