@@ -197,9 +197,11 @@ __global__ void __launch_bounds__(THREADS, NV <= 8 ? 8 : 4) logprobs_kernel(Logp
       }
     }
   };
-  // One fma an element, where m c is far from overflow.
+  // One fma an element, where the rounding of m c is 8 at most, so that no power of two
+  // of it overflows. (m is the thread's own maximum: one whose elements all have a mask
+  // of -1e10, say, is enough for the other way, which has no such limit.)
   const float mc = p.m * c;
-  if (__all(fabsf(mc) < 1e37f)) {
+  if (__all(fabsf(mc) < 0x1p28f)) {
     add_up([&](float x) { return fmaf(x, c, -mc); });
     // What was subtracted is m c rounded: back to m itself.
     const float d = fmaf(p.m, c, -mc), f = __builtin_amdgcn_exp2f(-d);
