@@ -61,7 +61,7 @@ int edsl_hip_rms_norm_backward_launch(const void *dy, int64_t lddy, const void *
                                       int64_t lddx, float *dweight, int64_t M, int64_t N, int type, void *stream);
 
 /* Log probabilities of given tokens under softmax(scale * logits) in each of
- * M rows of V logits (F32, BF16, F16), scale > 0:
+ * M rows of V logits (F32, BF16, F16), 0 < scale <= 2^127:
  *   lse = log sum_j exp(scale x_j);  logprobs = scale x_token - lse;
  *   entropy = lse - sum_j p_j scale x_j;
  *   top_logprobs, top_ids [M][k]: the k largest, in falling order, equal

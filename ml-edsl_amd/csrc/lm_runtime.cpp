@@ -94,7 +94,8 @@ void check_logits(int64_t M, int64_t V, int type, float scale) {
   check_sizes(M, V, "M", "V");
   check_float_type(type, "logits");
   if (V > kMostVocabulary) fail(kErrLimit, "V=%lld beyond 2^21", (long long)V);
-  if (!(scale > 0.0f) || !std::isfinite(scale)) fail(kErrArgument, "scale must be positive and finite");
+  // Its product with log2(e) has to be finite.
+  if (!(scale > 0.0f && scale <= 0x1p127f)) fail(kErrArgument, "scale must be positive and at most 2^127");
   if (M > 0 && V == 0) fail(kErrShape, "rows of no logits have no probabilities");
 }
 
