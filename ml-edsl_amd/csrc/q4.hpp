@@ -88,7 +88,7 @@ struct Q4Args {
   // are whole 16-byte aligned blocks of 16 bits.
   const void* xp;       // [planes][M][ldp]
   int64_t ldp, plane;   // elements
-  const float* xs;      // [blocks * spb][xs_ld]: minus the sums of x in each group, times offset + 8 without zero points
+  const float* xs;      // [blocks][xs_ld / 16][spb][16]: minus the sums of x in each group, times offset + 8 without zero points
   int64_t xs_ld;
 };
 

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(256 * TEAMS, 2) q4_tile_kernel(Q4Args a) {
   constexpr int SS = PLANES == 3 ? 2 : 4, CPR = 4 * SS, STAGES = 4 / SS;
   constexpr int ALL = PLANES * BM * CPR, CHUNKS = (ALL + 255) / 256;  // a thread's
   __shared__ u32x4 lds_all[TEAMS][2][ALL];
-  __shared__ f32x4 sums_all[TEAMS][2][SPB * BM / 4];  // a block's sums of x
+  __shared__ f32x4 sums_all[TEAMS][2][SPB * BM / 4];  // a block's sums of x: [BM / 16][SPB][16]
   const int tid = threadIdx.x % 256, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 256) : 0;
   auto& lds = lds_all[team];
@@ -86,10 +86,10 @@ __global__ void __launch_bounds__(256 * TEAMS, 2) q4_tile_kernel(Q4Args a) {
     }
   };
   const auto load_sums = [&](int b, f32x4* to) {
-    // 16-byte pieces of SPB runs of BM sums.
+    // The groups' sums of 16 rows lie together (Q4Args::xs), so that a block's sums of
+    // the tile's rows are one run and a lane's offset is small, however many rows there are.
     if (!OWN_SUMS && tid < SPB * BM / 4)
-      to_lds(a.xs + (int64_t)b * SPB * a.xs_ld + m0,
-             4u * (uint32_t)(tid / (BM / 4) * a.xs_ld + 4 * (tid % (BM / 4))), to + wave * 64);
+      to_lds(a.xs + ((int64_t)b * a.xs_ld + m0) * SPB, 16u * (uint32_t)tid, to + wave * 64);
   };
   const uint32_t scale_offset = lane % 16 * SPB * a.scale_bytes;
   struct Weights {
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(256 * TEAMS, 2) q4_tile_kernel(Q4Args a) {
             for (int t = 0; t < NT; ++t) acc[i][t] = own[i];
             continue;
           }
-          const f32x4 xs = sums_now[g * (BM / 4) + 4 * i + lane / 16];
+          const f32x4 xs = sums_now[4 * (i * SPB + g) + lane / 16];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             acc[i][t] = xs;
@@ -357,7 +357,10 @@ __global__ void __launch_bounds__(256) q4_prep_kernel(Q4PrepArgs a) {
     s += dpp<0x4E>(s);
     if (lanes > 4) s += dpp<0x141>(s);
     if (lanes > 8) s += dpp<0x140>(s);
-    if (a.xs && lane % lanes == 0) a.xs[(int64_t)(k0 / (8 * lanes)) * a.xs_ld + row] = a.factor * s;
+    if (a.xs && lane % lanes == 0) {
+      const int block = k0 / 128, group = k0 % 128 / (8 * lanes);
+      a.xs[((block * a.xs_ld + row / 16 * 16) * a.spb + 16 * group) + row % 16] = a.factor * s;
+    }
   }
 }
 
