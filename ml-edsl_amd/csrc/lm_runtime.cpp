@@ -184,12 +184,13 @@ size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 // 22.6), and for f32, where a CU holds one workgroup of eight (1 x 4096 x 50176 in
 // 45, on eight 58); and two for up to four blocks of a very wide layer (1 x 448 x
 // 50176 in 7.6, on four 9.4, on eight 13.3; but 16 x 448 x 32064 in 6.9 and 6.5).
+// More than 16 rows, two row tiles a wave, are on eight waves always.
 void q4_small_plan(const lm::Q4Args& a, int cus, int* nt, int* waves, int* ksplit) {
   const int64_t tiles = (a.N + 15) / 16;
   *nt = tiles > cus ? 2 : 1;
   const int64_t wgs = (tiles + *nt - 1) / *nt;
   *waves = 8;
-  if (*nt == 2) {
+  if (*nt == 2 && a.M <= 16) {
     if (a.blocks <= 4 && wgs > 4 * (int64_t)cus)
       *waves = 2;
     else if (a.blocks <= 8 || (a.x_type == lm::kF32 && wgs > cus) || wgs > 3 * (int64_t)cus)
