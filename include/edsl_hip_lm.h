@@ -107,7 +107,8 @@ int edsl_hip_q4_pack_launch(const uint8_t *q, int64_t ldq, const void *scales, i
  * optional; Y is F32, BF16 or F16, bias[N] of any of these; K, N, group,
  * scale_type and has_zeros as packed. Products are exact and sums 32-bit: no
  * weight or activation is rounded, f32 ones included. Sums are taken in a fixed
- * order. A row of X that holds an infinity or NaN gives NaN in all of Y's row. */
+ * order. A row of X that holds an infinity or NaN gives NaN in all of Y's row,
+ * but 0 with the epilogues that select (IF_RELU, y > 0 ? y : 0): NaN is not above 0. */
 int edsl_hip_q4_dense_launch(const void *X, int64_t ldx, int x_type, const float *x_scales, const void *packed,
                              const void *bias, int bias_type, void *Y, int64_t ldy, int y_type, int64_t M, int64_t N,
                              int64_t K, int group, int scale_type, int has_zeros, int epilogue, float alpha,

@@ -223,7 +223,8 @@ def q4_dense_launch(X, W: Q4Weight, b, Y, epilogue: int = _native.EPI_NONE, alph
     X is [M, K] in f32, bf16, f16, int8 or float8_e4m3fn, x_scales [M] f32
     (the 8-bit norm's, say), W from ``q4_pack``, Y [M, N] and b [N] in f32, bf16
     or f16. Nothing is rounded before the 32-bit sums. A row of X with an
-    infinity or NaN gives a row of NaN."""
+    infinity or NaN gives a row of NaN, or of 0 under the IF_RELU epilogues
+    (y > 0 ? y : 0)."""
     torch = _torch()
     if not isinstance(W, Q4Weight):
         raise TypeError("W is not a Q4Weight")
