@@ -26,13 +26,13 @@ namespace {
 // wave's own) + 16 lane. As the instruction itself: for its intrinsic the
 // compiler lets every later read of LDS wait for it, whichever buffer it reads,
 // which left nothing on the way while a stage was multiplied. It has no result
-// register; wait_loads() is what waits for it. (m0 holds nothing between uses.)
+// register; wait_loads() is what waits for it. m0 is declared as written.
 __device__ __forceinline__ void to_lds(const void* base, uint32_t offset, void* to) {
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(__builtin_amdgcn_readfirstlane((int)at)), "v"(offset), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 
 // Waits for the wave's loads, those to LDS among them (vmcnt 0).
