@@ -198,11 +198,14 @@ __device__ __forceinline__ void small_block(const Q4ScaleMask& mask, const Small
   __builtin_amdgcn_wave_barrier();
 }
 
-// Waves of a SIMD: two workgroups on a CU where what the two blocks, the operands
-// and the sums take fits half of its registers.
+// Waves of a SIMD: two workgroups on a CU where what the two blocks, the operands,
+// the sums and a second row tile's part of each group take fits half of its registers
+// (24 x 4096 x 4096 int8 in groups of 32 in 9.6 us on one, with 35 registers spilled for
+// two in 18.4). 16-bit x in two row and column tiles and groups of 32 spills 4 of 256.
 template <int XT, int NT, int MT, int SPB>
 constexpr int kSmallOccupancy = 2 * (4 * MT * SmallX<XT>::kLoads + 4 * NT + 2 * NT * SPB) +
-                                            4 * SmallX<XT>::kPlanes + 8 * MT * NT + 4 * NT + 44 <= 128
+                                            4 * SmallX<XT>::kPlanes + 8 * MT * NT + 2 * (MT - 1) * SPB + 4 * NT + 44 <=
+                                        128
                                     ? 4
                                     : 2;
 
