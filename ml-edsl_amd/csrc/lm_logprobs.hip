@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, NV <= 8 ? 8 : 4) logprobs_kernel(Logp
     __syncthreads();
     const int found = count;
     if (held <= kVectors && found <= kList) {
-      // Eight threads a candidate (65 x 32001 with 20 alternatives in 8.4 us, one
+      // Eight threads a candidate (65 x 32001 with 20 alternatives in 8.2 us, one
       // thread each in 9.9).
       for (int i = tid / 8; i < found; i += THREADS / 8) {
         const float value = list_v[i];
@@ -554,8 +554,9 @@ hipError_t launch_backward(const LogprobsBackwardArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// As few parts of a row as fit a workgroup's registers: with one there is no join
-// (1 x 50256 in 8.3 us, in 24 parts 10.4; 65 x 32001 in 9.7, in 3 parts 16.5).
+// As few parts of a row as fit a workgroup's registers: with one there is no join (1 x
+// 50256 with 8 alternatives in 8.2 us, in 24 parts 10.1; 65 x 32001 with 20 in 8.2, in 3
+// parts 12.4).
 // Twice the registers where there is no second row for the CU.
 int logprobs_chunks(int64_t M, int64_t V, int type, int cus) {
   const int vec = 16 / type_bytes(type);

@@ -78,7 +78,7 @@ __device__ __forceinline__ void load_weight(const void* w, bool f32, int64_t i0,
 // bits at most, so that its product with h w is exact where h w has 17 bits, and the
 // quotient is a correctly rounded one: values halfway between two codes are common
 // among products of few bits, and go to the even code. (The product of y and a
-// rounded 1 / s put 4 codes in 100000 of bf16 rows on the other side. It took 42.6 us
+// rounded 1 / s put 3 codes in 100000 of bf16 rows on the wrong side. It took 42.6 us
 // at 4096 x 8192 bf16 to int8, this takes 42.9; 2048 x 4096 to e4m3 10.7 and 11.0.)
 template <int OUT>
 struct RowCodes {
@@ -283,12 +283,13 @@ hipError_t launch_row(const NormArgs& a, hipStream_t stream) {
 }
 
 // Threads of a row x vectors of a thread. Short rows share a wave (262144 x 128 bf16
-// in 22 us on 16 threads each against 57 on 64) or take one without a barrier (65536
-// x 1024 in 38 on 64x2 against 57 on 256x1). More threads rather than vectors from 513
-// vectors on (4096 x 8192 bf16 to 8 bits 51 us on 512x2 against 56 on 256x4; 2048 x
-// 16384 49 on 1024x2 against 55 on 1024x4), and below where a CU has one row at most
-// (`few`; 256 x 4096 bf16 3.7 against 4.1), but not for many (2001 x 2001 f32 7.6 on
-// 256x2 against 8.2; 2048 x 4096 bf16 to 8 bits 8.2 against 10.4).
+// in 22 us on 16 threads each against 59 on 64) or take one without a barrier (65536
+// x 1024 in 46 on 64x2 against 76 on 256x1). More threads rather than vectors from 513
+// vectors on (4096 x 8192 bf16 to 8 bits 42.8 us on 512x2 against 44.1 on 256x4; 2048 x
+// 16384 49 on 1024x2 against 54 on 1024x4), and below where a CU has one row at most
+// (`few`; 256 x 4096 bf16 3.7 against 4.1), but not for many (2001 x 2001 f32 7.7 on
+// 256x2 against 8.2; 2048 x 4096 bf16 to 8 bits 11.0 against 12.3). Rows beyond 4096
+// vectors are read twice: 2048 x 40960 bf16 with a residual in 236 us, 201 of them its bytes.
 template <typename T, int OUT>
 hipError_t launch_norm(const NormArgs& a, bool few, hipStream_t stream, const char** plan) {
   const int64_t vecs = (a.N + kVec<T> - 1) / kVec<T>;
@@ -550,8 +551,11 @@ __global__ void __launch_bounds__(1024) dweight_kernel(const float* partials, in
 }
 
 // Threads of a row, 0 for rows of any length: a vector each, two of f32 (4096 x
-// 4096 f32 in 52 us, with one in 59); twice that of the longest rows, though four of f32 spill (2048 x
-// 16384 in 142 us, read twice in 173). 65536 x 128 bf16 in 22 us, 42 on 64 threads.
+// 4096 f32 in 52 us, with one in 59); twice that of the longest rows, though four of
+// f32 spill 7 registers (2048 x 16384 in 89 us, read twice in 156), 69 where rows are
+// not whole vectors, and with dh 141 or 171 (139 us, read twice 173). 65536 x 128 bf16
+// in 22 us, 42 on 64 threads. Rows read twice also add to their partials in memory:
+// 2048 x 20480 bf16 in 164 us, with dh 195.
 int backward_threads(int64_t N, int type) {
   int64_t vecs = (N * type_bytes(type) + 15) / 16;
   if (vecs > (type == kF32 ? 4096 : 2048)) return 0;

@@ -215,9 +215,9 @@ bool q4_small_takes(const lm::Q4Args& a, int cus) {
 // tiles a CU, two teams in a workgroup take K's blocks in turn (512 x 4096 x 4096 in 29 us against 33; 48 x 4096 x 50256
 // f32 in 65 against 66.5), not from there on (2048 x 4096 x 4096 in 88 against 85;
 // 1024 x 4096 x 4096 f32 in 106 against 99). Under one a CU (`few`), workgroups split
-// K too (33 x 8192 x 8192 bf16 in 49, 29, 20, 22 us on 1, 2, 4, 8 slices), and sum
+// K too (33 x 8192 x 8192 bf16 in 40, 25, 18, 20 us on 1, 2, 4, 8 slices), and sum
 // their x themselves where they read it in place: the prepared sums' launch costs
-// more (128 x 4096 x 4096 in 16.8 us against 18.8; 1024 rows in 54 against 47).
+// more (128 x 4096 x 4096 in 17.4 us against 19.7; 1024 rows in 54 against 47).
 struct Q4TilePlan {
   int config, teams, ksplit;
   bool few;  // fewer tiles than CUs

@@ -10,8 +10,8 @@
 // repeat the last one. The sums of x that the zero points multiply are a matrix
 // instruction with a constant operand.
 //
-// Bound by memory where the layer is large: 1 x 8192 x 8192 in 8.5 to 8.9 us, 4.1
-// TB/s with the weights in the Infinity Cache, 10.8 from HBM (a launch and the join
+// Bound by memory where the layer is large: 1 x 8192 x 8192 in 8.5 to 9.0 us, 4.1
+// TB/s with the weights in the Infinity Cache, 11.0 from HBM (a launch and the join
 // of the waves' sums are some 4 of them); else by latency: 16 x 4096 x 4097 int8 in
 // 7.2, four blocks a wave.
 #pragma once
