@@ -106,9 +106,11 @@ int edsl_hip_q4_pack_launch(const uint8_t *q, int64_t ldq, const void *scales, i
  * include/edsl_hip_device.h. X is F32, BF16, F16, I8 or E4M3, x_scales[M] (f32)
  * optional; Y is F32, BF16 or F16, bias[N] of any of these; K, N, group,
  * scale_type and has_zeros as packed. Products are exact and sums 32-bit: no
- * weight or activation is rounded, f32 ones included. Sums are taken in a fixed
- * order. A row of X that holds an infinity or NaN gives NaN in all of Y's row,
- * but 0 with the epilogues that select (IF_RELU, y > 0 ? y : 0): NaN is not above 0. */
+ * weight or activation is rounded, f32 ones included. X of 16 and 8 bits meets
+ * weights held as 16 + q, less its sum times 16 + zero, so that the sums' roundings
+ * are those of terms of |x| scale (32 + q + zero). Sums are taken in a fixed
+ * order. A row of X that holds an infinity or NaN gives NaN in all of Y's row, but
+ * 0 with the epilogues that select (IF_RELU, y > 0 ? y : 0): NaN is not above 0. */
 int edsl_hip_q4_dense_launch(const void *X, int64_t ldx, int x_type, const float *x_scales, const void *packed,
                              const void *bias, int bias_type, void *Y, int64_t ldy, int y_type, int64_t M, int64_t N,
                              int64_t K, int group, int scale_type, int has_zeros, int epilogue, float alpha,
