@@ -1,7 +1,8 @@
 /*
  * edsl_hip_lm.h -- device-resident operators of language models around the
- * dense layer: the root-mean-square norm, the dense layer on 4-bit weights, and
- * log probabilities of given tokens.
+ * dense layer: the root-mean-square norm, the dense layer on 4-bit weights, in
+ * 8-bit integers and on groups of rows, log probabilities of given tokens, and
+ * sampling.
  *
  * No counterpart in the reference, whose programs are dense layers. Calling
  * convention, streams, errors, workspaces and graph capture are those of
@@ -115,6 +116,72 @@ int edsl_hip_q4_dense_launch(const void *X, int64_t ldx, int x_type, const float
                              const void *bias, int bias_type, void *Y, int64_t ldy, int y_type, int64_t M, int64_t N,
                              int64_t K, int group, int scale_type, int has_zeros, int epilogue, float alpha,
                              void *stream);
+
+/* The dense layer in 8-bit integers, a scale for each column of W and, optionally,
+ * each row of X:
+ *   Y[m][n] = epilogue(x_scales[m] * scales[n] * sum_k X[m][k] q[k][n] (+ bias[n])).
+ * Sums are 32-bit integers and exact: 1 <= K < 2^17, values -128 .. 127. The sum is rounded to
+ * f32 once and then multiplied by scales[n] and by x_scales[m]. edsl_hip_i8_pack_launch
+ * lays q[K][N] and scales[N] (F32, BF16, F16) out once, in
+ * edsl_hip_i8_packed_bytes bytes (-1: arguments that it does not take) at a 256-byte
+ * aligned address. Y is F32, BF16 or F16, bias of any of these. */
+int64_t edsl_hip_i8_packed_bytes(int64_t K, int64_t N);
+int edsl_hip_i8_pack_launch(const int8_t *q, int64_t ldq, const void *scales, int scale_type, int64_t K, int64_t N,
+                            void *packed, size_t packed_bytes, void *stream);
+int edsl_hip_i8_dense_launch(const int8_t *X, int64_t ldx, const float *x_scales, const void *packed, const void *bias,
+                             int bias_type, void *Y, int64_t ldy, int y_type, int64_t M, int64_t N, int64_t K,
+                             int epilogue, float alpha, void *stream);
+
+/* The dense layer on groups of rows, each with weights of its own (experts):
+ *   Y[r] = epilogue(X[r] @ W[e] (+ bias[e]))   for offsets[e] <= r < offsets[e+1].
+ * X is [T][K], W [E][K][N] (w_stride elements from one group to the next; where
+ * w_turned, each is held as [N][K] with rows of ldw), bias [E][N] with rows of ldbias
+ * (0: one for all), Y [T][N], all of `type` (F32, BF16, F16). offsets[E+1] is
+ * device memory, int64_t when ids64, else int32_t; it rises from 0 or more to T or less, and may
+ * leave groups empty. Rows before the first and behind the last group are left as they are.
+ * Offsets outside 0 .. T are cut to it and falling ones make empty groups: nothing
+ * outside the operands is read or written, but which rows are is then unspecified.
+ * E <= 65535. Sums are 32-bit floats in a fixed order, rounded once to `type` after the epilogue. */
+int edsl_hip_grouped_dense_launch(const void *X, int64_t ldx, const void *W, int64_t ldw, int64_t w_stride,
+                                  int w_turned, const void *offsets, int ids64, int64_t E, const void *bias,
+                                  int64_t ldbias, void *Y, int64_t ldy, int64_t T, int64_t N, int64_t K, int type,
+                                  int epilogue, float alpha, void *stream);
+
+/* Its gradients, each optional. With dZ = dY where there is no activation, else
+ * dY * (Y > 0 ? 1 : slope), slope 0 or the leaky epilogue's alpha (>= 0), rounded to
+ * `type` (Y is what the forward pass gave, and may be null without an activation):
+ *   dX[r] = dZ[r] @ W[e]^T;  dW[e] = sum over the group's rows of X[r]^T dZ[r];
+ *   db[e] = sum of dZ[r], before that rounding.
+ * dX has `type`, dW and db that or F32 (dw_type, db_type); dW is [E][K][N], or turned as W
+ * may be. Groups without rows have dW and db 0; rows of no group leave dX as it is.
+ * dX may be dY's or X's memory only where neither is read by another gradient that is asked for:
+ * an output may not overlap an input. The same call gives the same bits. */
+int edsl_hip_grouped_dense_backward_launch(const void *dY, int64_t lddy, const void *X, int64_t ldx, const void *W,
+                                           int64_t ldw, int64_t w_stride, int w_turned, const void *offsets, int ids64,
+                                           int64_t E, const void *Y, int64_t ldy, void *dX, int64_t lddx, void *dW,
+                                           int64_t lddw, int64_t dw_stride, int dw_turned, int dw_type, void *db,
+                                           int64_t lddb, int db_type, int64_t T, int64_t N, int64_t K, int type,
+                                           int epilogue, float alpha, void *stream);
+
+/* Draws a token for each of M rows of V logits (F32, BF16, F16) with given numbers
+ * uniforms[M] in [0, 1). With w_i = exp((x_i - max x) / temperature), kept are
+ *   the top_k largest logits, equal ones in the order of their index;
+ *   of these, in falling order, those with less than top_p of their mass before them;
+ *   of these, the ones with w_i >= min_p;
+ * and the token is the first index at which the running sum of the kept w_i, by index,
+ * exceeds uniforms[m] times the whole of it. Temperature 0 takes the largest logit, the first of
+ * equal ones. top_k <= 0 or >= V, top_p >= 1 and min_p <= 0 leave their step out; the largest
+ * logit is always kept. logprobs[M] (optional) is the log probability with which the token was drawn.
+ * Each setting is one for all rows (`_all`) or, where its pointer is not null, M of them.
+ * w_i are held in units of 2^-46 (2^(ceil(log2 V) - 62) for V beyond 2^16), to nearest, and sums
+ * are exact: the same call gives the same tokens. Logits of -inf are never drawn; a row of
+ * nothing else gives token -1 and log probability -inf, and one that holds NaN or +inf, or whose
+ * settings or number are NaN or whose temperature is negative or infinite, -1 and NaN. Numbers outside [0, 1) count as
+ * the nearest inside. tokens are int64_t when ids64, else int32_t. V <= 2^21. */
+int edsl_hip_sample_tokens_launch(const void *logits, int64_t ldl, int type, const float *uniforms, void *tokens,
+                                  int ids64, float *logprobs, const float *temperature, float temperature_all,
+                                  const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all,
+                                  const float *min_p, float min_p_all, int64_t M, int64_t V, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,117 @@
+// The way back through the activation of a layer on groups of rows, and its
+// bias's gradient: dz = dy (y > 0), or dy times the slope elsewhere, and
+//   db_e = sum over e's rows of dz.
+// Bound by memory. Rows are summed in tiles of 64 whose sums a second launch adds in
+// their order, so that the same call gives the same bits.
+#include "lm_grouped.hpp"
+
+namespace edsl {
+namespace lm {
+
+namespace {
+
+constexpr int kActRows = kGroupedActRows, kActWaves = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(64 * kActWaves) grouped_act_kernel(GroupedActArgs a) {
+  constexpr int VEC = kVec<T>, COLS = 64 * VEC;
+  __shared__ float joined[kActWaves][COLS];
+  const int tiles_n = (int)((a.N + COLS - 1) / COLS);
+  const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  // The tile's number is its place among the partial sums: no other order.
+  const int w = (int)block_of(), tile = w / tiles_n;
+  const int64_t col = (int64_t)(w % tiles_n) * COLS + lane * VEC;
+  RowTile t;
+  if (!RowTiles{g, kActRows, 0}.find(tile, &t)) return;
+  const int64_t end = min(t.first + kActRows, t.end);
+  float sum[VEC] = {};
+  for (int64_t row = t.first + wave; row < end; row += kActWaves) {
+    if (col >= a.N) break;
+    const Packed<T, VEC> dy = load_guarded<T, VEC>(static_cast<const T*>(a.dy) + row * a.lddy, col, a.N);
+    if (a.y) {
+      const Packed<T, VEC> y = load_guarded<T, VEC>(static_cast<const T*>(a.y) + row * a.ldy, col, a.N);
+      Packed<T, VEC> dz;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = (float)dy.v[e], v = (float)y.v[e] > 0.0f ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
+        dz.v[e] = (T)v;
+        sum[e] += v;
+      }
+      if (col + VEC <= a.N)
+        *reinterpret_cast<Packed<T, VEC>*>(static_cast<T*>(a.dz) + row * a.lddz + col) = dz;
+      else
+        for (int e = 0; e < VEC; ++e)
+          if (col + e < a.N) static_cast<T*>(a.dz)[row * a.lddz + col + e] = dz.v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] += (float)dy.v[e];
+    }
+  }
+  if (!a.db) return;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = sum[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < COLS; c += 64 * kActWaves) {
+    float s = joined[0][c];
+#pragma unroll
+    for (int v = 1; v < kActWaves; ++v) s += joined[v][c];
+    const int64_t n = (int64_t)(w % tiles_n) * COLS + c;
+    if (n < a.N) a.partials[(int64_t)tile * a.N + n] = s;
+  }
+}
+
+__global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
+  const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
+  const int expert = blockIdx.y;
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const auto tiles_of = [&](int e) {
+    const int64_t rows = g.at(e + 1) - g.at(e);
+    return rows > 0 ? (rows + kActRows - 1) / kActRows : 0;
+  };
+  const int lane = threadIdx.x % 64;
+  int64_t before = 0;
+  for (int e = lane; e < expert; e += 64) before += tiles_of(e);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
+  if (n >= a.N) return;
+  const int64_t most = grouped_act_tiles(a.T, a.E);  // what the partial sums have room for
+  const int64_t tiles = min(tiles_of(expert), max(most - before, (int64_t)0));
+  float s = 0.0f;
+  for (int64_t t = 0; t < tiles; ++t) s += a.partials[(before + t) * a.N + n];
+  const int64_t at = expert * a.lddb + n;
+  if (a.db_type == kF32)
+    static_cast<float*>(a.db)[at] = s;
+  else if (a.db_type == kBf16)
+    static_cast<bf16*>(a.db)[at] = (bf16)s;
+  else
+    static_cast<f16*>(a.db)[at] = (f16)s;
+}
+
+template <typename T>
+hipError_t launch_act_type(const GroupedActArgs& a, hipStream_t stream) {
+  constexpr int COLS = 64 * kVec<T>;
+  const int64_t tiles = grouped_act_tiles(a.T, a.E) * ((a.N + COLS - 1) / COLS);
+  hipLaunchKernelGGL((grouped_act_kernel<T>), grid_of(tiles), dim3(64 * kActWaves), 0, stream, a);
+  return launched();
+}
+
+}  // namespace
+
+hipError_t launch_grouped_act(const GroupedActArgs& a, hipStream_t stream) {
+  if (a.T > 0) {
+    const hipError_t e = a.type == kF32    ? launch_act_type<float>(a, stream)
+                         : a.type == kBf16 ? launch_act_type<bf16>(a, stream)
+                                           : launch_act_type<f16>(a, stream);
+    if (e != hipSuccess) return e;
+  }
+  if (a.db) {
+    hipLaunchKernelGGL(grouped_bias_kernel, dim3((unsigned)((a.N + 255) / 256), (unsigned)a.E), dim3(256), 0, stream,
+                       a);
+    return launched();
+  }
+  return hipSuccess;
+}
+
+}  // namespace lm
+}  // namespace edsl

@@ -1,0 +1,21 @@
+// The layers on groups of rows (lm_grouped.hpp) in bf16.
+#include "lm_grouped_launch.hpp"
+
+namespace edsl {
+namespace lm {
+
+template <>
+hipError_t launch_grouped_rows<kBf16>(const GroupedArgs& a, int tile, hipStream_t stream) {
+  return GroupedLaunch<bf16>::rows(a, tile, stream);
+}
+template <>
+hipError_t launch_grouped_skinny<kBf16>(const GroupedArgs& a, hipStream_t stream) {
+  return GroupedLaunch<bf16>::skinny(a, stream);
+}
+template <>
+hipError_t launch_grouped_weights<kBf16>(const GroupedWeightArgs& a, int tile, hipStream_t stream) {
+  return GroupedLaunch<bf16>::weights(a, tile, stream);
+}
+
+}  // namespace lm
+}  // namespace edsl

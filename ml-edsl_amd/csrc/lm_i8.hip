@@ -1,0 +1,155 @@
+// The dense layer in 8-bit integers with a scale for each row of x and each column
+// of W:
+//   y[m][n] = epi(xs[m] ws[n] sum_k x[m][k] w[k][n] + b[n])
+// Sums are 32-bit integers: exact for K < 2^17.
+//
+// Weights are laid out once in blocks of 16 columns x 64 k, the 1024 bytes that a
+// wave's matrix instruction takes, successive k together.
+#include "lm_kernels.hpp"
+#include "lm_skinny.hpp"
+#include "lm_tile.hpp"
+
+namespace edsl {
+namespace lm {
+namespace {
+
+// 64 k x 64 columns a workgroup; zeros past K and N.
+__global__ void __launch_bounds__(256) i8_pack_kernel(I8PackArgs a) {
+  __shared__ uint8_t t[64][64 + 4];
+  const int64_t kblocks = i8_blocks(a.K), tiles = i8_tiles(a.N), groups = (tiles + 3) / 4;
+  const int64_t w = block_of();
+  if (w >= groups * kblocks) return;
+  const int64_t kb = w % kblocks, n0 = w / kblocks * 64;
+  const int tid = threadIdx.x;
+  {
+    const int64_t k = kb * 64 + tid / 4, n = n0 + tid % 4 * 16;
+    Packed<int8_t, 16> v{};
+    if (k < a.K && n < a.N) v = load_guarded<int8_t, 16>(a.q + k * a.ldq, n, a.N);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) t[tid / 4][tid % 4 * 16 + e] = (uint8_t)v.v[e];
+  }
+  __syncthreads();
+  const int64_t tile = n0 / 16 + tid / 64;
+  const int lane = tid % 64;
+  if (tile < tiles) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[i] |= (uint32_t)t[lane / 16 * 16 + 4 * i + e][tid / 64 * 16 + lane % 16] << (8 * e);
+    }
+    *reinterpret_cast<u32x4*>(a.packed + (tile * kblocks + kb) * 1024 + lane * 16) = r;
+    if (kb == 0 && lane < 16) {
+      const int64_t n = tile * 16 + lane;
+      reinterpret_cast<float*>(a.packed + i8_scales_at(a.K, a.N))[n] =
+          n < a.N ? get_typed(a.scales, n, a.scale_type) : 0.0f;
+    }
+  }
+}
+
+template <typename Tl>
+__global__ void __launch_bounds__(Tl::kThreads, 1) i8_tile_kernel(I8Args a) {
+  __shared__ u32x4 lds[2 * Tl::kStage];
+  const int tiles_m = (a.M + Tl::BM - 1) / Tl::BM, tiles_n = (a.N + Tl::BN - 1) / Tl::BN;
+  if (block_of() >= (uint32_t)tiles_m * tiles_n) return;
+  int at = xcd_order((int)block_of(), tiles_m * tiles_n);
+  constexpr int kGroup = 8;
+  const int group = at / (kGroup * tiles_n), first_m = group * kGroup, rows_m = min(tiles_m - first_m, kGroup);
+  at -= group * kGroup * tiles_n;
+  const int m0 = (first_m + at % rows_m) * Tl::BM, n0 = at / rows_m * Tl::BN;
+  const int64_t tile_bytes = i8_blocks(a.K) * 1024;
+  const TileOperand oa{reinterpret_cast<const char*>(a.x) + m0 * a.ldx, a.ldx, min(a.M - m0, Tl::BM)};
+  const TileOperand ob{a.w + n0 / 16 * tile_bytes, tile_bytes, min(a.N - n0, Tl::BN)};
+  typename Tl::Acc acc[Tl::MI][Tl::NI];
+  Tl::product(oa, ob, a.K, lds, acc);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  float xs[Tl::MI];
+#pragma unroll
+  for (int i = 0; i < Tl::MI; ++i) {
+    const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
+    xs[i] = a.x_scales && m < a.M ? a.x_scales[m] : 1.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < Tl::NI; ++j) {
+    const int n = n0 + 16 * (wave % Tl::WN * Tl::NI + j) + 4 * (lane / 16), left = a.N - n;
+    if (left <= 0) break;
+    float bias[4] = {};
+    if (a.bias) get4_typed(a.bias, n, a.bias_type, bias, left);
+    const f32x4 ws = *reinterpret_cast<const f32x4*>(a.w_scales + n);  // kept for whole blocks of 16
+#pragma unroll
+    for (int i = 0; i < Tl::MI; ++i) {
+      const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
+      if (m >= a.M) break;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = (float)acc[i][j][e] * ws[e] * xs[i];
+        if (a.bias) v[e] = __fadd_rn(v[e], bias[e]);
+      }
+      activate(v, a.epi, a.alpha);
+      put4_typed(a.y, m * a.ldy + n, a.y_type, v, left);
+    }
+  }
+}
+
+template <int MT, int NJ, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) i8_skinny_kernel(I8Args a) {
+  using S = Skinny<int8_t, kBlocks, MT, NJ, WAVES>;
+  __shared__ typename S::Acc lds[S::kSlots];
+  S::run(a.x, a.ldx, a.M, a.w, i8_blocks(a.K) * 1024, a.K, a.N, (int)blockIdx.x * S::kCols16, lds,
+         [&](int m, int n, int sum) {
+           float v[1] = {(float)sum * a.w_scales[n] * (a.x_scales ? a.x_scales[m] : 1.0f)};
+           if (a.bias) v[0] = __fadd_rn(v[0], get_typed(a.bias, n, a.bias_type));
+           activate(v, a.epi, a.alpha);
+           const int64_t at = m * a.ldy + n;
+           if (a.y_type == kF32)
+             static_cast<float*>(a.y)[at] = v[0];
+           else if (a.y_type == kBf16)
+             static_cast<bf16*>(a.y)[at] = (bf16)v[0];
+           else
+             static_cast<f16*>(a.y)[at] = (f16)v[0];
+         });
+}
+
+template <typename Tl>
+hipError_t launch_tile(const I8Args& a, hipStream_t stream) {
+  const int64_t tiles = (int64_t)((a.M + Tl::BM - 1) / Tl::BM) * ((a.N + Tl::BN - 1) / Tl::BN);
+  hipLaunchKernelGGL((i8_tile_kernel<Tl>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
+  return launched();
+}
+
+template <int MT>
+hipError_t launch_skinny(const I8Args& a, int cols16, hipStream_t stream) {
+  constexpr int kWaves = 8;
+  const unsigned blocks = (unsigned)((a.N + 16 * cols16 - 1) / (16 * cols16));
+  if (cols16 == 1)
+    hipLaunchKernelGGL((i8_skinny_kernel<MT, 1, kWaves>), dim3(blocks), dim3(64 * kWaves), 0, stream, a);
+  else
+    hipLaunchKernelGGL((i8_skinny_kernel<MT, 2, kWaves>), dim3(blocks), dim3(64 * kWaves), 0, stream, a);
+  return launched();
+}
+
+}  // namespace
+
+hipError_t launch_i8_pack(const I8PackArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(i8_pack_kernel, grid_of((i8_tiles(a.N) + 3) / 4 * i8_blocks(a.K)), dim3(256), 0, stream, a);
+  return launched();
+}
+
+hipError_t launch_i8_tile(const I8Args& a, int tile, hipStream_t stream) {
+  if (tile == kI8Tile256) return launch_tile<Tile<int8_t, kRows, kBlocks, 256, 256, 2, 4, true>>(a, stream);
+  if (tile == kI8Tile128) return launch_tile<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 2, true>>(a, stream);
+  return launch_tile<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 2, false>>(a, stream);
+}
+
+hipError_t launch_i8_skinny(const I8Args& a, int cols16, hipStream_t stream) {
+  if (a.M <= 16) return launch_skinny<1>(a, cols16, stream);
+  if (a.M <= 32) return launch_skinny<2>(a, cols16, stream);
+  if (a.M <= 48) return launch_skinny<3>(a, cols16, stream);
+  return launch_skinny<4>(a, cols16, stream);
+}
+
+}  // namespace lm
+}  // namespace edsl

@@ -83,5 +83,104 @@ struct LogprobsBackwardArgs {
 };
 hipError_t launch_token_logprobs_backward(const LogprobsBackwardArgs& a, hipStream_t stream);
 
+// ------------------------------------------------------------- sampling
+struct SampleArgs {
+  const void* x;
+  const float* uniforms;
+  void* tokens;
+  float* logprobs;           // or nullptr
+  const float* temperature;  // [M] each, or nullptr: `_all` for all rows
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t ldx, M, V;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  int shift;  // masses are in units of 2^-shift
+  int type;
+  bool ids64;
+};
+hipError_t launch_sample_tokens(const SampleArgs& a, hipStream_t stream);
+
+// --------------------------------------------------- layers on groups of rows
+struct GroupedArgs {
+  const void* x;
+  const void* w;        // expert e at w + e * stride_w
+  const void* bias;     // [E][N], rows of ldbias, or nullptr
+  const void* offsets;  // [E + 1]
+  void* y;
+  int64_t ldx, ldw, stride_w, ldbias, ldy, T, K, N;
+  int E, skip;  // experts of up to `skip` rows are left to the streaming kernel
+  int epi, type;
+  float alpha;
+  bool ids64;
+  bool turned;  // w's k are contiguous, not its columns
+};
+constexpr int kGroupedSkinnyRows = 32;  // experts with up to this many rows may stream their weights
+// Whether tiles read the operands where they are, by asynchronous loads.
+enum GroupedTile : int { kGroupedTile256 = 0, kGroupedTile128 = 1, kGroupedTileAny = 2 };
+template <int TYPE>
+hipError_t launch_grouped_rows(const GroupedArgs& a, int tile, hipStream_t stream);
+template <int TYPE>
+hipError_t launch_grouped_skinny(const GroupedArgs& a, hipStream_t stream);
+
+struct GroupedWeightArgs {
+  const void* a;  // dw[e] = a[e's rows]^T b[e's rows]
+  const void* b;
+  const void* offsets;
+  void* dw;
+  int64_t lda, ldb, lddw, stride_dw, T, M, N;
+  int E, type, dw_type;
+  bool ids64;
+};
+template <int TYPE>
+hipError_t launch_grouped_weights(const GroupedWeightArgs& a, int tile, hipStream_t stream);
+
+// dz = dy * act'(y), and the sums of dz over each expert's rows.
+struct GroupedActArgs {
+  const void* dy;
+  const void* y;   // or nullptr: no activation
+  void* dz;        // with y
+  float* partials; // [tiles][N], where the sums are wanted
+  void* db;        // [E][N], rows of lddb, or nullptr
+  const void* offsets;
+  int64_t lddy, ldy, lddz, lddb, T, N;
+  float slope;  // where y <= 0
+  int E, type, db_type;
+  bool ids64;
+};
+constexpr int kGroupedActRows = 64;  // rows whose sums are taken together
+// The most such tiles that T rows in E groups can have.
+constexpr int64_t grouped_act_tiles(int64_t T, int64_t E) { return T / kGroupedActRows + (E < T ? E : T); }
+hipError_t launch_grouped_act(const GroupedActArgs& a, hipStream_t stream);
+
+// ----------------------------------------------------------- 8-bit layer
+struct I8PackArgs {
+  const int8_t* q;
+  const void* scales;
+  char* packed;
+  int64_t ldq, K, N;
+  int scale_type;
+};
+constexpr int64_t i8_blocks(int64_t K) { return (K + 127) / 128 * 2; }  // of 64 k
+constexpr int64_t i8_tiles(int64_t N) { return (N + 15) / 16; }
+constexpr int64_t i8_scales_at(int64_t K, int64_t N) { return i8_tiles(N) * i8_blocks(K) * 1024; }
+hipError_t launch_i8_pack(const I8PackArgs& a, hipStream_t stream);
+
+struct I8Args {
+  const int8_t* x;
+  const float* x_scales;  // or nullptr
+  const char* w;          // as packed
+  const float* w_scales;
+  const void* bias;  // or nullptr
+  void* y;
+  int64_t ldx, ldy;
+  int M, N, K, epi, y_type, bias_type;
+  float alpha;
+};
+enum I8Tile : int { kI8Tile256 = 0, kI8Tile128 = 1, kI8TileAny = 2 };
+hipError_t launch_i8_tile(const I8Args& a, int tile, hipStream_t stream);
+hipError_t launch_i8_skinny(const I8Args& a, int cols16, hipStream_t stream);
+
 }  // namespace lm
 }  // namespace edsl

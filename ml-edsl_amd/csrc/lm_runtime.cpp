@@ -7,6 +7,7 @@
 
 #include "../../include/edsl_hip_lm.h"
 #include "dev_buf.hpp"
+#include "lm_checks.hpp"
 #include "lm_kernels.hpp"
 #include "q4.hpp"
 #include "runtime_internal.hpp"
@@ -15,32 +16,7 @@ namespace edsl {
 namespace rt {
 namespace {
 
-constexpr int64_t kMostDim = int64_t(1) << 30;
 constexpr int64_t kMostDepth = int64_t(1) << 23;  // of a 4-bit layer: 128 rows of x within 32-bit offsets
-constexpr int64_t kMostVocabulary = int64_t(1) << 21;
-
-void check_sizes(int64_t rows, int64_t cols, const char* rn, const char* cn) {
-  if (rows < 0 || cols < 0) fail(kErrShape, "negative dimension");
-  if (rows > kMostDim || cols > kMostDim)
-    fail(kErrLimit, "dimension beyond 2^30 (%s=%lld %s=%lld)", rn, (long long)rows, cn, (long long)cols);
-}
-
-void check_float_type(int type, const char* name) {
-  if (!lm::is_float_type(type)) fail(kErrDtype, "%s: type %d is not f32, bf16 or f16", name, type);
-}
-
-// A required operand of rows x cols elements (none needed where there are none).
-void check_mat(const void* p, int64_t ld, int64_t rows, int64_t cols, const char* name) {
-  if (rows > 0 && cols > 0 && !p) fail(kErrArgument, "%s is null", name);
-  if (rows > 1 && ld < cols) fail(kErrStride, "%s: row stride %lld < row length %lld", name, (long long)ld, (long long)cols);
-}
-
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
-
-const char* type_name(int t) {
-  static const char* const names[] = {"f32", "bf16", "f16", "i8", "e4m3"};
-  return names[t];
-}
 
 void rms_norm(lm::NormArgs a, void* stream) {
   check_sizes(a.M, a.N, "M", "N");
@@ -99,11 +75,6 @@ void check_logits(int64_t M, int64_t V, int type, float scale) {
   if (M > 0 && V == 0) fail(kErrShape, "rows of no logits have no probabilities");
 }
 
-void check_grid(int64_t M, int64_t parts) {
-  if (M * parts > 0x7fffffff)
-    fail(kErrLimit, "%lld rows of %lld parts are more than one launch takes", (long long)M, (long long)parts);
-}
-
 void token_logprobs(lm::LogprobsArgs a, void* stream) {
   check_logits(a.M, a.V, a.type, a.scale);
   if (a.k < 0 || a.k > lm::kMaxTop) fail(kErrLimit, "k=%d is not in 0 .. %d", a.k, lm::kMaxTop);
@@ -149,11 +120,6 @@ lm::Q4Layout q4_checked_layout(int64_t K, int64_t N, int group, int scale_type, 
   return lm::q4_layout(K, N, group, scale_type, zeros);
 }
 
-void check_packed(const void* p, const char* name) {
-  if (!p) fail(kErrArgument, "%s is null", name);
-  if (reinterpret_cast<uintptr_t>(p) % 256 != 0) fail(kErrArgument, "%s is not 256-byte aligned", name);
-}
-
 void q4_pack(lm::Q4PackArgs a, size_t bytes, void* stream) {
   a.layout = q4_checked_layout(a.K, a.N, a.group, a.scale_type, a.zeros != nullptr);
   if (bytes < (size_t)a.layout.bytes)
@@ -170,8 +136,6 @@ void q4_pack(lm::Q4PackArgs a, size_t bytes, void* stream) {
     set_plan("q4_pack group=%d", a.group);
   });
 }
-
-size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Up to 32 rows: column tiles of a workgroup, one where that is one workgroup a
 // CU at most (1 x 4096 x 4096 in 5.0 us against 7.6 on half the CUs), else two (1 x

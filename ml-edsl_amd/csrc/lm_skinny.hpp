@@ -1,0 +1,203 @@
+// A few rows against a layer's weights: what is read once is the weights, and the
+// time is theirs. The waves of a workgroup take K in turn, each with the next
+// block's loads on their way while it multiplies this one's, and meet in LDS once.
+// No operand goes through LDS before: rows of x come in the instruction's order, and
+// so do weights whose k are contiguous (kRows) or that are laid out so (kBlocks).
+// Where columns are contiguous (kCols), a lane reads kChunk successive k of NJ
+// successive columns and turns them in registers, so that NJ instructions take one
+// of its columns each; the order of the columns is put right where they are stored.
+#pragma once
+
+#include "lm_tile.hpp"
+
+namespace edsl {
+namespace lm {
+
+template <typename T, int KIND, int MT, int NJ, int WAVES>
+struct Skinny {
+  using E = TileElem<T>;
+  using Acc = typename E::Acc;
+  static constexpr int kChunk = E::kChunk, kStep = 4 * kChunk;
+  static constexpr int U = KIND == kCols ? 1 : MT <= 2 ? 4 : 2;  // steps of a block
+  static constexpr int kDepth = U * kStep;
+  static constexpr int kCols16 = 16 * NJ;         // columns of a workgroup
+  static constexpr int kSlots = WAVES * NJ * 64;  // Acc of LDS
+
+  struct Block {
+    u32x4 a[U][MT];
+    u32x4 b[KIND == kCols ? 1 : U][KIND == kCols ? 1 : NJ];
+    Packed<T, NJ> raw[KIND == kCols ? kChunk : 1];
+  };
+
+  const char* xrow[MT];  // the lane's rows, at its first k
+  const char* wcol[NJ];  // its columns (kCols: the first one)
+  int64_t ld;            // of the weights
+  int lane, chunk_at;
+
+  // `rows` of x and `n` columns of weights; columns from n0 on.
+  __device__ __forceinline__ void init(const void* x, int64_t ldx, int rows, const void* w, int64_t ldw, int N,
+                                       int n0) {
+    lane = threadIdx.x % 64;
+    chunk_at = lane / 16 * kChunk;
+    ld = ldw;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      xrow[i] = static_cast<const char*>(x) +
+                (min(16 * i + lane % 16, rows - 1) * ldx + chunk_at) * (int64_t)sizeof(T);
+    if constexpr (KIND == kCols) {
+      wcol[0] = static_cast<const char*>(w) + (chunk_at * ldw + column(0, lane % 16, N, n0)) * (int64_t)sizeof(T);
+    } else if constexpr (KIND == kRows) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        wcol[j] = static_cast<const char*>(w) +
+                  (min(column(j, lane % 16, N, n0), N - 1) * ldw + chunk_at) * (int64_t)sizeof(T);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        wcol[j] = static_cast<const char*>(w) + min(n0 / 16 + j, (N - 1) / 16) * ldw + lane * 16;
+    }
+  }
+
+  // The layer's column that instruction j gives in its column c. Past the last one
+  // kCols repeats columns before it (N is at least NJ), the others have no column.
+  static __device__ __forceinline__ int column(int j, int c, int N, int n0) {
+    return KIND == kCols ? min(n0 + NJ * c, N - NJ) + j : n0 + 16 * j + c;
+  }
+
+  __device__ __forceinline__ void load(Block& r, int k0) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        r.a[u][i] = __builtin_bit_cast(
+            u32x4, load_packed<T, kChunk>(reinterpret_cast<const T*>(xrow[i]) + k0 + u * kStep));
+    if constexpr (KIND == kCols) {
+#pragma unroll
+      for (int q = 0; q < kChunk; ++q)
+        r.raw[q] = load_packed<T, NJ>(reinterpret_cast<const T*>(wcol[0]) + (int64_t)(k0 + q) * ld);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if constexpr (KIND == kRows)
+            r.b[u][j] = __builtin_bit_cast(
+                u32x4, load_packed<T, kChunk>(reinterpret_cast<const T*>(wcol[j]) + k0 + u * kStep));
+          else
+            r.b[u][j] = *reinterpret_cast<const u32x4*>(wcol[j] + (int64_t)(k0 / kStep + u) * 1024);
+        }
+    }
+  }
+
+  // The same where the block goes past K: zeros there.
+  __device__ __forceinline__ void load_tail(Block& r, int k0, int K) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int left = K - (k0 + u * kStep + chunk_at);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        r.a[u][i] = __builtin_bit_cast(
+            u32x4, load_guarded<T, kChunk>(reinterpret_cast<const T*>(xrow[i]) + k0 + u * kStep, 0, left));
+      if constexpr (KIND == kRows)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          r.b[u][j] = __builtin_bit_cast(
+              u32x4, load_guarded<T, kChunk>(reinterpret_cast<const T*>(wcol[j]) + k0 + u * kStep, 0, left));
+      if constexpr (KIND == kBlocks)  // they hold zeros up to whole pairs of steps
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int step = k0 / kStep + u;
+          r.b[u][j] = step < (K + kStep - 1) / kStep ? *reinterpret_cast<const u32x4*>(wcol[j] + (int64_t)step * 1024)
+                                                     : u32x4{0, 0, 0, 0};
+        }
+    }
+    if constexpr (KIND == kCols)
+#pragma unroll
+      for (int q = 0; q < kChunk; ++q) {
+        r.raw[q] = Packed<T, NJ>{};
+        if (k0 + chunk_at + q < K)
+          r.raw[q] = load_packed<T, NJ>(reinterpret_cast<const T*>(wcol[0]) + (int64_t)(k0 + q) * ld);
+      }
+  }
+
+  // Column j of kChunk rows of NJ, as an operand.
+  static __device__ __forceinline__ u32x4 turned(const Packed<T, NJ> (&raw)[kChunk], int j) {
+    u32x4 v;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = __builtin_bit_cast(uint32_t, raw[q].v[j]);
+    } else {
+      typedef uint32_t Words __attribute__((ext_vector_type(NJ / 2)));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t x = __builtin_bit_cast(Words, raw[2 * q])[j / 2], y = __builtin_bit_cast(Words, raw[2 * q + 1])[j / 2];
+        v[q] = __builtin_amdgcn_perm(y, x, j % 2 ? 0x07060302u : 0x05040100u);
+      }
+    }
+    return v;
+  }
+
+  static __device__ __forceinline__ void multiply(const Block& r, Acc (&acc)[MT][NJ]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        u32x4 b;
+        if constexpr (KIND == kCols)
+          b = turned(r.raw, j);
+        else
+          b = r.b[u][j];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = E::mul(r.a[u][i], b, acc[i][j]);
+      }
+  }
+
+  // store(row, column, sum) of every output of the workgroup's columns.
+  template <typename Store>
+  static __device__ __forceinline__ void run(const void* x, int64_t ldx, int rows, const void* w, int64_t ldw, int K,
+                                             int N, int n0, Acc* lds, Store&& store) {
+    Skinny s;
+    s.init(x, ldx, rows, w, ldw, N, n0);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = s.lane;
+    Acc acc[MT][NJ];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = Acc{};
+    const int blocks = K / kDepth;
+    Block now, next;
+    if (wave < blocks) s.load(now, wave * kDepth);
+    for (int b = wave; b < blocks; b += WAVES) {
+      const int ahead = b + WAVES < blocks ? b + WAVES : b;  // the last turn reads its own again
+      s.load(next, ahead * kDepth);
+      multiply(now, acc);
+      now = next;
+    }
+    if (blocks * kDepth < K && wave == blocks % WAVES) {
+      s.load_tail(now, blocks * kDepth, K);
+      multiply(now, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (16 * i >= rows) break;  // uniform
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) lds[(wave * NJ + j) * 64 + lane] = acc[i][j];
+      __syncthreads();
+      for (int at = threadIdx.x; at < NJ * 64; at += 64 * WAVES) {
+        Acc sum = lds[at];
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) sum += lds[v * NJ * 64 + at];
+        const int l = at % 64, n = column(at / 64, l % 16, N, n0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = 16 * i + 4 * (l / 16) + e;
+          if (m < rows && n < N) store(m, n, sum[e]);
+        }
+      }
+    }
+  }
+};
+
+}  // namespace lm
+}  // namespace edsl

@@ -4,6 +4,7 @@
 // entry's status, or None where an argument is not taken: the Python path then
 // names what is wrong. Checking a norm's operands through Python takes 9 us, here
 // 0.4.
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/edsl_hip_lm.h"
@@ -260,6 +261,179 @@ PyObject* edsl_torch_token_logprobs_backward(PyObject*, PyObject* const* args, P
     return released([&] {
       return edsl_hip_token_logprobs_backward_launch(l.p, l.ld, l.type, tokens, ids64, lse, dlp, ent, dent, dl.p, dl.ld,
                                                      l.rows, l.cols, scale, stream);
+    });
+  });
+}
+
+namespace {
+
+// Whether a tensor is on the current device, and the caller's stream too.
+void require_here(const at::Tensor& t, PyObject* stream) {
+  const c10::impl::VirtualGuardImpl guard(t.device().type());
+  require(guard.getDevice() == t.device());
+  if (!given(stream)) return;
+  PyObject* const index = PyObject_GetAttrString(stream, "device_index");
+  if (index == nullptr) throw NotTaken{};
+  const long at = PyLong_AsLong(index);
+  Py_DECREF(index);
+  require(!PyErr_Occurred() && at == t.device().index());
+}
+
+// A stack of matrices [E][K][N] on `like`'s device, of K or N contiguous.
+struct Stack {
+  void* p = nullptr;
+  int64_t ld = 0, each = 0;
+  int type = 0, turned = 0;
+};
+Stack stack(PyObject* o, const at::Tensor& like, int64_t E, int64_t K, int64_t N) {
+  const at::Tensor& t = tensor(o);
+  require(t.is_cuda() && t.layout() == at::kStrided && t.dim() == 3 && t.device() == like.device());
+  require(t.size(0) == E && t.size(1) == K && t.size(2) == N);
+  const int64_t k = t.stride(1), n = t.stride(2);
+  Stack s{t.data_ptr(), k, t.stride(0), type_code(t.scalar_type()), 0};
+  if ((N <= 1 || n == 1) && (K <= 1 || k >= N)) return s;
+  require((K <= 1 || k == 1) && (N <= 1 || n >= K));
+  s.ld = n, s.turned = 1;
+  return s;
+}
+
+// Offsets of E groups.
+void* offsets_of(PyObject* o, const at::Tensor& like, int64_t E, int* ids64) {
+  require(given(o));
+  return ids(o, like, E + 1, ids64);
+}
+
+// A number for all rows, or one for each.
+struct Setting {
+  const void* each = nullptr;
+  double all = 0.0;
+};
+Setting setting(PyObject* o, const at::Tensor& like, int64_t n, at::ScalarType type) {
+  Setting s;
+  if (THPVariable_CheckExact(o)) {
+    const at::Tensor* const t = vec(o, like, n);
+    require(t->scalar_type() == type);
+    s.each = t->data_ptr();
+  } else if (type == at::kInt) {
+    require(PyLong_CheckExact(o));
+    const int64_t v = integer(o);
+    s.all = static_cast<double>(v < 0 ? 0 : v > 0x7fffffff ? 0x7fffffff : v);
+  } else {
+    require(PyFloat_CheckExact(o) || PyLong_CheckExact(o));
+    s.all = number(o);
+  }
+  return s;
+}
+
+}  // namespace
+
+// i8_dense(X, packed, K, N, b, Y, epilogue, alpha, x_scales, stream, current)
+PyObject* edsl_torch_i8_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return taken(args, n, 11, [](PyObject* const* a) {
+    const at::Tensor &X = tensor(a[0]), &W = tensor(a[1]);
+    const int64_t K = integer(a[2]), N = integer(a[3]);
+    const Mat x = mat(X), y = mat_like(a[5], X, x.rows, N);
+    require(x.cols == K && x.type == EDSL_LM_I8 && is_float(y.type) && W.is_cuda() && W.device() == X.device());
+    const at::Tensor* b = vec(a[4], X, N);
+    const int bt = b ? type_code(b->scalar_type()) : 0;
+    require(is_float(bt));
+    const float* const xs = vec_f32(a[8], X, x.rows);
+    const int epi = static_cast<int>(integer(a[6]));
+    const float alpha = number(a[7]);
+    require_here(X, a[9]);
+    void* const stream = stream_of(a[9], a[10]);
+    const void *const wp = W.data_ptr(), *const bp = b ? b->data_ptr() : nullptr;
+    return released([&] {
+      return edsl_hip_i8_dense_launch(static_cast<const int8_t*>(x.p), x.ld, xs, wp, bp, bt, y.p, y.ld, y.type, x.rows,
+                                      N, K, epi, alpha, stream);
+    });
+  });
+}
+
+// grouped_dense(X, W, offsets, b, Y, epilogue, alpha, stream, current)
+PyObject* edsl_torch_grouped_dense(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return taken(args, n, 9, [](PyObject* const* a) {
+    const at::Tensor &X = tensor(a[0]), &W = tensor(a[1]);
+    require(W.dim() == 3);
+    const Mat x = mat(X);
+    const int64_t E = W.size(0), N = W.size(2);
+    const Stack w = stack(a[1], X, E, x.cols, N);
+    int ids64 = 0;
+    void* const offsets = offsets_of(a[2], X, E, &ids64);
+    const Mat b = given(a[3]) ? mat_like(a[3], X, E, N) : Mat{};
+    const Mat y = mat_like(a[4], X, x.rows, N);
+    require(is_float(x.type) && w.type == x.type && y.type == x.type && (!given(a[3]) || b.type == x.type));
+    const int epi = static_cast<int>(integer(a[5]));
+    const float alpha = number(a[6]);
+    require_here(X, a[7]);
+    void* const stream = stream_of(a[7], a[8]);
+    return released([&] {
+      return edsl_hip_grouped_dense_launch(x.p, x.ld, w.p, w.ld, w.each, w.turned, offsets, ids64, E, b.p, b.ld, y.p,
+                                           y.ld, x.rows, N, x.cols, x.type, epi, alpha, stream);
+    });
+  });
+}
+
+// grouped_dense_backward(dY, X, W, offsets, dX, dW, db, Y, epilogue, alpha, stream, current)
+PyObject* edsl_torch_grouped_dense_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return taken(args, n, 12, [](PyObject* const* a) {
+    const at::Tensor &DY = tensor(a[0]), &O = tensor(a[3]);
+    const Mat dy = mat(DY);
+    require(is_float(dy.type) && O.dim() == 1 && O.size(0) > 0);
+    const int64_t E = O.size(0) - 1;
+    int ids64 = 0;
+    void* const offsets = offsets_of(a[3], DY, E, &ids64);
+    require((!given(a[4]) || given(a[2])) && (!given(a[5]) || given(a[1])));
+    int64_t K = 0;
+    for (const int i : {1, 4, 2, 5})
+      if (given(a[i])) {
+        require(tensor(a[i]).dim() >= 2);
+        K = tensor(a[i]).size(1);
+        break;
+      }
+    const Mat x = given(a[1]) ? mat_like(a[1], DY, dy.rows, K) : Mat{};
+    const Stack w = given(a[2]) ? stack(a[2], DY, E, K, dy.cols) : Stack{};
+    const Mat dx = given(a[4]) ? mat_like(a[4], DY, dy.rows, K) : Mat{};
+    const Stack dw = given(a[5]) ? stack(a[5], DY, E, K, dy.cols) : Stack{};
+    const Mat db = given(a[6]) ? mat_like(a[6], DY, E, dy.cols) : Mat{};
+    const Mat y = given(a[7]) ? mat_like(a[7], DY, dy.rows, dy.cols) : Mat{};
+    const auto same = [&](PyObject* o, int type) { return !given(o) || type == dy.type; };
+    const auto either = [&](PyObject* o, int type) { return same(o, type) || type == EDSL_LM_F32; };
+    require(same(a[1], x.type) && same(a[2], w.type) && same(a[4], dx.type) && same(a[7], y.type) &&
+            either(a[5], dw.type) && either(a[6], db.type));
+    require(!given(a[5]) || E <= 1 || dw.each != 0);
+    const int epi = static_cast<int>(integer(a[8]));
+    const float alpha = number(a[9]);
+    require_here(DY, a[10]);
+    void* const stream = stream_of(a[10], a[11]);
+    return released([&] {
+      return edsl_hip_grouped_dense_backward_launch(
+          dy.p, dy.ld, x.p, x.ld, w.p, w.ld, w.each, w.turned, offsets, ids64, E, y.p, y.ld, dx.p, dx.ld, dw.p, dw.ld,
+          dw.each, dw.turned, dw.type, db.p, db.ld, db.type, dy.rows, dy.cols, K, dy.type, epi, alpha, stream);
+    });
+  });
+}
+
+// sample_tokens(logits, uniforms, tokens, logprobs, temperature, top_k, top_p, min_p, stream, current)
+PyObject* edsl_torch_sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return taken(args, n, 10, [](PyObject* const* a) {
+    const at::Tensor& L = tensor(a[0]);
+    const Mat l = mat(L);
+    require(is_float(l.type) && given(a[1]) && given(a[2]));
+    const float* const u = vec_f32(a[1], L, l.rows);
+    int ids64 = 0;
+    void* const tokens = ids(a[2], L, l.rows, &ids64);
+    float* const lp = vec_f32(a[3], L, l.rows);
+    const Setting t = setting(a[4], L, l.rows, at::kFloat), k = setting(a[5], L, l.rows, at::kInt),
+                  p = setting(a[6], L, l.rows, at::kFloat), m = setting(a[7], L, l.rows, at::kFloat);
+    require_here(L, a[8]);
+    void* const stream = stream_of(a[8], a[9]);
+    return released([&] {
+      return edsl_hip_sample_tokens_launch(
+          l.p, l.ld, l.type, u, tokens, ids64, lp, static_cast<const float*>(t.each), static_cast<float>(t.all),
+          static_cast<const int32_t*>(k.each), static_cast<int>(k.all), static_cast<const float*>(p.each),
+          static_cast<float>(p.all), static_cast<const float*>(m.each), static_cast<float>(m.all), l.rows, l.cols,
+          stream);
     });
   });
 }

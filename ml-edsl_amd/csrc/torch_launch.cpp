@@ -108,6 +108,10 @@ PyMethodDef methods[] = {
     {"q4_dense", FAST(edsl_torch_q4_dense), "q4_dense_launch of lm.py"},
     {"token_logprobs", FAST(edsl_torch_token_logprobs), "token_logprobs_launch of lm.py"},
     {"token_logprobs_backward", FAST(edsl_torch_token_logprobs_backward), "token_logprobs_backward_launch of lm.py"},
+    {"i8_dense", FAST(edsl_torch_i8_dense), "i8_dense_launch of lm.py"},
+    {"grouped_dense", FAST(edsl_torch_grouped_dense), "grouped_dense_launch of lm.py"},
+    {"grouped_dense_backward", FAST(edsl_torch_grouped_dense_backward), "grouped_dense_backward_launch of lm.py"},
+    {"sample_tokens", FAST(edsl_torch_sample_tokens), "sample_tokens_launch of lm.py"},
     {nullptr, nullptr, 0, nullptr},
 };
 

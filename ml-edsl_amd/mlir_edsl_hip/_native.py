@@ -39,7 +39,9 @@ MEMREF_ENTRY_POINTS = {
 
 LM_ENTRY_POINTS = ("edsl_hip_rms_norm_launch", "edsl_hip_rms_norm_backward_launch",
                    "edsl_hip_token_logprobs_launch", "edsl_hip_token_logprobs_backward_launch",
-                   "edsl_hip_q4_pack_launch", "edsl_hip_q4_dense_launch")
+                   "edsl_hip_q4_pack_launch", "edsl_hip_q4_dense_launch",
+                   "edsl_hip_i8_pack_launch", "edsl_hip_i8_dense_launch", "edsl_hip_grouped_dense_launch",
+                   "edsl_hip_grouped_dense_backward_launch", "edsl_hip_sample_tokens_launch")
 LM_F32, LM_BF16, LM_F16, LM_I8, LM_E4M3 = range(5)  # EDSL_LM_* element types
 LM_MAX_TOP = 32  # EDSL_LM_MAX_TOP
 
@@ -105,10 +107,22 @@ def _declare(L: ctypes.CDLL) -> None:
     L.edsl_hip_q4_pack_launch.argtypes = [vp, i64, vp, i64, c_int, vp, i64, i64, i64, c_int, vp, ctypes.c_size_t, vp]
     L.edsl_hip_q4_dense_launch.argtypes = [vp, i64, c_int, vp, vp, vp, c_int, vp, i64, c_int, i64, i64, i64, c_int,
                                            c_int, c_int, c_int, c_float, vp]
+    L.edsl_hip_i8_pack_launch.argtypes = [vp, i64, vp, c_int, i64, i64, vp, ctypes.c_size_t, vp]
+    L.edsl_hip_i8_dense_launch.argtypes = [vp, i64, vp, vp, vp, c_int, vp, i64, c_int, i64, i64, i64, c_int, c_float,
+                                           vp]
+    L.edsl_hip_grouped_dense_launch.argtypes = [vp, i64, vp, i64, i64, c_int, vp, c_int, i64, vp, i64, vp, i64, i64,
+                                                i64, i64, c_int, c_int, c_float, vp]
+    L.edsl_hip_grouped_dense_backward_launch.argtypes = [
+        vp, i64, vp, i64, vp, i64, i64, c_int, vp, c_int, i64, vp, i64, vp, i64, vp, i64, i64, c_int, c_int, vp, i64,
+        c_int, i64, i64, i64, c_int, c_int, c_float, vp]
+    L.edsl_hip_sample_tokens_launch.argtypes = [vp, i64, c_int, vp, vp, c_int, vp, vp, c_float, vp, c_int, vp, c_float,
+                                                vp, c_float, i64, i64, vp]
     for name in LM_ENTRY_POINTS:
         getattr(L, name).restype = c_int
     L.edsl_hip_q4_packed_bytes.argtypes = [i64, i64, c_int, c_int, c_int]
     L.edsl_hip_q4_packed_bytes.restype = i64
+    L.edsl_hip_i8_packed_bytes.argtypes = [i64, i64]
+    L.edsl_hip_i8_packed_bytes.restype = i64
 
 
 def _share_torch_hip_runtime() -> None:

@@ -26,8 +26,10 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["gemm_f32.hip", "gemm_f32_m16.hip", "gemm_f32_direct.hip", "gemm_f32_small.hip", "gemm_f32_split.hip",
            "gemv_f32.hip", "gemm_i8.hip", "runtime.cpp", "plan_f32.cpp",
            "program.cpp", "host_stage.cpp", "noalloc.hip", "unfused.hip",
-           "lm_runtime.cpp", "lm_norm.hip", "lm_logprobs.hip", "q4_tile.hip", "q4_small_f32.hip",
-           "q4_small_bf16.hip", "q4_small_f16.hip", "q4_small_i8.hip", "q4_small_e4m3.hip"]
+           "lm_runtime.cpp", "lm_layers_runtime.cpp", "lm_norm.hip", "lm_logprobs.hip", "q4_tile.hip", "q4_small_f32.hip",
+           "q4_small_bf16.hip", "q4_small_f16.hip", "q4_small_i8.hip", "q4_small_e4m3.hip",
+           "lm_i8.hip", "lm_grouped_f32.hip", "lm_grouped_bf16.hip", "lm_grouped_f16.hip", "lm_grouped_act.hip",
+           "lm_sample.hip"]
 ARCH = "gfx950"
 
 # Packed fp32 VALU ops are disabled on purpose: the compiler would otherwise

@@ -14,8 +14,15 @@ and what the library refuses raises ``RuntimeError``.
   scales, and ``q4_quantize`` to make them.
 * ``token_logprobs_launch``, ``token_logprobs_backward_launch``: log
   probabilities of given tokens, log-sum-exp, entropy, top alternatives.
+* ``i8_pack``, ``i8_dense_launch``: the dense layer in 8-bit integers with a
+  scale for each row and column, and ``i8_quantize`` to make its weights.
+* ``grouped_dense_launch``, ``grouped_dense_backward_launch``: the dense layer
+  of experts, each on its own run of rows.
+* ``sample_tokens_launch``: tokens drawn with temperature, top-k, top-p, min-p.
 """
 from __future__ import annotations
+
+import operator
 
 from . import _native, device
 
@@ -323,3 +330,233 @@ def token_logprobs_backward_launch(logits, tokens, lse, dlogits, dlogprobs=None,
             _ptr(dlogprobs), _ptr(entropy), _ptr(dentropy), dlogits.data_ptr(), dlogits.stride(0), M, V, scale,
             _stream(stream)):
         _native.raise_on_error("token_logprobs_backward_launch")
+
+
+def _here(torch, t, name, stream):
+    """The launches below run on the current device."""
+    current = torch.cuda.current_device()
+    if t.device.index != current:
+        raise ValueError(f"{name} is on {t.device}, not on the current device cuda:{current}")
+    if stream is not None and stream.device != t.device:
+        raise ValueError(f"stream is of {stream.device}, {name} on {t.device}")
+
+
+class I8Weight:
+    """8-bit weights of a [K, N] layer as ``i8_pack`` laid them out."""
+
+    __slots__ = ("packed", "K", "N")
+
+    def __init__(self, packed, K, N):
+        self.packed, self.K, self.N = packed, K, N
+
+    def __repr__(self):
+        return f"I8Weight({self.K}x{self.N}, {self.packed.numel()} bytes on {self.packed.device})"
+
+
+def i8_quantize(W):
+    """8-bit integers [K, N] and scales [N] of a float matrix, each column's
+    largest value at 127: what ``i8_pack`` takes. Torch arithmetic, for the time
+    a model is loaded."""
+    torch = _torch()
+    if W.dim() != 2 or not W.is_floating_point() or W.shape[0] == 0:
+        raise ValueError(f"W must be a 2-D float matrix with rows, got {tuple(W.shape)} {W.dtype}")
+    w = W.float()
+    scales = w.abs().amax(0) / 127
+    q = torch.where(scales > 0, w / scales, 0.0).round().clamp(-127, 127)
+    return q.to(torch.int8), scales
+
+
+def i8_pack(Q, scales) -> I8Weight:
+    """Lays 8-bit weights out for ``i8_dense_launch``, once:
+    ``W[k, n] = scales[n] * Q[k, n]``, Q [K, N] int8 with 1 <= K < 2**17, scales
+    [N] in f32, bf16 or f16. Enqueued on the current stream."""
+    torch = _torch()
+    K, N = _matrix(Q, "Q", (torch.int8,))
+    _list(scales, "scales", (N,), _floats(torch), Q)
+    _here(torch, Q, "Q", None)
+    bytes_ = _native.lib().edsl_hip_i8_packed_bytes(K, N)
+    if bytes_ < 0:
+        _native.raise_on_error("i8_pack")
+    packed = torch.empty(bytes_, dtype=torch.uint8, device=Q.device)
+    if _native.lib().edsl_hip_i8_pack_launch(Q.data_ptr(), Q.stride(0), scales.data_ptr(), _types[scales.dtype], K, N,
+                                             packed.data_ptr(), bytes_, _stream(None)):
+        _native.raise_on_error("i8_pack")
+    return I8Weight(packed, K, N)
+
+
+def i8_dense_launch(X, W: I8Weight, b, Y, epilogue: int = _native.EPI_NONE, alpha: float = 0.0, x_scales=None,
+                    stream=None) -> None:
+    """``Y = epilogue(x_scales[:, None] * X @ W (+ b))``, with the epilogues of
+    ``device.dense_launch``.
+
+    X is [M, K] int8 and x_scales [M] f32 (the 8-bit norm's, say), W from
+    ``i8_pack``, Y [M, N] and b [N] in f32, bf16 or f16. Products and sums are
+    exact integers; the scales multiply the sum in 32 bits."""
+    torch = _torch()
+    if not isinstance(W, I8Weight):
+        raise TypeError("W is not an I8Weight")
+    if _native_module is not None and _done(
+            _native_module.i8_dense(X, W.packed, W.K, W.N, b, Y, epilogue, alpha, x_scales, stream,
+                                    device._raw_stream), "i8_dense_launch"):
+        return
+    M, K = _matrix(X, "X", (torch.int8,))
+    if K != W.K:
+        raise ValueError(f"shape mismatch: X{tuple(X.shape)} W{(W.K, W.N)}")
+    if W.packed.device != X.device:
+        raise ValueError(f"W is on {W.packed.device}, not on {X.device}")
+    _operand(Y, "Y", (M, W.N), _floats(torch), X)
+    if b is not None:
+        _list(b, "b", (W.N,), _floats(torch), X)
+    if x_scales is not None:
+        _list(x_scales, "x_scales", (M,), (torch.float32,), X)
+    _here(torch, X, "X", stream)
+    if _native.lib().edsl_hip_i8_dense_launch(
+            X.data_ptr(), X.stride(0), _ptr(x_scales), W.packed.data_ptr(), _ptr(b),
+            _types[b.dtype] if b is not None else 0, Y.data_ptr(), Y.stride(0), _types[Y.dtype], M, W.N, K, epilogue,
+            alpha, _stream(stream)):
+        _native.raise_on_error("i8_dense_launch")
+
+
+def _experts(t, name, shape, dtypes, like):
+    """A stack [E, K, N] of matrices: (row stride, stride between them, whether
+    K and not N is the contiguous index)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    (_, K, N), (each, k, n) = t.shape, t.stride()
+    if (N <= 1 or n == 1) and (K <= 1 or k >= N):
+        return k, each, False
+    if (K <= 1 or k == 1) and (N <= 1 or n >= K):
+        return n, each, True
+    raise ValueError(f"{name} must have unit stride along its rows or its columns, got strides {t.stride()}")
+
+
+def _offsets(torch, offsets, E, like):
+    _list(offsets, "offsets", (E + 1,), (torch.int32, torch.int64), like)
+    return offsets.dtype == torch.int64
+
+
+def grouped_dense_launch(X, W, offsets, b, Y, epilogue: int = _native.EPI_NONE, alpha: float = 0.0,
+                         stream=None) -> None:
+    """``Y[r] = epilogue(X[r] @ W[e] (+ b[e]))`` for the rows ``offsets[e] <= r <
+    offsets[e + 1]`` of each expert, with the epilogues of ``device.dense_launch``.
+
+    X is [T, K], W [E, K, N] with N or K contiguous (``transpose(1, 2)`` of [E,
+    N, K]), b [E, N], Y [T, N], all f32, bf16 or f16. offsets [E + 1], int32 or
+    int64, rise from 0 to T; they stay on the device, and experts may have no rows. Rows
+    of no expert are left as they are."""
+    torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.grouped_dense(X, W, offsets, b, Y, epilogue, alpha, stream, device._raw_stream),
+            "grouped_dense_launch"):
+        return
+    T, K = _matrix(X, "X", _floats(torch))
+    if W.dim() != 3:
+        raise ValueError(f"W must be 3-D, got {tuple(W.shape)}")
+    E, N = W.shape[0], W.shape[2]
+    ldw, each, turned = _experts(W, "W", (E, K, N), (X.dtype,), X)
+    ids64 = _offsets(torch, offsets, E, X)
+    if b is not None:
+        _operand(b, "b", (E, N), (X.dtype,), X)
+    _operand(Y, "Y", (T, N), (X.dtype,), X)
+    _here(torch, X, "X", stream)
+    if _native.lib().edsl_hip_grouped_dense_launch(
+            X.data_ptr(), X.stride(0), W.data_ptr(), ldw, each, turned, offsets.data_ptr(), ids64, E, _ptr(b), _ld(b),
+            Y.data_ptr(), Y.stride(0), T, N, K, _types[X.dtype], epilogue, alpha, _stream(stream)):
+        _native.raise_on_error("grouped_dense_launch")
+
+
+def grouped_dense_backward_launch(dY, X, W, offsets, dX=None, dW=None, db=None, Y=None,
+                                  epilogue: int = _native.EPI_NONE, alpha: float = 0.0, stream=None) -> None:
+    """The gradients of ``grouped_dense_launch``, each where it is given: dX
+    [T, K] of X's type (with W), dW [E, K, N] (with X) and db [E, N] in that type
+    or f32. dY is the gradient of Y; with an activation Y is what the forward pass
+    gave, and a leaky one needs alpha >= 0. Experts without rows have gradients
+    of 0; rows of no expert leave dX as it is. The same call gives the same bits."""
+    torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.grouped_dense_backward(dY, X, W, offsets, dX, dW, db, Y, epilogue, alpha, stream,
+                                                  device._raw_stream), "grouped_dense_backward_launch"):
+        return
+    T, N = _matrix(dY, "dY", _floats(torch))
+    if dX is not None and W is None:
+        raise ValueError("dX needs W")
+    if dW is not None and X is None:
+        raise ValueError("dW needs X")
+    if offsets.dim() != 1 or offsets.shape[0] == 0:
+        raise ValueError(f"offsets must be a vector of E + 1, got {tuple(offsets.shape)}")
+    E = offsets.shape[0] - 1
+    ids64 = _offsets(torch, offsets, E, dY)
+    either = (dY.dtype, torch.float32)
+    K = next((t.shape[1] for t in (X, dX, W, dW) if t is not None and t.dim() >= 2), 0)
+    ldw = each = lddw = each_dw = 0
+    turned = dw_turned = False
+    if X is not None:
+        _operand(X, "X", (T, K), (dY.dtype,), dY)
+    if W is not None:
+        ldw, each, turned = _experts(W, "W", (E, K, N), (dY.dtype,), dY)
+    if dX is not None:
+        _operand(dX, "dX", (T, K), (dY.dtype,), dY)
+    if dW is not None:
+        lddw, each_dw, dw_turned = _experts(dW, "dW", (E, K, N), either, dY)
+        if E > 1 and each_dw == 0:
+            raise ValueError("dW has one matrix for several experts")
+    if db is not None:
+        _operand(db, "db", (E, N), either, dY)
+    if Y is not None:
+        _operand(Y, "Y", (T, N), (dY.dtype,), dY)
+    _here(torch, dY, "dY", stream)
+    if _native.lib().edsl_hip_grouped_dense_backward_launch(
+            dY.data_ptr(), dY.stride(0), _ptr(X), _ld(X), _ptr(W), ldw, each, turned, offsets.data_ptr(), ids64, E,
+            _ptr(Y), _ld(Y), _ptr(dX), _ld(dX), _ptr(dW), lddw, each_dw, dw_turned,
+            _types[dW.dtype] if dW is not None else 0, _ptr(db), _ld(db), _types[db.dtype] if db is not None else 0,
+            T, N, K, _types[dY.dtype], epilogue, alpha, _stream(stream)):
+        _native.raise_on_error("grouped_dense_backward_launch")
+
+
+def sample_tokens_launch(logits, uniforms, tokens, logprobs=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                         stream=None) -> None:
+    """Draws a token for each row of logits [M, V] (f32, bf16, f16) with the
+    given numbers uniforms [M] f32 in [0, 1).
+
+    Under ``softmax(logits / temperature)`` kept are the top_k largest (equal
+    ones by their index), of these in falling order those with less than top_p
+    of their mass before them, and of these the ones with at least min_p of the
+    largest one's probability. The token is the first index at which the running sum of
+    the kept ones, by index, exceeds that share of their mass. temperature 0 takes
+    the largest; top_k 0, top_p 1 and min_p 0 leave their step out. Each setting
+    is a number or one for each row, [M] f32 (top_k int32).
+    tokens [M] int64 or int32; logprobs [M] f32 receives the log probability among
+    the kept ones. A row of -inf alone gives -1 and -inf, one with a NaN, +inf
+    or a setting of no meaning -1 and NaN. The same call gives the same tokens."""
+    torch = _torch()
+    if _native_module is not None and _done(
+            _native_module.sample_tokens(logits, uniforms, tokens, logprobs, temperature, top_k, top_p, min_p, stream,
+                                         device._raw_stream), "sample_tokens_launch"):
+        return
+    M, V = _matrix(logits, "logits", _floats(torch))
+    _list(uniforms, "uniforms", (M,), (torch.float32,), logits)
+    ids64 = _tokens(torch, tokens, logits)
+    if logprobs is not None:
+        _list(logprobs, "logprobs", (M,), (torch.float32,), logits)
+    settings = []
+    for value, name, dtype, kind in ((temperature, "temperature", torch.float32, float),
+                                     (top_k, "top_k", torch.int32, int), (top_p, "top_p", torch.float32, float),
+                                     (min_p, "min_p", torch.float32, float)):
+        if isinstance(value, torch.Tensor):
+            _list(value, name, (M,), (dtype,), logits)
+            settings += [value.data_ptr(), 0]
+        else:
+            if kind is int:
+                value = max(0, min(operator.index(value), 2**31 - 1))
+            settings += [None, kind(value)]
+    _here(torch, logits, "logits", stream)
+    if _native.lib().edsl_hip_sample_tokens_launch(
+            logits.data_ptr(), logits.stride(0), _types[logits.dtype], uniforms.data_ptr(), tokens.data_ptr(), ids64,
+            _ptr(logprobs), *settings, M, V, _stream(stream)):
+        _native.raise_on_error("sample_tokens_launch")
