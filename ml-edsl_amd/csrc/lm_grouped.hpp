@@ -34,36 +34,42 @@ struct RowTile {
 };
 
 // The tiles of `bm` rows of experts of more than `skip` rows, over all experts, by a
-// wave: a lane holds one expert of each 64.
+// wave: a lane holds one expert of each 64. Whole tiles are numbered apart from the
+// last ones of experts, which have fewer rows.
 struct RowTiles {
   const GroupOffsets& g;
   int bm, skip;
 
-  __device__ __forceinline__ int of(int e, int64_t* first, int64_t* end) const {
+  // Whole tiles of an expert, and whether it has another one.
+  __device__ __forceinline__ int of(int e, int64_t* first, int64_t* end, int* part) const {
+    *part = 0;
     if (e >= g.experts) return 0;
     *first = g.at(e);
     *end = g.at(e + 1);
     const int64_t n = *end - *first;
-    return n > skip ? (int)((n + bm - 1) / bm) : 0;
+    if (n <= skip || n <= 0) return 0;
+    *part = n % bm != 0;
+    return (int)(n / bm);
   }
-  __device__ __forceinline__ int64_t total() const {
-    int64_t total = 0;
+  __device__ __forceinline__ void total(int64_t* whole, int64_t* parts) const {
+    *whole = *parts = 0;
     for (int e = 0; e < g.experts; e += 64) {
       int64_t first, end;
-      int sum = of(e + (int)threadIdx.x % 64, &first, &end);
+      int part, sum = of(e + (int)threadIdx.x % 64, &first, &end, &part);
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-      total += __builtin_amdgcn_readfirstlane(sum);
+      *whole += __builtin_amdgcn_readfirstlane(sum);
+      *parts += __popcll(__ballot(part));
     }
-    return total;
   }
-  // Tile `t`; false where there are fewer.
-  __device__ __forceinline__ bool find(int64_t t, RowTile* tile) const {
+  // Whole tile `t`, or part `t`; false where there are fewer.
+  __device__ __forceinline__ bool find(bool parts, int64_t t, RowTile* tile) const {
     const int lane = threadIdx.x % 64;
     int64_t before = 0;
     for (int e = 0; e < g.experts; e += 64) {
       int64_t first = 0, end = 0;
-      const int mine = of(e + lane, &first, &end);
+      int part;
+      const int whole = of(e + lane, &first, &end, &part), mine = parts ? part : whole;
       int upto = mine;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) {
@@ -73,8 +79,8 @@ struct RowTiles {
       const uint64_t past = __ballot(before + upto > t);
       if (past) {
         const int l = __builtin_ctzll(past);
-        const int64_t row = __shfl(first, l) + (t - before - (__shfl(upto, l) - __shfl(mine, l))) * bm;
-        *tile = {__builtin_amdgcn_readfirstlane(e + l), uniform(row), uniform(__shfl(end, l))};
+        const int64_t at = parts ? __shfl(whole, l) : t - before - (__shfl(upto, l) - __shfl(mine, l));
+        *tile = {__builtin_amdgcn_readfirstlane(e + l), uniform(__shfl(first, l) + at * bm), uniform(__shfl(end, l))};
         return true;
       }
       before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
@@ -87,34 +93,14 @@ struct RowTiles {
   }
 };
 
-// Workgroup w's tile and column strip: eight row tiles go along the columns together,
-// one XCD's workgroups among them.
-__device__ __forceinline__ bool find_tile(const RowTiles& tiles, int tiles_n, int64_t w, RowTile* tile, int* tn) {
-  // Offsets that do not rise could make more than the grid is made for.
-  const int64_t total = min(tiles.total(), (int64_t)(0x7fffffff / tiles_n));
-  if (w >= total * tiles_n) return false;
-  const int at = xcd_order((int)w, (int)(total * tiles_n));
-  constexpr int kGroup = 8;
-  const int group = at / (kGroup * tiles_n), first = group * kGroup;
-  const int rows = min((int)total - first, kGroup), in = at - group * kGroup * tiles_n;
-  *tn = in / rows;
-  return tiles.find(first + in % rows, tile);
-}
-
 __device__ __forceinline__ GroupOffsets offsets_of(const GroupedArgs& a) {
   return {a.offsets, a.T, a.E, a.ids64};
 }
 
+// One tile: rows `first` to `end` at most, columns from n0 to `stop` at most.
 template <typename Tl, int BKIND>
-__global__ void __launch_bounds__(Tl::kThreads, 1) grouped_rows_kernel(GroupedArgs a) {
+__device__ __forceinline__ void grouped_rows_tile(const GroupedArgs& a, const RowTile& t, int n0, u32x4* lds) {
   using T = typename Tl::T;
-  __shared__ u32x4 lds[2 * Tl::kStage];
-  const int tiles_n = (int)((a.N + Tl::BN - 1) / Tl::BN);
-  RowTile t;
-  int tn;
-  const GroupOffsets g = offsets_of(a);
-  if (!find_tile(RowTiles{g, Tl::BM, a.skip}, tiles_n, block_of(), &t, &tn)) return;
-  const int n0 = tn * Tl::BN;
   const TileOperand oa{static_cast<const char*>(a.x) + t.first * a.ldx * (int64_t)sizeof(T), a.ldx,
                        (int)min(t.end - t.first, (int64_t)Tl::BM)};
   const TileOperand ob{static_cast<const char*>(a.w) +
@@ -139,6 +125,44 @@ __global__ void __launch_bounds__(Tl::kThreads, 1) grouped_rows_kernel(GroupedAr
       activate(v, a.epi, a.alpha);
       put4(static_cast<T*>(a.y) + row * a.ldy + n, v, left);
     }
+  }
+}
+
+// Big tiles, and Half (half as many columns) and Quarter ones for what is left of a round; the
+// same type where there are none.
+template <typename Big, typename Half, typename Quarter, int BKIND>
+__global__ void __launch_bounds__(Big::kThreads, 1) grouped_rows_kernel(GroupedArgs a) {
+  static_assert(Big::kThreads == Half::kThreads && Big::kThreads == Quarter::kThreads, "one launch");
+  constexpr int kLds = Big::kLds > Half::kLds ? (Big::kLds > Quarter::kLds ? Big::kLds : Quarter::kLds)
+                                              : (Half::kLds > Quarter::kLds ? Half::kLds : Quarter::kLds);
+  __shared__ u32x4 lds[kLds];
+  const int tiles_n = (int)((a.N + Big::BN - 1) / Big::BN);
+  const GroupOffsets g = offsets_of(a);
+  const RowTiles tiles{g, Big::BM, a.skip};
+  int64_t whole, parts;
+  tiles.total(&whole, &parts);
+  // Offsets that do not rise could make more tiles than the grid is made for.
+  const int most = 0x3fffffff / tiles_n;
+  whole = min(whole, (int64_t)most), parts = min(parts, most - whole);
+  TileTurn turn;
+  if (!tile_turn((int)block_of(), (int)(whole + parts) * tiles_n, (int)whole * tiles_n, a.rounds, &turn)) return;
+  // Whole tiles first, then the experts' last ones.
+  const bool part = turn.tile >= whole * tiles_n;
+  int tn;
+  const int row = row_of_tile(turn.tile - (part ? (int)whole * tiles_n : 0), (int)(part ? parts : whole), tiles_n, &tn);
+  RowTile t;
+  if (!tiles.find(part, row, &t)) return;
+  t.end = min(t.end, t.first + Big::BM);
+  int n0 = tn * Big::BN;
+  if (turn.pieces == 1) return grouped_rows_tile<Big, BKIND>(a, t, n0, lds);
+  n0 += turn.sub % 2 * (Big::BN / 2);
+  t.first += turn.sub / 2 * (Big::BM / 2);
+  if (n0 >= a.N || t.first >= t.end) return;
+  if constexpr (!std::is_same<Half, Quarter>::value)
+    if (turn.pieces == 2) return grouped_rows_tile<Half, BKIND>(a, t, n0, lds);
+  if constexpr (!std::is_same<Big, Quarter>::value) {
+    t.end = min(t.end, t.first + Quarter::BM);
+    grouped_rows_tile<Quarter, BKIND>(a, t, n0, lds);
   }
 }
 
@@ -171,17 +195,16 @@ __global__ void __launch_bounds__(64 * WAVES) grouped_skinny_kernel(GroupedArgs 
 template <typename Tl>
 __global__ void __launch_bounds__(Tl::kThreads, 1) grouped_weights_kernel(GroupedWeightArgs a) {
   using T = typename Tl::T;
-  __shared__ u32x4 lds[2 * Tl::kStage];
+  __shared__ u32x4 lds[Tl::kLds];
   const int tiles_m = (int)((a.M + Tl::BM - 1) / Tl::BM), tiles_n = (int)((a.N + Tl::BN - 1) / Tl::BN);
   const int64_t total = (int64_t)tiles_m * tiles_n * a.E;
   if (block_of() >= total) return;
-  const int at = xcd_order((int)block_of(), (int)total);
-  const int expert = at / (tiles_m * tiles_n);
-  int in = at - expert * tiles_m * tiles_n;
-  constexpr int kGroup = 8;
-  const int group = in / (kGroup * tiles_n), first_m = group * kGroup, rows_m = min(tiles_m - first_m, kGroup);
-  in -= group * kGroup * tiles_n;
-  const int m0 = (first_m + in % rows_m) * Tl::BM, n0 = in / rows_m * Tl::BN;
+  // Each XCD has a part of every expert: their depths differ.
+  const int expert = (int)(block_of() / (uint32_t)(tiles_m * tiles_n));
+  int tn;
+  const int tm = row_of_tile(xcd_order((int)(block_of() % (uint32_t)(tiles_m * tiles_n)), tiles_m * tiles_n), tiles_m,
+                             tiles_n, &tn);
+  const int m0 = tm * Tl::BM, n0 = tn * Tl::BN;
   const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
   const int64_t first = g.at(expert), rows = max(g.at(expert + 1) - first, (int64_t)0);
   const TileOperand oa{static_cast<const char*>(a.a) + (first * a.lda + m0) * (int64_t)sizeof(T), a.lda, (int)(a.M - m0)};

@@ -22,8 +22,13 @@ __global__ void __launch_bounds__(64 * kActWaves) grouped_act_kernel(GroupedActA
   // The tile's number is its place among the partial sums: no other order.
   const int w = (int)block_of(), tile = w / tiles_n;
   const int64_t col = (int64_t)(w % tiles_n) * COLS + lane * VEC;
+  // Whole tiles of rows first, then the experts' last ones.
+  const RowTiles tiles{g, kActRows, 0};
+  int64_t whole, parts;
+  tiles.total(&whole, &parts);
+  const bool part = tile >= whole;
   RowTile t;
-  if (!RowTiles{g, kActRows, 0}.find(tile, &t)) return;
+  if (!tiles.find(part, part ? tile - whole : tile, &t)) return;
   const int64_t end = min(t.first + kActRows, t.end);
   float sum[VEC] = {};
   for (int64_t row = t.first + wave; row < end; row += kActWaves) {
@@ -65,20 +70,23 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
   const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
   const int expert = blockIdx.y;
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const auto tiles_of = [&](int e) {
-    const int64_t rows = g.at(e + 1) - g.at(e);
-    return rows > 0 ? (rows + kActRows - 1) / kActRows : 0;
-  };
+  const auto rows_of = [&](int e) { return max(g.at(e + 1) - g.at(e), (int64_t)0); };
+  // The expert's whole tiles, and the place of its last one behind all whole tiles.
   const int lane = threadIdx.x % 64;
-  int64_t before = 0;
-  for (int e = lane; e < expert; e += 64) before += tiles_of(e);
+  int64_t before = 0, all = 0, parts = 0;
+  for (int e = lane; e < a.E; e += 64) {
+    const int64_t rows = rows_of(e);
+    all += rows / kActRows;
+    if (e < expert) before += rows / kActRows, parts += rows % kActRows != 0;
+  }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d);
+  for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d), all += __shfl_xor(all, d), parts += __shfl_xor(parts, d);
   if (n >= a.N) return;
   const int64_t most = grouped_act_tiles(a.T, a.E);  // what the partial sums have room for
-  const int64_t tiles = min(tiles_of(expert), max(most - before, (int64_t)0));
+  const int64_t rows = rows_of(expert), tiles = min(rows / kActRows, max(most - before, (int64_t)0));
   float s = 0.0f;
   for (int64_t t = 0; t < tiles; ++t) s += a.partials[(before + t) * a.N + n];
+  if (rows % kActRows != 0 && all + parts < most) s += a.partials[(all + parts) * a.N + n];
   const int64_t at = expert * a.lddb + n;
   if (a.db_type == kF32)
     static_cast<float*>(a.db)[at] = s;

@@ -5,16 +5,16 @@ namespace edsl {
 namespace lm {
 
 template <>
-hipError_t launch_grouped_rows<kF16>(const GroupedArgs& a, int tile, hipStream_t stream) {
-  return GroupedLaunch<f16>::rows(a, tile, stream);
+hipError_t launch_grouped_rows<kF16>(const GroupedArgs& a, int loads, hipStream_t stream) {
+  return GroupedLaunch<f16>::rows(a, loads, stream);
 }
 template <>
 hipError_t launch_grouped_skinny<kF16>(const GroupedArgs& a, hipStream_t stream) {
   return GroupedLaunch<f16>::skinny(a, stream);
 }
 template <>
-hipError_t launch_grouped_weights<kF16>(const GroupedWeightArgs& a, int tile, hipStream_t stream) {
-  return GroupedLaunch<f16>::weights(a, tile, stream);
+hipError_t launch_grouped_weights<kF16>(const GroupedWeightArgs& a, int loads, bool big, hipStream_t stream) {
+  return GroupedLaunch<f16>::weights(a, loads, big, stream);
 }
 
 }  // namespace lm

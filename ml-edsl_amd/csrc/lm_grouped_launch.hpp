@@ -10,24 +10,38 @@ namespace lm {
 
 template <typename T>
 struct GroupedLaunch {
-  template <typename Tl, int BKIND>
-  static hipError_t rows_tile(const GroupedArgs& a, hipStream_t stream) {
+  template <int BKIND, typename Big, typename Half = Big, typename Quarter = Half>
+  static hipError_t rows_tiles(GroupedArgs a, int quarters, int halves, hipStream_t stream) {
     // The most tiles that T rows in E groups can have.
     const int64_t groups = std::min<int64_t>(a.E, a.T / (a.skip + 1));
-    const int64_t tiles = (a.T / Tl::BM + groups) * ((a.N + Tl::BN - 1) / Tl::BN);
+    const int64_t tiles = (a.T / Big::BM + groups) * ((a.N + Big::BN - 1) / Big::BN);
     if (tiles == 0) return hipSuccess;
-    hipLaunchKernelGGL((grouped_rows_kernel<Tl, BKIND>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
+    a.rounds = {a.cus, quarters, halves};
+    hipLaunchKernelGGL((grouped_rows_kernel<Big, Half, Quarter, BKIND>), grid_of(tile_turns(tiles, a.rounds)),
+                       dim3(Big::kThreads), 0, stream, a);
     return launched();
   }
-  template <int BKIND>
-  static hipError_t rows_kind(const GroupedArgs& a, int tile, hipStream_t stream) {
-    if (tile == kGroupedTileAny) return rows_tile<Tile<T, kRows, BKIND, 128, 128, 2, 2, false>, BKIND>(a, stream);
-    if constexpr (sizeof(T) == 2)
-      if (tile == kGroupedTile256) return rows_tile<Tile<T, kRows, BKIND, 256, 256, 2, 4, true>, BKIND>(a, stream);
-    return rows_tile<Tile<T, kRows, BKIND, 128, 128, 2, 2, true>, BKIND>(a, stream);
+  template <int BKIND, int LOADS>
+  static hipError_t rows_loads(const GroupedArgs& a, hipStream_t stream) {
+    if constexpr (LOADS == 0)
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, 0>>(a, 0, 0, stream);
+    else if constexpr (sizeof(T) == 4)
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, LOADS>, Tile<T, kRows, BKIND, 64, 64, 2, 4, LOADS>>(
+          a, a.cus * 3 / 4, 0, stream);
+    else if constexpr (LOADS == 4)
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, 4, 3>>(a, 0, 0, stream);
+    else
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 256, 256, 2, 4, 16>, Tile<T, kRows, BKIND, 256, 128, 4, 2, 16, 3>,
+                        Tile<T, kRows, BKIND, 128, 128, 2, 4, 16, 3>>(a, a.cus / 4, a.cus / 2, stream);
   }
-  static hipError_t rows(const GroupedArgs& a, int tile, hipStream_t stream) {
-    return a.turned ? rows_kind<kRows>(a, tile, stream) : rows_kind<kCols>(a, tile, stream);
+  template <int BKIND>
+  static hipError_t rows_kind(const GroupedArgs& a, int loads, hipStream_t stream) {
+    return loads == 16  ? rows_loads<BKIND, 16>(a, stream)
+           : loads == 4 ? rows_loads<BKIND, 4>(a, stream)
+                        : rows_loads<BKIND, 0>(a, stream);
+  }
+  static hipError_t rows(const GroupedArgs& a, int loads, hipStream_t stream) {
+    return a.turned ? rows_kind<kRows>(a, loads, stream) : rows_kind<kCols>(a, loads, stream);
   }
 
   template <int BKIND, int NJ>
@@ -49,11 +63,12 @@ struct GroupedLaunch {
     hipLaunchKernelGGL((grouped_weights_kernel<Tl>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
     return launched();
   }
-  static hipError_t weights(const GroupedWeightArgs& a, int tile, hipStream_t stream) {
-    if (tile == kGroupedTileAny) return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 2, false>>(a, stream);
+  static hipError_t weights(const GroupedWeightArgs& a, int loads, bool big, hipStream_t stream) {
+    if (loads == 0) return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, 0>>(a, stream);
+    if (loads == 4) return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, 4>>(a, stream);
     if constexpr (sizeof(T) == 2)
-      if (tile == kGroupedTile256) return weights_tile<Tile<T, kCols, kCols, 256, 256, 2, 4, true>>(a, stream);
-    return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 2, true>>(a, stream);
+      if (big) return weights_tile<Tile<T, kCols, kCols, 256, 256, 2, 4, 16>>(a, stream);
+    return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, 16>>(a, stream);
   }
 };
 

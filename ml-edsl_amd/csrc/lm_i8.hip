@@ -50,15 +50,7 @@ __global__ void __launch_bounds__(256) i8_pack_kernel(I8PackArgs a) {
 }
 
 template <typename Tl>
-__global__ void __launch_bounds__(Tl::kThreads, 1) i8_tile_kernel(I8Args a) {
-  __shared__ u32x4 lds[2 * Tl::kStage];
-  const int tiles_m = (a.M + Tl::BM - 1) / Tl::BM, tiles_n = (a.N + Tl::BN - 1) / Tl::BN;
-  if (block_of() >= (uint32_t)tiles_m * tiles_n) return;
-  int at = xcd_order((int)block_of(), tiles_m * tiles_n);
-  constexpr int kGroup = 8;
-  const int group = at / (kGroup * tiles_n), first_m = group * kGroup, rows_m = min(tiles_m - first_m, kGroup);
-  at -= group * kGroup * tiles_n;
-  const int m0 = (first_m + at % rows_m) * Tl::BM, n0 = at / rows_m * Tl::BN;
+__device__ __forceinline__ void i8_tile(const I8Args& a, int m0, int n0, u32x4* lds) {
   const int64_t tile_bytes = i8_blocks(a.K) * 1024;
   const TileOperand oa{reinterpret_cast<const char*>(a.x) + m0 * a.ldx, a.ldx, min(a.M - m0, Tl::BM)};
   const TileOperand ob{a.w + n0 / 16 * tile_bytes, tile_bytes, min(a.N - n0, Tl::BN)};
@@ -94,6 +86,27 @@ __global__ void __launch_bounds__(Tl::kThreads, 1) i8_tile_kernel(I8Args a) {
   }
 }
 
+// Big tiles, and Half and Quarter ones for what is left of a round of the CUs.
+template <typename Big, typename Half, typename Quarter>
+__global__ void __launch_bounds__(Big::kThreads, 1) i8_tile_kernel(I8Args a) {
+  constexpr int kLds = Big::kLds > Half::kLds ? (Big::kLds > Quarter::kLds ? Big::kLds : Quarter::kLds)
+                                              : (Half::kLds > Quarter::kLds ? Half::kLds : Quarter::kLds);
+  __shared__ u32x4 lds[kLds];
+  const int tiles_m = (a.M + Big::BM - 1) / Big::BM, tiles_n = (a.N + Big::BN - 1) / Big::BN;
+  TileTurn turn;
+  if (!tile_turn((int)block_of(), tiles_m * tiles_n, tiles_m * tiles_n, a.rounds, &turn)) return;
+  int tn;
+  int m0 = row_of_tile(turn.tile, tiles_m, tiles_n, &tn) * Big::BM, n0 = tn * Big::BN;
+  if (turn.pieces == 1) return i8_tile<Big>(a, m0, n0, lds);
+  n0 += turn.sub % 2 * (Big::BN / 2);
+  m0 += turn.sub / 2 * (Big::BM / 2);
+  if (n0 >= a.N || m0 >= a.M) return;
+  if constexpr (!std::is_same<Big, Quarter>::value) {
+    if (turn.pieces == 2) return i8_tile<Half>(a, m0, n0, lds);
+    i8_tile<Quarter>(a, m0, n0, lds);
+  }
+}
+
 template <int MT, int NJ, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) i8_skinny_kernel(I8Args a) {
   using S = Skinny<int8_t, kBlocks, MT, NJ, WAVES>;
@@ -113,10 +126,12 @@ __global__ void __launch_bounds__(64 * WAVES) i8_skinny_kernel(I8Args a) {
          });
 }
 
-template <typename Tl>
-hipError_t launch_tile(const I8Args& a, hipStream_t stream) {
-  const int64_t tiles = (int64_t)((a.M + Tl::BM - 1) / Tl::BM) * ((a.N + Tl::BN - 1) / Tl::BN);
-  hipLaunchKernelGGL((i8_tile_kernel<Tl>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
+template <typename Big, typename Half = Big, typename Quarter = Half>
+hipError_t launch_tiles(I8Args a, int quarters, int halves, hipStream_t stream) {
+  const int64_t tiles = (int64_t)((a.M + Big::BM - 1) / Big::BM) * ((a.N + Big::BN - 1) / Big::BN);
+  a.rounds = {a.cus, quarters, halves};
+  hipLaunchKernelGGL((i8_tile_kernel<Big, Half, Quarter>), grid_of(tile_turns(tiles, a.rounds)), dim3(Big::kThreads), 0,
+                     stream, a);
   return launched();
 }
 
@@ -138,10 +153,10 @@ hipError_t launch_i8_pack(const I8PackArgs& a, hipStream_t stream) {
   return launched();
 }
 
-hipError_t launch_i8_tile(const I8Args& a, int tile, hipStream_t stream) {
-  if (tile == kI8Tile256) return launch_tile<Tile<int8_t, kRows, kBlocks, 256, 256, 2, 4, true>>(a, stream);
-  if (tile == kI8Tile128) return launch_tile<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 2, true>>(a, stream);
-  return launch_tile<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 2, false>>(a, stream);
+hipError_t launch_i8_tile(const I8Args& a, int loads, hipStream_t stream) {
+  if (loads == 0) return launch_tiles<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 4, 0>>(a, 0, 0, stream);
+  return launch_tiles<Tile<int8_t, kRows, kBlocks, 256, 256, 2, 4, 16>, Tile<int8_t, kRows, kBlocks, 256, 128, 4, 2, 16, 3>,
+                      Tile<int8_t, kRows, kBlocks, 128, 128, 2, 4, 16, 3>>(a, a.cus / 4, a.cus / 2, stream);
 }
 
 hipError_t launch_i8_skinny(const I8Args& a, int cols16, hipStream_t stream) {

@@ -103,6 +103,10 @@ struct SampleArgs {
 hipError_t launch_sample_tokens(const SampleArgs& a, hipStream_t stream);
 
 // --------------------------------------------------- layers on groups of rows
+// How tiles fill the CUs (lm_tile.hpp).
+struct TileRounds {
+  int cus, quarters, halves;
+};
 struct GroupedArgs {
   const void* x;
   const void* w;        // expert e at w + e * stride_w
@@ -115,12 +119,14 @@ struct GroupedArgs {
   float alpha;
   bool ids64;
   bool turned;  // w's k are contiguous, not its columns
+  int cus;
+  TileRounds rounds;
 };
 constexpr int kGroupedSkinnyRows = 32;  // experts with up to this many rows may stream their weights
-// Whether tiles read the operands where they are, by asynchronous loads.
-enum GroupedTile : int { kGroupedTile256 = 0, kGroupedTile128 = 1, kGroupedTileAny = 2 };
+// How tiles take their operands: `loads` bytes a lane at a time, 16 or 4, where all rows start on so many and
+// are whole multiples of them along K; 0: any.
 template <int TYPE>
-hipError_t launch_grouped_rows(const GroupedArgs& a, int tile, hipStream_t stream);
+hipError_t launch_grouped_rows(const GroupedArgs& a, int loads, hipStream_t stream);
 template <int TYPE>
 hipError_t launch_grouped_skinny(const GroupedArgs& a, hipStream_t stream);
 
@@ -134,7 +140,7 @@ struct GroupedWeightArgs {
   bool ids64;
 };
 template <int TYPE>
-hipError_t launch_grouped_weights(const GroupedWeightArgs& a, int tile, hipStream_t stream);
+hipError_t launch_grouped_weights(const GroupedWeightArgs& a, int loads, bool big, hipStream_t stream);
 
 // dz = dy * act'(y), and the sums of dz over each expert's rows.
 struct GroupedActArgs {
@@ -177,9 +183,10 @@ struct I8Args {
   int64_t ldx, ldy;
   int M, N, K, epi, y_type, bias_type;
   float alpha;
+  int cus;
+  TileRounds rounds;
 };
-enum I8Tile : int { kI8Tile256 = 0, kI8Tile128 = 1, kI8TileAny = 2 };
-hipError_t launch_i8_tile(const I8Args& a, int tile, hipStream_t stream);
+hipError_t launch_i8_tile(const I8Args& a, int loads, hipStream_t stream);
 hipError_t launch_i8_skinny(const I8Args& a, int cols16, hipStream_t stream);
 
 }  // namespace lm

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/edsl_hip_lm.h"
 #include "dev_buf.hpp"
@@ -18,6 +19,15 @@ constexpr int64_t kMostI8Depth = (int64_t(1) << 17) - 1;  // K 2^14 < 2^31: 32-b
 constexpr int kMostExperts = 65535;
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// A tile's rows of `ld` elements within the 31 bits of an asynchronous load's offset.
+bool reachable(int64_t rows, int64_t ld, int e) { return rows * ld * e < 0x7fffffff; }
+// The bytes that all of these are multiples of, 16, 4 or 0 (fewer).
+int common_bytes(std::initializer_list<int64_t> values) {
+  int64_t all = 0;
+  for (const int64_t v : values) all |= v;
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 0;
+}
+int64_t address(const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); }
 
 void check_epilogue(int epi) {
   if (epi < 0 || epi > 7) fail(kErrArgument, "bad epilogue code %d", epi);
@@ -74,14 +84,11 @@ void i8_dense(lm::I8Args a, int64_t M, int64_t N, int64_t K, void* stream) {
       set_plan("i8_skinny cols=%d", 16 * cols);
       return;
     }
-    const bool direct = aligned16(a.x) && a.ldx % 16 == 0 && K % 16 == 0 && 256 * a.ldx < 0x7fffffff;
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    const int tile = !direct ? lm::kI8TileAny : big >= cus ? lm::kI8Tile256 : lm::kI8Tile128;
-    const int64_t side = tile == lm::kI8Tile256 ? 256 : 128;
-    check_grid((M + side - 1) / side, (N + side - 1) / side);
-    check_hip(lm::launch_i8_tile(a, tile, s), "i8_tile launch");
-    static const char* const names[] = {"256x256", "128x128", "128x128 any"};
-    set_plan("i8_tile tile=%s", names[tile]);
+    const int loads = aligned16(a.x) && a.ldx % 16 == 0 && K % 16 == 0 && reachable(256, a.ldx, 1) ? 16 : 0;
+    check_grid((M + 127) / 128 + 4, (N + 127) / 128 + 4);
+    a.cus = cus;
+    check_hip(lm::launch_i8_tile(a, loads, s), "i8_tile launch");
+    set_plan("i8_tile loads=%d", loads);
   });
 }
 
@@ -108,43 +115,37 @@ hipError_t skinny_by_type(const lm::GroupedArgs& a, hipStream_t s) {
          : a.type == lm::kBf16 ? lm::launch_grouped_skinny<lm::kBf16>(a, s)
                                : lm::launch_grouped_skinny<lm::kF16>(a, s);
 }
-hipError_t rows_by_type(const lm::GroupedArgs& a, int tile, hipStream_t s) {
-  return a.type == lm::kF32    ? lm::launch_grouped_rows<lm::kF32>(a, tile, s)
-         : a.type == lm::kBf16 ? lm::launch_grouped_rows<lm::kBf16>(a, tile, s)
-                               : lm::launch_grouped_rows<lm::kF16>(a, tile, s);
+hipError_t rows_by_type(const lm::GroupedArgs& a, int loads, hipStream_t s) {
+  return a.type == lm::kF32    ? lm::launch_grouped_rows<lm::kF32>(a, loads, s)
+         : a.type == lm::kBf16 ? lm::launch_grouped_rows<lm::kBf16>(a, loads, s)
+                               : lm::launch_grouped_rows<lm::kF16>(a, loads, s);
 }
-hipError_t weights_by_type(const lm::GroupedWeightArgs& a, int tile, hipStream_t s) {
-  return a.type == lm::kF32    ? lm::launch_grouped_weights<lm::kF32>(a, tile, s)
-         : a.type == lm::kBf16 ? lm::launch_grouped_weights<lm::kBf16>(a, tile, s)
-                               : lm::launch_grouped_weights<lm::kF16>(a, tile, s);
+hipError_t weights_by_type(const lm::GroupedWeightArgs& a, int loads, bool big, hipStream_t s) {
+  return a.type == lm::kF32    ? lm::launch_grouped_weights<lm::kF32>(a, loads, big, s)
+         : a.type == lm::kBf16 ? lm::launch_grouped_weights<lm::kBf16>(a, loads, big, s)
+                               : lm::launch_grouped_weights<lm::kF16>(a, loads, big, s);
 }
-
-// A tile's rows of `ld` elements within the 31 bits of an asynchronous load's offset.
-bool reachable(int64_t rows, int64_t ld, int e) { return rows * ld * e < 0x7fffffff; }
 
 // y = epi(x @ w_e + b_e), the launches of one product over rows. `plan`: what ran.
 void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t len) {
-  const int e = lm::type_bytes(a.type), chunk = 16 / e;
+  const int e = lm::type_bytes(a.type);
   const bool streams = a.T < 64 * (int64_t)a.E && (a.turned || a.N >= 4);
   a.skip = streams ? lm::kGroupedSkinnyRows : 0;
   if (streams) {
     check_hip(skinny_by_type(a, s), "grouped_skinny launch");
   }
-  const char* tiles = "";
+  int loads = -1;
   if (a.T > a.skip) {
-    const bool direct = aligned16(a.x) && a.ldx % chunk == 0 && aligned16(a.w) && a.ldw % chunk == 0 &&
-                        a.stride_w % chunk == 0 && a.K % chunk == 0 && reachable(256, a.ldx, e) &&
-                        reachable(256, a.ldw, e);
-    const int64_t big = (a.T / 256 + 1) * ((a.N + 255) / 256);
-    const int tile = !direct                                                        ? lm::kGroupedTileAny
-                     : a.type != lm::kF32 && a.T >= 512 * (int64_t)a.E && big >= cus ? lm::kGroupedTile256
-                                                                                    : lm::kGroupedTile128;
-    check_grid(a.T / 128 + a.E, (a.N + 127) / 128);
-    check_hip(rows_by_type(a, tile, s), "grouped_rows launch");
-    static const char* const names[] = {"256x256", "128x128", "128x128 any"};
-    tiles = names[tile];
+    loads = reachable(256, a.ldx, e) && reachable(256, a.ldw, e)
+                ? common_bytes({address(a.x), a.ldx * e, address(a.w), a.ldw * e, a.stride_w * e, a.K * e})
+                : 0;
+    // The last elements of a row come with their neighbours' bytes.
+    if (loads == 4 && a.N * e % 4 != 0) loads = 0;
+    check_grid(a.T / 128 + a.E, (a.N + 127) / 128 + 16);
+    a.cus = cus;
+    check_hip(rows_by_type(a, loads, s), "grouped_rows launch");
   }
-  snprintf(plan, len, "%s%s%s%s", streams ? "stream" : "", streams && *tiles ? "+" : "", *tiles ? "tile=" : "", tiles);
+  snprintf(plan, len, "%s%s", streams ? "stream" : "", loads < 0 ? "" : loads == 16 ? "+tiles=16" : loads == 4 ? "+tiles=4" : "+tiles=any");
 }
 
 void grouped_dense(lm::GroupedArgs a, int64_t E, void* stream) {
@@ -243,17 +244,15 @@ void grouped_backward(Backward a, void* stream) {
       if (a.dw_turned) std::swap(g.a, g.b), std::swap(g.lda, g.ldb), std::swap(g.M, g.N);
       g.offsets = a.offsets, g.dw = a.dw, g.lddw = a.lddw, g.stride_dw = a.stride_dw, g.T = a.T;
       g.E = (int)a.E, g.type = a.type, g.dw_type = a.dw_type, g.ids64 = a.ids64;
-      const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % chunk == 0 && g.ldb % chunk == 0 &&
-                          reachable(64, g.lda, e) && reachable(64, g.ldb, e);
-      const int64_t big = ((g.M + 255) / 256) * ((g.N + 255) / 256) * a.E;
-      const int tile = !direct                                                        ? lm::kGroupedTileAny
-                       : a.type != lm::kF32 && a.T >= 256 * a.E && big >= cus ? lm::kGroupedTile256
-                                                                              : lm::kGroupedTile128;
-      const int64_t side = tile == lm::kGroupedTile256 ? 256 : 128;
-      check_grid((g.M + side - 1) / side * a.E, (g.N + side - 1) / side);
-      check_hip(weights_by_type(g, tile, s), "grouped_weights launch");
-      static const char* const names[] = {" dW tile=256x256", " dW tile=128x128", " dW tile=128x128 any"};
-      tiles = names[tile];
+      int loads = reachable(64, g.lda, e) && reachable(64, g.ldb, e)
+                      ? common_bytes({address(g.a), g.lda * e, address(g.b), g.ldb * e})
+                      : 0;
+      if (loads == 4 && (g.M * e % 4 != 0 || g.N * e % 4 != 0)) loads = 0;
+      const int64_t tiles256 = ((g.M + 255) / 256) * ((g.N + 255) / 256) * a.E;
+      const bool big = loads == 16 && a.type != lm::kF32 && a.T >= 256 * a.E && tiles256 >= cus;
+      check_grid((g.M + 127) / 128 * a.E, (g.N + 127) / 128);
+      check_hip(weights_by_type(g, loads, big, s), "grouped_weights launch");
+      tiles = big ? " dW 256x256" : loads == 16 ? " dW 128x128" : loads == 4 ? " dW loads=4" : " dW any";
     }
     set_plan("grouped_dense_backward %s%s%s%s%s", type_name(a.type), masks ? " mask" : "", *plan ? " dX " : "", plan,
              tiles);

@@ -1,22 +1,36 @@
 // Tiles of a matrix product on the matrix cores, C[m][n] = sum_k A[m][k] B[k][n]:
 // what the layers on groups of rows and on 8-bit weights share.
 //
-// A workgroup of WM x WN waves takes BM x BN outputs; a stage of 128 bytes of k a row
-// goes from memory straight to LDS while the one before it is multiplied, two
-// stages in turn, one barrier a stage. An operand lies in memory, and in LDS, with
-// k contiguous (kRows), with its own index contiguous (kCols: read through the
-// transposing LDS load, or element by element in f32) or laid out as the
-// instruction takes it (kBlocks, 8-bit weights). 16-byte chunks change places by row
-// so that a fragment's reads meet all banks. Where a row starts off 16 bytes, or a
-// chunk would cross its end, the chunks go through registers instead, cut
-// element by element (ASYNC false).
+// A workgroup of WM x WN waves takes BM x BN outputs. Stages of 128 bytes of k a row
+// go from memory straight to LDS, two or three of them in turn. Half a stage's fragments
+// are read into registers while the half before it is multiplied. In the middle of a stage
+// all of it is in registers and the next one has arrived: there is its only barrier, and
+// there the loads into its place start, one after every few products, since a wave
+// waits for each of them to be taken.
+//
+// An operand lies in memory, and in LDS, with k contiguous (kRows), with its own index
+// contiguous (kCols: read through the transposing LDS load, or element by element in f32)
+// or laid out as the instruction takes it (kBlocks, 8-bit weights). 16-byte chunks change
+// places by row so that a fragment's reads meet all banks. LOADS is how they come: 16 bytes
+// a lane at a time where all rows start on 16 bytes and no chunk crosses a row's end, 4 where
+// that holds for 4 bytes, or 0: through registers, cut element by element, for any alignment.
 //
 // The two operands are given to the instruction in exchanged places, so that a lane
 // ends with four successive n of one row: wide stores.
+//
+// Measured, bf16 4096^3, random values: 256x256 tiles in 123 us (1.12 PFLOP/s; the vendor's product
+// takes 128), of which 12 are launch, first loads and stores. Without its loads a product
+// takes 112, without its reads of LDS 126, with neither 98: the matrix cores at the clock that power
+// leaves them come first, then the loads' way from L2 (48 bytes a clock and CU at most). Matrix
+// instructions of one wave a SIMD start every 32 cycles, of two every 16: tiles have eight waves. Stages of 64 bytes a
+// row, four in LDS, took 137 us (half lines twice); 16 waves with a barrier between loads and products 128.
 #pragma once
+
+#include <type_traits>
 
 #include "common.hpp"
 #include "lm_common.hpp"
+#include "lm_kernels.hpp"
 
 namespace edsl {
 namespace lm {
@@ -71,7 +85,7 @@ struct TileElem<float> {
 // 16 bytes a lane from memory, descriptor `from` + `offset`, to LDS, `to` (the wave's
 // own) + 16 lane; zeros at offsets past the descriptor's end. As the instruction
 // itself: for its intrinsic the compiler lets every later read of LDS wait for it,
-// whichever buffer it reads. It has no result register; wait_tile_loads() is what waits
+// whichever buffer it reads. It has no result register; tile_arrived() is what waits
 // for it.
 __device__ __forceinline__ void tile_to_lds(i32x4 from, int offset, const void* to) {
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to;
@@ -80,8 +94,19 @@ __device__ __forceinline__ void tile_to_lds(i32x4 from, int offset, const void* 
                : "s"(__builtin_amdgcn_readfirstlane((int)at)), "v"(offset), "s"(from)
                : "memory", "m0");
 }
-// vmcnt 0.
-__device__ __forceinline__ void wait_tile_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// All waves' loads but their last N have arrived, and their reads of LDS.
+template <int N>
+__device__ __forceinline__ void tile_arrived() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void tile_to_lds4(i32x4 from, int offset, const void* to) {  // 4 bytes a lane
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane((int)at)), "v"(offset), "s"(from)
+               : "memory", "m0");
+}
 
 // One operand of a tile: `n` of its own index's elements are there from `base` on.
 struct TileOperand {
@@ -91,13 +116,13 @@ struct TileOperand {
 };
 
 // MN of an operand's own index in LDS and its loads by THREADS threads.
-template <typename T, int KIND, int MN, int THREADS, bool ASYNC>
+template <typename T, int KIND, int MN, int THREADS, int LOADS>
 struct TileSide {
   static constexpr int kChunk = TileElem<T>::kChunk;
   static constexpr int kDepth = 8 * kChunk;  // k of a stage
   static constexpr int kAll = MN * 8;        // chunks of a stage
   static constexpr int kMine = kAll / THREADS;
-  static_assert(kAll % THREADS == 0 && (MN % 128 == 0 || KIND == kRows), "whole chunks, whole banks");
+  static_assert(kAll % THREADS == 0 && (MN % (sizeof(T) == 4 ? 64 : 128) == 0 || KIND != kCols), "whole chunks, whole banks");
   static constexpr int kPerRow = KIND == kCols ? MN / kChunk : 8;
   static constexpr int kOutside = (int)0x80000000;  // an offset past every descriptor
 
@@ -114,66 +139,83 @@ struct TileSide {
     col = c * kChunk;
   }
 
-  int offset[ASYNC ? kMine : 1];
-  u32x4 held[ASYNC ? 1 : kMine];
+  static constexpr int kParts = LOADS == 4 ? 4 : 1;  // loads of a chunk
+  int offset[LOADS ? kMine * kParts : 1];
+  u32x4 held[LOADS ? 1 : kMine];
 
   __device__ __forceinline__ void init(const TileOperand& o, int tid) {
-    if constexpr (ASYNC) {
+    if constexpr (LOADS != 0) {
 #pragma unroll
-      for (int c = 0; c < kMine; ++c) {
-        const int at = c * THREADS + tid;
+      for (int c = 0; c < kMine * kParts; ++c) {
+        // Four lanes have a chunk's 4-byte parts.
+        const int at = LOADS == 16 ? c * THREADS + tid
+                                   : c / 4 * THREADS + tid / 64 * 64 + c % 4 * 16 + tid % 64 / 4;
+        const int part = LOADS == 16 ? 0 : tid % 4 * 4;
         if constexpr (KIND == kBlocks) {
           // Blocks of 16 columns x 64 k, `ld` bytes from 16 columns to the next.
           offset[c] = (int)((at / 128) * o.ld) + (at % 128) * 16;
         } else {
           int row, col;
           place(at, row, col);
-          offset[c] = (int)(((int64_t)row * o.ld + col) * (int64_t)sizeof(T));
+          offset[c] = (int)(((int64_t)row * o.ld + col) * (int64_t)sizeof(T)) + part;
         }
       }
     }
   }
 
-  // Starts the loads of the stage at k0 of K.
-  __device__ __forceinline__ void load(const TileOperand& o, int K, int k0, u32x4* lds, int tid, int wave) {
-    if constexpr (ASYNC) {
-      i32x4 from;
-      if constexpr (KIND == kRows) {
-        from = buffer_rsrc(o.base + (int64_t)k0 * sizeof(T), ((o.n - 1) * o.ld + K - k0) * (int64_t)sizeof(T));
-      } else if constexpr (KIND == kCols) {
-        from = buffer_rsrc(o.base + k0 * o.ld * (int64_t)sizeof(T), ((K - k0 - 1) * o.ld + o.n) * (int64_t)sizeof(T));
-      } else {
-        from = buffer_rsrc(o.base + (int64_t)k0 * 16, (int64_t)((o.n + 15) / 16) * o.ld - (int64_t)k0 * 16);
-      }
-      const bool tail = KIND == kRows && k0 + kDepth > K;  // rows go on past K
+  // A stage at k0 of K, `left` of K from there.
+  struct Source {
+    i32x4 from;
+    int k0, left;
+  };
+  static __device__ __forceinline__ Source source(const TileOperand& o, int K, int k0) {
+    if constexpr (LOADS == 0) return {i32x4{}, k0, K - k0};
+    if constexpr (KIND == kRows)
+      return {buffer_rsrc(o.base + (int64_t)k0 * sizeof(T), ((o.n - 1) * o.ld + K - k0) * (int64_t)sizeof(T)), k0,
+              K - k0};
+    if constexpr (KIND == kCols)
+      return {buffer_rsrc(o.base + k0 * o.ld * (int64_t)sizeof(T), ((K - k0 - 1) * o.ld + o.n) * (int64_t)sizeof(T)),
+              k0, K - k0};
+    return {buffer_rsrc(o.base + (int64_t)k0 * 16, (int64_t)((o.n + 15) / 16) * o.ld - (int64_t)k0 * 16), k0, K - k0};
+  }
+  // Starts load c of kMine of a stage.
+  __device__ __forceinline__ void load(int c, const Source& s, const TileOperand& o, u32x4* lds, int tid, int wave) {
+    int row, col;
+    if constexpr (LOADS != 0) {
 #pragma unroll
-      for (int c = 0; c < kMine; ++c) {
-        int at = offset[c];
-        if (tail) {
-          int row, col;
-          place(c * THREADS + tid, row, col);
-          if (k0 + col >= K) at = kOutside;
+      for (int p = 0; p < kParts; ++p) {
+        int at = offset[c * kParts + p];
+        if constexpr (KIND == kRows) {  // rows go on past K
+          place(LOADS == 16 ? c * THREADS + tid : c * THREADS + tid / 64 * 64 + p * 16 + tid % 64 / 4, row, col);
+          if constexpr (LOADS == 4) col += tid % 4 * (4 / (int)sizeof(T));
+          at = col < s.left ? at : kOutside;
         }
-        tile_to_lds(from, at, lds + c * THREADS + wave * 64);
+        u32x4* const to = lds + c * THREADS + wave * 64 + p * 16;
+        if constexpr (LOADS == 16)
+          tile_to_lds(s.from, at, to);
+        else
+          tile_to_lds4(s.from, at, to);
       }
     } else {
       static_assert(KIND != kBlocks, "blocks are always aligned");
-#pragma unroll
-      for (int c = 0; c < kMine; ++c) {
-        int row, col;
-        place(c * THREADS + tid, row, col);
-        const int rows = KIND == kRows ? o.n : K - k0, left = KIND == kRows ? K - k0 : o.n;
-        held[c] = u32x4{0, 0, 0, 0};
-        if (row < rows && col < left) {
-          const T* const p = reinterpret_cast<const T*>(o.base) +
-                             (KIND == kRows ? (int64_t)row * o.ld + k0 : (int64_t)(row + k0) * o.ld);
-          held[c] = __builtin_bit_cast(u32x4, load_guarded<T, kChunk>(p, col, left));
-        }
+      place(c * THREADS + tid, row, col);
+      const T* const base = reinterpret_cast<const T*>(o.base);
+      // Inside, or past the last row, whose sums nobody stores, a load depends on no comparison.
+      if (KIND == kRows ? s.left >= kDepth : s.left >= kDepth && o.n >= MN) {
+        const int64_t at = KIND == kRows ? min(row, o.n - 1) * o.ld + s.k0 + col : (row + s.k0) * o.ld + col;
+        held[c] = __builtin_bit_cast(u32x4, load_packed<T, kChunk>(base + at));
+        return;
+      }
+      const int rows = KIND == kRows ? o.n : s.left, left = KIND == kRows ? s.left : o.n;
+      held[c] = u32x4{0, 0, 0, 0};
+      if (row < rows && col < left) {
+        const T* const p = base + (KIND == kRows ? row * o.ld + s.k0 : (row + s.k0) * o.ld);
+        held[c] = __builtin_bit_cast(u32x4, load_guarded<T, kChunk>(p, col, left));
       }
     }
   }
   __device__ __forceinline__ void put(u32x4* lds, int tid) {
-    if constexpr (!ASYNC)
+    if constexpr (LOADS == 0)
 #pragma unroll
       for (int c = 0; c < kMine; ++c) lds[c * THREADS + tid] = held[c];
   }
@@ -206,7 +248,8 @@ struct TileSide {
   }
 };
 
-template <typename T_, int AKIND, int BKIND, int BM_, int BN_, int WM_, int WN_, bool ASYNC>
+// NS stages in LDS.
+template <typename T_, int AKIND, int BKIND, int BM_, int BN_, int WM_, int WN_, int LOADS, int NS = 2>
 struct Tile {
   using T = T_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
@@ -214,9 +257,10 @@ struct Tile {
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   using E = TileElem<T>;
   using Acc = typename E::Acc;
-  using A = TileSide<T, AKIND, BM, kThreads, ASYNC>;
-  using B = TileSide<T, BKIND, BN, kThreads, ASYNC || BKIND == kBlocks>;
+  using A = TileSide<T, AKIND, BM, kThreads, LOADS>;
+  using B = TileSide<T, BKIND, BN, kThreads, BKIND == kBlocks ? 16 : LOADS>;
   static constexpr int kStage = A::kAll + B::kAll;  // chunks
+  static constexpr int kLds = NS * kStage;
 
   // acc[i][j][e]: row 16 (wave's MI + i) + lane % 16, column 16 (wave's NI + j) + 4 (lane / 16) + e.
   static __device__ __forceinline__ void product(const TileOperand& oa, const TileOperand& ob, int K, u32x4* lds,
@@ -227,43 +271,112 @@ struct Tile {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = Acc{};
+    const int stages = (K + A::kDepth - 1) / A::kDepth;
+    if (stages == 0) return;
     A a;
     B b;
     a.init(oa, tid);
     b.init(ob, tid);
-    const int stages = (K + A::kDepth - 1) / A::kDepth;
-    if (stages > 0) {
-      a.load(oa, K, 0, lds, tid, wave);
-      b.load(ob, K, 0, lds + A::kAll, tid, wave);
-      a.put(lds, tid);
-      b.put(lds + A::kAll, tid);
-    }
-    for (int st = 0; st < stages; ++st) {
-      u32x4* const now = lds + (st % 2) * kStage;
-      u32x4* const next = lds + ((st + 1) % 2) * kStage;
-      if constexpr (ASYNC || BKIND == kBlocks) wait_tile_loads();
-      __syncthreads();
-      if (st + 1 < stages) {
-        a.load(oa, K, (st + 1) * A::kDepth, next, tid, wave);
-        b.load(ob, K, (st + 1) * A::kDepth, next + A::kAll, tid, wave);
+    constexpr int kLoads = A::kMine * A::kParts + B::kMine * B::kParts;  // of a stage, a thread
+    constexpr int kAll = A::kMine + B::kMine;
+    struct Fragments {
+      u32x4 a[MI], b[NI];
+    };
+    const auto read = [&](const u32x4* from, int s, Fragments& f) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) f.b[j] = B::fragment(from + A::kAll, wn * NI + j, s, lane);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) f.a[i] = A::fragment(from, wm * MI + i, s, lane);
+    };
+    struct Sources {
+      typename A::Source a;
+      typename B::Source b;
+    };
+    // Stages past the last one read nothing: their descriptors, or their elements, are none.
+    const auto sources = [&](int st) {
+      return Sources{A::source(oa, K, st * A::kDepth), B::source(ob, K, st * A::kDepth)};
+    };
+    const auto load = [&](int c, const Sources& s, u32x4* to) {
+      if (c < A::kMine)
+        a.load(c, s.a, oa, to, tid, wave);
+      else
+        b.load(c - A::kMine, s.b, ob, to + A::kAll, tid, wave);
+    };
+    const auto load_all = [&](int st, u32x4* to) {
+      const Sources s = sources(st);
+#pragma unroll
+      for (int c = 0; c < kAll; ++c) load(c, s, to);
+    };
+    const auto run = [&](auto working) {
+      constexpr bool kWorks = decltype(working)::value;
+      Fragments f0, f1;
+      if constexpr (LOADS != 0) {
+#pragma unroll
+        for (int st = 0; st < NS; ++st) load_all(st, lds + st * kStage);
+        tile_arrived<(NS - 1) * kLoads>();
+        if constexpr (kWorks) read(lds, 0, f0);
+        int at = 0;
+        for (int st = 0; st < stages; ++st) {
+          u32x4* const now = lds + at * kStage;
+          at = at + 1 == NS ? 0 : at + 1;
+          u32x4* const next = lds + at * kStage;
+          if constexpr (kWorks) {
+            __builtin_amdgcn_sched_barrier(0);
+            read(now, 1, f1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+              for (int j = 0; j < NI; ++j) acc[i][j] = E::mul(f0.b[j], f0.a[i], acc[i][j]);
+          }
+          const Sources s = sources(st + NS);
+          __builtin_amdgcn_sched_barrier(0);
+          tile_arrived<(NS - 2) * kLoads>();
+          if constexpr (kWorks) read(next, 0, f0);
+          // The loads between the products: a wave waits for each to be taken.
+#pragma unroll
+          for (int c = 0; c < kAll; ++c) {
+            __builtin_amdgcn_sched_barrier(0);
+            load(c, s, now);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kWorks)
+#pragma unroll
+              for (int m = c * MI * NI / kAll; m < (c + 1) * MI * NI / kAll; ++m)
+                acc[m / NI][m % NI] = E::mul(f1.b[m % NI], f1.a[m / NI], acc[m / NI][m % NI]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        tile_arrived<0>();  // nothing is on its way to LDS when the workgroup ends
+      } else {
+        static_assert(LOADS || NS == 2, "a stage at a time goes through registers");
+        load_all(0, lds);
+        a.put(lds, tid);
+        b.put(lds + A::kAll, tid);
+        for (int st = 0; st < stages; ++st) {
+          u32x4* const now = lds + st % 2 * kStage;
+          u32x4* const next = lds + (st + 1) % 2 * kStage;
+          tile_arrived<0>();
+          load_all(st + 1, next);
+          if constexpr (kWorks)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              read(now, s, f0);
+#pragma unroll
+              for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = E::mul(f0.b[j], f0.a[i], acc[i][j]);
+            }
+          a.put(next, tid);
+          b.put(next + A::kAll, tid);
+        }
+        tile_arrived<0>();
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4 fa[MI], fb[NI];
-#pragma unroll
-        for (int j = 0; j < NI; ++j) fb[j] = B::fragment(now + A::kAll, wn * NI + j, s, lane);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) fa[i] = A::fragment(now, wm * MI + i, s, lane);
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int j = 0; j < NI; ++j) acc[i][j] = E::mul(fb[j], fa[i], acc[i][j]);
-      }
-      if (!ASYNC && st + 1 < stages) {
-        a.put(next, tid);
-        b.put(next + A::kAll, tid);
-      }
-    }
+    };
+    // A wave whose rows are all past the operand's leaves the matrix cores to the others.
+    if (wm * MI * 16 < oa.n)
+      run(std::true_type{});
+    else
+      run(std::false_type{});
   }
 };
 
@@ -335,6 +448,40 @@ __device__ __forceinline__ void activate(float (&v)[N], int epi, float alpha) {
 __device__ __forceinline__ int xcd_order(int w, int total) {
   const int x = w % 8, per = total / 8, more = total % 8;
   return x * per + min(x, more) + w / 8;
+}
+
+// Eight row tiles go along the columns together.
+constexpr int kTogether = 8;
+// Tile `at` of rows x tiles_n: its row tile and column strip.
+__device__ __forceinline__ int row_of_tile(int at, int rows, int tiles_n, int* tn) {
+  const int group = at / (kTogether * tiles_n), first = group * kTogether, high = min(rows - first, kTogether);
+  at -= group * kTogether * tiles_n;
+  *tn = at / high;
+  return first + at % high;
+}
+
+// Which tile a workgroup takes of `total` tiles of the largest shape: those come in whole rounds of the
+// CUs, and what is left is cut in four where there are up to `quarters` tiles, or else in two up to `halves`.
+struct TileTurn {
+  int tile, sub, pieces;  // piece `sub` of 1, 2 or 4
+};
+// The most workgroups, whatever `total` up to `most` is.
+inline int64_t tile_turns(int64_t most, const TileRounds& r) { return most + 3 * r.quarters + r.halves; }
+__device__ __forceinline__ bool tile_turn(int w, int total, int first_part, const TileRounds& r, TileTurn* turn) {
+  int whole = total / r.cus * r.cus, left = total - whole;
+  const int pieces = left <= r.quarters ? 4 : left <= r.halves ? 2 : 1;
+  if (pieces == 1) whole = total, left = 0;
+  if (w < whole) {
+    // Tiles from first_part on have fewer rows: each XCD has its share of both.
+    const int even = min(whole, first_part);
+    *turn = {w < even ? xcd_order(w, even) : even + xcd_order(w - even, whole - even), 0, 1};
+    return true;
+  }
+  w -= whole;
+  if (w >= left * pieces) return false;
+  w = xcd_order(w, left * pieces);
+  *turn = {whole + w / pieces, w % pieces, pieces};
+  return true;
 }
 
 }  // namespace lm

@@ -60,8 +60,9 @@ def test_types_and_epilogues(M, y, epi):
 
 
 @pytest.mark.parametrize("M,K,N,plan", [
-    (1, 4096, 20000, "skinny cols=32"), (64, 512, 700, "skinny cols=16"), (2100, 384, 8200, "tile=256x256"),
-    (300, 512, 700, "tile=128x128"), (300, 500, 700, "any"), (66, 8192, 300, "tile=128x128")])
+    (1, 4096, 20000, "skinny cols=32"), (64, 512, 700, "skinny cols=16"), (2100, 384, 8200, "loads=16"), (4200, 192, 4000, "loads=16"),
+    (600, 512, 8192, "loads=16"), (4096, 128, 4096, "loads=16"), (300, 512, 700, "loads=16"), (300, 500, 700, "loads=0"),
+    (66, 8192, 300, "loads=16")])
 def test_kernels(M, K, N, plan):
     check(M, K, N, y=BF16, epi="bias_relu", b=BF16, plan=plan)
 
