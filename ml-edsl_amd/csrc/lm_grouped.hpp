@@ -167,10 +167,10 @@ __global__ void __launch_bounds__(Big::kThreads, 1) grouped_rows_kernel(GroupedA
 }
 
 // Experts of up to kGroupedSkinnyRows rows: a workgroup an expert and column block.
-template <typename T, int BKIND, int NJ, int WAVES>
+template <typename T, int BKIND, int NJ, int WAVES, int U, int AHEAD>
 __global__ void __launch_bounds__(64 * WAVES) grouped_skinny_kernel(GroupedArgs a) {
-  using S1 = Skinny<T, BKIND, 1, NJ, WAVES>;
-  using S2 = Skinny<T, BKIND, 2, NJ, WAVES>;
+  using S1 = Skinny<T, BKIND, 1, NJ, WAVES, U, AHEAD>;
+  using S2 = Skinny<T, BKIND, 2, NJ, WAVES, U, AHEAD>;
   __shared__ typename S1::Acc lds[S1::kSlots];
   const GroupOffsets g = offsets_of(a);
   const int e = blockIdx.y;

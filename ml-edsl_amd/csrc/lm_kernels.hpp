@@ -187,7 +187,7 @@ struct I8Args {
   TileRounds rounds;
 };
 hipError_t launch_i8_tile(const I8Args& a, int loads, hipStream_t stream);
-hipError_t launch_i8_skinny(const I8Args& a, int cols16, hipStream_t stream);
+hipError_t launch_i8_skinny(const I8Args& a, int rows16, int cols16, hipStream_t stream);
 
 }  // namespace lm
 }  // namespace edsl

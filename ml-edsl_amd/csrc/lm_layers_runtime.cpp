@@ -78,10 +78,17 @@ void i8_dense(lm::I8Args a, int64_t M, int64_t N, int64_t K, void* stream) {
   a.w_scales = reinterpret_cast<const float*>(a.w + lm::i8_scales_at(K, N));
   device_launch(0, stream, [&](char*, int cus) {
     const hipStream_t s = as_stream(stream);
-    if (M <= 64) {
-      const int cols = lm::i8_tiles(N) > 2 * cus ? 2 : 1;
-      check_hip(lm::launch_i8_skinny(a, cols, s), "i8_skinny launch");
-      set_plan("i8_skinny cols=%d", 16 * cols);
+    const int64_t tiles = lm::i8_tiles(N), parts = (M + 63) / 64;
+    // Streaming, in parts of up to 64 rows: up to 64 rows, 32 of a wide layer (64 x 4096 x 50256 in 73 us against 55 on
+    // tiles), and more where all parts together are two rounds of workgroups (256 x 8192 x 2048 ...).
+    if (M <= (tiles >= 8 * (int64_t)cus ? 32 : 64) || (parts <= 64 && parts * tiles <= 2 * (int64_t)cus)) {
+      // Each workgroup reads all of x: more columns a workgroup where there are many (32 x 4096 x 50256 in 49 us on
+      // 64 columns, on 16 in 90; 16 rows in 42 and 53), and where one more than a round of 16 each would run (33 x 4096 x
+      // 4097 in 10.2 us, in 13.7 on 16), but not where CUs would be idle (32 x 4096 x 4096 in 8.4, on 32 in 9.2).
+      const int cols = tiles >= 8 * (int64_t)cus ? 4 : tiles > (M <= 16 ? 2 : 1) * (int64_t)cus ? 2 : 1;
+      const int rows = (int)(((M + parts - 1) / parts + 15) / 16);
+      check_hip(lm::launch_i8_skinny(a, rows, cols, s), "i8_skinny launch");
+      set_plan("i8_skinny rows=%d cols=%d", 16 * rows, 16 * cols);
       return;
     }
     const int loads = aligned16(a.x) && a.ldx % 16 == 0 && K % 16 == 0 && reachable(256, a.ldx, 1) ? 16 : 0;
@@ -131,6 +138,7 @@ void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t 
   const int e = lm::type_bytes(a.type);
   const bool streams = a.T < 64 * (int64_t)a.E && (a.turned || a.N >= 4);
   a.skip = streams ? lm::kGroupedSkinnyRows : 0;
+  a.cus = cus;
   if (streams) {
     check_hip(skinny_by_type(a, s), "grouped_skinny launch");
   }
@@ -142,7 +150,6 @@ void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t 
     // The last elements of a row come with their neighbours' bytes.
     if (loads == 4 && a.N * e % 4 != 0) loads = 0;
     check_grid(a.T / 128 + a.E, (a.N + 127) / 128 + 16);
-    a.cus = cus;
     check_hip(rows_by_type(a, loads, s), "grouped_rows launch");
   }
   snprintf(plan, len, "%s%s", streams ? "stream" : "", loads < 0 ? "" : loads == 16 ? "+tiles=16" : loads == 4 ? "+tiles=4" : "+tiles=any");

@@ -1,6 +1,6 @@
 // A few rows against a layer's weights: what is read once is the weights, and the
-// time is theirs. The waves of a workgroup take K in turn, each with the next
-// block's loads on their way while it multiplies this one's, and meet in LDS once.
+// time is theirs. The waves of a workgroup take blocks of K in turn, each with the next ones'
+// loads on their way while it multiplies this one, and meet in LDS once.
 // No operand goes through LDS before: rows of x come in the instruction's order, and
 // so do weights whose k are contiguous (kRows) or that are laid out so (kBlocks).
 // Where columns are contiguous (kCols), a lane reads kChunk successive k of NJ
@@ -13,20 +13,21 @@
 namespace edsl {
 namespace lm {
 
-template <typename T, int KIND, int MT, int NJ, int WAVES>
+template <typename T, int KIND, int MT, int NJ, int WAVES, int U, int AHEAD>
 struct Skinny {
   using E = TileElem<T>;
   using Acc = typename E::Acc;
   static constexpr int kChunk = E::kChunk, kStep = 4 * kChunk;
-  static constexpr int U = KIND == kCols ? 1 : MT <= 2 ? 4 : 2;  // steps of a block
-  static constexpr int kDepth = U * kStep;
+  static constexpr int kDepth = U * kStep;        // k of a block: U steps
   static constexpr int kCols16 = 16 * NJ;         // columns of a workgroup
   static constexpr int kSlots = WAVES * NJ * 64;  // Acc of LDS
 
-  struct Block {
-    u32x4 a[U][MT];
+  struct Rows {
+    u32x4 v[U][MT];
+  };
+  struct Weights {
     u32x4 b[KIND == kCols ? 1 : U][KIND == kCols ? 1 : NJ];
-    Packed<T, NJ> raw[KIND == kCols ? kChunk : 1];
+    Packed<T, NJ> raw[KIND == kCols ? U : 1][KIND == kCols ? kChunk : 1];
   };
 
   const char* xrow[MT];  // the lane's rows, at its first k
@@ -64,20 +65,22 @@ struct Skinny {
     return KIND == kCols ? min(n0 + NJ * c, N - NJ) + j : n0 + 16 * j + c;
   }
 
-  __device__ __forceinline__ void load(Block& r, int k0) const {
+  __device__ __forceinline__ void load(Rows& r, int k0) const {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        r.a[u][i] = __builtin_bit_cast(
+        r.v[u][i] = __builtin_bit_cast(
             u32x4, load_packed<T, kChunk>(reinterpret_cast<const T*>(xrow[i]) + k0 + u * kStep));
-    if constexpr (KIND == kCols) {
+  }
+  __device__ __forceinline__ void load(Weights& r, int k0) const {
 #pragma unroll
-      for (int q = 0; q < kChunk; ++q)
-        r.raw[q] = load_packed<T, NJ>(reinterpret_cast<const T*>(wcol[0]) + (int64_t)(k0 + q) * ld);
-    } else {
+    for (int u = 0; u < U; ++u) {
+      if constexpr (KIND == kCols)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int q = 0; q < kChunk; ++q)
+          r.raw[u][q] = load_packed<T, NJ>(reinterpret_cast<const T*>(wcol[0]) + (int64_t)(k0 + u * kStep + q) * ld);
+      else
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if constexpr (KIND == kRows)
@@ -90,38 +93,36 @@ struct Skinny {
   }
 
   // The same where the block goes past K: zeros there.
-  __device__ __forceinline__ void load_tail(Block& r, int k0, int K) const {
+  __device__ __forceinline__ void load_tail(Rows& r, Weights& w, int k0, int K) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int left = K - (k0 + u * kStep + chunk_at);
+      const int k = k0 + u * kStep, left = K - (k + chunk_at);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        r.a[u][i] = __builtin_bit_cast(
-            u32x4, load_guarded<T, kChunk>(reinterpret_cast<const T*>(xrow[i]) + k0 + u * kStep, 0, left));
+        r.v[u][i] = __builtin_bit_cast(
+            u32x4, load_guarded<T, kChunk>(reinterpret_cast<const T*>(xrow[i]) + k, 0, left));
       if constexpr (KIND == kRows)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          r.b[u][j] = __builtin_bit_cast(
-              u32x4, load_guarded<T, kChunk>(reinterpret_cast<const T*>(wcol[j]) + k0 + u * kStep, 0, left));
+          w.b[u][j] =
+              __builtin_bit_cast(u32x4, load_guarded<T, kChunk>(reinterpret_cast<const T*>(wcol[j]) + k, 0, left));
       if constexpr (KIND == kBlocks)  // they hold zeros up to whole pairs of steps
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int step = k0 / kStep + u;
-          r.b[u][j] = step < (K + kStep - 1) / kStep ? *reinterpret_cast<const u32x4*>(wcol[j] + (int64_t)step * 1024)
-                                                     : u32x4{0, 0, 0, 0};
+        for (int j = 0; j < NJ; ++j)
+          w.b[u][j] = k < K ? *reinterpret_cast<const u32x4*>(wcol[j] + (int64_t)(k / kStep) * 1024) : u32x4{0, 0, 0, 0};
+      if constexpr (KIND == kCols)
+#pragma unroll
+        for (int q = 0; q < kChunk; ++q) {
+          w.raw[u][q] = Packed<T, NJ>{};
+          if (q < left)
+            w.raw[u][q] = load_packed<T, NJ>(reinterpret_cast<const T*>(wcol[0]) + (int64_t)(k + q) * ld);
         }
     }
-    if constexpr (KIND == kCols)
-#pragma unroll
-      for (int q = 0; q < kChunk; ++q) {
-        r.raw[q] = Packed<T, NJ>{};
-        if (k0 + chunk_at + q < K)
-          r.raw[q] = load_packed<T, NJ>(reinterpret_cast<const T*>(wcol[0]) + (int64_t)(k0 + q) * ld);
-      }
   }
 
   // Column j of kChunk rows of NJ, as an operand.
-  static __device__ __forceinline__ u32x4 turned(const Packed<T, NJ> (&raw)[kChunk], int j) {
+  template <int Q>
+  static __device__ __forceinline__ u32x4 turned(const Packed<T, NJ> (&raw)[Q], int j) {
     u32x4 v;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -137,18 +138,18 @@ struct Skinny {
     return v;
   }
 
-  static __device__ __forceinline__ void multiply(const Block& r, Acc (&acc)[MT][NJ]) {
+  static __device__ __forceinline__ void multiply(const Rows& r, const Weights& w, Acc (&acc)[MT][NJ]) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         u32x4 b;
         if constexpr (KIND == kCols)
-          b = turned(r.raw, j);
+          b = turned(w.raw[u], j);
         else
-          b = r.b[u][j];
+          b = w.b[u][j];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][j] = E::mul(r.a[u][i], b, acc[i][j]);
+        for (int i = 0; i < MT; ++i) acc[i][j] = E::mul(r.v[u][i], b, acc[i][j]);
       }
   }
 
@@ -165,17 +166,31 @@ struct Skinny {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = Acc{};
     const int blocks = K / kDepth;
-    Block now, next;
-    if (wave < blocks) s.load(now, wave * kDepth);
-    for (int b = wave; b < blocks; b += WAVES) {
-      const int ahead = b + WAVES < blocks ? b + WAVES : b;  // the last turn reads its own again
-      s.load(next, ahead * kDepth);
-      multiply(now, acc);
-      now = next;
+    // The wave's blocks: AHEAD of weights on their way, from memory, and one of x, from the caches. Past the
+    // last one it reads that again.
+    const int last = blocks - 1 - (blocks - 1 - wave) % WAVES;
+    Rows x_now, x_next;
+    Weights ring[AHEAD];
+    if (wave < blocks) {
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) s.load(ring[a], min(wave + a * WAVES, last) * kDepth);
+      s.load(x_now, wave * kDepth);
+#pragma unroll 1
+      for (int b = wave; b < blocks; b += AHEAD * WAVES) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          const int at = b + a * WAVES;
+          if (a > 0 && at >= blocks) break;  // uniform
+          s.load(x_next, min(at + WAVES, last) * kDepth);
+          multiply(x_now, ring[a], acc);
+          s.load(ring[a], min(at + AHEAD * WAVES, last) * kDepth);
+          x_now = x_next;
+        }
+      }
     }
     if (blocks * kDepth < K && wave == blocks % WAVES) {
-      s.load_tail(now, blocks * kDepth, K);
-      multiply(now, acc);
+      s.load_tail(x_now, ring[0], blocks * kDepth, K);
+      multiply(x_now, ring[0], acc);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {

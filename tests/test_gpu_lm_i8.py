@@ -52,31 +52,33 @@ def test_sizes(M, K, N):
     check(M, K, N)
 
 
-@pytest.mark.parametrize("M", [3, 40, 100])
+@pytest.mark.parametrize("M,N", [(3, 100), (40, 100), (100, 100), (700, 1502)])
 @pytest.mark.parametrize("y", [F32, BF16, F16])
 @pytest.mark.parametrize("epi", list(EPI))
-def test_types_and_epilogues(M, y, epi):
-    check(M, 320, 100, y=y, epi=epi, scales=y, b=F16 if y == F32 else y)
+def test_types_and_epilogues(M, N, y, epi):
+    check(M, 320, N, y=y, epi=epi, scales=y, b=F16 if y == F32 else y)
 
 
 @pytest.mark.parametrize("M,K,N,plan", [
-    (1, 4096, 20000, "skinny cols=32"), (64, 512, 700, "skinny cols=16"), (2100, 384, 8200, "loads=16"), (4200, 192, 4000, "loads=16"),
-    (600, 512, 8192, "loads=16"), (4096, 128, 4096, "loads=16"), (300, 512, 700, "loads=16"), (300, 500, 700, "loads=0"),
-    (66, 8192, 300, "loads=16")])
+    (1, 4096, 20000, "skinny rows=16 cols=32"), (5, 64, 40000, "skinny rows=16 cols=64"), (64, 512, 700, "skinny rows=64 cols=16"),
+    (33, 200, 6000, "skinny rows=48 cols=32"), (300, 512, 700, "skinny rows=64 cols=16"), (130, 8192, 300, "skinny rows=48"),
+    (70, 63, 17, "skinny rows=48"), (2100, 384, 8200, "loads=16"), (4200, 192, 4000, "loads=16"), (600, 512, 8192, "loads=16"),
+    (4096, 128, 4096, "loads=16"), (700, 512, 1500, "loads=16"), (701, 500, 1501, "loads=0"), (65, 640, 40000, "loads=16"),
+    (700, 1, 1500, "loads=0"), (4097, 16, 130, "loads=16")])
 def test_kernels(M, K, N, plan):
     check(M, K, N, y=BF16, epi="bias_relu", b=BF16, plan=plan)
 
 
-@pytest.mark.parametrize("M", [5, 70, 260])
+@pytest.mark.parametrize("M,N", [(5, 130), (70, 130), (260, 130), (900, 1130)])
 @pytest.mark.parametrize("pad", [1, 8, 16])
-def test_strides_and_alignments(M, pad):
-    check(M, 272, 130, y=F16, pad=pad, ypad=3, xs=False)
+def test_strides_and_alignments(M, N, pad):
+    check(M, 272, N, y=F16, pad=pad, ypad=3, xs=False)
 
 
-@pytest.mark.parametrize("M", [1, 70])
-def test_largest_sums_are_exact(M):
+@pytest.mark.parametrize("M,N", [(1, 33), (70, 33), (513, 1040)])
+def test_largest_sums_are_exact(M, N):
     # All values at an end: the largest sum that 32 bits hold, and the deepest layer.
-    K, N = 2 ** 17 - 1, 33
+    K = 2 ** 17 - 1
     for a, b in ((-128, -128), (127, -128)):
         x, q = torch.full((M, K), a, dtype=I8, device="cuda"), torch.full((K, N), b, dtype=I8, device="cuda")
         Y = torch.empty(M, N, device="cuda")
@@ -112,8 +114,8 @@ def test_a_column_of_zeros_and_no_rows():
 
 
 def test_another_stream_and_graph_replays():
-    x, q = integers(70, 256, 1), integers(256, 200, 2)
-    P, Y = lm.i8_pack(q, floats(200, seed=3)), torch.zeros(70, 200, device="cuda")
+    x, q = integers(700, 256, 1), integers(256, 1400, 2)
+    P, Y = lm.i8_pack(q, floats(1400, seed=3)), torch.zeros(700, 1400, device="cuda")
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     lm.i8_dense_launch(x, P, None, Y, stream=side)
@@ -124,7 +126,7 @@ def test_another_stream_and_graph_replays():
     with torch.cuda.graph(graph):
         lm.i8_dense_launch(x, P, None, Y)
     for i in range(4):
-        x.copy_(integers(70, 256, 10 + i))
+        x.copy_(integers(700, 256, 10 + i))
         Y.zero_()
         graph.replay()
         got = Y.clone()
