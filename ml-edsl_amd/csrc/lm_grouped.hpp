@@ -102,28 +102,38 @@ template <typename Tl, int BKIND>
 __device__ __forceinline__ void grouped_rows_tile(const GroupedArgs& a, const RowTile& t, int n0, u32x4* lds) {
   using T = typename Tl::T;
   const TileOperand oa{static_cast<const char*>(a.x) + t.first * a.ldx * (int64_t)sizeof(T), a.ldx,
-                       (int)min(t.end - t.first, (int64_t)Tl::BM)};
+                       (int)min(t.end - t.first, (int64_t)Tl::BM), a.T};
   const TileOperand ob{static_cast<const char*>(a.w) +
                            (t.expert * a.stride_w + (BKIND == kRows ? n0 * a.ldw : (int64_t)n0)) * (int64_t)sizeof(T),
-                       a.ldw, (int)(a.N - n0)};
+                       a.ldw, (int)(a.N - n0), a.N};
   typename Tl::Acc acc[Tl::MI][Tl::NI];
   Tl::product(oa, ob, (int)a.K, lds, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const auto finish = [&](float (&v)[4], typename Tl::Acc sum, const float (&bias)[4]) {
 #pragma unroll
-  for (int j = 0; j < Tl::NI; ++j) {
-    const int n = n0 + 16 * (wave % Tl::WN * Tl::NI + j) + 4 * (lane / 16), left = (int)a.N - n;
-    if (left <= 0) break;
-    float bias[4] = {};
-    if (a.bias) get4_typed(a.bias, t.expert * a.ldbias + n, a.type, bias, left);
+    for (int e = 0; e < 4; ++e) v[e] = a.bias ? __fadd_rn(sum[e], bias[e]) : sum[e];
+    activate(v, a.epi, a.alpha);
+  };
+#pragma unroll
+  for (int j = 0; j < Tl::NI; j += 2) {
+    const int first = n0 + 16 * (wave % Tl::WN * Tl::NI + j), n = first + 4 * (lane / 16);
+    float bias[2][4] = {};
+    if (a.bias)
+#pragma unroll
+      for (int b = 0; b < 2 && j + b < Tl::NI; ++b)
+        if (n + 16 * b < a.N) get4_typed(a.bias, t.expert * a.ldbias + n + 16 * b, a.type, bias[b], (int)a.N - n - 16 * b);
 #pragma unroll
     for (int i = 0; i < Tl::MI; ++i) {
       const int64_t row = t.first + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
-      if (row >= t.end) break;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = a.bias ? __fadd_rn(acc[i][j][e], bias[e]) : acc[i][j][e];
-      activate(v, a.epi, a.alpha);
-      put4(static_cast<T*>(a.y) + row * a.ldy + n, v, left);
+      T* const to = static_cast<T*>(a.y) + row * a.ldy;
+      float v0[4], v1[4];
+      finish(v0, acc[i][j], bias[0]);
+      if constexpr (Tl::NI > 1) {
+        finish(v1, acc[i][j + 1], bias[1]);
+        put_blocks(to, first, a.N, v0, v1, row < t.end);
+      } else {
+        put4(to, n, a.N, v0, row < t.end);
+      }
     }
   }
 }
@@ -131,7 +141,7 @@ __device__ __forceinline__ void grouped_rows_tile(const GroupedArgs& a, const Ro
 // Big tiles, and Half (half as many columns) and Quarter ones for what is left of a round; the
 // same type where there are none.
 template <typename Big, typename Half, typename Quarter, int BKIND>
-__global__ void __launch_bounds__(Big::kThreads, 1) grouped_rows_kernel(GroupedArgs a) {
+__global__ void __launch_bounds__(Big::kThreads, Big::kWavesPerSimd) grouped_rows_kernel(GroupedArgs a) {
   static_assert(Big::kThreads == Half::kThreads && Big::kThreads == Quarter::kThreads, "one launch");
   constexpr int kLds = Big::kLds > Half::kLds ? (Big::kLds > Quarter::kLds ? Big::kLds : Quarter::kLds)
                                               : (Half::kLds > Quarter::kLds ? Half::kLds : Quarter::kLds);
@@ -193,7 +203,7 @@ __global__ void __launch_bounds__(64 * WAVES) grouped_skinny_kernel(GroupedArgs 
 
 // dW: an expert's tile of [M][N], its rows the depth. Experts without rows get zeros.
 template <typename Tl>
-__global__ void __launch_bounds__(Tl::kThreads, 1) grouped_weights_kernel(GroupedWeightArgs a) {
+__global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesPerSimd) grouped_weights_kernel(GroupedWeightArgs a) {
   using T = typename Tl::T;
   __shared__ u32x4 lds[Tl::kLds];
   const int tiles_m = (int)((a.M + Tl::BM - 1) / Tl::BM), tiles_n = (int)((a.N + Tl::BN - 1) / Tl::BN);
@@ -207,20 +217,24 @@ __global__ void __launch_bounds__(Tl::kThreads, 1) grouped_weights_kernel(Groupe
   const int m0 = tm * Tl::BM, n0 = tn * Tl::BN;
   const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
   const int64_t first = g.at(expert), rows = max(g.at(expert + 1) - first, (int64_t)0);
-  const TileOperand oa{static_cast<const char*>(a.a) + (first * a.lda + m0) * (int64_t)sizeof(T), a.lda, (int)(a.M - m0)};
-  const TileOperand ob{static_cast<const char*>(a.b) + (first * a.ldb + n0) * (int64_t)sizeof(T), a.ldb, (int)(a.N - n0)};
+  const TileOperand oa{static_cast<const char*>(a.a) + (first * a.lda + m0) * (int64_t)sizeof(T), a.lda, (int)(a.M - m0), a.M};
+  const TileOperand ob{static_cast<const char*>(a.b) + (first * a.ldb + n0) * (int64_t)sizeof(T), a.ldb, (int)(a.N - n0), a.N};
   typename Tl::Acc acc[Tl::MI][Tl::NI];
   Tl::product(oa, ob, (int)rows, lds, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
   for (int i = 0; i < Tl::MI; ++i) {
     const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
-    if (m >= a.M) continue;
+    const int64_t at = expert * a.stride_dw + m * a.lddw;
 #pragma unroll
-    for (int j = 0; j < Tl::NI; ++j) {
-      const int n = n0 + 16 * (wave % Tl::WN * Tl::NI + j) + 4 * (lane / 16);
-      const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (n < a.N) put4_typed(a.dw, expert * a.stride_dw + m * a.lddw + n, a.dw_type, v, (int)a.N - n);
+    for (int j = 0; j < Tl::NI; j += 2) {
+      const int first = n0 + 16 * (wave % Tl::WN * Tl::NI + j);
+      const float v0[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      const float v1[4] = {acc[i][j + 1][0], acc[i][j + 1][1], acc[i][j + 1][2], acc[i][j + 1][3]};
+      if (a.dw_type == kF32)
+        put_blocks(static_cast<float*>(a.dw) + at, first, a.N, v0, v1, m < a.M);
+      else
+        put_blocks(static_cast<T*>(a.dw) + at, first, a.N, v0, v1, m < a.M);
     }
   }
 }

@@ -1,7 +1,7 @@
 // The way back through the activation of a layer on groups of rows, and its
 // bias's gradient: dz = dy (y > 0), or dy times the slope elsewhere, and
 //   db_e = sum over e's rows of dz.
-// Bound by memory. Rows are summed in tiles of 64 whose sums a second launch adds in
+// Bound by memory. Rows are summed in tiles of 32 whose sums a second launch adds in
 // their order, so that the same call gives the same bits.
 #include "lm_grouped.hpp"
 
@@ -10,60 +10,64 @@ namespace lm {
 
 namespace {
 
-constexpr int kActRows = kGroupedActRows, kActWaves = 4;
+constexpr int kActRows = kGroupedActRows, kActThreads = 256, kAhead = 8;
 
+// A workgroup takes rows of one expert and a strip of columns, a thread its own columns of them.
 template <typename T>
-__global__ void __launch_bounds__(64 * kActWaves) grouped_act_kernel(GroupedActArgs a) {
-  constexpr int VEC = kVec<T>, COLS = 64 * VEC;
-  __shared__ float joined[kActWaves][COLS];
+__global__ void __launch_bounds__(kActThreads) grouped_act_kernel(GroupedActArgs a) {
+  constexpr int VEC = kVec<T>, COLS = kActThreads * VEC;
   const int tiles_n = (int)((a.N + COLS - 1) / COLS);
   const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  // The tile's number is its place among the partial sums: no other order.
+  // The tile's number is its place among the partial sums: whole tiles of rows first, then the experts'
+  // last ones.
   const int w = (int)block_of(), tile = w / tiles_n;
-  const int64_t col = (int64_t)(w % tiles_n) * COLS + lane * VEC;
-  // Whole tiles of rows first, then the experts' last ones.
+  const int64_t col = (int64_t)(w % tiles_n) * COLS + (int)threadIdx.x * VEC;
   const RowTiles tiles{g, kActRows, 0};
   int64_t whole, parts;
   tiles.total(&whole, &parts);
   const bool part = tile >= whole;
   RowTile t;
   if (!tiles.find(part, part ? tile - whole : tile, &t)) return;
+  if (col >= a.N) return;
   const int64_t end = min(t.first + kActRows, t.end);
+  const bool inside = (w % tiles_n + 1) * (int64_t)COLS <= a.N;  // uniform: no load waits at a branch then
+  const auto get = [&](const void* p, int64_t ld, int64_t row) {
+    const T* const from = static_cast<const T*>(p) + row * ld;
+    return inside ? load_packed<T, VEC>(from + col) : load_guarded<T, VEC>(from, col, a.N);
+  };
   float sum[VEC] = {};
-  for (int64_t row = t.first + wave; row < end; row += kActWaves) {
-    if (col >= a.N) break;
-    const Packed<T, VEC> dy = load_guarded<T, VEC>(static_cast<const T*>(a.dy) + row * a.lddy, col, a.N);
-    if (a.y) {
-      const Packed<T, VEC> y = load_guarded<T, VEC>(static_cast<const T*>(a.y) + row * a.ldy, col, a.N);
+  for (int64_t row = t.first; row < end; row += kAhead) {
+    // Rows past the last one are read as it is, and do not count.
+    Packed<T, VEC> dy[kAhead], y[kAhead];
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) dy[r] = get(a.dy, a.lddy, min(row + r, end - 1));
+    if (a.y)
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) y[r] = get(a.y, a.ldy, min(row + r, end - 1));
+#pragma unroll
+    for (int r = 0; r < kAhead; ++r) {
+      if (row + r >= end) break;
       Packed<T, VEC> dz;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = (float)dy.v[e], v = (float)y.v[e] > 0.0f ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
+        const float d = (float)dy[r].v[e];
+        const float v = !a.y || (float)y[r].v[e] > 0.0f ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
         dz.v[e] = (T)v;
         sum[e] += v;
       }
+      if (!a.y) continue;
+      T* const to = static_cast<T*>(a.dz) + (row + r) * a.lddz;
       if (col + VEC <= a.N)
-        *reinterpret_cast<Packed<T, VEC>*>(static_cast<T*>(a.dz) + row * a.lddz + col) = dz;
+        *reinterpret_cast<Packed<T, VEC>*>(to + col) = dz;
       else
         for (int e = 0; e < VEC; ++e)
-          if (col + e < a.N) static_cast<T*>(a.dz)[row * a.lddz + col + e] = dz.v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] += (float)dy.v[e];
+          if (col + e < a.N) to[col + e] = dz.v[e];
     }
   }
   if (!a.db) return;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = sum[e];
-  __syncthreads();
-  for (int c = threadIdx.x; c < COLS; c += 64 * kActWaves) {
-    float s = joined[0][c];
-#pragma unroll
-    for (int v = 1; v < kActWaves; ++v) s += joined[v][c];
-    const int64_t n = (int64_t)(w % tiles_n) * COLS + c;
-    if (n < a.N) a.partials[(int64_t)tile * a.N + n] = s;
-  }
+  for (int e = 0; e < VEC; ++e)
+    if (col + e < a.N) a.partials[(int64_t)tile * a.N + col + e] = sum[e];
 }
 
 __global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
@@ -85,7 +89,15 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
   const int64_t most = grouped_act_tiles(a.T, a.E);  // what the partial sums have room for
   const int64_t rows = rows_of(expert), tiles = min(rows / kActRows, max(most - before, (int64_t)0));
   float s = 0.0f;
-  for (int64_t t = 0; t < tiles; ++t) s += a.partials[(before + t) * a.N + n];
+  int64_t t = 0;
+  for (; t + 8 <= tiles; t += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = a.partials[(before + t + i) * a.N + n];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i];
+  }
+  for (; t < tiles; ++t) s += a.partials[(before + t) * a.N + n];
   if (rows % kActRows != 0 && all + parts < most) s += a.partials[(all + parts) * a.N + n];
   const int64_t at = expert * a.lddb + n;
   if (a.db_type == kF32)
@@ -98,9 +110,9 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
 
 template <typename T>
 hipError_t launch_act_type(const GroupedActArgs& a, hipStream_t stream) {
-  constexpr int COLS = 64 * kVec<T>;
+  constexpr int COLS = kActThreads * kVec<T>;
   const int64_t tiles = grouped_act_tiles(a.T, a.E) * ((a.N + COLS - 1) / COLS);
-  hipLaunchKernelGGL((grouped_act_kernel<T>), grid_of(tiles), dim3(64 * kActWaves), 0, stream, a);
+  hipLaunchKernelGGL((grouped_act_kernel<T>), grid_of(tiles), dim3(kActThreads), 0, stream, a);
   return launched();
 }
 

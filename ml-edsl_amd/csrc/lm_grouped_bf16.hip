@@ -5,16 +5,16 @@ namespace edsl {
 namespace lm {
 
 template <>
-hipError_t launch_grouped_rows<kBf16>(const GroupedArgs& a, int loads, hipStream_t stream) {
-  return GroupedLaunch<bf16>::rows(a, loads, stream);
+hipError_t launch_grouped_rows<kBf16>(const GroupedArgs& a, bool direct, hipStream_t stream) {
+  return GroupedLaunch<bf16>::rows(a, direct, stream);
 }
 template <>
 hipError_t launch_grouped_skinny<kBf16>(const GroupedArgs& a, hipStream_t stream) {
   return GroupedLaunch<bf16>::skinny(a, stream);
 }
 template <>
-hipError_t launch_grouped_weights<kBf16>(const GroupedWeightArgs& a, int loads, bool big, hipStream_t stream) {
-  return GroupedLaunch<bf16>::weights(a, loads, big, stream);
+hipError_t launch_grouped_weights<kBf16>(const GroupedWeightArgs& a, bool direct, bool big, hipStream_t stream) {
+  return GroupedLaunch<bf16>::weights(a, direct, big, stream);
 }
 
 }  // namespace lm

@@ -21,27 +21,23 @@ struct GroupedLaunch {
                        dim3(Big::kThreads), 0, stream, a);
     return launched();
   }
-  template <int BKIND, int LOADS>
-  static hipError_t rows_loads(const GroupedArgs& a, hipStream_t stream) {
-    if constexpr (LOADS == 0)
-      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, 0>>(a, 0, 0, stream);
-    else if constexpr (sizeof(T) == 4)
-      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, LOADS>, Tile<T, kRows, BKIND, 64, 64, 2, 4, LOADS, 4>>(
-          a, a.cus * 3 / 4, 0, stream);
-    else if constexpr (LOADS == 4)
-      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, 4, 3>>(a, 0, 0, stream);
-    else
-      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 256, 256, 2, 4, 16>, Tile<T, kRows, BKIND, 256, 128, 4, 2, 16, 3>,
-                        Tile<T, kRows, BKIND, 128, 128, 2, 4, 16, 3>>(a, a.cus / 4, a.cus / 2, stream);
+  template <int BKIND, bool DIRECT>
+  static hipError_t rows_kind(const GroupedArgs& a, hipStream_t stream) {
+    if constexpr (sizeof(T) == 4) {
+      // Bound by the matrix cores, which f32 keeps eight times as long: small tiles up to a round of large ones.
+      const int64_t tiles = (a.T / 128 + std::min<int64_t>(a.E, a.T)) * ((a.N + 127) / 128);
+      if (tiles <= a.cus) return rows_tiles<BKIND, Tile<T, kRows, BKIND, 64, 64, 2, 4, DIRECT, DIRECT ? 3 : 2>>(a, 0, 0, stream);
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, DIRECT>>(a, 0, 0, stream);
+    } else if constexpr (!DIRECT) {
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, false>>(a, 0, 0, stream);
+    } else {
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 256, 256, 2, 4, true>, Tile<T, kRows, BKIND, 256, 128, 4, 2, true, 3>,
+                        Tile<T, kRows, BKIND, 128, 128, 2, 4, true, 3>>(a, a.cus / 4, a.cus / 2, stream);
+    }
   }
-  template <int BKIND>
-  static hipError_t rows_kind(const GroupedArgs& a, int loads, hipStream_t stream) {
-    return loads == 16  ? rows_loads<BKIND, 16>(a, stream)
-           : loads == 4 ? rows_loads<BKIND, 4>(a, stream)
-                        : rows_loads<BKIND, 0>(a, stream);
-  }
-  static hipError_t rows(const GroupedArgs& a, int loads, hipStream_t stream) {
-    return a.turned ? rows_kind<kRows>(a, loads, stream) : rows_kind<kCols>(a, loads, stream);
+  static hipError_t rows(const GroupedArgs& a, bool direct, hipStream_t stream) {
+    if (a.turned) return direct ? rows_kind<kRows, true>(a, stream) : rows_kind<kRows, false>(a, stream);
+    return direct ? rows_kind<kCols, true>(a, stream) : rows_kind<kCols, false>(a, stream);
   }
 
   template <int BKIND, int NJ, int U, int AHEAD>
@@ -75,12 +71,11 @@ struct GroupedLaunch {
     hipLaunchKernelGGL((grouped_weights_kernel<Tl>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
     return launched();
   }
-  static hipError_t weights(const GroupedWeightArgs& a, int loads, bool big, hipStream_t stream) {
-    if (loads == 0) return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, 0>>(a, stream);
-    if (loads == 4) return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, 4>>(a, stream);
+  static hipError_t weights(const GroupedWeightArgs& a, bool direct, bool big, hipStream_t stream) {
+    if (!direct) return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, false>>(a, stream);
     if constexpr (sizeof(T) == 2)
-      if (big) return weights_tile<Tile<T, kCols, kCols, 256, 256, 2, 4, 16>>(a, stream);
-    return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, 16>>(a, stream);
+      if (big) return weights_tile<Tile<T, kCols, kCols, 256, 256, 2, 4, true>>(a, stream);
+    return weights_tile<Tile<T, kCols, kCols, 128, 128, 2, 4, true>>(a, stream);
   }
 };
 

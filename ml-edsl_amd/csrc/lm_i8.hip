@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(256) i8_pack_kernel(I8PackArgs a) {
 template <typename Tl>
 __device__ __forceinline__ void i8_tile(const I8Args& a, int m0, int n0, u32x4* lds) {
   const int64_t tile_bytes = i8_blocks(a.K) * 1024;
-  const TileOperand oa{reinterpret_cast<const char*>(a.x) + m0 * a.ldx, a.ldx, min(a.M - m0, Tl::BM)};
-  const TileOperand ob{a.w + n0 / 16 * tile_bytes, tile_bytes, min(a.N - n0, Tl::BN)};
+  const TileOperand oa{reinterpret_cast<const char*>(a.x) + m0 * a.ldx, a.ldx, min(a.M - m0, Tl::BM), a.M};
+  const TileOperand ob{a.w + n0 / 16 * tile_bytes, tile_bytes, min(a.N - n0, Tl::BN), a.N};
   typename Tl::Acc acc[Tl::MI][Tl::NI];
   Tl::product(oa, ob, a.K, lds, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -63,32 +63,44 @@ __device__ __forceinline__ void i8_tile(const I8Args& a, int m0, int n0, u32x4* 
     const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
     xs[i] = a.x_scales && m < a.M ? a.x_scales[m] : 1.0f;
   }
+  const auto finish = [&](float (&v)[4], i32x4 sum, f32x4 ws, float scale, const float (&bias)[4]) {
 #pragma unroll
-  for (int j = 0; j < Tl::NI; ++j) {
-    const int n = n0 + 16 * (wave % Tl::WN * Tl::NI + j) + 4 * (lane / 16), left = a.N - n;
-    if (left <= 0) break;
-    float bias[4] = {};
-    if (a.bias) get4_typed(a.bias, n, a.bias_type, bias, left);
-    const f32x4 ws = *reinterpret_cast<const f32x4*>(a.w_scales + n);  // kept for whole blocks of 16
+    for (int e = 0; e < 4; ++e) {
+      v[e] = (float)sum[e] * ws[e] * scale;
+      if (a.bias) v[e] = __fadd_rn(v[e], bias[e]);
+    }
+    activate(v, a.epi, a.alpha);
+  };
+#pragma unroll
+  for (int j = 0; j < Tl::NI; j += 2) {
+    const int first = n0 + 16 * (wave % Tl::WN * Tl::NI + j), n = first + 4 * (lane / 16);
+    float bias[2][4] = {};
+    f32x4 ws[2] = {};
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      if (n + 16 * b < a.N) {
+        if (a.bias) get4_typed(a.bias, n + 16 * b, a.bias_type, bias[b], a.N - n - 16 * b);
+        ws[b] = *reinterpret_cast<const f32x4*>(a.w_scales + n + 16 * b);  // kept for whole blocks of 16
+      }
 #pragma unroll
     for (int i = 0; i < Tl::MI; ++i) {
       const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
-      if (m >= a.M) break;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = (float)acc[i][j][e] * ws[e] * xs[i];
-        if (a.bias) v[e] = __fadd_rn(v[e], bias[e]);
-      }
-      activate(v, a.epi, a.alpha);
-      put4_typed(a.y, m * a.ldy + n, a.y_type, v, left);
+      float v0[4], v1[4];
+      finish(v0, acc[i][j], ws[0], xs[i], bias[0]);
+      finish(v1, acc[i][j + 1], ws[1], xs[i], bias[1]);
+      if (a.y_type == kF32)
+        put_blocks(static_cast<float*>(a.y) + m * a.ldy, first, a.N, v0, v1, m < a.M);
+      else if (a.y_type == kBf16)
+        put_blocks(static_cast<bf16*>(a.y) + m * a.ldy, first, a.N, v0, v1, m < a.M);
+      else
+        put_blocks(static_cast<f16*>(a.y) + m * a.ldy, first, a.N, v0, v1, m < a.M);
     }
   }
 }
 
 // Big tiles, and Half and Quarter ones for what is left of a round of the CUs.
 template <typename Big, typename Half, typename Quarter>
-__global__ void __launch_bounds__(Big::kThreads, 1) i8_tile_kernel(I8Args a) {
+__global__ void __launch_bounds__(Big::kThreads, Big::kWavesPerSimd) i8_tile_kernel(I8Args a) {
   constexpr int kLds = Big::kLds > Half::kLds ? (Big::kLds > Quarter::kLds ? Big::kLds : Quarter::kLds)
                                               : (Half::kLds > Quarter::kLds ? Half::kLds : Quarter::kLds);
   __shared__ u32x4 lds[kLds];
@@ -161,10 +173,10 @@ hipError_t launch_i8_pack(const I8PackArgs& a, hipStream_t stream) {
   return launched();
 }
 
-hipError_t launch_i8_tile(const I8Args& a, int loads, hipStream_t stream) {
-  if (loads == 0) return launch_tiles<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 4, 0>>(a, 0, 0, stream);
-  return launch_tiles<Tile<int8_t, kRows, kBlocks, 256, 256, 2, 4, 16>, Tile<int8_t, kRows, kBlocks, 256, 128, 4, 2, 16, 3>,
-                      Tile<int8_t, kRows, kBlocks, 128, 128, 2, 4, 16, 3>>(a, a.cus / 4, a.cus / 2, stream);
+hipError_t launch_i8_tile(const I8Args& a, bool direct, hipStream_t stream) {
+  if (!direct) return launch_tiles<Tile<int8_t, kRows, kBlocks, 128, 128, 2, 4, false>>(a, 0, 0, stream);
+  return launch_tiles<Tile<int8_t, kRows, kBlocks, 256, 256, 2, 4, true>, Tile<int8_t, kRows, kBlocks, 256, 128, 4, 2, true, 3>,
+                      Tile<int8_t, kRows, kBlocks, 128, 128, 2, 4, true, 3>>(a, a.cus / 4, a.cus / 2, stream);
 }
 
 hipError_t launch_i8_skinny(const I8Args& a, int rows16, int cols16, hipStream_t stream) {

@@ -123,10 +123,9 @@ struct GroupedArgs {
   TileRounds rounds;
 };
 constexpr int kGroupedSkinnyRows = 32;  // experts with up to this many rows may stream their weights
-// How tiles take their operands: `loads` bytes a lane at a time, 16 or 4, where all rows start on so many and
-// are whole multiples of them along K; 0: any.
+// direct: all rows start on 16 bytes, and K (of the product over rows) is whole pieces of 16 bytes.
 template <int TYPE>
-hipError_t launch_grouped_rows(const GroupedArgs& a, int loads, hipStream_t stream);
+hipError_t launch_grouped_rows(const GroupedArgs& a, bool direct, hipStream_t stream);
 template <int TYPE>
 hipError_t launch_grouped_skinny(const GroupedArgs& a, hipStream_t stream);
 
@@ -140,7 +139,7 @@ struct GroupedWeightArgs {
   bool ids64;
 };
 template <int TYPE>
-hipError_t launch_grouped_weights(const GroupedWeightArgs& a, int loads, bool big, hipStream_t stream);
+hipError_t launch_grouped_weights(const GroupedWeightArgs& a, bool direct, bool big, hipStream_t stream);
 
 // dz = dy * act'(y), and the sums of dz over each expert's rows.
 struct GroupedActArgs {
@@ -155,7 +154,7 @@ struct GroupedActArgs {
   int E, type, db_type;
   bool ids64;
 };
-constexpr int kGroupedActRows = 64;  // rows whose sums are taken together
+constexpr int kGroupedActRows = 32;  // rows whose sums are taken together
 // The most such tiles that T rows in E groups can have.
 constexpr int64_t grouped_act_tiles(int64_t T, int64_t E) { return T / kGroupedActRows + (E < T ? E : T); }
 hipError_t launch_grouped_act(const GroupedActArgs& a, hipStream_t stream);
@@ -186,7 +185,7 @@ struct I8Args {
   int cus;
   TileRounds rounds;
 };
-hipError_t launch_i8_tile(const I8Args& a, int loads, hipStream_t stream);
+hipError_t launch_i8_tile(const I8Args& a, bool direct, hipStream_t stream);
 hipError_t launch_i8_skinny(const I8Args& a, int rows16, int cols16, hipStream_t stream);
 
 }  // namespace lm

@@ -18,14 +18,13 @@ namespace {
 constexpr int64_t kMostI8Depth = (int64_t(1) << 17) - 1;  // K 2^14 < 2^31: 32-bit sums are exact
 constexpr int kMostExperts = 65535;
 
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 // A tile's rows of `ld` elements within the 31 bits of an asynchronous load's offset.
 bool reachable(int64_t rows, int64_t ld, int e) { return rows * ld * e < 0x7fffffff; }
-// The bytes that all of these are multiples of, 16, 4 or 0 (fewer).
-int common_bytes(std::initializer_list<int64_t> values) {
+// Whether all of these are multiples of 16.
+bool whole16(std::initializer_list<int64_t> values) {
   int64_t all = 0;
   for (const int64_t v : values) all |= v;
-  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 0;
+  return all % 16 == 0;
 }
 int64_t address(const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); }
 
@@ -91,11 +90,11 @@ void i8_dense(lm::I8Args a, int64_t M, int64_t N, int64_t K, void* stream) {
       set_plan("i8_skinny rows=%d cols=%d", 16 * rows, 16 * cols);
       return;
     }
-    const int loads = aligned16(a.x) && a.ldx % 16 == 0 && K % 16 == 0 && reachable(256, a.ldx, 1) ? 16 : 0;
+    const bool direct = whole16({address(a.x), a.ldx, K}) && reachable(256, a.ldx, 1);
     check_grid((M + 127) / 128 + 4, (N + 127) / 128 + 4);
     a.cus = cus;
-    check_hip(lm::launch_i8_tile(a, loads, s), "i8_tile launch");
-    set_plan("i8_tile loads=%d", loads);
+    check_hip(lm::launch_i8_tile(a, direct, s), "i8_tile launch");
+    set_plan("i8_tile %s", direct ? "direct" : "any");
   });
 }
 
@@ -122,15 +121,15 @@ hipError_t skinny_by_type(const lm::GroupedArgs& a, hipStream_t s) {
          : a.type == lm::kBf16 ? lm::launch_grouped_skinny<lm::kBf16>(a, s)
                                : lm::launch_grouped_skinny<lm::kF16>(a, s);
 }
-hipError_t rows_by_type(const lm::GroupedArgs& a, int loads, hipStream_t s) {
-  return a.type == lm::kF32    ? lm::launch_grouped_rows<lm::kF32>(a, loads, s)
-         : a.type == lm::kBf16 ? lm::launch_grouped_rows<lm::kBf16>(a, loads, s)
-                               : lm::launch_grouped_rows<lm::kF16>(a, loads, s);
+hipError_t rows_by_type(const lm::GroupedArgs& a, bool direct, hipStream_t s) {
+  return a.type == lm::kF32    ? lm::launch_grouped_rows<lm::kF32>(a, direct, s)
+         : a.type == lm::kBf16 ? lm::launch_grouped_rows<lm::kBf16>(a, direct, s)
+                               : lm::launch_grouped_rows<lm::kF16>(a, direct, s);
 }
-hipError_t weights_by_type(const lm::GroupedWeightArgs& a, int loads, bool big, hipStream_t s) {
-  return a.type == lm::kF32    ? lm::launch_grouped_weights<lm::kF32>(a, loads, big, s)
-         : a.type == lm::kBf16 ? lm::launch_grouped_weights<lm::kBf16>(a, loads, big, s)
-                               : lm::launch_grouped_weights<lm::kF16>(a, loads, big, s);
+hipError_t weights_by_type(const lm::GroupedWeightArgs& a, bool direct, bool big, hipStream_t s) {
+  return a.type == lm::kF32    ? lm::launch_grouped_weights<lm::kF32>(a, direct, big, s)
+         : a.type == lm::kBf16 ? lm::launch_grouped_weights<lm::kBf16>(a, direct, big, s)
+                               : lm::launch_grouped_weights<lm::kF16>(a, direct, big, s);
 }
 
 // y = epi(x @ w_e + b_e), the launches of one product over rows. `plan`: what ran.
@@ -142,17 +141,15 @@ void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t 
   if (streams) {
     check_hip(skinny_by_type(a, s), "grouped_skinny launch");
   }
-  int loads = -1;
+  const char* tiles = "";
   if (a.T > a.skip) {
-    loads = reachable(256, a.ldx, e) && reachable(256, a.ldw, e)
-                ? common_bytes({address(a.x), a.ldx * e, address(a.w), a.ldw * e, a.stride_w * e, a.K * e})
-                : 0;
-    // The last elements of a row come with their neighbours' bytes.
-    if (loads == 4 && a.N * e % 4 != 0) loads = 0;
-    check_grid(a.T / 128 + a.E, (a.N + 127) / 128 + 16);
-    check_hip(rows_by_type(a, loads, s), "grouped_rows launch");
+    const bool direct = whole16({address(a.x), a.ldx * e, address(a.w), a.ldw * e, a.stride_w * e, a.K * e}) &&
+                        reachable(256, a.ldx, e) && reachable(256, a.ldw, e);
+    check_grid(a.T / 64 + a.E, (a.N + 63) / 64 + 16);
+    check_hip(rows_by_type(a, direct, s), "grouped_rows launch");
+    tiles = direct ? "+tiles direct" : "+tiles any";
   }
-  snprintf(plan, len, "%s%s", streams ? "stream" : "", loads < 0 ? "" : loads == 16 ? "+tiles=16" : loads == 4 ? "+tiles=4" : "+tiles=any");
+  snprintf(plan, len, "%s%s", streams ? "stream" : "", tiles);
 }
 
 void grouped_dense(lm::GroupedArgs a, int64_t E, void* stream) {
@@ -221,7 +218,7 @@ void grouped_backward(Backward a, void* stream) {
   const int64_t lddz = (a.N + chunk - 1) / chunk * chunk;
   const size_t dz_bytes = masks ? aligned((size_t)a.T * lddz * e) : 0;
   const size_t sums = a.db ? (size_t)lm::grouped_act_tiles(a.T, (int)a.E) * a.N * sizeof(float) : 0;
-  if (masks || a.db) check_grid(a.T / 64 + a.E, a.N / 256 + 1);
+  if (masks || a.db) check_grid(a.T / lm::kGroupedActRows + a.E, a.N / 256 + 1);
   device_launch(dz_bytes + sums, stream, [&](char* ws, int cus) {
     const hipStream_t s = as_stream(stream);
     const void* dz = a.dy;
@@ -251,15 +248,13 @@ void grouped_backward(Backward a, void* stream) {
       if (a.dw_turned) std::swap(g.a, g.b), std::swap(g.lda, g.ldb), std::swap(g.M, g.N);
       g.offsets = a.offsets, g.dw = a.dw, g.lddw = a.lddw, g.stride_dw = a.stride_dw, g.T = a.T;
       g.E = (int)a.E, g.type = a.type, g.dw_type = a.dw_type, g.ids64 = a.ids64;
-      int loads = reachable(64, g.lda, e) && reachable(64, g.ldb, e)
-                      ? common_bytes({address(g.a), g.lda * e, address(g.b), g.ldb * e})
-                      : 0;
-      if (loads == 4 && (g.M * e % 4 != 0 || g.N * e % 4 != 0)) loads = 0;
+      const bool direct = whole16({address(g.a), g.lda * e, address(g.b), g.ldb * e}) && reachable(64, g.lda, e) &&
+                          reachable(64, g.ldb, e);
       const int64_t tiles256 = ((g.M + 255) / 256) * ((g.N + 255) / 256) * a.E;
-      const bool big = loads == 16 && a.type != lm::kF32 && a.T >= 256 * a.E && tiles256 >= cus;
+      const bool big = direct && a.type != lm::kF32 && a.T >= 256 * a.E && tiles256 >= cus;
       check_grid((g.M + 127) / 128 * a.E, (g.N + 127) / 128);
-      check_hip(weights_by_type(g, loads, big, s), "grouped_weights launch");
-      tiles = big ? " dW 256x256" : loads == 16 ? " dW 128x128" : loads == 4 ? " dW loads=4" : " dW any";
+      check_hip(weights_by_type(g, direct, big, s), "grouped_weights launch");
+      tiles = big ? " dW 256x256" : direct ? " dW 128x128" : " dW any";
     }
     set_plan("grouped_dense_backward %s%s%s%s%s", type_name(a.type), masks ? " mask" : "", *plan ? " dX " : "", plan,
              tiles);

@@ -11,9 +11,8 @@
 // An operand lies in memory, and in LDS, with k contiguous (kRows), with its own index
 // contiguous (kCols: read through the transposing LDS load, or element by element in f32)
 // or laid out as the instruction takes it (kBlocks, 8-bit weights). 16-byte chunks change
-// places by row so that a fragment's reads meet all banks. LOADS is how they come: 16 bytes
-// a lane at a time where all rows start on 16 bytes and no chunk crosses a row's end, 4 where
-// that holds for 4 bytes, or 0: through registers, cut element by element, for any alignment.
+// places by row so that a fragment's reads meet all banks. Where a row starts off 16 bytes, or a
+// chunk would cross its end (DIRECT false), they go through registers instead, loaded from any address.
 //
 // The two operands are given to the instruction in exchanged places, so that a lane
 // ends with four successive n of one row: wide stores.
@@ -100,23 +99,19 @@ __device__ __forceinline__ void tile_arrived() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ void tile_to_lds4(i32x4 from, int offset, const void* to) {  // 4 bytes a lane
-  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)to;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane((int)at)), "v"(offset), "s"(from)
-               : "memory", "m0");
-}
+// All waves' reads and writes of LDS have ended; loads to registers go on.
+__device__ __forceinline__ void tile_met() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // One operand of a tile: `n` of its own index's elements are there from `base` on.
 struct TileOperand {
   const char* base;  // its first element at k = 0
   int64_t ld;        // elements from one row of memory to the next
   int n;
+  int64_t all;  // of its own index's elements, those before `base` too
 };
 
 // MN of an operand's own index in LDS and its loads by THREADS threads.
-template <typename T, int KIND, int MN, int THREADS, int LOADS>
+template <typename T, int KIND, int MN, int THREADS, bool DIRECT>
 struct TileSide {
   static constexpr int kChunk = TileElem<T>::kChunk;
   static constexpr int kDepth = 8 * kChunk;  // k of a stage
@@ -139,25 +134,33 @@ struct TileSide {
     col = c * kChunk;
   }
 
-  static constexpr int kParts = LOADS == 4 ? 4 : 1;  // loads of a chunk
-  int offset[LOADS ? kMine * kParts : 1];
-  u32x4 held[LOADS ? 1 : kMine];
+  int offset[DIRECT ? kMine : 1];
+  const T* from[DIRECT ? 1 : kMine];  // of the first stage
+  int by[!DIRECT && KIND == kCols ? kMine : 1];  // columns that a chunk starts before its place
+  u32x4 held[2][DIRECT ? 1 : kMine];  // two stages
 
   __device__ __forceinline__ void init(const TileOperand& o, int tid) {
-    if constexpr (LOADS != 0) {
 #pragma unroll
-      for (int c = 0; c < kMine * kParts; ++c) {
-        // Four lanes have a chunk's 4-byte parts.
-        const int at = LOADS == 16 ? c * THREADS + tid
-                                   : c / 4 * THREADS + tid / 64 * 64 + c % 4 * 16 + tid % 64 / 4;
-        const int part = LOADS == 16 ? 0 : tid % 4 * 4;
-        if constexpr (KIND == kBlocks) {
-          // Blocks of 16 columns x 64 k, `ld` bytes from 16 columns to the next.
-          offset[c] = (int)((at / 128) * o.ld) + (at % 128) * 16;
+    for (int c = 0; c < kMine; ++c) {
+      const int at = c * THREADS + tid;
+      if constexpr (KIND == kBlocks) {
+        // Blocks of 16 columns x 64 k, `ld` bytes from 16 columns to the next.
+        offset[c] = (int)((at / 128) * o.ld) + (at % 128) * 16;
+      } else {
+        int row, col;
+        place(at, row, col);
+        if constexpr (DIRECT) {
+          offset[c] = (int)(((int64_t)row * o.ld + col) * (int64_t)sizeof(T));
         } else {
-          int row, col;
-          place(at, row, col);
-          offset[c] = (int)(((int64_t)row * o.ld + col) * (int64_t)sizeof(T)) + part;
+          // Rows past the last one repeat it: nobody stores their sums. Chunks past the last column are its row's
+          // last elements.
+          if constexpr (KIND == kRows) {
+            row = min(row, o.n - 1);
+          } else {
+            by[c] = o.all >= kChunk ? max(col - (o.n - kChunk), 0) : 0;
+            col -= by[c];
+          }
+          from[c] = reinterpret_cast<const T*>(o.base) + row * o.ld + col;
         }
       }
     }
@@ -169,7 +172,7 @@ struct TileSide {
     int k0, left;
   };
   static __device__ __forceinline__ Source source(const TileOperand& o, int K, int k0) {
-    if constexpr (LOADS == 0) return {i32x4{}, k0, K - k0};
+    if constexpr (!DIRECT) return {i32x4{}, k0, K - k0};
     if constexpr (KIND == kRows)
       return {buffer_rsrc(o.base + (int64_t)k0 * sizeof(T), ((o.n - 1) * o.ld + K - k0) * (int64_t)sizeof(T)), k0,
               K - k0};
@@ -179,45 +182,57 @@ struct TileSide {
     return {buffer_rsrc(o.base + (int64_t)k0 * 16, (int64_t)((o.n + 15) / 16) * o.ld - (int64_t)k0 * 16), k0, K - k0};
   }
   // Starts load c of kMine of a stage.
-  __device__ __forceinline__ void load(int c, const Source& s, const TileOperand& o, u32x4* lds, int tid, int wave) {
+  __device__ __forceinline__ void load(int c, const Source& s, const TileOperand& o, u32x4* lds, int tid, int wave,
+                                       int hold = 0) {
     int row, col;
-    if constexpr (LOADS != 0) {
-#pragma unroll
-      for (int p = 0; p < kParts; ++p) {
-        int at = offset[c * kParts + p];
-        if constexpr (KIND == kRows) {  // rows go on past K
-          place(LOADS == 16 ? c * THREADS + tid : c * THREADS + tid / 64 * 64 + p * 16 + tid % 64 / 4, row, col);
-          if constexpr (LOADS == 4) col += tid % 4 * (4 / (int)sizeof(T));
-          at = col < s.left ? at : kOutside;
-        }
-        u32x4* const to = lds + c * THREADS + wave * 64 + p * 16;
-        if constexpr (LOADS == 16)
-          tile_to_lds(s.from, at, to);
-        else
-          tile_to_lds4(s.from, at, to);
+    if constexpr (DIRECT) {
+      int at = offset[c];
+      if constexpr (KIND == kRows) {  // rows go on past K
+        place(c * THREADS + tid, row, col);
+        at = col < s.left ? at : kOutside;
       }
+      tile_to_lds(s.from, at, lds + c * THREADS + wave * 64);
     } else {
       static_assert(KIND != kBlocks, "blocks are always aligned");
-      place(c * THREADS + tid, row, col);
-      const T* const base = reinterpret_cast<const T*>(o.base);
-      // Inside, or past the last row, whose sums nobody stores, a load depends on no comparison.
-      if (KIND == kRows ? s.left >= kDepth : s.left >= kDepth && o.n >= MN) {
-        const int64_t at = KIND == kRows ? min(row, o.n - 1) * o.ld + s.k0 + col : (row + s.k0) * o.ld + col;
-        held[c] = __builtin_bit_cast(u32x4, load_packed<T, kChunk>(base + at));
-        return;
-      }
-      const int rows = KIND == kRows ? o.n : s.left, left = KIND == kRows ? s.left : o.n;
-      held[c] = u32x4{0, 0, 0, 0};
-      if (row < rows && col < left) {
-        const T* const p = base + (KIND == kRows ? row * o.ld + s.k0 : (row + s.k0) * o.ld);
-        held[c] = __builtin_bit_cast(u32x4, load_guarded<T, kChunk>(p, col, left));
+      if constexpr (KIND == kRows) {
+        if (s.left >= kDepth) {  // uniform
+          held[hold][c] = __builtin_bit_cast(u32x4, load_packed<T, kChunk>(from[c] + s.k0));
+        } else {
+          place(c * THREADS + tid, row, col);
+          held[hold][c] = __builtin_bit_cast(u32x4, load_guarded<T, kChunk>(from[c] + s.k0, 0, s.left - col));
+        }
+      } else {
+        // What depends on a loaded value waits for it: chunks are moved to their places as they are put.
+        const T* const p = from[c] + s.k0 * o.ld;
+        place(c * THREADS + tid, row, col);
+        if (s.left >= kDepth && o.all >= kChunk) {  // uniform
+          held[hold][c] = __builtin_bit_cast(u32x4, load_packed<T, kChunk>(p));
+        } else {
+          held[hold][c] = u32x4{0, 0, 0, 0};
+          if (row < s.left)
+            held[hold][c] = o.all >= kChunk
+                                ? __builtin_bit_cast(u32x4, load_packed<T, kChunk>(p))
+                                : __builtin_bit_cast(u32x4, load_guarded<T, kChunk>(p, col, o.n));
+        }
       }
     }
   }
-  __device__ __forceinline__ void put(u32x4* lds, int tid) {
-    if constexpr (LOADS == 0)
+  // The elements from `by` on, from the first place on.
+  static __device__ __forceinline__ u32x4 moved(u32x4 v, int by) {
+    const unsigned bits = (unsigned)by * 8 * sizeof(T);
+    const uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+    const uint64_t up = bits < 64 ? hi >> bits : 0;
+    const uint64_t low = bits == 0 ? lo : bits < 64 ? lo >> bits | hi << (64 - bits) : bits < 128 ? hi >> (bits - 64) : 0;
+    return u32x4{(uint32_t)low, (uint32_t)(low >> 32), (uint32_t)up, (uint32_t)(up >> 32)};
+  }
+  __device__ __forceinline__ void put(const TileOperand& o, u32x4* lds, int tid, int hold) {
+    if constexpr (!DIRECT) {
+      if (KIND == kCols && o.n < MN && o.all >= kChunk)  // uniform
 #pragma unroll
-      for (int c = 0; c < kMine; ++c) lds[c * THREADS + tid] = held[c];
+        for (int c = 0; c < kMine; ++c) held[hold][c] = moved(held[hold][c], by[KIND == kCols ? c : 0]);
+#pragma unroll
+      for (int c = 0; c < kMine; ++c) lds[c * THREADS + tid] = held[hold][c];
+    }
   }
 
   // The fragment of block `b` (16 of the operand's index) at step s (half a stage).
@@ -249,7 +264,7 @@ struct TileSide {
 };
 
 // NS stages in LDS.
-template <typename T_, int AKIND, int BKIND, int BM_, int BN_, int WM_, int WN_, int LOADS, int NS = 2>
+template <typename T_, int AKIND, int BKIND, int BM_, int BN_, int WM_, int WN_, bool DIRECT, int NS = 2>
 struct Tile {
   using T = T_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
@@ -257,10 +272,12 @@ struct Tile {
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   using E = TileElem<T>;
   using Acc = typename E::Acc;
-  using A = TileSide<T, AKIND, BM, kThreads, LOADS>;
-  using B = TileSide<T, BKIND, BN, kThreads, BKIND == kBlocks ? 16 : LOADS>;
+  using A = TileSide<T, AKIND, BM, kThreads, DIRECT>;
+  using B = TileSide<T, BKIND, BN, kThreads, DIRECT || BKIND == kBlocks>;
   static constexpr int kStage = A::kAll + B::kAll;  // chunks
   static constexpr int kLds = NS * kStage;
+  // Waves a SIMD that LDS leaves room for: two workgroups of eight waves a CU, or one.
+  static constexpr int kWavesPerSimd = kLds * 16 <= 80 * 1024 ? 4 : 2;
 
   // acc[i][j][e]: row 16 (wave's MI + i) + lane % 16, column 16 (wave's NI + j) + 4 (lane / 16) + e.
   static __device__ __forceinline__ void product(const TileOperand& oa, const TileOperand& ob, int K, u32x4* lds,
@@ -277,7 +294,7 @@ struct Tile {
     B b;
     a.init(oa, tid);
     b.init(ob, tid);
-    constexpr int kLoads = A::kMine * A::kParts + B::kMine * B::kParts;  // of a stage, a thread
+    constexpr int kLoads = A::kMine + B::kMine;  // of a stage, a thread
     constexpr int kAll = A::kMine + B::kMine;
     struct Fragments {
       u32x4 a[MI], b[NI];
@@ -296,23 +313,27 @@ struct Tile {
     const auto sources = [&](int st) {
       return Sources{A::source(oa, K, st * A::kDepth), B::source(ob, K, st * A::kDepth)};
     };
-    const auto load = [&](int c, const Sources& s, u32x4* to) {
+    const auto load = [&](int c, const Sources& s, u32x4* to, int hold) {
       if (c < A::kMine)
-        a.load(c, s.a, oa, to, tid, wave);
+        a.load(c, s.a, oa, to, tid, wave, hold);
       else
-        b.load(c - A::kMine, s.b, ob, to + A::kAll, tid, wave);
+        b.load(c - A::kMine, s.b, ob, to + A::kAll, tid, wave, hold);
     };
-    const auto load_all = [&](int st, u32x4* to) {
+    const auto load_all = [&](int st, u32x4* to, int hold) {
       const Sources s = sources(st);
 #pragma unroll
-      for (int c = 0; c < kAll; ++c) load(c, s, to);
+      for (int c = 0; c < kAll; ++c) load(c, s, to, hold);
+    };
+    const auto put_all = [&](u32x4* to, int hold) {
+      a.put(oa, to, tid, hold);
+      b.put(ob, to + A::kAll, tid, hold);
     };
     const auto run = [&](auto working) {
       constexpr bool kWorks = decltype(working)::value;
       Fragments f0, f1;
-      if constexpr (LOADS != 0) {
+      if constexpr (DIRECT) {
 #pragma unroll
-        for (int st = 0; st < NS; ++st) load_all(st, lds + st * kStage);
+        for (int st = 0; st < NS; ++st) load_all(st, lds + st * kStage, 0);
         tile_arrived<(NS - 1) * kLoads>();
         if constexpr (kWorks) read(lds, 0, f0);
         int at = 0;
@@ -337,7 +358,7 @@ struct Tile {
 #pragma unroll
           for (int c = 0; c < kAll; ++c) {
             __builtin_amdgcn_sched_barrier(0);
-            load(c, s, now);
+            load(c, s, now, 0);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (kWorks)
 #pragma unroll
@@ -348,15 +369,20 @@ struct Tile {
         }
         tile_arrived<0>();  // nothing is on its way to LDS when the workgroup ends
       } else {
-        static_assert(LOADS || NS == 2, "a stage at a time goes through registers");
-        load_all(0, lds);
-        a.put(lds, tid);
-        b.put(lds + A::kAll, tid);
-        for (int st = 0; st < stages; ++st) {
+        static_assert(DIRECT || NS == 2, "a stage at a time goes through registers");
+        // One stage in LDS, two on their way in registers. Blocks of weights go straight to LDS, a stage ahead.
+        const auto turn = [&](int st, int hold) {
           u32x4* const now = lds + st % 2 * kStage;
           u32x4* const next = lds + (st + 1) % 2 * kStage;
-          tile_arrived<0>();
-          load_all(st + 1, next);
+          if constexpr (BKIND == kBlocks)
+            tile_arrived<0>();
+          else
+            tile_met();
+          if constexpr (BKIND == kBlocks) {
+            const Sources s = sources(st + 1);
+#pragma unroll
+            for (int c = 0; c < B::kMine; ++c) b.load(c, s.b, ob, next + A::kAll, tid, wave);
+          }
           if constexpr (kWorks)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -366,9 +392,22 @@ struct Tile {
 #pragma unroll
                 for (int j = 0; j < NI; ++j) acc[i][j] = E::mul(f0.b[j], f0.a[i], acc[i][j]);
             }
-          a.put(next, tid);
-          b.put(next + A::kAll, tid);
+          put_all(next, hold);
+          const Sources s = sources(st + 3);
+#pragma unroll
+          for (int c = 0; c < (BKIND == kBlocks ? A::kMine : kAll); ++c) load(c, s, next, hold);
+        };
+        load_all(0, lds, 0);
+        put_all(lds, 0);
+        const Sources one = sources(1), two = sources(2);
+#pragma unroll
+        for (int c = 0; c < (BKIND == kBlocks ? A::kMine : kAll); ++c) load(c, one, lds, 0), load(c, two, lds, 1);
+        int st = 0;
+        for (; st + 2 <= stages; st += 2) {
+          turn(st, 0);
+          turn(st + 1, 1);
         }
+        if (st < stages) turn(st, 0);
         tile_arrived<0>();
       }
     };
@@ -405,26 +444,43 @@ __device__ __forceinline__ void get4_typed(const void* p, int64_t at, int type, 
   }
 }
 
-// Four values to successive elements of a row of `type`, of which `n` are there.
+// A row's outputs that a lane has of two neighbouring blocks of 16 columns, four of each (Tile::product), to
+// the row from column n0 on, where the first block starts; the row has `cols` columns. 16 bytes a lane: of
+// 16-bit outputs, lanes 16 apart exchange halves, so that the even ones have eight of the first block and the
+// odd ones of the second. Past the caches: gradients of 8 x 4096 x 4096 in f32 from 8192 rows in 326 us, with plain
+// stores in 388, from 512 rows in 130 and 189.
 template <typename To>
-__device__ __forceinline__ void put4(To* p, const float (&v)[4], int n) {
+__device__ __forceinline__ void put_blocks(To* row, int n0, int64_t cols, const float (&v0)[4], const float (&v1)[4],
+                                           bool there) {
+  const int g = threadIdx.x % 64 / 16;
+  if constexpr (sizeof(To) == 4) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      Packed<To, 4> r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.v[e] = (To)(b ? v1[e] : v0[e]);
+      if (there) store_guarded<To, 4>(row, n0 + 16 * b + 4 * g, cols, r);
+    }
+  } else {
+    typedef uint32_t Two __attribute__((ext_vector_type(2)));
+    Packed<To, 4> r0, r1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r0.v[e] = (To)v0[e], r1.v[e] = (To)v1[e];
+    const Two a = __builtin_bit_cast(Two, r0), b = __builtin_bit_cast(Two, r1);
+    const auto low = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto high = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    const u32x4 all{low[0], high[0], low[1], high[1]};
+    if (there)
+      store_guarded<To, 8>(row, n0 + 16 * (g % 2) + 8 * (g / 2), cols, __builtin_bit_cast(Packed<To, 8>, all));
+  }
+}
+// The same of one block.
+template <typename To>
+__device__ __forceinline__ void put4(To* row, int n, int64_t cols, const float (&v)[4], bool there) {
   Packed<To, 4> r;
 #pragma unroll
   for (int e = 0; e < 4; ++e) r.v[e] = (To)v[e];
-  if (n >= 4)
-    *reinterpret_cast<Packed<To, 4>*>(p) = r;
-  else
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (e < n) p[e] = r.v[e];
-}
-__device__ __forceinline__ void put4_typed(void* p, int64_t at, int type, const float (&v)[4], int n) {
-  if (type == 0)
-    put4(static_cast<float*>(p) + at, v, n);
-  else if (type == 1)
-    put4(static_cast<bf16*>(p) + at, v, n);
-  else
-    put4(static_cast<f16*>(p) + at, v, n);
+  if (there) store_guarded<To, 4>(row, n, cols, r);
 }
 __device__ __forceinline__ float get_typed(const void* p, int64_t at, int type) {
   if (type == 0) return static_cast<const float*>(p)[at];

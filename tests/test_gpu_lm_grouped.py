@@ -85,14 +85,14 @@ def test_epilogues(dtype, order, counts, epi):
 def test_kernels(dtype, order):
     t = TYPES[dtype]
     forward([2, 5, 0, 9], 512, 640, t, order, plan="stream")
-    forward([2, 60, 0, 9], 512, 640, t, order, plan="stream+tiles=16")
-    forward([200, 500], 128, 384, t, order, plan="tiles=16")
-    # Rows of whole 4 bytes, and of fewer.
-    forward([200, 500], 130, 382, t, order, plan="tiles=4")
-    forward([200, 500], 129, 381, t, order, plan="tiles=4" if dtype == "f32" else "tiles=any")
+    forward([2, 60, 0, 9], 512, 640, t, order, plan="stream+tiles direct")
+    forward([200, 500], 128, 384, t, order, plan="tiles direct")
+    # Rows off 16 bytes.
+    forward([200, 500], 130, 382, t, order, plan="tiles any")
+    forward([200, 500], 129, 381, t, order, plan="tiles any")
     # Whole rounds of large tiles with halves, with quarters and with none left; quarters alone.
     for counts, N in (([700, 0, 1500, 900], 8192), ([1500, 2000, 700], 4000), ([4096], 4096), ([300, 130], 2048)):
-        forward(counts, 192, N, t, order, epi=_native.EPI_BIAS_RELU, plan="tiles=16")
+        forward(counts, 192, N, t, order, epi=_native.EPI_BIAS_RELU, plan="tiles direct")
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -158,8 +158,8 @@ def test_gradients_of_large_groups(dtype):
     wide = dtype != "f32"
     backward([900, 1100, 0], 4096, 1536, TYPES[dtype], "kn", _native.EPI_BIAS_RELU,
              plan="dW 256x256" if wide else "dW 128x128")
-    backward([150, 90, 0], 130, 258, TYPES[dtype], "kn", _native.EPI_BIAS_RELU, plan="dW loads=4")
-    backward([150, 90, 0], 131, 259, TYPES[dtype], "kn", plan="dW loads=4" if dtype == "f32" else "dW any")
+    backward([150, 90, 0], 130, 258, TYPES[dtype], "kn", _native.EPI_BIAS_RELU, plan="dW any")
+    backward([150, 90, 0], 131, 259, TYPES[dtype], "kn", plan="dW any")
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
