@@ -30,40 +30,41 @@ __global__ void __launch_bounds__(kActThreads) grouped_act_kernel(GroupedActArgs
   if (!tiles.find(part, part ? tile - whole : tile, &t)) return;
   if (col >= a.N) return;
   const int64_t end = min(t.first + kActRows, t.end);
-  const bool inside = (w % tiles_n + 1) * (int64_t)COLS <= a.N;  // uniform: no load waits at a branch then
-  const auto get = [&](const void* p, int64_t ld, int64_t row) {
-    const T* const from = static_cast<const T*>(p) + row * ld;
-    return inside ? load_packed<T, VEC>(from + col) : load_guarded<T, VEC>(from, col, a.N);
-  };
   float sum[VEC] = {};
-  for (int64_t row = t.first; row < end; row += kAhead) {
-    // Rows past the last one are read as it is, and do not count.
-    Packed<T, VEC> dy[kAhead], y[kAhead];
+  const auto rows = [&](auto inside) {
+    const auto get = [&](const void* p, int64_t ld, int64_t row) {
+      const T* const from = static_cast<const T*>(p) + row * ld;
+      if constexpr (decltype(inside)::value) return load_packed<T, VEC>(from + col);
+      return load_guarded<T, VEC>(from, col, a.N);
+    };
+    for (int64_t row = t.first; row < end; row += kAhead) {
+      // Rows past the last one are read as it is, and do not count.
+      Packed<T, VEC> dy[kAhead], y[kAhead];
 #pragma unroll
-    for (int r = 0; r < kAhead; ++r) dy[r] = get(a.dy, a.lddy, min(row + r, end - 1));
-    if (a.y)
+      for (int r = 0; r < kAhead; ++r) dy[r] = get(a.dy, a.lddy, min(row + r, end - 1));
+      if (a.y)
 #pragma unroll
-      for (int r = 0; r < kAhead; ++r) y[r] = get(a.y, a.ldy, min(row + r, end - 1));
+        for (int r = 0; r < kAhead; ++r) y[r] = get(a.y, a.ldy, min(row + r, end - 1));
 #pragma unroll
-    for (int r = 0; r < kAhead; ++r) {
-      if (row + r >= end) break;
-      Packed<T, VEC> dz;
+      for (int r = 0; r < kAhead; ++r) {
+        if (row + r >= end) break;
+        Packed<T, VEC> dz;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = (float)dy[r].v[e];
-        const float v = !a.y || (float)y[r].v[e] > 0.0f ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
-        dz.v[e] = (T)v;
-        sum[e] += v;
+        for (int e = 0; e < VEC; ++e) {
+          const float d = (float)dy[r].v[e];
+          const float v = !a.y || (float)y[r].v[e] > 0.0f ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
+          dz.v[e] = (T)v;
+          sum[e] += v;
+        }
+        if (a.y) store_guarded<T, VEC>(static_cast<T*>(a.dz) + (row + r) * a.lddz, col, a.N, dz);
       }
-      if (!a.y) continue;
-      T* const to = static_cast<T*>(a.dz) + (row + r) * a.lddz;
-      if (col + VEC <= a.N)
-        *reinterpret_cast<Packed<T, VEC>*>(to + col) = dz;
-      else
-        for (int e = 0; e < VEC; ++e)
-          if (col + e < a.N) to[col + e] = dz.v[e];
     }
-  }
+  };
+  // Loads in flight wait at a branch of their own: whole vectors have none.
+  if (col + VEC <= a.N)
+    rows(std::true_type{});
+  else
+    rows(std::false_type{});
   if (!a.db) return;
 #pragma unroll
   for (int e = 0; e < VEC; ++e)
