@@ -176,8 +176,10 @@ struct TileSide {
     if constexpr (KIND == kRows)
       return {buffer_rsrc(o.base + (int64_t)k0 * sizeof(T), ((o.n - 1) * o.ld + K - k0) * (int64_t)sizeof(T)), k0,
               K - k0};
+    // Of a word that is not all inside nothing is read: the last row's end is its last word's.
     if constexpr (KIND == kCols)
-      return {buffer_rsrc(o.base + k0 * o.ld * (int64_t)sizeof(T), ((K - k0 - 1) * o.ld + o.n) * (int64_t)sizeof(T)),
+      return {buffer_rsrc(o.base + k0 * o.ld * (int64_t)sizeof(T),
+                          (((K - k0 - 1) * o.ld + o.n) * (int64_t)sizeof(T) + 3) & ~(int64_t)3),
               k0, K - k0};
     return {buffer_rsrc(o.base + (int64_t)k0 * 16, (int64_t)((o.n + 15) / 16) * o.ld - (int64_t)k0 * 16), k0, K - k0};
   }
