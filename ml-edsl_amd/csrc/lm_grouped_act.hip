@@ -27,6 +27,8 @@ __global__ void __launch_bounds__(kActThreads) grouped_act_kernel(GroupedActArgs
   tiles.total(&whole, &parts);
   const bool part = tile >= whole;
   RowTile t;
+  // Past what the partial sums have room for: the grid's last workgroups, where offsets do not rise.
+  if (tile >= grouped_act_tiles(a.T, a.E)) return;
   if (!tiles.find(part, part ? tile - whole : tile, &t)) return;
   if (col >= a.N) return;
   const int64_t end = min(t.first + kActRows, t.end);

@@ -17,6 +17,8 @@ namespace {
 
 constexpr int64_t kMostI8Depth = (int64_t(1) << 17) - 1;  // K 2^14 < 2^31: 32-bit sums are exact
 constexpr int kMostExperts = 65535;
+// The streaming kernels' columns go along one axis of the grid, 512 threads for 16 of them: under 2^32.
+constexpr int64_t kMostStreamed = int64_t(1) << 26;
 
 // A tile's rows of `ld` elements within the 31 bits of an asynchronous load's offset.
 bool reachable(int64_t rows, int64_t ld, int e) { return rows * ld * e < 0x7fffffff; }
@@ -80,7 +82,8 @@ void i8_dense(lm::I8Args a, int64_t M, int64_t N, int64_t K, void* stream) {
     const int64_t tiles = lm::i8_tiles(N), parts = (M + 63) / 64;
     // Streaming, in parts of up to 64 rows: up to 64 rows, 32 of a wide layer (64 x 4096 x 50256 in 73 us against 55 on
     // tiles), and more where all parts together are two rounds of workgroups (256 x 8192 x 2048 ...).
-    if (M <= (tiles >= 8 * (int64_t)cus ? 32 : 64) || (parts <= 64 && parts * tiles <= 2 * (int64_t)cus)) {
+    if (N <= kMostStreamed &&
+        (M <= (tiles >= 8 * (int64_t)cus ? 32 : 64) || (parts <= 64 && parts * tiles <= 2 * (int64_t)cus))) {
       // Each workgroup reads all of x: more columns a workgroup where there are many (32 x 4096 x 50256 in 49 us on
       // 64 columns, on 16 in 90; 16 rows in 42 and 53), and where one more than a round of 16 each would run (33 x 4096 x
       // 4097 in 10.2 us, in 13.7 on 16), but not where CUs would be idle (32 x 4096 x 4096 in 8.4, on 32 in 9.2).
@@ -135,7 +138,7 @@ hipError_t weights_by_type(const lm::GroupedWeightArgs& a, bool direct, bool big
 // y = epi(x @ w_e + b_e), the launches of one product over rows. `plan`: what ran.
 void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t len) {
   const int e = lm::type_bytes(a.type);
-  const bool streams = a.T < 64 * (int64_t)a.E && (a.turned || a.N >= 4);
+  const bool streams = a.T < 64 * (int64_t)a.E && (a.turned || a.N >= 4) && a.N <= kMostStreamed;
   a.skip = streams ? lm::kGroupedSkinnyRows : 0;
   a.cus = cus;
   if (streams) {
