@@ -24,10 +24,17 @@ struct GroupedLaunch {
   template <int BKIND, bool DIRECT>
   static hipError_t rows_kind(const GroupedArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 4) {
-      // Bound by the matrix cores, which f32 keeps eight times as long: small tiles up to a round of large ones.
-      const int64_t tiles = (a.T / 128 + std::min<int64_t>(a.E, a.T)) * ((a.N + 127) / 128);
-      if (tiles <= a.cus) return rows_tiles<BKIND, Tile<T, kRows, BKIND, 64, 64, 2, 4, DIRECT, DIRECT ? 3 : 2>>(a, 0, 0, stream);
-      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, DIRECT>>(a, 0, 0, stream);
+      // Bound by the matrix cores, which f32 keeps eight times as long, so that small tiles are nearly as good: 32 x 64
+      // where these are one round of the CUs (300 x 512 x 1024 in 11.8 us, on 64 x 64 in 15.9; 100 x 4096 x 4096 in 61 and 86;
+      // 2000 x 1008 x 1008, four rounds, in 53.5 and 50.5), 64 x 64 up to a round of 128 x 128 (2000 x 1008 x 1008 of five
+      // experts in 50.5 us, cut from 128 x 128 in 62), and for what rounds of those leave (2049^3 in 190 us, 288 on 128 x 128 alone).
+      constexpr int kStages = DIRECT ? 3 : 2;
+      using Small = Tile<T, kRows, BKIND, 64, 64, 2, 4, DIRECT, kStages>;
+      const int64_t groups = std::min<int64_t>(a.E, a.T);
+      if ((a.T / 32 + groups) * ((a.N + 63) / 64) <= a.cus)
+        return rows_tiles<BKIND, Tile<T, kRows, BKIND, 32, 64, 1, 4, DIRECT, kStages>>(a, 0, 0, stream);
+      if ((a.T / 128 + groups) * ((a.N + 127) / 128) <= a.cus) return rows_tiles<BKIND, Small>(a, 0, 0, stream);
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, DIRECT>, Small>(a, a.cus, 0, stream);
     } else if constexpr (!DIRECT) {
       return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, false>>(a, 0, 0, stream);
     } else {
