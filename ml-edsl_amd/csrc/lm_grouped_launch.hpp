@@ -24,17 +24,21 @@ struct GroupedLaunch {
   template <int BKIND, bool DIRECT>
   static hipError_t rows_kind(const GroupedArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 4) {
-      // Bound by the matrix cores, which f32 keeps eight times as long, so that small tiles are nearly as good: 32 x 64
-      // where these are one round of the CUs (300 x 512 x 1024 in 11.8 us, on 64 x 64 in 15.9; 100 x 4096 x 4096 in 61 and 86;
-      // 2000 x 1008 x 1008, four rounds, in 53.5 and 50.5), 64 x 64 up to a round of 128 x 128 (2000 x 1008 x 1008 of five
-      // experts in 50.5 us, cut from 128 x 128 in 62), and for what rounds of those leave (2049^3 in 190 us, 288 on 128 x 128 alone).
+      // Bound by the matrix cores, which f32 keeps eight times as long, so that small tiles are nearly as good. Up to
+      // a round of 128 x 128: of 64 x 64 and 32 x 64 the one whose rounds of the CUs take less, one of 32 x 64 0.6 of
+      // the other's (300 x 512 x 1024 in 11.8 and 15.9 us on 32 x 64 and 64 x 64, 700 x 900 x 1500 of three experts in 34 and 40,
+      // 1000 x 1024 x 1024 in 27.6 and 27.0, 2000 x 1008 x 1008 of five in 61 and 57). Beyond it 128 x 128, with 64 x 64 for
+      // what rounds leave (2049^3 in 190 us, 288 on 128 x 128 alone; 2000 x 1008 x 1008 so in 62 against 50 on 64 x 64).
       constexpr int kStages = DIRECT ? 3 : 2;
       using Small = Tile<T, kRows, BKIND, 64, 64, 2, 4, DIRECT, kStages>;
-      const int64_t groups = std::min<int64_t>(a.E, a.T);
-      if ((a.T / 32 + groups) * ((a.N + 63) / 64) <= a.cus)
-        return rows_tiles<BKIND, Tile<T, kRows, BKIND, 32, 64, 1, 4, DIRECT, kStages>>(a, 0, 0, stream);
-      if ((a.T / 128 + groups) * ((a.N + 127) / 128) <= a.cus) return rows_tiles<BKIND, Small>(a, 0, 0, stream);
-      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, DIRECT>, Small>(a, a.cus, 0, stream);
+      const auto tiles = [&](int64_t rows, int64_t cols) {
+        return (a.T / rows + std::min<int64_t>(a.E, a.T)) * ((a.N + cols - 1) / cols);
+      };
+      if (tiles(128, 128) > a.cus)
+        return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, DIRECT>, Small>(a, a.cus, 0, stream);
+      const auto rounds = [&](int64_t rows) { return (tiles(rows, 64) + a.cus - 1) / a.cus; };
+      if (5 * rounds(64) <= 3 * rounds(32)) return rows_tiles<BKIND, Small>(a, 0, 0, stream);
+      return rows_tiles<BKIND, Tile<T, kRows, BKIND, 32, 64, 1, 4, DIRECT, kStages>>(a, 0, 0, stream);
     } else if constexpr (!DIRECT) {
       return rows_tiles<BKIND, Tile<T, kRows, BKIND, 128, 128, 2, 4, false>>(a, 0, 0, stream);
     } else {

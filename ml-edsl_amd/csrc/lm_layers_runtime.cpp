@@ -148,7 +148,7 @@ void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t 
   if (a.T > a.skip) {
     const bool direct = whole16({address(a.x), a.ldx * e, address(a.w), a.ldw * e, a.stride_w * e, a.K * e}) &&
                         reachable(256, a.ldx, e) && reachable(256, a.ldw, e);
-    check_grid(a.T / 64 + a.E, (a.N + 63) / 64 + 16);  // 32 x 64 tiles are one round
+    check_grid(a.T / 64 + a.E, (a.N + 63) / 64 + 16);
     check_hip(rows_by_type(a, direct, s), "grouped_rows launch");
     tiles = direct ? "+tiles direct" : "+tiles any";
   }

@@ -183,7 +183,8 @@ struct TileSide {
               k0, K - k0};
     return {buffer_rsrc(o.base + (int64_t)k0 * 16, (int64_t)((o.n + 15) / 16) * o.ld - (int64_t)k0 * 16), k0, K - k0};
   }
-  // Starts load c of kMine of a stage.
+  // Starts load c of kMine of a stage, which has all its rows and columns where WHOLE.
+  template <bool WHOLE = false>
   __device__ __forceinline__ void load(int c, const Source& s, const TileOperand& o, u32x4* lds, int tid, int wave,
                                        int hold = 0) {
     int row, col;
@@ -197,7 +198,7 @@ struct TileSide {
     } else {
       static_assert(KIND != kBlocks, "blocks are always aligned");
       if constexpr (KIND == kRows) {
-        if (s.left >= kDepth) {  // uniform
+        if (WHOLE || s.left >= kDepth) {  // uniform
           held[hold][c] = __builtin_bit_cast(u32x4, load_packed<T, kChunk>(from[c] + s.k0));
         } else {
           place(c * THREADS + tid, row, col);
@@ -207,7 +208,7 @@ struct TileSide {
         // What depends on a loaded value waits for it: chunks are moved to their places as they are put.
         const T* const p = from[c] + s.k0 * o.ld;
         place(c * THREADS + tid, row, col);
-        if (s.left >= kDepth && o.all >= kChunk) {  // uniform
+        if (WHOLE || (s.left >= kDepth && o.all >= kChunk)) {  // uniform
           held[hold][c] = __builtin_bit_cast(u32x4, load_packed<T, kChunk>(p));
         } else {
           held[hold][c] = u32x4{0, 0, 0, 0};
@@ -315,16 +316,17 @@ struct Tile {
     const auto sources = [&](int st) {
       return Sources{A::source(oa, K, st * A::kDepth), B::source(ob, K, st * A::kDepth)};
     };
-    const auto load = [&](int c, const Sources& s, u32x4* to, int hold) {
+    const auto load = [&](int c, const Sources& s, u32x4* to, int hold, auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
       if (c < A::kMine)
-        a.load(c, s.a, oa, to, tid, wave, hold);
+        a.template load<kWhole>(c, s.a, oa, to, tid, wave, hold);
       else
-        b.load(c - A::kMine, s.b, ob, to + A::kAll, tid, wave, hold);
+        b.template load<kWhole>(c - A::kMine, s.b, ob, to + A::kAll, tid, wave, hold);
     };
-    const auto load_all = [&](int st, u32x4* to, int hold) {
+    const auto load_all = [&](int st, u32x4* to, int hold, auto whole) {
       const Sources s = sources(st);
 #pragma unroll
-      for (int c = 0; c < kAll; ++c) load(c, s, to, hold);
+      for (int c = 0; c < kAll; ++c) load(c, s, to, hold, whole);
     };
     const auto put_all = [&](u32x4* to, int hold) {
       a.put(oa, to, tid, hold);
@@ -335,7 +337,7 @@ struct Tile {
       Fragments f0, f1;
       if constexpr (DIRECT) {
 #pragma unroll
-        for (int st = 0; st < NS; ++st) load_all(st, lds + st * kStage, 0);
+        for (int st = 0; st < NS; ++st) load_all(st, lds + st * kStage, 0, std::false_type{});
         tile_arrived<(NS - 1) * kLoads>();
         if constexpr (kWorks) read(lds, 0, f0);
         int at = 0;
@@ -360,7 +362,7 @@ struct Tile {
 #pragma unroll
           for (int c = 0; c < kAll; ++c) {
             __builtin_amdgcn_sched_barrier(0);
-            load(c, s, now, 0);
+            load(c, s, now, 0, std::false_type{});
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (kWorks)
 #pragma unroll
@@ -372,8 +374,9 @@ struct Tile {
         tile_arrived<0>();  // nothing is on its way to LDS when the workgroup ends
       } else {
         static_assert(DIRECT || NS == 2, "a stage at a time goes through registers");
+        constexpr int kHeld = BKIND == kBlocks ? A::kMine : kAll;
         // One stage in LDS, two on their way in registers. Blocks of weights go straight to LDS, a stage ahead.
-        const auto turn = [&](int st, int hold) {
+        const auto turn = [&](int st, int hold, auto whole) {
           u32x4* const now = lds + st % 2 * kStage;
           u32x4* const next = lds + (st + 1) % 2 * kStage;
           if constexpr (BKIND == kBlocks)
@@ -397,19 +400,37 @@ struct Tile {
           put_all(next, hold);
           const Sources s = sources(st + 3);
 #pragma unroll
-          for (int c = 0; c < (BKIND == kBlocks ? A::kMine : kAll); ++c) load(c, s, next, hold);
+          for (int c = 0; c < kHeld; ++c) load(c, s, next, hold, whole);
         };
-        load_all(0, lds, 0);
-        put_all(lds, 0);
-        const Sources one = sources(1), two = sources(2);
+        const auto start = [&](auto whole) {
+          load_all(0, lds, 0, whole);
+          put_all(lds, 0);
+          const Sources one = sources(1), two = sources(2);
 #pragma unroll
-        for (int c = 0; c < (BKIND == kBlocks ? A::kMine : kAll); ++c) load(c, one, lds, 0), load(c, two, lds, 1);
+          for (int c = 0; c < kHeld; ++c) load(c, one, lds, 0, whole);
+#pragma unroll
+          for (int c = 0; c < kHeld; ++c) load(c, two, lds, 1, whole);
+        };
+        // Turns that start loads of whole stages have no branch between their loads: where paths of more and of
+        // fewer loads meet, the compiler waits for all.
+        const int even = ((AKIND == kRows || oa.all >= A::kChunk) && (BKIND != kCols || ob.all >= A::kChunk)
+                              ? K / A::kDepth - 3 : 0) / 2 * 2;
         int st = 0;
-        for (; st + 2 <= stages; st += 2) {
-          turn(st, 0);
-          turn(st + 1, 1);
+        if (even > 0) {
+          start(std::true_type{});
+          for (; st < even; st += 2) {
+            turn(st, 0, std::true_type{});
+            turn(st + 1, 1, std::true_type{});
+          }
+        } else {
+          start(std::false_type{});
         }
-        if (st < stages) turn(st, 0);
+#pragma unroll 1
+        for (; st + 2 <= stages; st += 2) {
+          turn(st, 0, std::false_type{});
+          turn(st + 1, 1, std::false_type{});
+        }
+        if (st < stages) turn(st, 0, std::false_type{});
         tile_arrived<0>();
       }
     };
