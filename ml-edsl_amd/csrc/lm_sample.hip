@@ -19,7 +19,8 @@
 // keys' digits where they are many). As soon as a bound of the kept logits is known, those above
 // it are candidates in LDS and the row is read no more: for top-k that is the k-th largest of the
 // threads' maxima, for min-p alone its weight, for top-p its border's bin. More than
-// 4096 candidates are read from the row, in the caches, each time.
+// 12288 candidates are read from the row, in the caches, each time: 0.9 of the mass of 50256 normal logits of
+// deviation 2.5, some 6000 of them, in 52.6 us for 256 rows, with room for 4096 in 63.5.
 #include <algorithm>
 
 #include "lm_common.hpp"
@@ -39,7 +40,8 @@ constexpr int kBins = 2048;
 constexpr int kMostRow = 1 << 21;
 constexpr float kRange = 48.0f;  // octaves below the maximum that the bins cover: past 47 a weight is 0
 constexpr int kList = 1024;      // logits of a border's bin that are ranked
-constexpr int kKept = 4096;      // candidates that are kept apart from the row
+// Candidates that are kept apart from the row; the registers leave room for one workgroup a CU in any case.
+constexpr int kKept = 12288;
 constexpr int kFew = 256;        // of those, so many are ranked against each other
 
 // v or 0, without a branch: the compiler would put all that v takes into it, one element after the other.
