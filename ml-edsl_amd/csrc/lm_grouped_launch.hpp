@@ -61,13 +61,13 @@ struct GroupedLaunch {
   }
   static hipError_t skinny(const GroupedArgs& a, hipStream_t stream) {
     // Workgroups of 16 columns of the experts that may have rows, and of more columns where these are many:
-    // 2 rows of 8 experts of 4096 x 4096 bf16 in 8.3 us on 16 columns, on 32 in 13.8; 96 rows of 64 of 2048 x 1024 in 57.7 on
-    // 16, 49.4 on 32; 600 rows of 24 of 2048 x 2048, 25 rows each, in 88, 55 and 49.5 on 16, 32 and 64.
+    // 2 rows of 8 experts of 4096 x 4096 bf16 in 8.3 us on 16 columns, on 32 in 13.8; 96 rows at 64 of 2048 x 1024 in 57.7 on
+    // 16, 52 on 32 and 54 on 64; 200 there in 64 on 32 and 57 on 64, 16 at 8 of 4096 x 4096 in 57 and 50.
     const int64_t groups = (a.N + 15) / 16 * std::min<int64_t>(a.E, a.T);
     const bool many = groups > 2 * (int64_t)a.cus;
     if (a.turned) {
       if (!many) return skinny_cols<kRows, 1, 2, 2>(a, stream);
-      return a.T > 8 * (int64_t)a.E ? skinny_cols<kRows, 4, 2, 1>(a, stream) : skinny_cols<kRows, 2, 2, 2>(a, stream);
+      return 2 * a.T > 3 * (int64_t)a.E ? skinny_cols<kRows, 4, 2, 1>(a, stream) : skinny_cols<kRows, 2, 2, 2>(a, stream);
     }
     // Columns contiguous: 64, with 8 bytes a lane and row; 128 of 16 bits where these are many (96 rows of 64 experts in
     // 46.5 us against 49; 2 rows of 8 in 15.7 against 12.1).

@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(64 * WAVES) i8_skinny_kernel(I8Args a) {
   // Few operands a block are read further ahead: 33 x 4096 x 4097 in 10.2 us with two blocks of weights on
   // their way, with one in 11.8; 1 x 8192 x 8192 in 11.3 with one of four steps, in 11.9 with two.
   constexpr int U = MT * NJ == 1 ? 4 : MT * NJ <= 8 && MT < 4 ? 2 : 1;
-  constexpr int AHEAD = MT * NJ == 1 || NJ == 4 && MT <= 2 || NJ == 1 && MT > 2 ? 1 : 2;
+  constexpr int AHEAD = MT * NJ == 1 || NJ == 4 || (NJ == 1 && MT > 2) ? 1 : 2;
   using S = Skinny<int8_t, kBlocks, MT, NJ, WAVES, U, AHEAD>;
   __shared__ typename S::Acc lds[S::kSlots];
   const int m0 = (int)blockIdx.y * 16 * MT;
@@ -153,6 +153,7 @@ hipError_t launch_tiles(I8Args a, int quarters, int halves, hipStream_t stream) 
   return launched();
 }
 
+// 64 columns: of up to 32 rows.
 template <int MT>
 hipError_t launch_skinny(const I8Args& a, int cols16, hipStream_t stream) {
   constexpr int kWaves = 8;
@@ -161,7 +162,7 @@ hipError_t launch_skinny(const I8Args& a, int cols16, hipStream_t stream) {
     hipLaunchKernelGGL((i8_skinny_kernel<MT, 1, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
   else if (cols16 == 2)
     hipLaunchKernelGGL((i8_skinny_kernel<MT, 2, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
-  else
+  else if constexpr (MT <= 2)
     hipLaunchKernelGGL((i8_skinny_kernel<MT, 4, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
   return launched();
 }

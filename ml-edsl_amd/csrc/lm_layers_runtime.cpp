@@ -80,14 +80,14 @@ void i8_dense(lm::I8Args a, int64_t M, int64_t N, int64_t K, void* stream) {
   device_launch(0, stream, [&](char*, int cus) {
     const hipStream_t s = as_stream(stream);
     const int64_t tiles = lm::i8_tiles(N), parts = (M + 63) / 64;
-    // Streaming, in parts of up to 64 rows: up to 64 rows, 32 of a wide layer (64 x 4096 x 50256 in 73 us against 55 on
-    // tiles), and more where all parts together are two rounds of workgroups (256 x 8192 x 2048 ...).
-    if (N <= kMostStreamed &&
-        (M <= (tiles >= 8 * (int64_t)cus ? 32 : 64) || (parts <= 64 && parts * tiles <= 2 * (int64_t)cus))) {
-      // Each workgroup reads all of x: more columns a workgroup where there are many (32 x 4096 x 50256 in 49 us on
-      // 64 columns, on 16 in 90; 16 rows in 42 and 53), and where one more than a round of 16 each would run (33 x 4096 x
-      // 4097 in 10.2 us, in 13.7 on 16), but not where CUs would be idle (32 x 4096 x 4096 in 8.4, on 32 in 9.2).
-      const int cols = tiles >= 8 * (int64_t)cus ? 4 : tiles > (M <= 16 ? 2 : 1) * (int64_t)cus ? 2 : 1;
+    // Streaming, in parts of up to 64 rows: up to 64 rows (33 x 4096 x 4097 in 11.5 us against 16.7 on tiles), 32 of a layer
+    // of more columns than two rounds (64 x 4096 x 16000 in 26 against 17.7; 32 x 4096 x 50256 in 40 against 44), and
+    // more rows where all parts together are one round (128 x 8192 x 2048 in 23 against 32; two, 256 rows, in 39 against 32).
+    if (N <= kMostStreamed && (M <= (tiles > 2 * (int64_t)cus ? 32 : 64) || (parts <= 64 && parts * tiles <= cus))) {
+      // Each workgroup reads all of x: more columns a workgroup where there are many (32 x 4096 x 30000 in 22.8 us on
+      // 64 columns, on 32 in 32.4; 1 x 4096 x 30000 in 19.5 and 19.3), and where one more than a round of 16 each would run
+      // (33 x 4096 x 4097 in 10.2 us, in 13.7 on 16), but not where CUs would be idle (32 x 4096 x 4096 in 8.4, on 32 in 9.2).
+      const int cols = tiles > 4 * (int64_t)cus ? 4 : tiles > (M <= 16 ? 2 : 1) * (int64_t)cus ? 2 : 1;
       const int rows = (int)(((M + parts - 1) / parts + 15) / 16);
       check_hip(lm::launch_i8_skinny(a, rows, cols, s), "i8_skinny launch");
       set_plan("i8_skinny rows=%d cols=%d", 16 * rows, 16 * cols);
@@ -138,7 +138,11 @@ hipError_t weights_by_type(const lm::GroupedWeightArgs& a, bool direct, bool big
 // y = epi(x @ w_e + b_e), the launches of one product over rows. `plan`: what ran.
 void rows_product(lm::GroupedArgs a, int cus, hipStream_t s, char* plan, size_t len) {
   const int e = lm::type_bytes(a.type);
-  const bool streams = a.T < 64 * (int64_t)a.E && (a.turned || a.N >= 4) && a.N <= kMostStreamed;
+  // Streaming, where no group has more rows than that takes (32 x 4096 x 4096 bf16 in 19 us, on tiles in 32) or most
+  // have few (200 rows at 64 of 2048 x 1024 in 56 to 62 us against 59 to 72; 400 rows in 59 to 67 against 60 to 74; 300 at 16 of
+  // 2048 x 2048 in 39 against 32 to 38, since groups on both sides of the limit take two launches).
+  const bool streams = (a.T <= lm::kGroupedSkinnyRows || a.T < 16 * (int64_t)a.E) && (a.turned || a.N >= 4) &&
+                       a.N <= kMostStreamed;
   a.skip = streams ? lm::kGroupedSkinnyRows : 0;
   a.cus = cus;
   if (streams) {

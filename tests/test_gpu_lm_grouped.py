@@ -85,7 +85,8 @@ def test_epilogues(dtype, order, counts, epi):
 def test_kernels(dtype, order):
     t = TYPES[dtype]
     forward([2, 5, 0, 9], 512, 640, t, order, plan="stream")
-    forward([2, 60, 0, 9], 512, 640, t, order, plan="stream+tiles direct")
+    forward([2, 40, 0, 9], 512, 640, t, order, plan="stream+tiles direct")
+    forward([2, 60, 0, 9], 512, 640, t, order, plan=" +tiles direct")
     forward([200, 500], 128, 384, t, order, plan="tiles direct")
     # Rows off 16 bytes.
     forward([200, 500], 130, 382, t, order, plan="tiles any")

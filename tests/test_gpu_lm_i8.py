@@ -60,7 +60,8 @@ def test_types_and_epilogues(M, N, y, epi):
 
 
 @pytest.mark.parametrize("M,K,N,plan", [
-    (1, 4096, 20000, "skinny rows=16 cols=32"), (5, 64, 40000, "skinny rows=16 cols=64"), (64, 512, 700, "skinny rows=64 cols=16"),
+    (1, 4096, 12000, "skinny rows=16 cols=32"), (1, 4096, 20000, "skinny rows=16 cols=64"), (40, 64, 9000, "direct"),
+    (5, 64, 40000, "skinny rows=16 cols=64"), (64, 512, 700, "skinny rows=64 cols=16"),
     (33, 200, 6000, "skinny rows=48 cols=32"), (300, 512, 700, "skinny rows=64 cols=16"), (130, 8192, 300, "skinny rows=48"),
     (70, 63, 17, "skinny rows=48"), (2100, 384, 8200, "direct"), (4200, 192, 4000, "direct"), (600, 512, 8192, "direct"),
     (4096, 128, 4096, "direct"), (700, 512, 1500, "direct"), (701, 500, 1501, "any"), (65, 640, 40000, "direct"),
