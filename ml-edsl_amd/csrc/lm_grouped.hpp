@@ -128,15 +128,15 @@ __device__ __forceinline__ void grouped_rows_tile(const GroupedArgs& a, const Ro
         if (n + 16 * b < a.N) get4_typed(a.bias, t.expert * a.ldbias + n + 16 * b, a.type, bias[b], (int)a.N - n - 16 * b);
 #pragma unroll
     for (int i = 0; i < Tl::MI; ++i) {
-      const int64_t row = t.first + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
+      const int64_t row = t.first + 16 * (wave / Tl::WN * Tl::MI + i);
       T* const to = static_cast<T*>(a.y) + row * a.ldy;
       float v0[4], v1[4];
       finish(v0, acc[i][j], bias[0]);
       if constexpr (Tl::NI > 1) {
         finish(v1, acc[i][j + 1], bias[1]);
-        put_blocks(to, first, a.N, v0, v1, row < t.end);
+        put_blocks(to, a.ldy, t.end - row, first, a.N, v0, v1);
       } else {
-        put4(to, n, a.N, v0, row < t.end);
+        put4(to + lane % 16 * a.ldy, n, a.N, v0, row + lane % 16 < t.end);
       }
     }
   }
@@ -225,10 +225,10 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesPerSimd) grouped_weigh
   const TileOperand ob{static_cast<const char*>(a.b) + (first * a.ldb + n0) * (int64_t)sizeof(T), a.ldb, (int)(a.N - n0), a.N};
   typename Tl::Acc acc[Tl::MI][Tl::NI];
   Tl::product(oa, ob, (int)rows, lds, acc);
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int wave = threadIdx.x / 64;
 #pragma unroll
   for (int i = 0; i < Tl::MI; ++i) {
-    const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
+    const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i);
     const int64_t at = expert * a.stride_dw + m * a.lddw;
 #pragma unroll
     for (int j = 0; j < Tl::NI; j += 2) {
@@ -236,9 +236,9 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesPerSimd) grouped_weigh
       const float v0[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
       const float v1[4] = {acc[i][j + 1][0], acc[i][j + 1][1], acc[i][j + 1][2], acc[i][j + 1][3]};
       if (a.dw_type == kF32)
-        put_blocks(static_cast<float*>(a.dw) + at, first, a.N, v0, v1, m < a.M);
+        put_blocks(static_cast<float*>(a.dw) + at, a.lddw, a.M - m, first, a.N, v0, v1);
       else
-        put_blocks(static_cast<T*>(a.dw) + at, first, a.N, v0, v1, m < a.M);
+        put_blocks(static_cast<T*>(a.dw) + at, a.lddw, a.M - m, first, a.N, v0, v1);
     }
   }
 }

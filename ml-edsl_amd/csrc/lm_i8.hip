@@ -90,16 +90,16 @@ __device__ __forceinline__ void i8_tile(const I8Args& a, int m0, int n0, u32x4* 
       }
 #pragma unroll
     for (int i = 0; i < Tl::MI; ++i) {
-      const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i) + lane % 16;
+      const int m = m0 + 16 * (wave / Tl::WN * Tl::MI + i);
       float v0[4], v1[4];
       finish(v0, acc[i][j], ws[0], xs[i], bias[0]);
       finish(v1, acc[i][j + 1], ws[1], xs[i], bias[1]);
       if (a.y_type == kF32)
-        put_blocks(static_cast<float*>(a.y) + m * a.ldy, first, a.N, v0, v1, m < a.M);
+        put_blocks(static_cast<float*>(a.y) + m * a.ldy, a.ldy, a.M - m, first, a.N, v0, v1);
       else if (a.y_type == kBf16)
-        put_blocks(static_cast<bf16*>(a.y) + m * a.ldy, first, a.N, v0, v1, m < a.M);
+        put_blocks(static_cast<bf16*>(a.y) + m * a.ldy, a.ldy, a.M - m, first, a.N, v0, v1);
       else
-        put_blocks(static_cast<f16*>(a.y) + m * a.ldy, first, a.N, v0, v1, m < a.M);
+        put_blocks(static_cast<f16*>(a.y) + m * a.ldy, a.ldy, a.M - m, first, a.N, v0, v1);
     }
   }
 }

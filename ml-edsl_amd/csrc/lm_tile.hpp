@@ -469,23 +469,28 @@ __device__ __forceinline__ void get4_typed(const void* p, int64_t at, int type, 
   }
 }
 
-// A row's outputs that a lane has of two neighbouring blocks of 16 columns, four of each (Tile::product), to
-// the row from column n0 on, where the first block starts; the row has `cols` columns. 16 bytes a lane: of
-// 16-bit outputs, lanes 16 apart exchange halves, so that the even ones have eight of the first block and the
-// odd ones of the second. Past the caches: gradients of 8 x 4096 x 4096 in f32 from 8192 rows in 326 us, with plain
-// stores in 388, from 512 rows in 130 and 189.
+// What a wave has of 16 rows and of two neighbouring blocks of 16 columns, a lane four of each of its row
+// (Tile::product), to the rows from `first` on, `ld` apart, of which `rows` are there, and from column n0 on of `cols`. 16 bytes a
+// lane: of 16-bit outputs, lanes 16 apart exchange halves, so that the even ones have eight of the first block and the
+// odd ones of the second; of 32-bit ones, lanes eight rows apart exchange a block, so that a store has 128 bytes of each of
+// eight rows (gradients of 8 x 4096 x 4096 in f32 from 8192 rows in 354 us, in pieces of 64 bytes in 374). Past the
+// caches: these in 326 us and with plain stores in 388, from 512 rows in 130 and 189.
 template <typename To>
-__device__ __forceinline__ void put_blocks(To* row, int n0, int64_t cols, const float (&v0)[4], const float (&v1)[4],
-                                           bool there) {
-  const int g = threadIdx.x % 64 / 16;
+__device__ __forceinline__ void put_blocks(To* first, int64_t ld, int64_t rows, int n0, int64_t cols, const float (&v0)[4],
+                                           const float (&v1)[4]) {
+  const int lane = threadIdx.x % 64, g = lane / 16;
   if constexpr (sizeof(To) == 4) {
+    const bool upper = lane & 8;
+    Packed<float, 4> low, high;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      Packed<To, 4> r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r.v[e] = (To)(b ? v1[e] : v0[e]);
-      if (there) store_guarded<To, 4>(row, n0 + 16 * b + 4 * g, cols, r);
+    for (int e = 0; e < 4; ++e) {
+      const float got = dpp<0x128>(upper ? v0[e] : v1[e]);  // the other's, of a row's 16 lanes eight on
+      low.v[e] = upper ? got : v0[e];
+      high.v[e] = upper ? v1[e] : got;
     }
+    const int row = lane % 8, n = n0 + (upper ? 16 : 0) + 4 * g;
+    if (row < rows) store_guarded<float, 4>(first + row * ld, n, cols, low);
+    if (row + 8 < rows) store_guarded<float, 4>(first + (row + 8) * ld, n, cols, high);
   } else {
     typedef uint32_t Two __attribute__((ext_vector_type(2)));
     Packed<To, 4> r0, r1;
@@ -495,11 +500,12 @@ __device__ __forceinline__ void put_blocks(To* row, int n0, int64_t cols, const 
     const auto low = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
     const auto high = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
     const u32x4 all{low[0], high[0], low[1], high[1]};
-    if (there)
-      store_guarded<To, 8>(row, n0 + 16 * (g % 2) + 8 * (g / 2), cols, __builtin_bit_cast(Packed<To, 8>, all));
+    const int row = lane % 16;
+    if (row < rows)
+      store_guarded<To, 8>(first + row * ld, n0 + 16 * (g % 2) + 8 * (g / 2), cols, __builtin_bit_cast(Packed<To, 8>, all));
   }
 }
-// The same of one block.
+// A row's outputs of one block, four a lane.
 template <typename To>
 __device__ __forceinline__ void put4(To* row, int n, int64_t cols, const float (&v)[4], bool there) {
   Packed<To, 4> r;
