@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(64 * WAVES) grouped_skinny_kernel(GroupedArgs 
     S2::run(x, a.ldx, rows, w, a.ldw, (int)a.K, (int)a.N, n0, lds, store);
 }
 
-// dW: an expert's tile of [M][N], its rows the depth. Experts without rows get zeros.
-template <typename Tl>
+// dW: an expert's tile of [M][N], its rows the depth. Experts without rows get zeros. MORE: of two products.
+template <typename Tl, bool MORE>
 __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesPerSimd) grouped_weights_kernel(GroupedWeightArgs a) {
   using T = typename Tl::T;
   __shared__ u32x4 lds[Tl::kLds];
@@ -221,10 +221,23 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesPerSimd) grouped_weigh
   const int m0 = tm * Tl::BM, n0 = tn * Tl::BN;
   const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
   const int64_t first = g.at(expert), rows = max(g.at(expert + 1) - first, (int64_t)0);
-  const TileOperand oa{static_cast<const char*>(a.a) + (first * a.lda + m0) * (int64_t)sizeof(T), a.lda, (int)(a.M - m0), a.M};
-  const TileOperand ob{static_cast<const char*>(a.b) + (first * a.ldb + n0) * (int64_t)sizeof(T), a.ldb, (int)(a.N - n0), a.N};
   typename Tl::Acc acc[Tl::MI][Tl::NI];
-  Tl::product(oa, ob, (int)rows, lds, acc);
+#pragma unroll
+  for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < Tl::NI; ++j) acc[i][j] = typename Tl::Acc{};
+  const auto operand = [&](const void* p, int64_t ld, int at, int64_t all) {
+    return TileOperand{static_cast<const char*>(p) + (first * ld + at) * (int64_t)sizeof(T), ld, (int)(all - at), all};
+  };
+  if constexpr (MORE) {
+    Tl::add_product(operand(a.more_is_a ? a.more : a.a, a.lda, m0, a.M), operand(a.more_is_a ? a.b : a.more, a.ldb, n0, a.N),
+                    (int)rows, lds, acc);
+#pragma unroll
+    for (int i = 0; i < Tl::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < Tl::NI; ++j) acc[i][j] *= a.scale;
+  }
+  Tl::add_product(operand(a.a, a.lda, m0, a.M), operand(a.b, a.ldb, n0, a.N), (int)rows, lds, acc);
   const int wave = threadIdx.x / 64;
 #pragma unroll
   for (int i = 0; i < Tl::MI; ++i) {

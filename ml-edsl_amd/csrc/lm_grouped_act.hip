@@ -2,7 +2,9 @@
 // bias's gradient: dz = dy (y > 0), or dy times the slope elsewhere, and
 //   db_e = sum over e's rows of dz.
 // Bound by memory: 8192 x 4096 bf16 with both in 42 us (201 MB at 4.8 TB/s), sums alone in 22.
-// dz is rounded to its type, the matrix instructions' operand; db sums it before that, in 32 bits. Rows are
+// dz is rounded to its type, the matrix instructions' operand, for results of that type; db sums it before that, in
+// 32 bits, and dW in f32 through a slope takes dy's two parts as they are, the lower one's product scaled (a 16-bit
+// dy times a slope of 0.01 would be 2^-9 or 2^-12 of it off). Rows are
 // summed in tiles of 32 whose sums a second launch adds in their order (8 of those 42 us), so that the same call
 // gives the same bits. A thread has its own 8 or 4 columns and eight rows on their way; with a wave's threads
 // along the rows, joined through LDS, the same took 92 us.
@@ -53,15 +55,22 @@ __global__ void __launch_bounds__(kActThreads) grouped_act_kernel(GroupedActArgs
 #pragma unroll
       for (int r = 0; r < kAhead; ++r) {
         if (row + r >= end) break;
-        Packed<T, VEC> dz;
+        Packed<T, VEC> dz, up, down;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const float d = (float)dy[r].v[e];
-          const float v = !a.y || (float)y[r].v[e] > 0.0f ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
+          const bool is_up = !a.y || (float)y[r].v[e] > 0.0f;
+          const float v = is_up ? d : a.slope == 0.0f ? 0.0f : d * a.slope;
           dz.v[e] = (T)v;
+          up.v[e] = is_up ? dy[r].v[e] : (T)0.0f;
+          down.v[e] = is_up ? (T)0.0f : dy[r].v[e];
           sum[e] += v;
         }
-        if (a.y) store_guarded<T, VEC>(static_cast<T*>(a.dz) + (row + r) * a.lddz, col, a.N, dz);
+        const auto put = [&](void* to, const Packed<T, VEC>& v) {
+          store_guarded<T, VEC>(static_cast<T*>(to) + (row + r) * a.lddz, col, a.N, v);
+        };
+        if (a.dz) put(a.dz, dz);
+        if (a.up) put(a.up, up), put(a.down, down);
       }
     }
   };

@@ -82,7 +82,12 @@ struct GroupedLaunch {
   template <typename Tl>
   static hipError_t weights_tile(const GroupedWeightArgs& a, hipStream_t stream) {
     const int64_t tiles = ((a.M + Tl::BM - 1) / Tl::BM) * ((a.N + Tl::BN - 1) / Tl::BN) * a.E;
-    hipLaunchKernelGGL((grouped_weights_kernel<Tl>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
+    if constexpr (sizeof(T) == 2 && Tl::BM == 128)
+      if (a.more) {
+        hipLaunchKernelGGL((grouped_weights_kernel<Tl, true>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
+        return launched();
+      }
+    hipLaunchKernelGGL((grouped_weights_kernel<Tl, false>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
     return launched();
   }
   static hipError_t weights(const GroupedWeightArgs& a, bool direct, bool big, hipStream_t stream) {

@@ -130,10 +130,13 @@ template <int TYPE>
 hipError_t launch_grouped_skinny(const GroupedArgs& a, hipStream_t stream);
 
 struct GroupedWeightArgs {
-  const void* a;  // dw[e] = a[e's rows]^T b[e's rows]
+  const void* a;  // dw[e] = a[e's rows]^T b[e's rows], plus `scale` times that of `more`, in b's place
   const void* b;
+  const void* more;  // or nullptr
   const void* offsets;
   void* dw;
+  float scale;
+  bool more_is_a;  // in a's place
   int64_t lda, ldb, lddw, stride_dw, T, M, N;
   int E, type, dw_type;
   bool ids64;
@@ -145,7 +148,9 @@ hipError_t launch_grouped_weights(const GroupedWeightArgs& a, bool direct, bool 
 struct GroupedActArgs {
   const void* dy;
   const void* y;   // or nullptr: no activation
-  void* dz;        // with y
+  void* dz;        // or nullptr
+  void* up;        // dy where y > 0, else 0, or nullptr
+  void* down;      // with it: dy elsewhere
   float* partials; // [tiles][N], where the sums are wanted
   void* db;        // [E][N], rows of lddb, or nullptr
   const void* offsets;

@@ -223,16 +223,21 @@ void grouped_backward(Backward a, void* stream) {
   const int e = lm::type_bytes(a.type), chunk = 16 / e;
   const bool masks = act != 0 && a.T > 0 && a.N > 0;
   const int64_t lddz = (a.N + chunk - 1) / chunk * chunk;
-  const size_t dz_bytes = masks ? aligned((size_t)a.T * lddz * e) : 0;
+  // dW in f32 through a slope: of dy's two parts, unrounded.
+  const bool split = masks && act == 2 && a.dw && a.type != lm::kF32 && a.dw_type == lm::kF32;
+  const bool whole = masks && ((a.dx && a.K > 0) || (a.dw && !split));
+  const size_t one = masks ? aligned((size_t)a.T * lddz * e) : 0, dz_bytes = one * ((whole ? 1 : 0) + (split ? 2 : 0));
   const size_t sums = a.db ? (size_t)lm::grouped_act_tiles(a.T, (int)a.E) * a.N * sizeof(float) : 0;
   if (masks || a.db) check_grid(a.T / lm::kGroupedActRows + a.E, a.N / 256 + 1);
   device_launch(dz_bytes + sums, stream, [&](char* ws, int cus) {
     const hipStream_t s = as_stream(stream);
-    const void* dz = a.dy;
+    const void *dz = a.dy, *up = nullptr, *down = nullptr;
     int64_t ldz = a.lddy;
     if (masks || a.db) {
       lm::GroupedActArgs g{};
-      g.dy = a.dy, g.y = masks ? a.y : nullptr, g.dz = ws;
+      g.dy = a.dy, g.y = masks ? a.y : nullptr, g.dz = whole ? ws : nullptr;
+      g.up = split ? ws + (whole ? one : 0) : nullptr, g.down = split ? static_cast<char*>(g.up) + one : nullptr;
+      up = g.up, down = g.down;
       g.partials = reinterpret_cast<float*>(ws + dz_bytes), g.db = a.db, g.offsets = a.offsets;
       g.lddy = a.lddy, g.ldy = a.ldy, g.lddz = lddz, g.lddb = a.lddb, g.T = a.T, g.N = a.N;
       g.slope = act == 2 ? a.alpha : 0.0f;
@@ -251,7 +256,8 @@ void grouped_backward(Backward a, void* stream) {
     const char* tiles = "";
     if (a.dw && a.K > 0) {
       lm::GroupedWeightArgs g{};
-      g.a = a.x, g.lda = a.ldx, g.b = dz, g.ldb = ldz, g.M = a.K, g.N = a.N;
+      g.a = a.x, g.lda = a.ldx, g.b = split ? up : dz, g.ldb = ldz, g.M = a.K, g.N = a.N;
+      g.more = down, g.scale = a.alpha, g.more_is_a = a.dw_turned;
       if (a.dw_turned) std::swap(g.a, g.b), std::swap(g.lda, g.ldb), std::swap(g.M, g.N);
       g.offsets = a.offsets, g.dw = a.dw, g.lddw = a.lddw, g.stride_dw = a.stride_dw, g.T = a.T;
       g.E = (int)a.E, g.type = a.type, g.dw_type = a.dw_type, g.ids64 = a.ids64;
@@ -260,8 +266,8 @@ void grouped_backward(Backward a, void* stream) {
       const int64_t tiles256 = ((g.M + 255) / 256) * ((g.N + 255) / 256) * a.E;
       // 256 x 256 where they fill the CUs and are deep enough: 8192 rows at 8 bf16 experts of 4096 x 4096 in 283 us, 128 x 128
       // in 333; 2048 rows in 122 and 127, 1024 in 102 and 98. f32 results, twice the bytes, 8192 rows: 379 and 435, 4096: 243
-      // and 237, 2048: 200 and 178.
-      const bool big = direct && a.type != lm::kF32 && tiles256 >= cus &&
+      // and 237, 2048: 200 and 178. Two products spill there: the whole way back through a slope in 1041 and 986, 622 without one.
+      const bool big = !split && direct && a.type != lm::kF32 && tiles256 >= cus &&
                        a.T >= (a.dw_type == lm::kF32 ? 768 : 256) * a.E;
       check_grid((g.M + 127) / 128 * a.E, (g.N + 127) / 128);
       check_hip(weights_by_type(g, direct, big, s), "grouped_weights launch");

@@ -287,12 +287,16 @@ struct Tile {
   // acc[i][j][e]: row 16 (wave's MI + i) + lane % 16, column 16 (wave's NI + j) + 4 (lane / 16) + e.
   static __device__ __forceinline__ void product(const TileOperand& oa, const TileOperand& ob, int K, u32x4* lds,
                                                  Acc (&acc)[MI][NI]) {
-    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int wm = wave / WN, wn = wave % WN;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = Acc{};
+    add_product(oa, ob, K, lds, acc);
+  }
+  static __device__ __forceinline__ void add_product(const TileOperand& oa, const TileOperand& ob, int K, u32x4* lds,
+                                                     Acc (&acc)[MI][NI]) {
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = wave / WN, wn = wave % WN;
     const int stages = (K + A::kDepth - 1) / A::kDepth;
     if (stages == 0) return;
     A a;
