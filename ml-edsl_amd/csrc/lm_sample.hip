@@ -11,7 +11,7 @@
 // A token next to a border changes with the last bits of a sum, so masses are
 // integers: w_i 2^s to nearest, s = 46 for up to 2^16 logits and one less for each
 // doubling, from a 64-bit exponential. Their sums are exact in 64 bits, whatever the order,
-// so that atomics give the same bits each time. A weight below 2^-47 of the largest is 0.
+// so that atomics give the same bits each time. A weight below half a unit, 2^-(s+1) of the largest, is 0.
 //
 // One workgroup takes a row, a wave a run of it. Top-k and top-p: the logits fall into
 // 2048 bins by their distance from m, with counts and masses; the bin that holds a border is
@@ -42,7 +42,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kMostRow = 1 << 21;
-constexpr float kRange = 48.0f;  // octaves below the maximum that the bins cover: past 47 a weight is 0
+constexpr float kRange = 48.0f;  // octaves below the maximum that the bins cover: past s + 1, 47 at most, a weight is 0
 constexpr int kList = 1024;      // logits of a border's bin that are ranked
 // Candidates that are kept apart from the row; the registers leave room for one workgroup a CU in any case.
 constexpr int kKept = 12288;
@@ -147,7 +147,7 @@ struct Row {
   static constexpr int kLine = 64 * kVec<T>;
   const T* x;
   int V;
-  float m, to_bins;
+  float m, half_m, to_bins;  // to_bins: of half a difference
   double octaves;  // log2(e) / T
   double grid, units;  // weight_on's; 2^s
   int kept;  // candidates, or -1: all of the row
@@ -213,7 +213,10 @@ struct Row {
     __syncthreads();
   }
 
-  __device__ __forceinline__ int bin_of(float v) const { return (int)fminf((m - v) * to_bins, (float)(kBins - 1)); }
+  // Of half the difference: that of two finite logits may be past the largest f32, and only -inf is infinitely far.
+  __device__ __forceinline__ int bin_of(float v) const {
+    return (int)fminf(fmaf(-0.5f, v, half_m) * to_bins, (float)(kBins - 1));
+  }
   // log2 of an element's weight.
   __device__ __forceinline__ double exponent(float v) const { return ((double)v - (double)m) * octaves; }
   __device__ __forceinline__ u64 weight(float v) const { return units_of(weight_on(exponent(v), grid)); }
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
   const int64_t row = block_of();
   if (row >= a.M) return;
   const int tid = threadIdx.x, V = (int)a.V;
-  Row<T> r{static_cast<const T*>(a.x) + row * a.ldx, V, 0.0f, 0.0f, 0.0, ldexp(1.0, 52 - a.shift), ldexp(1.0, a.shift), -1};
+  Row<T> r{static_cast<const T*>(a.x) + row * a.ldx, V, 0.0f, 0.0f, 0.0f, 0.0, ldexp(1.0, 52 - a.shift), ldexp(1.0, a.shift), -1};
 
   const float temperature = setting(a.temperature, a.temperature_all, row);
   const float top_p = setting(a.top_p, a.top_p_all, row), min_p = setting(a.min_p, a.min_p_all, row);
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
                     uniform == uniform;
   if (!(most < __builtin_inff()) || !fine) return done(-1, __builtin_nanf(""));
   if (most == -__builtin_inff()) return done(-1, most);
-  r.m = most;
+  r.m = most, r.half_m = 0.5f * most;
   if (temperature == 0.0f) {
     int first = V;
     r.template scan<6>([&](const auto& some) INLINE {
@@ -472,7 +475,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a) {
   }
   r.octaves = 1.4426950408889634074 / (double)temperature;
   // Finite, so that the maximum is in the first bin.
-  r.to_bins = fminf((float)(kBins / kRange * r.octaves), 1e30f);
+  r.to_bins = fminf((float)(2 * (kBins / kRange) * r.octaves), 1e30f);
 
   const bool use_k = top_k > 0 && top_k < V, use_p = top_p < 1.0f;
   // The least logit of a weight of min_p of the largest, by halving the keys between two that are and are
