@@ -223,8 +223,10 @@ void grouped_backward(Backward a, void* stream) {
   const int e = lm::type_bytes(a.type), chunk = 16 / e;
   const bool masks = act != 0 && a.T > 0 && a.N > 0;
   const int64_t lddz = (a.N + chunk - 1) / chunk * chunk;
-  // dW in f32 through a slope: of dy's two parts, unrounded.
-  const bool split = masks && act == 2 && a.dw && a.type != lm::kF32 && a.dw_type == lm::kF32;
+  // dW in f32 through a slope: of dy's two parts, unrounded. Products with 0, 1 and infinity are what 16 bits hold, and
+  // scaling a sum by 0 or infinity is not scaling its terms (0 times an infinite one, infinity times none).
+  const bool rounds = act == 2 && a.alpha != 0.0f && a.alpha != 1.0f && std::isfinite(a.alpha);
+  const bool split = masks && rounds && a.dw && a.type != lm::kF32 && a.dw_type == lm::kF32;
   const bool whole = masks && ((a.dx && a.K > 0) || (a.dw && !split));
   const size_t one = masks ? aligned((size_t)a.T * lddz * e) : 0, dz_bytes = one * ((whole ? 1 : 0) + (split ? 2 : 0));
   const size_t sums = a.db ? (size_t)lm::grouped_act_tiles(a.T, (int)a.E) * a.N * sizeof(float) : 0;
