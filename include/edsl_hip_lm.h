@@ -156,7 +156,7 @@ int edsl_hip_grouped_dense_launch(const void *X, int64_t ldx, const void *W, int
  * dX has `type`, dW and db that or F32 (dw_type, db_type); dW is [E][K][N], or turned as W
  * may be. Groups without rows have dW and db 0; rows of no group leave dX as it is.
  * dW in F32 through a slope of 16-bit dY is the sum of two products, of dY where Y > 0 and slope times dY elsewhere,
- * but where the slope is 0 or 1: there an infinite X gives NaN. An output may not overlap an input or another output. The same call gives the same bits. */
+ * without that rounding. An output may not overlap an input or another output. The same call gives the same bits. */
 int edsl_hip_grouped_dense_backward_launch(const void *dY, int64_t lddy, const void *X, int64_t ldx, const void *W,
                                            int64_t ldw, int64_t w_stride, int w_turned, const void *offsets, int ids64,
                                            int64_t E, const void *Y, int64_t ldy, void *dX, int64_t lddx, void *dW,
