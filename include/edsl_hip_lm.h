@@ -150,13 +150,13 @@ int edsl_hip_grouped_dense_launch(const void *X, int64_t ldx, const void *W, int
 
 /* Its gradients, each optional. With dZ = dY where there is no activation, else
  * dY * (Y > 0 ? 1 : slope), slope 0 or the leaky epilogue's alpha (>= 0; where it is 0, dZ is 0 whatever dY holds),
- * rounded to `type` for dX and for dW of that type (Y is what the forward pass gave, and may be null without an activation):
+ * rounded to `type` for dX and for BF16 dW (Y is what the forward pass gave, and may be null without an activation):
  *   dX[r] = dZ[r] @ W[e]^T;  dW[e] = sum over the group's rows of X[r]^T dZ[r];
  *   db[e] = sum of dZ[r], without that rounding.
  * dX has `type`, dW and db that or F32 (dw_type, db_type); dW is [E][K][N], or turned as W
  * may be. Groups without rows have dW and db 0; rows of no group leave dX as it is.
- * dW in F32 through a slope of 16-bit dY is the sum of two products, of dY where Y > 0 and slope times dY elsewhere,
- * without that rounding. An output may not overlap an input or another output. The same call gives the same bits. */
+ * dW in F32 or F16 through a slope of 16-bit dY is the sum of two products, of dY where Y > 0 and of dY elsewhere, that
+ * one times the slope. An output may not overlap an input or another output. The same call gives the same bits. */
 int edsl_hip_grouped_dense_backward_launch(const void *dY, int64_t lddy, const void *X, int64_t ldx, const void *W,
                                            int64_t ldw, int64_t w_stride, int w_turned, const void *offsets, int ids64,
                                            int64_t E, const void *Y, int64_t ldy, void *dX, int64_t lddx, void *dW,

@@ -2,9 +2,9 @@
 // bias's gradient: dz = dy (y > 0), or dy times the slope elsewhere, and
 //   db_e = sum over e's rows of dz.
 // Bound by memory: 8192 x 4096 bf16 with both in 42 us (201 MB at 4.8 TB/s), sums alone in 22.
-// dz is rounded to its type, the matrix instructions' operand, for results of that type; db sums it before that, in
-// 32 bits, and dW in f32 through a slope takes dy's two parts as they are, the lower one's product scaled (a 16-bit
-// dy times a slope of 0.01 would be 2^-9 or 2^-12 of it off). Rows are
+// dz is rounded to its type, the matrix instructions' operand, for dX and bf16 dW (a 16-bit dy times a slope of 0.01 is 2^-9 or
+// 2^-12 of it off, f16 below 2^-14 half of 2^-24); db sums it before that, and dW in f32 and of f16 through a slope
+// takes dy's two parts as they are, the lower one's product scaled. Rows are
 // summed in tiles of 32 whose sums a second launch adds in their order (8 of those 42 us), so that the same call
 // gives the same bits. A thread has its own 8 or 4 columns and eight rows on their way; with a wave's threads
 // along the rows, joined through LDS, the same took 92 us.

@@ -476,7 +476,10 @@ def grouped_dense_backward_launch(dY, X, W, offsets, dX=None, dW=None, db=None, 
     """The gradients of ``grouped_dense_launch``, each where it is given: dX
     [T, K] of X's type (with W), dW [E, K, N] (with X) and db [E, N] in that type
     or f32. dY is the gradient of Y; with an activation Y is what the forward pass
-    gave, and a leaky one needs alpha >= 0. Experts without rows have gradients
+    gave, and a leaky one needs alpha >= 0. dX and bf16 dW are products of dY's part
+    that passes, times the slope, rounded to its type: of f16 gradients whose product is below 6e-5
+    steps of 6e-8 are left (scale the loss); db, and dW in f32 or f16, are sums without
+    that rounding. Experts without rows have gradients
     of 0; rows of no expert leave dX as it is. The same call gives the same bits."""
     torch = _torch()
     if _native_module is not None and _done(

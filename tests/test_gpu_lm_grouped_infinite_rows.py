@@ -13,7 +13,7 @@ from test_gpu_lm_grouped import TYPES, offsets_of, stack
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("dtype,grad", [("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("dtype,grad", [("bf16", "f32"), ("f16", "f32"), ("f16", "f16")])
 @pytest.mark.parametrize("order", ["kn", "nk"])
 @pytest.mark.parametrize("counts,K,N", [([3, 0, 20], 40, 24), ([150, 90, 0], 131, 259), ([150, 0, 300], 264, 136)], ids=str)
 def test_infinities(dtype, grad, order, counts, K, N):
