@@ -1,13 +1,15 @@
 // The way back through the activation of a layer on groups of rows, and its
 // bias's gradient: dz = dy (y > 0), or dy times the slope elsewhere, and
 //   db_e = sum over e's rows of dz.
-// Bound by memory: 8192 x 4096 bf16 with both in 42 us (201 MB at 4.8 TB/s), sums alone in 22.
+// Bound by memory: 8192 x 4096 bf16 with both in 42 us (201 MB at 4.8 TB/s), sums alone in 21.
 // dz is rounded to its type, the matrix instructions' operand, for dX and bf16 dW (a 16-bit dy times a slope of 0.01 is 2^-9 or
 // 2^-12 of it off, f16 below 2^-14 half of 2^-24); db sums it before that, and dW in f32 and of f16 through a slope
 // takes dy's two parts as they are, the lower one's product scaled. Rows are
-// summed in tiles of 32 whose sums a second launch adds in their order (8 of those 42 us), so that the same call
+// summed in tiles of 32 whose sums a second launch adds in their order, in 64 bits (8 of those 42 us), so that the same call
 // gives the same bits. A thread has its own 8 or 4 columns and eight rows on their way; with a wave's threads
 // along the rows, joined through LDS, the same took 92 us.
+#include <algorithm>
+
 #include "lm_grouped.hpp"
 
 namespace edsl {
@@ -85,13 +87,16 @@ __global__ void __launch_bounds__(kActThreads) grouped_act_kernel(GroupedActArgs
     if (col + e < a.N) a.partials[(int64_t)tile * a.N + col + e] = sum[e];
 }
 
-__global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
+// A wave has a quarter of an expert's tiles, successive ones, and a lane one column: sums of 2^20 bf16 rows of one expert
+// and 64 columns, 32768 tiles, in 632 us, with one thread for all of a column's tiles in 1386; 8192 rows at 8 of 4096 columns
+// in 20.8 and 21.3.
+constexpr int kBiasWaves = 4;
+__global__ void __launch_bounds__(64 * kBiasWaves) grouped_bias_kernel(GroupedActArgs a) {
   const GroupOffsets g{a.offsets, a.T, a.E, a.ids64};
-  const int expert = blockIdx.y;
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int expert = blockIdx.y, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t n = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 64 + lane;
   const auto rows_of = [&](int e) { return max(g.at(e + 1) - g.at(e), (int64_t)0); };
   // The expert's whole tiles, and the place of its last one behind all whole tiles.
-  const int lane = threadIdx.x % 64;
   int64_t before = 0, all = 0, parts = 0;
   for (int e = lane; e < a.E; e += 64) {
     const int64_t rows = rows_of(e);
@@ -100,20 +105,31 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(GroupedActArgs a) {
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) before += __shfl_xor(before, d), all += __shfl_xor(all, d), parts += __shfl_xor(parts, d);
-  if (n >= a.N) return;
   const int64_t most = grouped_act_tiles(a.T, a.E);  // what the partial sums have room for
   const int64_t rows = rows_of(expert), tiles = min(rows / kActRows, max(most - before, (int64_t)0));
-  float s = 0.0f;
-  int64_t t = 0;
-  for (; t + 8 <= tiles; t += 8) {
-    float v[8];
+  // In 64 bits: their number does not add to the error of a tile's own sum, 31 roundings.
+  double sum = 0.0;
+  if (n < a.N) {
+    const int64_t share = (tiles + kBiasWaves - 1) / kBiasWaves, end = min((wave + 1) * share, tiles);
+    int64_t t = wave * share;
+    for (; t + 8 <= end; t += 8) {
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = a.partials[(before + t + i) * a.N + n];
+      for (int i = 0; i < 8; ++i) v[i] = a.partials[(before + t + i) * a.N + n];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += v[i];
+      for (int i = 0; i < 8; ++i) sum += (double)v[i];
+    }
+    for (; t < end; ++t) sum += (double)a.partials[(before + t) * a.N + n];
+    if (wave == kBiasWaves - 1 && rows % kActRows != 0 && all + parts < most)
+      sum += (double)a.partials[(all + parts) * a.N + n];
   }
-  for (; t < tiles; ++t) s += a.partials[(before + t) * a.N + n];
-  if (rows % kActRows != 0 && all + parts < most) s += a.partials[(all + parts) * a.N + n];
+  __shared__ double sums[kBiasWaves][64];
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || n >= a.N) return;
+#pragma unroll
+  for (int w = 1; w < kBiasWaves; ++w) sum += sums[w][lane];
+  const float s = (float)sum;
   const int64_t at = expert * a.lddb + n;
   if (a.db_type == kF32)
     static_cast<float*>(a.db)[at] = s;
@@ -141,8 +157,9 @@ hipError_t launch_grouped_act(const GroupedActArgs& a, hipStream_t stream) {
     if (e != hipSuccess) return e;
   }
   if (a.db) {
-    hipLaunchKernelGGL(grouped_bias_kernel, dim3((unsigned)((a.N + 255) / 256), (unsigned)a.E), dim3(256), 0, stream,
-                       a);
+    const int64_t blocks = (a.N + 63) / 64, along = std::min<int64_t>(blocks, 1 << 20);  // under 2^32 threads an axis
+    hipLaunchKernelGGL(grouped_bias_kernel, dim3((unsigned)along, (unsigned)a.E, (unsigned)((blocks + along - 1) / along)),
+                       dim3(64 * kBiasWaves), 0, stream, a);
     return launched();
   }
   return hipSuccess;
