@@ -159,10 +159,11 @@ hipError_t launch_tiles(I8Args a, int quarters, int halves, hipStream_t stream) 
   return launched();
 }
 
-// 64 columns: of up to 32 rows.
+// 64 columns: of up to 32 rows. What no kernel is made for is an error: Y would keep what it held.
 template <int MT>
 hipError_t launch_skinny(const I8Args& a, int cols16, hipStream_t stream) {
   constexpr int kWaves = 8;
+  if (cols16 != 1 && cols16 != 2 && (cols16 != 4 || MT > 2)) return hipErrorInvalidValue;
   const dim3 grid((unsigned)((a.N + 16 * cols16 - 1) / (16 * cols16)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
   if (cols16 == 1)
     hipLaunchKernelGGL((i8_skinny_kernel<MT, 1, kWaves>), grid, dim3(64 * kWaves), 0, stream, a);
@@ -190,7 +191,8 @@ hipError_t launch_i8_skinny(const I8Args& a, int rows16, int cols16, hipStream_t
   if (rows16 == 1) return launch_skinny<1>(a, cols16, stream);
   if (rows16 == 2) return launch_skinny<2>(a, cols16, stream);
   if (rows16 == 3) return launch_skinny<3>(a, cols16, stream);
-  return launch_skinny<4>(a, cols16, stream);
+  if (rows16 == 4) return launch_skinny<4>(a, cols16, stream);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace lm
