@@ -87,6 +87,7 @@ struct GroupedLaunch {
         hipLaunchKernelGGL((grouped_weights_kernel<Tl, true>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
         return launched();
       }
+    if (a.more) return hipErrorInvalidValue;  // half of dW would be left out
     hipLaunchKernelGGL((grouped_weights_kernel<Tl, false>), grid_of(tiles), dim3(Tl::kThreads), 0, stream, a);
     return launched();
   }

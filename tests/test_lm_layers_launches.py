@@ -24,3 +24,14 @@ def test_streamed_8_bit_layers_of_other_widths(rows16, cols16):
     launch.restype = ctypes.c_int
     args = ctypes.create_string_buffer(512)  # of no rows and columns
     assert launch(args, rows16, cols16, None) == INVALID_VALUE
+
+
+@pytest.mark.parametrize("kind,direct,big", [(0, 0, 0), (0, 1, 0), (1, 1, 1), (2, 1, 1)])
+def test_two_products_of_tiles_that_take_one(kind, direct, big):
+    """f32, and the largest tiles: the second operand's pointer, the third of the arguments, is given."""
+    launch = exported(f"launch_grouped_weightsILi{kind}E")
+    launch.argtypes = [ctypes.c_void_p, ctypes.c_bool, ctypes.c_bool, ctypes.c_void_p]
+    launch.restype = ctypes.c_int
+    args = ctypes.create_string_buffer(512)
+    ctypes.c_void_p.from_buffer(args, 2 * ctypes.sizeof(ctypes.c_void_p)).value = 0x1000
+    assert launch(args, direct, big, None) == INVALID_VALUE
