@@ -8,7 +8,7 @@
 // real number end at once. Offsets are cut to 0 .. T, so that none leads outside.
 //
 // Three kernels. Groups of a few rows stream their weights (lm_skinny.hpp), bound by memory: 2 rows at 8 bf16
-// experts of 4096 x 4096 in 12.4 us (4.5 TB/s of the weights in use), 96 at 64 of 2048 x 1024 in 51 (4.1 TB/s). Others take tiles (lm_tile.hpp),
+// experts of 4096 x 4096 in 12.4 us (4.5 TB/s of the weights in use), 96 at 64 of 2048 x 1024 in 50 to 53 (4.1 TB/s). Others take tiles (lm_tile.hpp),
 // bound by the matrix cores: 8192 rows at 8 of 4096 x 4096 in 276 to 284 us (0.97 to 1.0 PFLOP/s; one group of 4096 rows there in
 // 124 to 142, the vendor's product in 128); f32 4096 x 4096 x 4096 at 134 to 141 TFLOP/s of 157. dW has the rows as its
 // depth: 345 us from the same 8192 rows, 104 of them the 537 MB of f32 results at the copy's rate.

@@ -5,7 +5,7 @@
 // dz is rounded to its type, the matrix instructions' operand, for dX and bf16 dW (a 16-bit dy times a slope of 0.01 is 2^-9 or
 // 2^-12 of it off, f16 below 2^-14 half of 2^-24); db sums it before that, and dW in f32 and of f16 through a slope
 // takes dy's two parts as they are, the lower one's product scaled. Rows are
-// summed in tiles of 32 whose sums a second launch adds in their order, in 64 bits (8 of those 42 us), so that the same call
+// summed in tiles of 32 whose sums a second launch adds in their order, in 64 bits (6 of those 42 us), so that the same call
 // gives the same bits. A thread has its own 8 or 4 columns and eight rows on their way; with a wave's threads
 // along the rows, joined through LDS, the same took 92 us.
 #include <algorithm>

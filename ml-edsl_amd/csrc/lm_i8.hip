@@ -7,10 +7,11 @@
 // wave's matrix instruction takes, successive k together: any load of them is one run.
 //
 // A few rows stream the weights (lm_skinny.hpp), bound by memory: 1 x 8192 x 8192 in 11.4 us, 5.9 TB/s (three sets
-// of weights in turn stay in the Infinity Cache; the copy's rate is 5.2); at 33 x 4096 x 4097, 11.3 to 12.4 us, the way of
+// of weights in turn stay in the Infinity Cache; the copy's rate is 5.2); at 33 x 4096 x 4097, 12.4 us, the way of
 // eight blocks a wave one after the other is the time. More rows take tiles (lm_tile.hpp), bound by the matrix cores and their
 // power: 4096 x 4096 x 4096 in 57.5 to 67 us by box, 2.0 to 2.4 POP/s (the vendor's product 69 to 86), 8192 x 8192 x 8192 in 480 (2.3). Rows of x
-// off 16 bytes go through registers: 4097 x 4097 x 4097 in 142.
+// off 16 bytes go through registers: 4097 x 4097 x 4097 in 137 to 142, since a turn's wait for its packed weights is also one
+// for the two stages of x on their way.
 #include "lm_kernels.hpp"
 #include "lm_skinny.hpp"
 #include "lm_tile.hpp"
@@ -127,8 +128,8 @@ __global__ void __launch_bounds__(Big::kThreads, Big::kWavesPerSimd) i8_tile_ker
 
 template <int MT, int NJ, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) i8_skinny_kernel(I8Args a) {
-  // Few operands a block are read further ahead: 33 x 4096 x 4097 in 10.2 us with two blocks of weights on
-  // their way, with one in 11.8; 1 x 8192 x 8192 in 11.3 with one of four steps, in 11.9 with two.
+  // Few operands a block are read further ahead: 33 x 4096 x 4097 in 12.4 us with two blocks of weights on
+  // their way, with one in 14.0; 1 x 8192 x 8192 in 11.3 with one of four steps, in 11.9 with two.
   constexpr int U = MT * NJ == 1 ? 4 : MT * NJ <= 8 && MT < 4 ? 2 : 1;
   constexpr int AHEAD = MT * NJ == 1 || NJ == 4 || (NJ == 1 && MT > 2) ? 1 : 2;
   using S = Skinny<int8_t, kBlocks, MT, NJ, WAVES, U, AHEAD>;

@@ -80,13 +80,13 @@ void i8_dense(lm::I8Args a, int64_t M, int64_t N, int64_t K, void* stream) {
   device_launch(0, stream, [&](char*, int cus) {
     const hipStream_t s = as_stream(stream);
     const int64_t tiles = lm::i8_tiles(N), parts = (M + 63) / 64;
-    // Streaming, in parts of up to 64 rows: up to 64 rows (33 x 4096 x 4097 in 11.5 us against 16.7 on tiles), 32 of a layer
+    // Streaming, in parts of up to 64 rows: up to 64 rows (33 x 4096 x 4097 in 12.4 us against 18.3 on tiles), 32 of a layer
     // of more columns than two rounds (64 x 4096 x 16000 in 26 against 17.7; 32 x 4096 x 50256 in 40 against 44), and
     // more rows where all parts together are one round (128 x 8192 x 2048 in 23 against 32; two, 256 rows, in 39 against 32).
     if (N <= kMostStreamed && (M <= (tiles > 2 * (int64_t)cus ? 32 : 64) || (parts <= 64 && parts * tiles <= cus))) {
       // Each workgroup reads all of x: more columns a workgroup where there are many (32 x 4096 x 30000 in 22.8 us on
       // 64 columns, on 32 in 32.4; 1 x 4096 x 30000 in 19.5 and 19.3), and where one more than a round of 16 each would run
-      // (33 x 4096 x 4097 in 10.2 us, in 13.7 on 16), but not where CUs would be idle (32 x 4096 x 4096 in 8.4, on 32 in 9.2).
+      // (33 x 4096 x 4097 in 12.4 us, in 15.8 on 16), but not where CUs would be idle (32 x 4096 x 4096 in 8.4, on 32 in 9.2).
       const int cols = tiles > 4 * (int64_t)cus ? 4 : tiles > (M <= 16 ? 2 : 1) * (int64_t)cus ? 2 : 1;
       const int rows = (int)(((M + parts - 1) / parts + 15) / 16);
       check_hip(lm::launch_i8_skinny(a, rows, cols, s), "i8_skinny launch");
@@ -271,7 +271,7 @@ void grouped_backward(Backward a, void* stream) {
       const int64_t tiles256 = ((g.M + 255) / 256) * ((g.N + 255) / 256) * a.E;
       // 256 x 256 where they fill the CUs and are deep enough: 8192 rows at 8 bf16 experts of 4096 x 4096 in 283 us, 128 x 128
       // in 333; 2048 rows in 122 and 127, 1024 in 102 and 98. f32 results, twice the bytes, 8192 rows: 379 and 435, 4096: 243
-      // and 237, 2048: 200 and 178. Two products spill there: the whole way back through a slope in 1041 and 986, 622 without one.
+      // and 237, 2048: 200 and 178. Two products spill there: the whole way back through a slope in 1041 with it and 986 without, through ReLU in 622.
       const bool big = !split && direct && a.type != lm::kF32 && tiles256 >= cus &&
                        a.T >= (a.dw_type == lm::kF32 ? 768 : 256) * a.E;
       check_grid((g.M + 127) / 128 * a.E, (g.N + 127) / 128);
