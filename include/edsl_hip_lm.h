@@ -150,7 +150,8 @@ int edsl_hip_grouped_dense_launch(const void *X, int64_t ldx, const void *W, int
 
 /* Its gradients, each optional. With dZ = dY where there is no activation, else
  * dY * (Y > 0 ? 1 : slope), slope 0 or the leaky epilogue's alpha (>= 0; where it is 0, dZ is 0 whatever dY holds),
- * rounded to `type` for dX and for BF16 dW (Y is what the forward pass gave, and may be null without an activation):
+ * rounded to `type` for dX and, where that is BF16 or F32, for dW of that type (Y is what the forward pass gave, and may be
+ * null without an activation):
  *   dX[r] = dZ[r] @ W[e]^T;  dW[e] = sum over the group's rows of X[r]^T dZ[r];
  *   db[e] = sum of dZ[r], without that rounding.
  * dX has `type`, dW and db that or F32 (dw_type, db_type); dW is [E][K][N], or turned as W

@@ -41,3 +41,35 @@ def test_infinities(dtype, grad, order, counts, K, N):
         assert torch.equal(got[~fine].nan_to_num(nan=0.0), want[~fine].nan_to_num(nan=0.0))
         bound = (max(counts) + 65) * 2.0 ** -23 * size + ref.HALF_ULP[dw.dtype] * want.abs() + ref.TINY[dw.dtype]
         assert bool(((got - want).abs() <= bound)[fine].all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_captured(dtype):
+    """A captured call whose rows, groups and infinities change between its replays: the eager call's bits."""
+    t, T, E, K, N = TYPES[dtype], 160, 3, 72, 136
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).to(t).cuda()  # noqa: E731
+    dy, x, y, w, off = r(T, N), r(T, K), r(T, N), r(E, K, N), offsets_of([100, 20, 40])
+    outs = [torch.zeros(T, K, dtype=t, device="cuda"), torch.zeros(E, K, N, dtype=t if dtype == "f16" else torch.float32,
+                                                                   device="cuda"), torch.zeros(E, N, device="cuda")]
+
+    def step(outs):
+        lm.grouped_dense_backward_launch(dy, x, w, off, *outs, y, _native.EPI_BIAS_LEAKY, 0.3)
+    step(outs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(outs)
+    for i, counts in enumerate(([0, 160, 0], [1, 30, 129], [60, 60, 40], [10, 5, 2])):
+        dy.copy_(r(T, N))
+        x.copy_(r(T, K))
+        x[i, ::3], x[150 - i, ::4] = math.inf, math.nan if i % 2 else -math.inf
+        off.copy_(offsets_of(counts))
+        for out in outs:
+            out.fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = [torch.full_like(out, -7.0) for out in outs]
+        step(eager)
+        for got, want in zip(outs, eager):
+            assert torch.equal(got.double().nan_to_num(nan=12345.0), want.double().nan_to_num(nan=12345.0))
